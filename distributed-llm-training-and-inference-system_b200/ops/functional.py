@@ -14,9 +14,10 @@ can attribute speed-ups.
 """
 from __future__ import annotations
 
+import contextlib
 import threading
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -85,6 +86,11 @@ def _whole_units(t: torch.Tensor) -> torch.Tensor:
     """``t`` contiguous from a 16-byte boundary, as the kernels read it."""
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _on_device(t: torch.Tensor):
+    """Launches go to the current device's stream: a context in which that is the tensor's device."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 _NORM_BWD_CTAS = 148 * 4
@@ -723,6 +729,100 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor, ignore_index: int
         return _CrossEntropyFn.apply(logits2, t.contiguous(), ignore_index, grad_scale, assume_unit_grad)
     loss = F.cross_entropy(logits2.float(), t, ignore_index=ignore_index)
     return loss * grad_scale if grad_scale != 1.0 else loss
+
+
+# ------------------------------------------------------------------------------------------------
+# Log probabilities of given tokens, entropy, most probable tokens — csrc/loss/token_logprobs.cu
+# ------------------------------------------------------------------------------------------------
+MAX_TOP_LOGPROBS = 64
+
+
+class TokenLogprobs(NamedTuple):
+    """``logprobs`` and ``entropy``: fp32, one per row of logits (natural logarithms); ``top_ids`` (int64) and ``top_logprobs`` (fp32) [..., top]: the most
+    probable tokens, largest first, of equal ones the lowest id first; None where ``top`` is 0."""
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: Optional[torch.Tensor] = None
+    top_logprobs: Optional[torch.Tensor] = None
+
+
+def _rows_like(logits: torch.Tensor) -> torch.Tensor:
+    """Uninitialised rows of the same sizes, type and place in 16-byte units (where the kernel loads whole units it stores whole ones)."""
+    rows, V = logits.shape
+    size, units = logits.element_size(), 16 // logits.element_size()
+    ld = V + (logits.stride(0) - V) % units if rows > 1 else V
+    shift = logits.data_ptr() % 16 // size
+    buf = torch.empty(shift + rows * ld, dtype=logits.dtype, device=logits.device)
+    return buf.as_strided((rows, V), (ld, 1), shift)
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top):
+        rows, V = logits.shape
+        f32 = {"dtype": torch.float32, "device": logits.device}
+        logprobs, entropy = torch.empty(rows, **f32), torch.empty(rows, **f32)
+        stats = torch.empty(rows, 2, **f32) if ctx.needs_input_grad else None
+        top_ids = torch.empty(rows, top, dtype=torch.int64, device=logits.device) if top else None
+        top_logprobs = torch.empty(rows, top, **f32) if top else None
+        native.call("llmctl_token_logprobs", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), tokens.data_ptr(), rows, V, top,
+                    logprobs.data_ptr(), entropy.data_ptr(), native.ptr(stats), native.ptr(top_ids), native.ptr(top_logprobs), native.stream_ptr())
+        if stats is not None:
+            native.keep(ctx, logits, tokens, stats, entropy, top_ids)
+            ctx.top = top
+            ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(top_ids)
+        return logprobs, entropy, top_ids, top_logprobs
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_logprobs, d_entropy, _, d_top):
+        logits, tokens, stats, entropy, top_ids = native.kept(ctx)
+        if logits.stride(1) != 1:
+            logits = logits.contiguous()
+        tokens, stats, entropy = tokens.contiguous(), stats.contiguous(), entropy.contiguous()
+        top_ids = None if top_ids is None else top_ids.contiguous()
+        d_logprobs, d_entropy, d_top = (None if d is None else d.float().contiguous() for d in (d_logprobs, d_entropy, d_top))
+        dx = _rows_like(logits)
+        with _on_device(logits):
+            native.call("llmctl_token_logprobs_bwd", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), tokens.data_ptr(), *logits.shape,
+                        ctx.top, stats.data_ptr(), entropy.data_ptr(), native.ptr(top_ids), native.ptr(d_logprobs), native.ptr(d_entropy), native.ptr(d_top),
+                        dx.data_ptr(), dx.stride(0), native.stream_ptr())
+        return dx, None, None
+
+
+def _token_logprobs_torch(x: torch.Tensor, tokens: torch.Tensor, top: int) -> TokenLogprobs:
+    lp = torch.log_softmax(x, -1)
+    p = lp.exp()
+    entropy = -torch.where(p == 0, 0.0, p * lp.clamp(min=-1e4)).sum(-1)
+    given = (tokens >= 0) & (tokens < x.shape[-1])
+    logprobs = lp.gather(-1, torch.where(given, tokens, 0).unsqueeze(-1)).squeeze(-1)
+    logprobs = torch.where(given, logprobs, torch.zeros_like(logprobs))
+    if not top:
+        return TokenLogprobs(logprobs, entropy)
+    ids = torch.sort(torch.where(x.isnan(), float("-inf"), x.detach()), dim=-1, descending=True, stable=True).indices[..., :top]
+    return TokenLogprobs(logprobs, entropy, ids, lp.gather(-1, ids))
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` (int64 [...]; a number that is no token of the vocabulary has 0 and no gradient) under ``logits`` [..., vocabulary], the
+    entropy of each row and its ``top`` most probable tokens.  ``logits`` are left as they are; gradients of the log probabilities (``top_logprobs`` among
+    them) and of the entropy flow back to them.  A row that holds a NaN or +inf, or nothing but -inf, has NaN for each."""
+    V = logits.shape[-1]
+    if tokens.shape != logits.shape[:-1] or tokens.dtype != torch.int64 or tokens.device != logits.device:
+        raise ValueError(f"token_logprobs: int64 tokens of sizes {list(logits.shape[:-1])} beside the logits, not {tokens.dtype} {list(tokens.shape)} on {tokens.device}")
+    if not logits.is_floating_point() or not 0 <= top <= min(V, MAX_TOP_LOGPROBS):
+        raise ValueError(f"token_logprobs: floating logits and 0 to {min(V, MAX_TOP_LOGPROBS)} most probable tokens, not {logits.dtype} and {top}")
+    if logits.is_cuda and _cfg.elementwise == "native" and logits.dtype in (torch.bfloat16, torch.float32) and logits.numel():
+        rows = logits.reshape(-1, V)
+        if rows.stride(1) != 1:
+            rows = rows.contiguous()
+        with _on_device(rows):
+            out = native.apply(_TokenLogprobsFn, rows, tokens.reshape(-1).contiguous(), top)
+        lead = logits.shape[:-1]
+        return TokenLogprobs(out[0].view(lead), out[1].view(lead), *(None if t is None else t.view(*lead, top) for t in out[2:]))
+    return _token_logprobs_torch(logits if logits.dtype == torch.float64 else logits.float(), tokens, top)
 
 
 # ------------------------------------------------------------------------------------------------

@@ -74,6 +74,8 @@ _SIGNATURES = {
     "llmctl_cross_entropy_mean": [c_void_p, c_ll, c_void_p, c_void_p, c_int, c_int, c_ll, c_float, c_int, c_void_p, c_void_p],
     "llmctl_cross_entropy_partial": [c_void_p, c_ll, c_void_p, c_void_p, c_int, c_int, c_ll, c_void_p],
     "llmctl_cross_entropy_finalize": [c_void_p, c_ll, c_void_p, c_void_p, c_int, c_int, c_ll, c_ll, c_float, c_void_p, c_void_p],
+    "llmctl_token_logprobs": [c_void_p, c_int, c_ll, c_void_p, c_int, c_int, c_int] + [c_void_p] * 6,
+    "llmctl_token_logprobs_bwd": [c_void_p, c_int, c_ll, c_void_p, c_int, c_int, c_int] + [c_void_p] * 7 + [c_ll, c_void_p],
     "llmctl_gemm_bf16": [c_void_p] * 3 + [c_int] * 3 + [c_ll] * 3 + [c_int] * 6 + [c_void_p],
     "llmctl_gemm_bf16_bgated": [c_void_p] * 3 + [c_int] * 3 + [c_ll] * 3 + [c_int] * 6 + [c_void_p, ctypes.c_uint, c_ll, c_ll, c_void_p],
     "llmctl_gemm_swiglu_bf16": [c_void_p] * 4 + [c_int] * 3 + [c_ll] * 4 + [c_void_p],

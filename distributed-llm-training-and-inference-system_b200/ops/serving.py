@@ -1,7 +1,11 @@
-"""Serving ops: paged KV append (K13), paged decode attention (K12), batched sampling (K14).  CUDA/bf16 runs
-the native kernels; CPU tensors run a plain PyTorch restatement (used by the CPU tests and as the oracle)."""
+"""Serving ops: paged KV append (K13) with or without the rotation, paged decode attention (K12) over caches of 16 or 8 bits, batched sampling (K14).
+CUDA/bf16 runs the native kernels; CPU tensors run a plain PyTorch restatement (used by the CPU tests and as the oracle).
+
+A cache of 8 bits is [blocks, kv_heads, block_size, head_dim] of ``torch.float8_e4m3fn`` with scales, fp32 [blocks, kv_heads]: a number is its code times
+its block's scale (``allocate_fp8_cache``)."""
 from __future__ import annotations
 
+import contextlib
 import math
 from functools import lru_cache
 from typing import Optional
@@ -16,6 +20,10 @@ native.register_signature("llmctl_paged_attn_decode",
                           [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_ll, c_void_p,
                            c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p])
 native.register_signature("llmctl_paged_attn_scratch_elems", [c_int, c_int, c_int, c_int], restype=c_ll)
+native.register_signature("llmctl_rope_kv_append", [c_void_p, c_ll] + [c_int] * 4 + [c_void_p, c_void_p, c_int] + [c_void_p] * 4 + [c_ll, c_void_p])
+native.register_signature("llmctl_rope_kv_append_fp8", [c_void_p, c_ll] + [c_int] * 4 + [c_void_p, c_void_p, c_int] + [c_void_p] * 6 + [c_int, c_int, c_void_p])
+native.register_signature("llmctl_paged_attn_fp8_scratch_elems", [c_int] * 4, restype=c_ll)
+native.register_signature("llmctl_paged_attn_decode_fp8", [c_void_p, c_ll] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 8 + [c_float, c_void_p])
 native.register_signature("llmctl_sample", [c_void_p, c_int, c_ll, c_int, c_int] + [c_void_p] * 6 + [c_void_p])
 
 
@@ -128,6 +136,167 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         v = v_cache.view(-1, H, D)[slots].float()
         s = torch.einsum("hd,nhd->hn", q[b].float(), k) * scale
         out[b] = torch.einsum("hn,nhd->hd", torch.softmax(s, -1), v).to(q.dtype)
+    return out
+
+
+# ---- rotation and append in one pass; caches of 8 bits ---------------------------------------------------------------------------------------------
+FP8 = torch.float8_e4m3fn
+_FP8_MAX = 448.0
+
+
+def allocate_fp8_cache(num_blocks: int, block_size: int, kv_heads: int, head_dim: int, device=None):
+    """``(codes, scales)`` of an empty cache of 8 bits for keys or for values."""
+    return (torch.zeros(num_blocks, kv_heads, block_size, head_dim, dtype=FP8, device=device), torch.zeros(num_blocks, kv_heads, dtype=torch.float32, device=device))
+
+
+def _on_device(t: torch.Tensor):
+    """Launches go to the current device's stream: a context in which that is the tensor's device."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _check_fp8_caches(k_cache, v_cache, k_scale, v_scale, head_dim: int, device) -> None:
+    for c, s in ((k_cache, k_scale), (v_cache, v_scale)):
+        _check(c.dim() == 4 and c.dtype == FP8 and c.is_contiguous() and c.device == device and c.shape[3] == head_dim and c.data_ptr() % 16 == 0,
+               f"a cache of 8 bits is contiguous [blocks, kv_heads, block_size, {head_dim}] of {FP8} beside the rows, from a 16-byte boundary")
+        _check(s is not None and s.dtype == torch.float32 and s.is_contiguous() and s.device == device and s.shape == c.shape[:2],
+               "scales of a cache of 8 bits: contiguous float32 [blocks, kv_heads] beside it")
+    _check(k_cache.shape == v_cache.shape, "k_cache and v_cache: of one shape")
+
+
+def _quantise_rows(x: torch.Tensor, cache: torch.Tensor, scale: torch.Tensor, slots: torch.Tensor) -> None:
+    """x: fp32 [T, kv_heads, head_dim] to the rows ``slots`` of a cache of 8 bits, as the kernel does it (csrc/serve/rope_kv_append.cu)."""
+    size = cache.shape[2]
+    last = {int(s): i for i, s in enumerate(slots.tolist()) if 0 <= s < cache.shape[0] * size}      # of a slot's tokens the last
+    for block in sorted({s // size for s in last}):
+        rows = [r for r in range(size) if block * size + r in last]
+        new = x[[last[block * size + r] for r in rows]].transpose(0, 1)                              # [kv_heads, rows, head_dim]
+        most = torch.where(new.isfinite(), new.abs(), 0.0).amax((1, 2))
+        mantissa, exponent = torch.frexp(most)
+        need = torch.where(most > 0, torch.ldexp(torch.ones_like(most), (exponent - 9 + (mantissa > _FP8_MAX / 512).int()).clamp(min=-126)), 0.0)
+        old = torch.zeros_like(need) if rows[0] == 0 else scale[block].clamp(min=0.0)
+        to = torch.maximum(need, old)
+        if rows[0] != 0:
+            grown = (to > old).nonzero().reshape(-1)
+            others = torch.tensor([r for r in range(size) if block * size + r not in last], dtype=torch.int64)
+            for h in grown.tolist():
+                cache[block, h, others] = (cache[block, h, others].float() * (old[h] / to[h])).to(FP8)
+        inv = torch.where(to > 0, 1.0 / to, 0.0)[:, None, None]
+        cache[block][:, torch.tensor(rows)] = torch.where(new.isfinite(), new * inv, float("nan")).to(FP8)
+        scale[block] = to
+
+
+def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   slot_mapping: torch.Tensor, heads: int, head_dim: int, *, kv_heads: Optional[int] = None, k_scale: Optional[torch.Tensor] = None,
+                   v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotates q and k of the packed rows ``qkv`` [T, (heads + 2 kv_heads) * head_dim] in place to their ``positions`` (int32 [T], rows of the tables ``cos`` /
+    ``sin``, fp32 [positions, head_dim / 2]) and writes k and v to the rows ``slot_mapping`` (int64 [T]; outside of the cache = skip) of the caches:
+    [blocks, block_size, kv_heads, head_dim] of the rows' type, or caches of 8 bits with their scales.  Returns ``qkv``.
+
+    Where the call names a row of a cache of 16 bits more than once any of its tokens is kept.  In a cache of 8 bits a block's scale is the smallest power of two under which the largest number written to it fits.  The tokens of a block may
+    stand anywhere in the call; where it names a slot more than once the last is kept.  A block whose first row is written begins anew; in any
+    other the rows that the call does not write keep what they stand for, in codes of the larger scale where it grows.  NaN and infinities become NaN."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    fp8 = k_cache.dtype == FP8
+    T, width = qkv.shape[0], (heads + 2 * kv_heads) * head_dim
+    _check(heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and head_dim > 0 and head_dim % 16 == 0, "heads: a multiple of kv_heads; head_dim: a multiple of 16")
+    _check(qkv.dim() == 2 and qkv.shape[1] >= width, f"qkv: rows of at least {width} numbers")
+    _check(not (torch.is_grad_enabled() and qkv.requires_grad), "rope_kv_append has no backward: call it under no_grad")
+    for t in (cos, sin):
+        _check(t.dim() == 2 and t.shape == cos.shape and t.shape[0] > 0 and t.shape[1] == head_dim // 2 and t.dtype == torch.float32 and t.device == qkv.device,
+               f"cos and sin: float32 [positions, {head_dim // 2}] beside the rows")
+    _check(positions.shape == (T,) and positions.dtype == torch.int32 and positions.device == qkv.device, "positions: int32 beside the rows, one per row")
+    _check(slot_mapping.shape == (T,) and slot_mapping.dtype == torch.int64 and slot_mapping.device == qkv.device, "slot_mapping: int64 beside the rows, one per row")
+    if fp8:
+        _check_fp8_caches(k_cache, v_cache, k_scale, v_scale, head_dim, qkv.device)
+        _check(k_cache.shape[1] == kv_heads and 1 <= k_cache.shape[2] <= 4096 and head_dim <= 512, f"a cache of 8 bits of {kv_heads} heads, blocks of at most 4096 rows, heads of at most 512")
+    else:
+        _check(k_scale is None and v_scale is None, "scales belong to caches of 8 bits")
+        for c in (k_cache, v_cache):
+            _check(c.dtype == qkv.dtype and c.device == qkv.device and c.is_contiguous() and c.dim() == 4 and c.shape[2:] == (kv_heads, head_dim) and c.data_ptr() % 16 == 0,
+                   f"a cache is contiguous [blocks, block_size, {kv_heads}, {head_dim}] of the rows' type beside them, from a 16-byte boundary")
+        _check(k_cache.shape == v_cache.shape, "k_cache and v_cache: of one shape")
+    if qkv.is_cuda:
+        _check(qkv.dtype == torch.bfloat16, "qkv: bfloat16")
+        cos, sin, positions, slot_mapping = (t.contiguous() for t in (cos, sin, positions, slot_mapping))
+        cos, sin = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (cos, sin))
+        rows = qkv if qkv.stride(1) == 1 and qkv.stride(0) % 8 == 0 and qkv.stride(0) >= width and qkv.data_ptr() % 16 == 0 else _aligned_rows(qkv, width)
+        args = (rows.data_ptr(), rows.stride(0), T, heads, kv_heads, head_dim, cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(),
+                slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr())
+        with _on_device(qkv):
+            if fp8:
+                native.call("llmctl_rope_kv_append_fp8", *args, k_scale.data_ptr(), v_scale.data_ptr(), k_cache.shape[0], k_cache.shape[2], native.stream_ptr())
+            else:
+                native.call("llmctl_rope_kv_append", *args, k_cache.shape[0] * k_cache.shape[1], native.stream_ptr())
+            if rows is not qkv:
+                qkv[:, :width].copy_(rows)
+            elif not qkv.is_inference():
+                torch.autograd.graph.increment_version(qkv)
+        return qkv
+    x = qkv[:, :width].view(T, heads + 2 * kv_heads, head_dim)
+    half = head_dim // 2
+    at = positions.long().clamp(0, cos.shape[0] - 1)
+    c, s = cos[at].unsqueeze(1), sin[at].unsqueeze(1)
+    a, b = x[:, :heads + kv_heads, :half].float(), x[:, :heads + kv_heads, half:].float()
+    rotated = torch.cat([a * c - b * s, b * c + a * s], dim=-1)
+    x[:, :heads + kv_heads] = rotated.to(x.dtype)
+    if fp8:
+        _quantise_rows(rotated[:, heads:], k_cache, k_scale, slot_mapping)
+        _quantise_rows(x[:, heads + kv_heads:].float(), v_cache, v_scale, slot_mapping)
+        return qkv
+    ok = (slot_mapping >= 0) & (slot_mapping < k_cache.shape[0] * k_cache.shape[1])
+    k_cache.view(-1, kv_heads, head_dim)[slot_mapping[ok]] = x[ok, heads:heads + kv_heads]
+    v_cache.view(-1, kv_heads, head_dim)[slot_mapping[ok]] = x[ok, heads + kv_heads:]
+    return qkv
+
+
+def _aligned_rows(x: torch.Tensor, width: int) -> torch.Tensor:
+    """A copy of the first ``width`` columns in rows that begin at 16-byte boundaries."""
+    return x[:, :width].clone(memory_format=torch.contiguous_format)
+
+
+def paged_attention_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                               block_tables: torch.Tensor, context_lens: torch.Tensor, max_context: int, scale: Optional[float] = None,
+                               num_splits: Optional[int] = None) -> torch.Tensor:
+    """``paged_attention_decode`` over caches of 8 bits: q [B, heads, head_dim], a token per sequence; block_tables: int32 [B, max_blocks]; context_lens: int32
+    [B], at most ``max_context`` (tokens beyond it, or beyond the table, are left out) -> [B, heads, head_dim].  heads may be a multiple of the cache's heads:
+    query head h reads head h // (heads / kv_heads).  A sequence without tokens gets zeros.  What the cache holds behind a sequence's last token does not matter."""
+    B, H, D = q.shape
+    blocks, kv_heads, block_size = k_cache.shape[:3]
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    _check(not (torch.is_grad_enabled() and q.requires_grad), "paged_attention_decode_fp8 has no backward: call it under no_grad")
+    _check_fp8_caches(k_cache, v_cache, k_scale, v_scale, D, q.device)
+    _check(H % kv_heads == 0, "heads: a multiple of the cache's")
+    _check(block_tables.dim() == 2 and block_tables.shape[0] >= B and block_tables.dtype == torch.int32 and block_tables.device == q.device, "block_tables: int32 beside the queries, a row per sequence")
+    _check(context_lens.dim() == 1 and context_lens.numel() >= B and context_lens.dtype == torch.int32 and context_lens.device == q.device, "context_lens: int32 beside the queries, one per sequence")
+    max_context = max(0, min(int(max_context), block_tables.shape[1] * block_size))
+    if q.is_cuda:
+        _check(q.dtype == torch.bfloat16 and D in (64, 128), "q: bfloat16, heads of 64 or 128")
+        _check(num_splits is None or 1 <= num_splits <= 256, "num_splits: 1 to 256")
+        out = torch.empty(B, H, D, dtype=q.dtype, device=q.device)
+        if B == 0:
+            return out
+        ns = num_splits or choose_splits(B, H, max_context, block_size)
+        block_tables, context_lens = block_tables.contiguous(), context_lens.contiguous()
+        if q.stride(2) != 1 or q.stride(1) != D or q.data_ptr() % 16 or q.stride(0) % 8:
+            q = q.clone(memory_format=torch.contiguous_format)
+        need = native.lib().llmctl_paged_attn_fp8_scratch_elems(B, H, D, ns)
+        scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+        with _on_device(q):
+            native.call("llmctl_paged_attn_decode_fp8", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                        v_scale.data_ptr(), block_tables.data_ptr(), block_tables.shape[1], context_lens.data_ptr(), out.data_ptr(), native.ptr(scratch), B, H,
+                        kv_heads, D, blocks, block_size, max_context, ns, float(scale), native.stream_ptr())
+        if need:
+            native.count_launches(1)        # the merge kernel
+        return out
+    out = torch.zeros(B, H, D, dtype=q.dtype)
+    for b in range(B):
+        n = min(int(context_lens[b]), max_context)
+        if n <= 0:
+            continue
+        pages = block_tables[b, :(n + block_size - 1) // block_size].long()
+        k, v = ((c[pages].float() * s[pages][..., None, None]).transpose(0, 1).reshape(kv_heads, -1, D)[:, :n] for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
+        s = torch.einsum("kgd,knd->kgn", q[b].float().view(kv_heads, H // kv_heads, D), k) * scale
+        out[b] = torch.einsum("kgn,knd->kgd", torch.softmax(s, -1), v).reshape(H, D).to(q.dtype)
     return out
 
 

@@ -86,6 +86,13 @@ void* llmctl_wait_status_word(void);
 int llmctl_wait_status_report(int which, void* stream);
 /* 0 unless a bounded wait of the loss kernel ran out since the last clearing call (synchronises the device). */
 int llmctl_cross_entropy_status(int clear);
+/* Log probabilities of given tokens, entropies and the most probable tokens of rows of V bf16 (is_fp32: fp32) logits, and the logits' gradient
+ * (csrc/loss/token_logprobs.cu).  stats: fp32 [rows, 2] for the gradient, or NULL; top: 0 .. 64.  dx lies to 16-byte boundaries as logits does. */
+int llmctl_token_logprobs(const void* logits, int is_fp32, long long ld, const long long* tokens, int rows, int V, int top, float* logprobs,
+                          float* entropy, float* stats, long long* top_ids, float* top_logprobs, void* stream);
+int llmctl_token_logprobs_bwd(const void* logits, int is_fp32, long long ld, const long long* tokens, int rows, int V, int top, const float* stats,
+                              const float* entropy, const long long* top_ids, const float* d_logprobs, const float* d_entropy, const float* d_top,
+                              void* dx, long long ldd, void* stream);
 int llmctl_cross_entropy_partial(const void* logits, long long ld, const long long* targets,
                                  float* stats, int rows, int V_local, long long vocab_start,
                                  void* stream);
@@ -117,6 +124,20 @@ int llmctl_paged_attn_decode(const void* q, long long q_stride, const void* k_ca
                              const int* context_lens, void* out, long long out_stride, float* scratch,
                              int batch, int heads, int head_dim, int block_size, int max_context,
                              int num_splits, float scale, void* stream);
+
+/* Rotation of packed q | k | v rows in place with the append of k and v to paged caches of 16 bits, or of 8 bits (e4m3, a power of two as scale for each
+ * block and head; csrc/serve/rope_kv_append.cu), and decode attention over the latter (csrc/serve/paged_attention_fp8.cu). */
+int llmctl_rope_kv_append(void* qkv, long long row_stride, int tokens, int heads, int kv_heads, int head_dim, const float* cos_t, const float* sin_t,
+                          int table_rows, const int* positions, const long long* slots, void* k_cache, void* v_cache, long long cache_rows,
+                          void* stream);
+int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int tokens, int heads, int kv_heads, int head_dim, const float* cos_t,
+                              const float* sin_t, int table_rows, const int* positions, const long long* slots, void* k_cache, void* v_cache,
+                              float* k_scale, float* v_scale, int blocks, int block_size, void* stream);
+long long llmctl_paged_attn_fp8_scratch_elems(int batch, int heads, int head_dim, int num_splits);
+int llmctl_paged_attn_decode_fp8(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const float* k_scale,
+                                 const float* v_scale, const int* block_tables, int max_blocks, const int* context_lens, void* out, float* scratch,
+                                 int batch, int heads, int kv_heads, int head_dim, int blocks, int block_size, int max_context, int num_splits,
+                                 float scale, void* stream);
 
 /* ---- K14 sampling.  Reference: per-request Python loop with .item() syncs (server.py:209-235). ---- */
 int llmctl_sample(const void* logits, int logits_is_fp32, long long ld, int rows, int V,
