@@ -48,7 +48,7 @@ static std::unordered_map<Key, CUtensorMap, KeyHash> g_cache;
 
 static int encode_cached(CUtensorMap* out, const Key& key, int rank, const void* base,
                          const cuuint64_t* dims, const cuuint64_t* strides_bytes,
-                         const cuuint32_t* box, int swizzle128) {
+                         const cuuint32_t* box, CUtensorMapSwizzle swizzle, CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16) {
   {
     std::lock_guard<std::mutex> lk(g_mu);
     auto it = g_cache.find(key);
@@ -68,9 +68,9 @@ static int encode_cached(CUtensorMap* out, const Key& key, int rank, const void*
     ctx_bound = true;
   }
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims,
+  CUresult r = fn(out, type, rank, const_cast<void*>(base), dims,
                   strides_bytes, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     if (getenv("LLMCTL_DEBUG"))
@@ -100,7 +100,20 @@ int get_tmap_2d_bf16(CUtensorMap* out, const void* base, uint64_t rows, uint64_t
   cuuint64_t dims[2] = {cols, rows};
   cuuint64_t strides[1] = {ld * 2};
   cuuint32_t box[2] = {box_cols, box_rows};
-  return encode_cached(out, key, 2, base, dims, strides, box, swizzle128);
+  return encode_cached(out, key, 2, base, dims, strides, box, swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+int get_tmap_2d_bytes(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes, uint64_t pitch, uint32_t box_rows, uint32_t box_bytes) {
+  Key key;
+  memset(&key, 0, sizeof(key));
+  const uint64_t all[6] = {reinterpret_cast<uint64_t>(base), rows, row_bytes, pitch, box_rows, box_bytes};
+  memcpy(key.v, all, sizeof(all));
+  key.v[13] = 8;                // of bytes
+  cuuint64_t dims[2] = {row_bytes, rows};
+  cuuint64_t strides[1] = {pitch};
+  cuuint32_t box[2] = {box_bytes, box_rows};
+  return encode_cached(out, key, 2, base, dims, strides, box, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                       CU_TENSOR_MAP_DATA_TYPE_UINT8);
 }
 
 int get_tmap_4d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t d3,
@@ -115,7 +128,7 @@ int get_tmap_4d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d
   cuuint64_t dims[4] = {d0, d1, d2, d3};
   cuuint64_t strides[3] = {s1 * 2, s2 * 2, s3 * 2};
   cuuint32_t box[4] = {b0, b1, b2, b3};
-  return encode_cached(out, key, 4, base, dims, strides, box, swizzle128);
+  return encode_cached(out, key, 4, base, dims, strides, box, swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 }  // namespace llmctl

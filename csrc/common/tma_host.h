@@ -19,4 +19,7 @@ int get_tmap_4d_bf16(CUtensorMap* out, const void* base, uint64_t d0, uint64_t d
                      uint64_t s1, uint64_t s2, uint64_t s3, uint32_t b0, uint32_t b1, uint32_t b2, uint32_t b3,
                      int swizzle128);
 
+// 2D map over rows of bytes, `pitch` bytes apart: box = [box_rows, box_bytes], 128- or 64-byte swizzle (box_bytes).
+int get_tmap_2d_bytes(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes, uint64_t pitch, uint32_t box_rows, uint32_t box_bytes);
+
 }  // namespace llmctl

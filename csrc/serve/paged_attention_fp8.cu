@@ -6,8 +6,8 @@
 // over the tokens j < context_lens[b] of the blocks in the sequence's table; query head h reads head h / (heads / kv_heads) of the cache.  A sequence
 // without tokens gets zeros.
 //
-// This kernel: a warp takes every fourth token, a lane D / 32 dimensions of it; fp32 throughout.  Splits of the context are
-// merged by a second kernel.
+// Blocks of a multiple of 8 tokens go to the tensor cores (paged_attention_fp8_t5.cu).  Of any other size: a warp takes every fourth token, a lane D / 32 dimensions of it; fp32 throughout.  Splits of the context are
+// in both merged by a second kernel.
 //
 // Reference: none — the reference re-runs the model over the whole sequence (reference llmctl/serve/server.py:199-204).
 #include "../common/dependent.cuh"
@@ -15,6 +15,11 @@
 #include "../common/util.cuh"
 
 namespace llmctl {
+
+bool paged_attn_fp8_t5_ok(int head_dim, int block_size);
+int launch_paged_attn_fp8_t5(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                             const int* block_tables, int max_blocks, const int* context_lens, void* out, float* partial, int batch, int heads, int kv_heads,
+                             int head_dim, int blocks, int block_size, int limit, int tokens_per_split, int splits, float scale, cudaStream_t s);
 
 namespace decode8 {
 constexpr float kLog2e = 1.4426950408889634f;
@@ -152,13 +157,21 @@ LLMCTL_API int llmctl_paged_attn_decode_fp8(const void* q, long long q_stride, c
   LLMCTL_REQUIRE(aligned16(k_cache, v_cache));
   cudaStream_t s = (cudaStream_t)stream;
   const long long room = static_cast<long long>(max_blocks) * block_size;
-  const int limit = max_context < room ? max_context : static_cast<int>(room), per = limit > 0 ? (limit - 1) / num_splits + 1 : 1;
-  auto launch = [&](auto kern) {
-    return launch_dependent(kern, dim3(heads, num_splits, batch), 128, 0, s, (const __nv_bfloat16*)q, q_stride, (const uint8_t*)k_cache,
-                            (const uint8_t*)v_cache, k_scale, v_scale, block_tables, max_blocks, context_lens, scratch, (__nv_bfloat16*)out, blocks,
-                            block_size, heads / kv_heads, limit, per, scale * decode8::kLog2e);
-  };
-  LLMCTL_CHECK(head_dim == 128 ? launch(paged_attn_decode_fp8_kernel<128>) : launch(paged_attn_decode_fp8_kernel<64>));
+  const int limit = max_context < room ? max_context : static_cast<int>(room);
+  int per = limit > 0 ? (limit - 1) / num_splits + 1 : 1;
+  if (paged_attn_fp8_t5_ok(head_dim, block_size) && blocks > 0) {
+    per = (per + 127) / 128 * 128;             // whole tiles
+    const int rc = launch_paged_attn_fp8_t5(q, q_stride, k_cache, v_cache, k_scale, v_scale, block_tables, max_blocks, context_lens, out, scratch, batch,
+                                            heads, kv_heads, head_dim, blocks, block_size, limit, per, num_splits, scale, s);
+    if (rc) LLMCTL_FAIL(rc, "decode over 8 bits");
+  } else {
+    auto launch = [&](auto kern) {
+      return launch_dependent(kern, dim3(heads, num_splits, batch), 128, 0, s, (const __nv_bfloat16*)q, q_stride, (const uint8_t*)k_cache,
+                              (const uint8_t*)v_cache, k_scale, v_scale, block_tables, max_blocks, context_lens, scratch, (__nv_bfloat16*)out, blocks,
+                              block_size, heads / kv_heads, limit, per, scale * decode8::kLog2e);
+    };
+    LLMCTL_CHECK(head_dim == 128 ? launch(paged_attn_decode_fp8_kernel<128>) : launch(paged_attn_decode_fp8_kernel<64>));
+  }
   if (num_splits > 1) {
     if (head_dim == 128)
       LLMCTL_CHECK(launch_dependent(paged_attn_merge_fp8_kernel<128>, dim3(heads, batch), 128, 0, s, scratch, (__nv_bfloat16*)out, num_splits));

@@ -47,7 +47,7 @@ struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
   LLMCTL_ENTRIES(X)
 #undef X
-  const volatile uint32_t* waits = nullptr;      // != 0: a bounded wait of a kernel ran out (csrc/common/wait_status.h)
+  const volatile uint64_t* waits = nullptr;      // != 0: a bounded wait of a kernel ran out (csrc/common/wait_status.h)
   void* (*wait_word)() = nullptr;
 } lib;                                           // entries that a partial build leaves out stay null
 
@@ -62,7 +62,7 @@ bool ready(F* f) {
   if (f == nullptr) return false;
   if (lib.waits == nullptr) {
     if (lib.wait_word == nullptr) return false;
-    lib.waits = static_cast<const volatile uint32_t*>(lib.wait_word());
+    lib.waits = static_cast<const volatile uint64_t*>(lib.wait_word());
   }
   return lib.waits != nullptr && *lib.waits == 0;
 }

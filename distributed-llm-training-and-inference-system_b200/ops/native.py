@@ -253,7 +253,8 @@ class NativeError(RuntimeError):
 # the entry points that read and clear their device-side status.
 _WAITS = (("flash attention forward", "llmctl_flash_fwd_status"), ("flash attention backward", "llmctl_flash_bwd_status"),
           ("cross-entropy", "llmctl_cross_entropy_status"), ("latent attention", "llmctl_latent_attention_t5_status"))
-_wait_word = ctypes.c_uint32(0)         # the library's word once a kernel has been launched
+_OTHER_WAITS = ("paged decode attention over 8 bits",)      # behind those: kernels that keep no status on the device
+_wait_word = ctypes.c_uint64(0)         # the library's word once a kernel has been launched
 _wait_bound = False
 
 
@@ -262,7 +263,7 @@ def _bind_waits() -> None:
     register_signature("llmctl_wait_status_word", [], restype=c_void_p)
     address = _function("llmctl_wait_status_word")()
     if address:
-        _wait_word = ctypes.c_uint32.from_address(address)
+        _wait_word = ctypes.c_uint64.from_address(address)
     _wait_bound = True
 
 
@@ -272,7 +273,7 @@ def check_waits(context: str = "") -> None:
     value = _wait_word.value
     if value:
         _wait_word.value = 0
-        names = [name for i, (name, _) in enumerate(_WAITS) if value >> 8 * i & 0xff]
+        names = [name for i, name in enumerate([*(name for name, _ in _WAITS), *_OTHER_WAITS]) if value >> 8 * i & 0xff]
         for _, status in _WAITS:
             if has_symbol(status):
                 _function(status)(1)

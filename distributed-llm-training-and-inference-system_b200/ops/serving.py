@@ -254,6 +254,13 @@ def _aligned_rows(x: torch.Tensor, width: int) -> torch.Tensor:
     return x[:, :width].clone(memory_format=torch.contiguous_format)
 
 
+def _fp8_splits(batch: int, heads: int, kv_heads: int, max_context: int, block_size: int, sms: int = 148) -> int:
+    if block_size % 8:
+        return choose_splits(batch, heads, max_context, block_size, sms)
+    pairs = batch * kv_heads * -(-heads // kv_heads // 16)
+    return max(1, min(-(-4 * sms // pairs), max_context // 256, 64))
+
+
 def paged_attention_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                                block_tables: torch.Tensor, context_lens: torch.Tensor, max_context: int, scale: Optional[float] = None,
                                num_splits: Optional[int] = None) -> torch.Tensor:
@@ -275,7 +282,7 @@ def paged_attention_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         out = torch.empty(B, H, D, dtype=q.dtype, device=q.device)
         if B == 0:
             return out
-        ns = num_splits or choose_splits(B, H, max_context, block_size)
+        ns = num_splits or _fp8_splits(B, H, kv_heads, max_context, block_size)
         block_tables, context_lens = block_tables.contiguous(), context_lens.contiguous()
         if q.stride(2) != 1 or q.stride(1) != D or q.data_ptr() % 16 or q.stride(0) % 8:
             q = q.clone(memory_format=torch.contiguous_format)
