@@ -393,6 +393,9 @@ __device__ __forceinline__ void umma_commit_mc2(uint64_t* bar, uint16_t mask) {
 
 // TMEM -> registers: 32 lanes x 32-bit, N consecutive columns per thread (thread i of the warp
 // reads lane (warp%4)*32+i).  taddr = (lane << 16) | column.
+__device__ __forceinline__ void tmem_ld_x4(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_ld_x8(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"

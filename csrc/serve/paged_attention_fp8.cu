@@ -16,10 +16,12 @@
 
 namespace llmctl {
 
+// paged_attention_fp8_t5.cu
 bool paged_attn_fp8_t5_ok(int head_dim, int block_size);
+long long paged_attn_fp8_t5_scratch(int batch, int heads, int kv_heads, int head_dim, int limit, int runs);
 int launch_paged_attn_fp8_t5(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
                              const int* block_tables, int max_blocks, const int* context_lens, void* out, float* partial, int batch, int heads, int kv_heads,
-                             int head_dim, int blocks, int block_size, int limit, int tokens_per_split, int splits, float scale, cudaStream_t s);
+                             int head_dim, int blocks, int block_size, int limit, int runs, float scale, cudaStream_t s);
 
 namespace decode8 {
 constexpr float kLog2e = 1.4426950408889634f;
@@ -138,45 +140,61 @@ paged_attn_merge_fp8_kernel(const float* __restrict__ partial, __nv_bfloat16* __
 
 using namespace llmctl;
 
+static int decode8_limit(int max_blocks, int block_size, int max_context) {
+  const long long room = static_cast<long long>(max_blocks) * block_size;
+  return max_context < room ? max_context : static_cast<int>(room);
+}
+// Splits of a context where a block is not of whole boxes: some 8 CTAs to an SM, of 64 tokens and more.
+static int decode8_splits(int batch, int heads, int limit, int splits) {
+  if (splits > 0) return splits;
+  const long long want = (8LL * kNumSMs + static_cast<long long>(batch) * heads - 1) / (static_cast<long long>(batch) * heads);
+  const int most = limit / 64 < 256 ? limit / 64 : 256;
+  return want < most ? static_cast<int>(want) : most > 1 ? most : 1;
+}
+
 // Number of fp32 scratch elements llmctl_paged_attn_decode_fp8 needs for a given launch.
-LLMCTL_API long long llmctl_paged_attn_fp8_scratch_elems(int batch, int heads, int head_dim, int num_splits) {
-  return num_splits == 1 ? 0 : static_cast<long long>(batch) * heads * num_splits * (head_dim + 2);
+LLMCTL_API long long llmctl_paged_attn_fp8_scratch_elems(int batch, int heads, int kv_heads, int head_dim, int max_blocks, int block_size, int max_context,
+                                                         int num_splits) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || block_size <= 0) return 0;
+  const int limit = decode8_limit(max_blocks, block_size, max_context);
+  if (paged_attn_fp8_t5_ok(head_dim, block_size)) return paged_attn_fp8_t5_scratch(batch, heads, kv_heads, head_dim, limit, num_splits);
+  const int splits = decode8_splits(batch, heads, limit, num_splits);
+  return splits == 1 ? 0 : static_cast<long long>(batch) * heads * splits * (head_dim + 2);
 }
 
 // q: bf16 [batch, heads, head_dim], rows q_stride apart; caches [blocks, kv_heads, block_size, head_dim] e4m3, scales fp32 [blocks, kv_heads]; out: bf16
-// [batch, heads, head_dim].  scratch: fp32 [llmctl_paged_attn_fp8_scratch_elems(...)] (may be null when that is 0).  num_splits >= 1.
+// [batch, heads, head_dim].  scratch: fp32 [llmctl_paged_attn_fp8_scratch_elems(...)] (may be null when that is 0).  num_splits: parts of a context, or (blocks
+// of whole boxes) of the batch; 0: as many as fill the chip; 1: none is merged.
 LLMCTL_API int llmctl_paged_attn_decode_fp8(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const float* k_scale,
                                             const float* v_scale, const int* block_tables, int max_blocks, const int* context_lens, void* out,
                                             float* scratch, int batch, int heads, int kv_heads, int head_dim, int blocks, int block_size,
                                             int max_context, int num_splits, float scale, void* stream) {
   LLMCTL_BEGIN();
   LLMCTL_REQUIRE((head_dim == 128 || head_dim == 64) && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && batch >= 0 && batch < 65536);
-  LLMCTL_REQUIRE(num_splits >= 1 && num_splits < 65536 && block_size >= 1 && blocks >= 0 && max_blocks >= 0 && max_context >= 0);
-  LLMCTL_REQUIRE(num_splits == 1 || scratch != nullptr);
+  LLMCTL_REQUIRE(num_splits >= 0 && num_splits < 65536 && block_size >= 1 && blocks >= 0 && max_blocks >= 0 && max_context >= 0);
   if (batch == 0) return 0;
   LLMCTL_REQUIRE(aligned16(k_cache, v_cache));
   cudaStream_t s = (cudaStream_t)stream;
-  const long long room = static_cast<long long>(max_blocks) * block_size;
-  const int limit = max_context < room ? max_context : static_cast<int>(room);
-  int per = limit > 0 ? (limit - 1) / num_splits + 1 : 1;
+  const int limit = decode8_limit(max_blocks, block_size, max_context);
   if (paged_attn_fp8_t5_ok(head_dim, block_size) && blocks > 0) {
-    per = (per + 127) / 128 * 128;             // whole tiles
     const int rc = launch_paged_attn_fp8_t5(q, q_stride, k_cache, v_cache, k_scale, v_scale, block_tables, max_blocks, context_lens, out, scratch, batch,
-                                            heads, kv_heads, head_dim, blocks, block_size, limit, per, num_splits, scale, s);
+                                            heads, kv_heads, head_dim, blocks, block_size, limit, num_splits, scale, s);
     if (rc) LLMCTL_FAIL(rc, "decode over 8 bits");
-  } else {
-    auto launch = [&](auto kern) {
-      return launch_dependent(kern, dim3(heads, num_splits, batch), 128, 0, s, (const __nv_bfloat16*)q, q_stride, (const uint8_t*)k_cache,
-                              (const uint8_t*)v_cache, k_scale, v_scale, block_tables, max_blocks, context_lens, scratch, (__nv_bfloat16*)out, blocks,
-                              block_size, heads / kv_heads, limit, per, scale * decode8::kLog2e);
-    };
-    LLMCTL_CHECK(head_dim == 128 ? launch(paged_attn_decode_fp8_kernel<128>) : launch(paged_attn_decode_fp8_kernel<64>));
+    LLMCTL_RETURN_LAST();
   }
-  if (num_splits > 1) {
+  const int splits = decode8_splits(batch, heads, limit, num_splits), per = limit > 0 ? (limit - 1) / splits + 1 : 1;
+  LLMCTL_REQUIRE(splits == 1 || scratch != nullptr);
+  auto launch = [&](auto kern) {
+    return launch_dependent(kern, dim3(heads, splits, batch), 128, 0, s, (const __nv_bfloat16*)q, q_stride, (const uint8_t*)k_cache, (const uint8_t*)v_cache,
+                            k_scale, v_scale, block_tables, max_blocks, context_lens, scratch, (__nv_bfloat16*)out, blocks, block_size, heads / kv_heads,
+                            limit, per, scale * decode8::kLog2e);
+  };
+  LLMCTL_CHECK(head_dim == 128 ? launch(paged_attn_decode_fp8_kernel<128>) : launch(paged_attn_decode_fp8_kernel<64>));
+  if (splits > 1) {
     if (head_dim == 128)
-      LLMCTL_CHECK(launch_dependent(paged_attn_merge_fp8_kernel<128>, dim3(heads, batch), 128, 0, s, scratch, (__nv_bfloat16*)out, num_splits));
+      LLMCTL_CHECK(launch_dependent(paged_attn_merge_fp8_kernel<128>, dim3(heads, batch), 128, 0, s, scratch, (__nv_bfloat16*)out, splits));
     else
-      LLMCTL_CHECK(launch_dependent(paged_attn_merge_fp8_kernel<64>, dim3(heads, batch), 64, 0, s, scratch, (__nv_bfloat16*)out, num_splits));
+      LLMCTL_CHECK(launch_dependent(paged_attn_merge_fp8_kernel<64>, dim3(heads, batch), 64, 0, s, scratch, (__nv_bfloat16*)out, splits));
   }
   LLMCTL_RETURN_LAST();
 }

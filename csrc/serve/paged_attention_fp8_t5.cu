@@ -13,9 +13,13 @@
 //     O = 2^(M - m) sum_j w_j cv_j / l,    w_j = 2^(s_j + log2 sv_j - M),    l = sum_j 2^(s_j - m)
 // O of a tile is read from tensor memory and added up in registers, where the reference of the tiles before is caught up with.
 //
-//   warp 0      TMA producer: 128 tokens of keys and of values, a box for each block that they stand in, a ring of stages
-//   warp 1      MMA issuer
+//   warp 0      TMA producer: 128 tokens of keys and of values, a box for each block that they stand in, a ring of stages; their scales beside them
+//   warps 1, 6  MMA issuers, of scores and of values
 //   warps 2-5   the columns of Q, then a token per thread: S^T -> P^T; a dimension per thread: O^T
+//
+// The work is one row of tiles: those of every sequence and head behind one another.  As many CTAs as fit on the chip take equal runs of it, so that
+// batches of unlike contexts end together; a sequence and head that more than one CTA has a part of is merged by a second kernel.
+// Where contexts are of a few tiles only the runs are cut between heads, and nothing is merged.
 //
 // Every wait is bounded, as in latent_attention_t5.cu.
 // Reference: none.
@@ -32,10 +36,12 @@ using namespace ptx;
 
 namespace dec8 {
 constexpr int kTile = 128;                   // tokens
-constexpr int kThreads = 192;
-constexpr int kPieces = 4, kMaxStages = 8;
+constexpr int kThreads = 224;
+constexpr int kPieces = 4, kMaxStages = 8, kMaxBoxes = 16;
+constexpr int kWholeTokens = 512, kLeast = 2;
 constexpr float kStep = 16.f;                // between the columns of a number
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int columns(int GP) { return GP < 4 ? 16 : kPieces * GP; }     // of a product: 16 at least, of which those past 4 GP are nobody's
 constexpr int stage_bytes(int D) { return 2 * kTile * D; }
 constexpr int fixed_smem(int D, int N) { return N * D + 2 * kTile * N + 1024; }       // Q, two of P, alignment
 
@@ -57,33 +63,151 @@ __device__ __forceinline__ float joined(const uint32_t* c, int g) {
   x = fmaf(x, 1.f / kStep, __uint_as_float(c[GP + g]));
   return fmaf(x, 1.f / kStep, __uint_as_float(c[g]));
 }
-template <int N>
+template <int C>
 __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t* r) {
-  if constexpr (N == 16) tmem_ld_x16(at, r);
-  else if constexpr (N == 32) tmem_ld_x32(at, r);
+  if constexpr (C == 4) tmem_ld_x4(at, r);
+  else if constexpr (C == 8) tmem_ld_x8(at, r);
+  else if constexpr (C == 16) tmem_ld_x16(at, r);
+  else if constexpr (C == 32) tmem_ld_x32(at, r);
   else {
     tmem_ld_x32(at, r);
     tmem_ld_x32(at + 32, r + 32);
   }
 }
+
+// Place in the ring of stages.  (A quotient and a remainder by a number known at launch are 200 clocks in the issuing warp's way, three of them in
+// each turn of its loop: 2600 clocks a tile, 16 contexts up to 4096, 32 heads 66.1 us instead of XX.)
+struct Place {
+  int st = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++st == stages) {
+      st = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// The row of tiles.  Item: a sequence and up to 16 query heads of one head of the cache, b * per_sequence + x.
+struct Work {
+  const int* context_lens;
+  int batch, per_sequence, limit, least;                 // least: tiles of the shortest run
+  int whole, items, items_rest;                          // != 0: runs are of `items` items, the first `items_rest` of one more
+  FastDiv by_sequence;
+  __device__ __forceinline__ int tokens(int b) const { return b < batch ? max(min(context_lens[b], limit), 0) : 0; }
+  __device__ __forceinline__ int tiles(int b) const { return (tokens(b) + kTile - 1) / kTile; }
+};
+struct Run {
+  int b, x, t, left;                                     // first tile, tiles left
+  int last_b;                                            // of the last item (runs of whole items)
+};
+// Tiles of all sequences before `b` and, in `all`, of the whole batch, for one head; by one warp.
+__device__ __forceinline__ int tiles_before(const Work& w, int b, int& all) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  all = 0;
+  for (int i = lane; i < w.batch; i += 32) {
+    const int n = w.tiles(i);
+    all += n;
+    if (i < b) before += n;
+  }
+  all = __reduce_add_sync(0xffffffffu, all);
+  return __reduce_add_sync(0xffffffffu, before);
+}
+__device__ __forceinline__ int run_length(const Work& w, int all, int ctas) { return max((all * w.per_sequence + ctas - 1) / ctas, w.least); }
+
+// The run of a CTA, by one warp.
+__device__ __forceinline__ Run run_of(const Work& w, int cta, int ctas) {
+  const int lane = threadIdx.x & 31;
+  Run r = {0, 0, 0, 0, 0};
+  uint32_t x;
+  if (w.whole) {
+    const int first = cta * w.items + min(cta, w.items_rest), last = first + w.items + (cta < w.items_rest ? 1 : 0);
+    r.last_b = static_cast<int>(w.by_sequence.divide(last - 1, x));
+    r.b = static_cast<int>(w.by_sequence.divide(first, x));
+    r.x = static_cast<int>(x);
+    int n = 0;
+    for (int i = first + lane; i < last; i += 32) n += w.tiles(static_cast<int>(w.by_sequence.divide(i, x)));
+    r.left = __reduce_add_sync(0xffffffffu, n);
+    return r;
+  }
+  int all;
+  tiles_before(w, 0, all);
+  const int length = run_length(w, all, ctas);
+  const long long start = static_cast<long long>(length) * cta;
+  const int total = all * w.per_sequence;
+  if (start >= total) return r;
+  const int first = static_cast<int>(start);
+  r.left = min(total - first, length);
+  int before = 0;                                        // tiles of the items in front of the chunk of 32 sequences
+  for (int b0 = 0; b0 < w.batch; b0 += 32) {
+    const int n = w.tiles(b0 + lane);
+    int end = n;                                         // of the sequences up to this lane's
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += other;
+    }
+    const int upto = before + end * w.per_sequence;
+    const unsigned here = __ballot_sync(0xffffffffu, upto > first);
+    if (here != 0u) {
+      const int at = __ffs(here) - 1, nb = __shfl_sync(0xffffffffu, n, at), in = first - __shfl_sync(0xffffffffu, upto, at) + nb * w.per_sequence;
+      r.b = b0 + at;
+      r.x = in / nb;
+      r.t = in - r.x * nb;
+      return r;
+    }
+    before = __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return r;
+}
+// A run item by item: tiles t .. t + n of the nt of (b, x), whose sequence has `tokens`.
+struct Items {
+  Run r;
+  int nt, n, tokens;
+  __device__ __forceinline__ Items(const Run& run, const Work& w) : r(run), nt(0), n(0), tokens(0) {
+    if (r.left > 0) skip(w);
+  }
+  __device__ __forceinline__ void skip(const Work& w) {          // sequences without tokens
+    while ((tokens = w.tokens(r.b)) == 0) ++r.b, r.x = 0;
+    nt = (tokens + kTile - 1) / kTile;
+    n = min(nt - r.t, r.left);
+  }
+  __device__ __forceinline__ bool more() const { return r.left > 0; }
+  __device__ __forceinline__ void next(const Work& w) {
+    r.left -= n;
+    r.t = 0;
+    n = 0;
+    if (r.left == 0) return;
+    if (++r.x == w.per_sequence) {
+      r.x = 0;
+      ++r.b;
+      skip(w);
+    } else {
+      n = min(nt, r.left);
+    }
+  }
+};
 }  // namespace dec8
 
-// Grid: (heads of the cache x groups of N / 4 query heads, splits, batch).  partial: as in paged_attention_fp8.cu.
-template <int D, int N>
-__global__ void __launch_bounds__(dec8::kThreads)
+// Grid: as many CTAs as there are runs.  GP: query heads of an item.  partial: two rows of items [2 ctas, GP, D + 2] = {sum of w cv at the reference m, m (log2), sum of p}: of the
+// item that the run begins inside of, and of the one that it ends inside of.
+template <int D, int GP>
+__global__ void __launch_bounds__(dec8::kThreads, GP == 16 ? 1 : 2)
 paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __nv_bfloat16* __restrict__ q,
                                 long long q_stride, const float* __restrict__ k_scale, const float* __restrict__ v_scale,
-                                const int* __restrict__ block_tables, int max_blocks, const int* __restrict__ context_lens, float* __restrict__ partial,
+                                const int* __restrict__ block_tables, int max_blocks, dec8::Work work, float* __restrict__ partial,
                                 __nv_bfloat16* __restrict__ out, int blocks, int block_size, FastDiv by_block, int box_rows, int kv_heads, int group,
-                                int limit, int tokens_per_split, int stages, float scale_log2, unsigned char* wait_byte) {
+                                int stages, float scale_log2, unsigned char* wait_byte) {
   using namespace dec8;
-  constexpr int GP = N / kPieces, kStage = stage_bytes(D), kHalf = kTile * D;
+  constexpr int C = kPieces * GP, N = columns(GP), kStage = stage_bytes(D), kHalf = kTile * D;
   constexpr uint32_t kSwizzle = D == 128 ? 2 : 4, kEight = 8 * D;          // layout of the tiles, bytes of eight rows
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bar_q, bar_full[kMaxStages], bar_empty[kMaxStages], bar_s[2], bar_p[2], bar_o[2];
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
   __shared__ float top[2][4][2 * GP];                                      // per softmax warp: the tile's largest s and s + log2 sv
+  __shared__ float2 box_scale[kMaxStages][kMaxBoxes];                      // of a stage's boxes: sk, log2 sv
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -111,49 +235,68 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_smem, tO = tmem_base + 2 * N;
-  wait_for_previous(q, k_scale, v_scale, block_tables, context_lens, partial, out);
+  wait_for_previous(q, k_scale, v_scale, block_tables, work.context_lens, partial, out);
   release_dependents();
   volatile int* abort = &abort_flag;
-
-  const int b = blockIdx.z, split = blockIdx.y, nsplit = gridDim.y;
-  const int kv_head = blockIdx.x % kv_heads, g0 = blockIdx.x / kv_heads * GP, ng = min(GP, group - g0), heads = kv_heads * group;
-  const int head0 = kv_head * group + g0;
-  const int ctx = min(context_lens[b], limit);
-  const int t0 = split * tokens_per_split, t1 = min(ctx, t0 + tokens_per_split);
-  const int nt = t1 > t0 ? (t1 - t0 + kTile - 1) / kTile : 0;
-  const int* bt = block_tables + static_cast<long long>(b) * max_blocks;
-  auto block_of = [&](int token, int& row) {
-    uint32_t r;
-    const uint32_t i = by_block.divide(static_cast<uint32_t>(token), r);
-    row = static_cast<int>(r);
-    return bt[i];
-  };
+  const int heads = kv_heads * group;
+  const Run run = run_of(work, blockIdx.x, gridDim.x);                     // every warp finds it for itself
 
   if (warp == 0) {
     // ------------------------------------ TMA producer: a lane per box ------------------------------------
     const int boxes = kTile / box_rows, all_rows = blocks * kv_heads * block_size;
-    auto row_of = [&](int n) {                            // cache row of the lane's box, -1: none.  A block outside of the cache is filled with zeros
-      const int token = t0 + n * kTile + lane * box_rows;
-      if (lane >= boxes || n >= nt || token >= t1) return -1;
-      int row;
-      const int block = block_of(token, row);
-      return block >= 0 && block < blocks ? (block * kv_heads + kv_head) * block_size + row : all_rows;
+    // Three tiles are under way: the block of the one after next is asked for, the scales of the next, and this one is copied: the producer waits for
+    // no load that it has just asked for.  A block outside of the cache is filled with zeros, its scales are no numbers.
+    struct Box {
+      int block, row, head;                               // row: of the block; < 0: no box
     };
-    int row = row_of(0), loaded = 0;
-    for (int n = 0; n < nt; ++n) {
-      const int st = n % stages, next = row_of(n + 1);
-      const bool given = n < stages || mbar_wait_bounded(&bar_empty[st], ((n / stages) & 1u) ^ 1u, abort);
+    auto find = [&](const Items& it, int tile) {
+      const int token = (it.r.t + tile) * kTile + lane * box_rows;
+      Box box = {0, -1, 0};
+      if (!it.more() || lane >= boxes || token >= it.tokens) return box;
+      uint32_t row;
+      box.block = block_tables[static_cast<long long>(it.r.b) * max_blocks + by_block.divide(static_cast<uint32_t>(token), row)];
+      box.row = static_cast<int>(row);
+      box.head = it.r.x < kv_heads ? it.r.x : it.r.x % kv_heads;
+      return box;
+    };
+    auto scale_of = [&](const float* s, const Box& box) {
+      return box.row < 0 ? 0.f : box.block >= 0 && box.block < blocks ? s[static_cast<long long>(box.block) * kv_heads + box.head] : NAN;
+    };
+    Items it(run, work);
+    int tile = 0, loaded = 0;                             // within the item's part; so far
+    auto advance = [&] {
+      if (it.more() && ++tile == it.n) {
+        it.next(work);
+        tile = 0;
+      }
+    };
+    Box box = find(it, 0);
+    advance();
+    Box next = find(it, tile);
+    float sk = scale_of(k_scale, box), sv = scale_of(v_scale, box);
+    Place at;
+    for (; loaded < run.left; ++loaded, at.next(stages)) {
+      const int st = at.st;
+      advance();
+      const Box after = find(it, tile);
+      const float next_sk = scale_of(k_scale, next), next_sv = scale_of(v_scale, next);
+      const bool given = loaded < stages || mbar_wait_bounded(&bar_empty[st], at.phase ^ 1u, abort);
       if (!__all_sync(0xffffffffu, given)) break;
-      const int count = __popc(__ballot_sync(0xffffffffu, row >= 0));
+      if (lane < kMaxBoxes) box_scale[st][lane] = make_float2(sk, __log2f(sv));
+      const int count = __popc(__ballot_sync(0xffffffffu, box.row >= 0));
+      __syncwarp();                                       // the scales are there for whom the barrier lets through
       if (lane == 0) mbar_expect_tx(&bar_full[st], count * box_rows * D * 2);
-      ++loaded;
       __syncwarp();
-      if (row >= 0) {
+      if (box.row >= 0) {
+        const int row = box.block >= 0 && box.block < blocks ? (box.block * kv_heads + box.head) * block_size + box.row : all_rows;
         uint8_t* dst = smem + st * kStage + lane * box_rows * D;
         tma_load_2d(dst, &tmK, &bar_full[st], 0, row);
         tma_load_2d(dst + kHalf, &tmV, &bar_full[st], 0, row);
       }
-      row = next;
+      box = next;
+      next = after;
+      sk = next_sk;
+      sv = next_sv;
     }
     // Copies still in flight when a wait ran out land before the CTA's shared memory is given back.
     if (*abort && lane == 0)
@@ -162,91 +305,76 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
         mbar_wait_bounded(&bar_full[i % stages], (i / stages) & 1u, &none);
       }
   } else if (warp == 1) {
-    // ------------------------------------ MMA issuer: whichever is there first, the next tile or the weights of this one ------------------------------------
-    constexpr uint32_t id_s = make_idesc_e4m3(kTile, N, 0u, 0u);       // A, B K-major
-    constexpr uint32_t id_o = make_idesc_e4m3(D, N, 1u, 1u);           // A, B MN-major
-    if (nt > 0) mbar_wait_or_abort(&bar_q, 0u, abort);
-    const long long since = clock64();
-    for (int ns = 0, np = 0; np < nt;) {
-      const int st = ns % stages, sp = np % stages;
-      const bool tile = ns < nt && ns <= np + 1 && __any_sync(0xffffffffu, mbar_test(&bar_full[st], (ns / stages) & 1u));
-      const bool weights = !tile && np < ns && __any_sync(0xffffffffu, mbar_test(&bar_p[np & 1], (np >> 1) & 1u));
-      if (tile) {
-        mbar_wait_or_abort(&bar_full[st], (ns / stages) & 1u, abort);
+    // ------------------------------------ scores ------------------------------------
+    constexpr uint32_t id = make_idesc_e4m3(kTile, N, 0u, 0u);          // A, B K-major
+    const uint64_t a0 = make_smem_desc(smem_base, 16, kEight, kSwizzle), b0 = make_smem_desc(smem_base + q_at, 16, kEight, kSwizzle);
+    Place at;
+    int n = 0, item = 0;
+    for (Items it(run, work); it.more(); it.next(work), ++item) {
+      mbar_wait_or_abort(&bar_q, item & 1u, abort);
+      for (int i = 0; i < it.n; ++i, ++n, at.next(stages)) {
+        if (n >= 2) mbar_wait_or_abort(&bar_p[n & 1], ((n >> 1) & 1u) ^ 1u, abort);       // the scores before last have been read
+        mbar_wait_or_abort(&bar_full[at.st], at.phase, abort);
         __syncwarp();
         tc_fence_after();
-        const uint64_t a = make_smem_desc(smem_base + st * kStage, 16, kEight, kSwizzle), bq = make_smem_desc(smem_base + q_at, 16, kEight, kSwizzle);
         if (elect_one()) {
+          const uint64_t a = a0 + (at.st * kStage >> 4);
 #pragma unroll
-          for (int k = 0; k < D / 32; ++k) umma_f8_ss(tmem_base + (ns & 1) * N, a + (k * 32 >> 4), bq + (k * 32 >> 4), id_s, k != 0 ? 1u : 0u);
-          umma_commit<1>(&bar_s[ns & 1]);
+          for (int k = 0; k < D / 32; ++k) umma_f8_ss(tmem_base + (n & 1) * N, a + (k * 32 >> 4), b0 + (k * 32 >> 4), id, k != 0 ? 1u : 0u);
+          umma_commit<1>(&bar_s[n & 1]);
         }
-        ++ns;
-      } else if (weights) {
-        mbar_wait_or_abort(&bar_p[np & 1], (np >> 1) & 1u, abort);
-        __syncwarp();
-        tc_fence_after();
-        const uint64_t a = make_smem_desc(smem_base + sp * kStage + kHalf, 16, kEight, kSwizzle);
-        const uint64_t bp = make_smem_desc(smem_base + p_at + (np & 1) * kTile * N, 128, kTile * 16, 0);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kTile / 32; ++k) umma_f8_ss(tO + (np & 1) * N, a + (k * 32 * D >> 4), bp + (k * 512 >> 4), id_o, k != 0 ? 1u : 0u);
-          umma_commit<1>(&bar_empty[sp]);
-          umma_commit<1>(&bar_o[np & 1]);
-        }
-        ++np;
-      } else {
-        const bool late = clock64() - since > kBoundedWaitCycles;
-        if (late) *abort = 1;
-        if (__any_sync(0xffffffffu, late || *abort)) break;
       }
+      if (__any_sync(0xffffffffu, *abort)) break;
+    }
+  } else if (warp == 6) {
+    // ------------------------------------ values, by a warp of their own: each issuer then waits for one thing after the other and never polls ------------------------------------
+    constexpr uint32_t id = make_idesc_e4m3(D, N, 1u, 1u);              // A, B MN-major
+    const uint64_t a0 = make_smem_desc(smem_base + kHalf, 16, kEight, kSwizzle), b0 = make_smem_desc(smem_base + p_at, 128, kTile * 16, 0);
+    Place at;
+    for (int n = 0; n < run.left; ++n, at.next(stages)) {
+      mbar_wait_or_abort(&bar_p[n & 1], (n >> 1) & 1u, abort);
+      __syncwarp();
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t a = a0 + (at.st * kStage >> 4), b = b0 + ((n & 1) * kTile * N >> 4);
+#pragma unroll
+        for (int k = 0; k < kTile / 32; ++k) umma_f8_ss(tO + (n & 1) * N, a + (k * 32 * D >> 4), b + (k * 512 >> 4), id, k != 0 ? 1u : 0u);
+        umma_commit<1>(&bar_empty[at.st]);
+        umma_commit<1>(&bar_o[n & 1]);
+      }
+      if (__any_sync(0xffffffffu, *abort)) break;
     }
   } else {
     // ------------------------------------ softmax warps ------------------------------------
-    const int w = warp - 2, quad = warp & 3, t = quad * 32 + lane;
+    const int w = warp - 2, quad = warp & 3, t = quad * 32 + lane, box = t / box_rows;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
     const int dim = D == 128 ? t : quad * 16 + lane;      // of O^T: 64 rows stand in 16 lanes of each quadrant
     const bool has_dim = D == 128 || lane < 16;
-    const long long row0 = static_cast<long long>(b) * heads + head0;
 
-    // scales of this thread's token, two tiles ahead in the block table
-    auto block_at = [&](int n) {
-      const int token = t0 + n * kTile + t;
-      int row;
-      return n < nt && token < t1 ? block_of(token, row) : 0;
-    };
-    auto scale_at = [&](const float* s, int block) { return block >= 0 && block < blocks ? s[static_cast<long long>(block) * kv_heads + kv_head] : NAN; };
-    int block1 = block_at(1);
-    float sk = 0.f, sv = 0.f;
-    if (nt > 0) {
-      const int block0 = block_at(0);
-      sk = scale_at(k_scale, block0);
-      sv = scale_at(v_scale, block0);
-    }
-
-    // Q: a row's largest number comes to stand in 128 .. 255, its four columns K-major, swizzled as TMA swizzles the tiles
-    float factor[GP];
-    {
-      float x[GP];
+    // A row of Q whose largest number comes to stand in 128 .. 255, as four columns K-major, swizzled as TMA swizzles the tiles
+    auto load_q = [&](const Items& it, float (&x)[GP]) {
+      const int g0 = it.r.x / kv_heads * GP;
+      const __nv_bfloat16* src = q + it.r.b * q_stride + static_cast<long long>(it.r.x % kv_heads * group + g0) * D + t;
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
-        x[g] = nt > 0 && t < D && g < ng ? __bfloat162float(q[b * q_stride + static_cast<long long>(head0 + g) * D + t]) : 0.f;
+        x[g] = it.more() && t < D && g < group - g0 ? __bfloat162float(src[g * D]) : 0.f;
         if (!isfinite(x[g])) x[g] = NAN;                  // an infinity has no columns, and no scores that are numbers
       }
+    };
+    auto write_q = [&](float (&x)[GP], float (&factor)[GP], int buf) {
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
         const float m = warp_max_all(fabsf(x[g]));
-        if (lane == 0) top[0][w][g] = m;
+        if (lane == 0) top[buf][w][g] = m;
       }
       named_bar_sync(1, 128);
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
-        const float m = fmaxf(fmaxf(top[0][0][g], top[0][1][g]), fmaxf(top[0][2][g], top[0][3][g]));
-        const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23), 16), 254);           // biased; what is smaller than 2^-111 is 0 here
-        x[g] *= __uint_as_float(static_cast<uint32_t>(max(261 - e, 1)) << 23);                  // 2^(7 - (e - 127))
+        const float m = fmaxf(fmaxf(top[buf][0][g], top[buf][1][g]), fmaxf(top[buf][2][g], top[buf][3][g]));
+        const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23), 16), 254);           // biased
+        x[g] *= __uint_as_float(static_cast<uint32_t>(261 - e) << 23);                          // 2^(7 - (e - 127))
         factor[g] = __uint_as_float(static_cast<uint32_t>(e - 7) << 23) * scale_log2;
       }
-      named_bar_sync(1, 128);                             // top[0] is written again by the first tile
       uint8_t* qs = smem + q_at;
       if (t < D) {
         auto at = [&](int n) {                            // byte t of row n
@@ -255,127 +383,147 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
 #pragma unroll
         for (int g = 0; g < GP; g += 2) {
           uint32_t codes[kPieces];
-          split2(x[g], x[g + 1], codes);
+          split2(x[g], GP > 1 ? x[g + 1] : 0.f, codes);
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) {
             qs[at(i * GP + g)] = static_cast<uint8_t>(codes[i]);
-            qs[at(i * GP + g + 1)] = static_cast<uint8_t>(codes[i] >> 8);
+            if (GP > 1) qs[at(i * GP + g + 1)] = static_cast<uint8_t>(codes[i] >> 8);
           }
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar_q);
-    }
+    };
 
-    float m[GP], M[GP], l[GP], acc[GP], catch_up[GP];     // catch_up: from the reference of the tile before last to that of the last
-#pragma unroll
-    for (int g = 0; g < GP; ++g) {
-      m[g] = M[g] = -INFINITY;
-      l[g] = acc[g] = 0.f;
-    }
+    float m[GP], M[GP], l[GP], acc[GP], catch_up[GP], factor[GP];     // catch_up: from the reference of the tile before last to that of the last
     auto add_tile = [&](int n) {
       mbar_wait_or_abort(&bar_o[n & 1], (n >> 1) & 1u, abort);
       __syncwarp();
       tc_fence_after();
-      uint32_t o[N];
-      tmem_ld<N>(tO + (n & 1) * N + lane_off, o);
+      uint32_t o[C];
+      tmem_ld<C>(tO + (n & 1) * N + lane_off, o);
       tmem_ld_wait();
 #pragma unroll
       for (int g = 0; g < GP; ++g) acc[g] = fmaf(acc[g], catch_up[g], joined<GP>(o, g));
     };
-    for (int n = 0; n < nt; ++n) {
-      const int block2 = block_at(n + 2);
-      const float next_sk = n + 1 < nt ? scale_at(k_scale, block1) : 0.f, next_sv = n + 1 < nt ? scale_at(v_scale, block1) : 0.f;
-      const int j = t0 + n * kTile + t;
-      const bool seen = j < t1;
-      const float lv = seen ? __log2f(sv) : 0.f;
-      mbar_wait_or_abort(&bar_s[n & 1], (n >> 1) & 1u, abort);
-      __syncwarp();
-      tc_fence_after();
-      float s[GP];
-      {
-        uint32_t c[N];
-        tmem_ld<N>(tmem_base + (n & 1) * N + lane_off, c);
-        tmem_ld_wait();
-#pragma unroll
-        for (int g = 0; g < GP; ++g) s[g] = seen ? joined<GP>(c, g) * (sk * factor[g]) : -INFINITY;
-      }
+    Items it(run, work);
+    float x[GP];
+    load_q(it, x);
+    if (work.whole)                                       // sequences without tokens are in nobody's run (of runs with parts: paged_attn_merge_fp8_t5_kernel)
+      for (int b = run.b; b <= run.last_b; ++b)
+        if (work.tokens(b) == 0)
+          for (int i = t; i < heads * D; i += 128) out[static_cast<long long>(b) * heads * D + i] = __float2bfloat16(0.f);
+    Place at;
+    int n = 0, part = 0;                                  // tiles so far; use of top: items and tiles so far
+    while (it.more()) {
+      write_q(x, factor, part++ & 1);
+      const int first = n, end = n + it.n, b = it.r.b, g0 = it.r.x / kv_heads * GP, kv_head = it.r.x % kv_heads;
+      const int t0 = it.r.t * kTile, t1 = it.tokens;
+      const bool whole_item = it.n == it.nt, begins_inside = it.r.t > 0;
+      it.next(work);
+      load_q(it, x);                                      // of the next item, while this one's tiles come in
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
-        const float a = warp_max_all(s[g]), c = warp_max_all(s[g] + lv);
-        if (lane == 0) {
-          top[n & 1][w][g] = a;
-          top[n & 1][w][GP + g] = c;
+        m[g] = M[g] = -INFINITY;
+        l[g] = acc[g] = catch_up[g] = 0.f;
+      }
+      for (; n < end; ++n, ++part, at.next(stages)) {
+        const bool seen = t0 + (n - first) * kTile + t < t1;
+        const int st = at.st;
+        float (&most)[4][2 * GP] = top[part & 1];
+        mbar_wait_or_abort(&bar_s[n & 1], (n >> 1) & 1u, abort);
+        mbar_wait_or_abort(&bar_full[st], at.phase, abort);                // it is: the scales, and values that are written below
+        __syncwarp();
+        tc_fence_after();
+        const float2 scale = box_scale[st][box];
+        const float lv = seen ? scale.y : 0.f;
+        float s[GP];
+        {
+          uint32_t c[C];
+          tmem_ld<C>(tmem_base + (n & 1) * N + lane_off, c);
+          tmem_ld_wait();
+#pragma unroll
+          for (int g = 0; g < GP; ++g) s[g] = seen ? joined<GP>(c, g) * (scale.x * factor[g]) : -INFINITY;
         }
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          const float a = warp_max_all(s[g]), c = warp_max_all(s[g] + lv);
+          if (lane == 0) {
+            most[w][g] = a;
+            most[w][GP + g] = c;
+          }
+        }
+        named_bar_sync(1, 128);
+        uint32_t codes[C / 4];                            // this token's row of P: C bytes, piece after piece
+        float from[GP];
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          auto over = [&](int i) { return fmaxf(fmaxf(most[0][i], most[1][i]), fmaxf(most[2][i], most[3][i])); };
+          const float m1 = fmaxf(m[g], over(g)), M1 = fmaxf(M[g], over(GP + g));
+          const float ref = m1 == -INFINITY ? 0.f : m1, Ref = M1 == -INFINITY ? 0.f : M1;
+          l[g] = fmaf(l[g], ex2_approx(m[g] - ref), ex2_approx(s[g] - ref));
+          from[g] = ex2_approx(M[g] - Ref);
+          m[g] = m1;
+          M[g] = M1;
+          s[g] = ex2_approx(s[g] + lv - Ref) * 256.f;
+        }
+#pragma unroll
+        for (int i = 0; i < C / 4; ++i) codes[i] = 0u;
+#pragma unroll
+        for (int g = 0; g < GP; g += 2) {
+          uint32_t two[kPieces];
+          split2(s[g], GP > 1 ? s[g + 1] : 0.f, two);
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) codes[(i * GP + g) / 4] |= two[i] << ((i * GP + g) % 4 * 8);
+        }
+        uint8_t* dst = smem + p_at + (n & 1) * kTile * N + t * 16;
+        if constexpr (C == 4) *reinterpret_cast<uint32_t*>(dst) = codes[0];
+        else if constexpr (C == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(codes[0], codes[1]);
+        else {
+#pragma unroll
+          for (int i = 0; i < C / 16; ++i) *reinterpret_cast<uint4*>(dst + i * kTile * 16) = make_uint4(codes[4 * i], codes[4 * i + 1], codes[4 * i + 2], codes[4 * i + 3]);
+        }
+        // Values past the last token: nothing that the cache holds there may meet a weight of zero.
+        if (!seen) {
+          uint8_t* row = smem + st * kStage + kHalf + t * D;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) *reinterpret_cast<uint4*>(row + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_p[n & 1]);
+        if (n > first) add_tile(n - 1);
+#pragma unroll
+        for (int g = 0; g < GP; ++g) catch_up[g] = from[g];
+      }
+      add_tile(n - 1);
+
+      // ---- sums over the tokens, read-out ----
+      float (&sums)[4][2 * GP] = top[part++ & 1];
+#pragma unroll
+      for (int g = 0; g < GP; ++g) {
+        const float v = warp_sum(l[g]);
+        if (lane == 0) sums[w][g] = v;
       }
       named_bar_sync(1, 128);
-      uint32_t codes[N / 4];                              // this token's row of P: N bytes, piece after piece
-      float from[GP];
+      const long long row0 = static_cast<long long>(b) * heads + kv_head * group + g0;
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
-        auto over = [&](int i) { return fmaxf(fmaxf(top[n & 1][0][i], top[n & 1][1][i]), fmaxf(top[n & 1][2][i], top[n & 1][3][i])); };
-        const float m1 = fmaxf(m[g], over(g)), M1 = fmaxf(M[g], over(GP + g));
-        const float ref = m1 == -INFINITY ? 0.f : m1, Ref = M1 == -INFINITY ? 0.f : M1;
-        l[g] = fmaf(l[g], ex2_approx(m[g] - ref), ex2_approx(s[g] - ref));
-        from[g] = ex2_approx(M[g] - Ref);
-        m[g] = m1;
-        M[g] = M1;
-        s[g] = ex2_approx(s[g] + lv - Ref) * 256.f;
-      }
-#pragma unroll
-      for (int i = 0; i < N / 4; ++i) codes[i] = 0u;
-#pragma unroll
-      for (int g = 0; g < GP; g += 2) {
-        uint32_t two[kPieces];
-        split2(s[g], s[g + 1], two);
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) codes[(i * GP + g) / 4] |= two[i] << ((i * GP + g) % 4 * 8);
-      }
-      uint8_t* dst = smem + p_at + (n & 1) * kTile * N + t * 16;
-#pragma unroll
-      for (int i = 0; i < N / 16; ++i) *reinterpret_cast<uint4*>(dst + i * kTile * 16) = make_uint4(codes[4 * i], codes[4 * i + 1], codes[4 * i + 2], codes[4 * i + 3]);
-      // Values past the last token: nothing that the cache holds there may meet a weight of zero.
-      if (n == nt - 1 && !seen) {
-        mbar_wait_or_abort(&bar_full[n % stages], (n / stages) & 1u, abort);
-        uint8_t* row = smem + (n % stages) * kStage + kHalf + t * D;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) *reinterpret_cast<uint4*>(row + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-      }
-      fence_proxy_async_smem();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar_p[n & 1]);
-      if (n > 0) add_tile(n - 1);
-#pragma unroll
-      for (int g = 0; g < GP; ++g) catch_up[g] = from[g];
-      sk = next_sk;
-      sv = next_sv;
-      block1 = block2;
-    }
-    if (nt > 0) add_tile(nt - 1);
-
-    // ---- sums over the tokens, read-out ----
-#pragma unroll
-    for (int g = 0; g < GP; ++g) {
-      const float x = warp_sum(l[g]);
-      if (lane == 0) top[nt & 1][w][g] = x;
-    }
-    named_bar_sync(1, 128);
-#pragma unroll
-    for (int g = 0; g < GP; ++g) {
-      if (g >= ng || !has_dim) continue;
-      const float total = (top[nt & 1][0][g] + top[nt & 1][1][g]) + (top[nt & 1][2][g] + top[nt & 1][3][g]);
-      const float o = acc[g] * (M[g] == -INFINITY ? 1.f / 256.f : exp2f(M[g] - m[g]) * (1.f / 256.f));
-      if (nsplit > 1) {
-        float* dst = partial + ((row0 + g) * nsplit + split) * (D + 2);
-        dst[dim] = o;
-        if (t == 0) {
-          dst[D] = m[g];
-          dst[D + 1] = total;
+        if (g >= group - g0 || !has_dim) continue;
+        const float total = (sums[0][g] + sums[1][g]) + (sums[2][g] + sums[3][g]);
+        const float o = acc[g] * (M[g] == -INFINITY ? 1.f / 256.f : exp2f(M[g] - m[g]) * (1.f / 256.f));
+        if (whole_item) {
+          out[(row0 + g) * D + dim] = __float2bfloat16(o / total);
+        } else {
+          float* dst = partial + ((2LL * blockIdx.x + (begins_inside ? 0 : 1)) * GP + g) * (D + 2);
+          dst[dim] = o;
+          if (t == 0) {
+            dst[D] = m[g];
+            dst[D + 1] = total;
+          }
         }
-      } else {
-        out[(row0 + g) * D + dim] = __float2bfloat16(nt > 0 ? o / total : 0.f);
       }
     }
   }
@@ -389,11 +537,67 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
   }
 }
 
+// Items of more than one run.  Grid: (items of a sequence x GP, batch), a thread per dimension.
+template <int D, int GP>
+__global__ void __launch_bounds__(D)
+paged_attn_merge_fp8_t5_kernel(const float* __restrict__ partial, __nv_bfloat16* __restrict__ out, dec8::Work work, int ctas, int kv_heads, int group) {
+  using namespace dec8;
+  wait_for_previous(partial, out, work.context_lens);
+  release_dependents();
+  const int b = blockIdx.y, x = blockIdx.x / GP, g = blockIdx.x % GP, nt = work.tiles(b), g0 = x / kv_heads * GP;
+  if (g >= group - g0) return;
+  const long long row = (static_cast<long long>(b) * kv_heads + x % kv_heads) * group + g0 + g;
+  if (nt == 0) {
+    out[row * D + threadIdx.x] = __float2bfloat16(0.f);
+    return;
+  }
+  int all;
+  const int before = tiles_before(work, b, all);                          // every warp for itself
+  const int length = run_length(work, all, ctas), start = before * work.per_sequence + x * nt;
+  const int c0 = start / length, c1 = (start + nt - 1) / length;
+  if (c0 == c1) return;
+  float m = -INFINITY, l = 0.f, o = 0.f;
+  for (int c = c0; c <= c1; ++c) {
+    const float* p = partial + ((2LL * c + (c * length > start ? 0 : 1)) * GP + g) * (D + 2);
+    const float pm = p[D], pl = p[D + 1], po = p[threadIdx.x], to = fmaxf(m, pm), ref = to == -INFINITY ? 0.f : to;
+    const float u = exp2f(m - ref), w = exp2f(pm - ref);
+    l = l * u + pl * w;
+    o = o * u + po * w;
+    m = to;
+  }
+  out[row * D + threadIdx.x] = __float2bfloat16(o / l);
+}
+
 bool paged_attn_fp8_t5_ok(int head_dim, int block_size) { return (head_dim == 64 || head_dim == 128) && block_size % 8 == 0; }
+
+namespace dec8 {
+struct Plan {
+  int GP, parts, ctas, per_sm, whole;
+  long long items, partial;
+};
+static Plan plan_of(int batch, int heads, int kv_heads, int head_dim, int limit, int runs) {
+  Plan p;
+  const int group = heads / kv_heads;
+  for (p.GP = 1; p.GP < group && p.GP < 16;) p.GP *= 2;
+  p.parts = (group + p.GP - 1) / p.GP;
+  p.per_sm = p.GP == 16 ? 1 : 2;
+  p.items = static_cast<long long>(batch) * kv_heads * p.parts;
+  const long long tiles = p.items * ((limit + kTile - 1) / kTile);
+  p.whole = runs == 1 || limit <= kWholeTokens;
+  const long long most = p.whole ? p.items : runs > 1 ? runs : (tiles + kLeast - 1) / kLeast;
+  p.ctas = static_cast<int>(most < p.per_sm * kNumSMs ? (most > 1 ? most : 1) : p.per_sm * kNumSMs);
+  p.partial = p.whole ? 0 : 2LL * p.ctas * p.GP * (head_dim + 2);
+  return p;
+}
+}  // namespace dec8
+
+long long paged_attn_fp8_t5_scratch(int batch, int heads, int kv_heads, int head_dim, int limit, int runs) {
+  return dec8::plan_of(batch, heads, kv_heads, head_dim, limit, runs).partial;
+}
 
 int launch_paged_attn_fp8_t5(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
                              const int* block_tables, int max_blocks, const int* context_lens, void* out, float* partial, int batch, int heads, int kv_heads,
-                             int head_dim, int blocks, int block_size, int limit, int tokens_per_split, int splits, float scale, cudaStream_t s) {
+                             int head_dim, int blocks, int block_size, int limit, int runs, float scale, cudaStream_t s) {
   using namespace dec8;
   int box_rows = 8;
   while (box_rows < kTile && block_size % (2 * box_rows) == 0) box_rows *= 2;
@@ -406,22 +610,29 @@ int launch_paged_attn_fp8_t5(const void* q, long long q_stride, const void* k_ca
   unsigned char* const wait_byte = wait_report(kWaitPagedFp8);
   if (wait_byte == nullptr) return static_cast<int>(cudaErrorMemoryAllocation);
   const int group = heads / kv_heads;
-  auto launch = [&](auto kern, int N) {
-    const int room = 110 * 1024, fit = (room - fixed_smem(head_dim, N)) / stage_bytes(head_dim), stages = fit < kMaxStages ? fit : kMaxStages;
-    const int smem = fixed_smem(head_dim, N) + stages * stage_bytes(head_dim);
-    const cudaError_t e = allow_smem(kern, smem);
-    if (e != cudaSuccess) return e;
-    const int parts = (group + N / kPieces - 1) / (N / kPieces);
-    return launch_dependent(kern, dim3(kv_heads * parts, splits, batch), kThreads, smem, s, tmK, tmV, (const __nv_bfloat16*)q, q_stride, k_scale, v_scale,
-                            block_tables, max_blocks, context_lens, splits > 1 ? partial : nullptr, (__nv_bfloat16*)out, blocks, block_size,
-                            FastDiv(static_cast<uint32_t>(block_size)), box_rows, kv_heads, group, limit, tokens_per_split, stages,
-                            scale * kLog2e, wait_byte);
+  const Plan p = plan_of(batch, heads, kv_heads, head_dim, limit, runs);
+  if (p.partial > 0 && partial == nullptr) return static_cast<int>(cudaErrorInvalidValue);
+  if (p.items * ((limit + kTile - 1) / kTile) >= (1LL << 30)) return static_cast<int>(cudaErrorInvalidValue);      // tiles are counted in 31 bits
+  const int items = static_cast<int>(p.items);
+  const Work work{context_lens, batch, kv_heads * p.parts, limit, kLeast, p.whole, items / p.ctas, items % p.ctas, FastDiv(static_cast<uint32_t>(kv_heads * p.parts))};
+  auto launch = [&](auto kern, auto merge) {
+    const int room = (p.per_sm == 1 ? 225 : 110) * 1024, fit = (room - fixed_smem(head_dim, columns(p.GP))) / stage_bytes(head_dim);
+    const int stages = fit < kMaxStages ? fit : kMaxStages, smem = fixed_smem(head_dim, columns(p.GP)) + stages * stage_bytes(head_dim);
+    cudaError_t e = allow_smem(kern, smem);
+    if (e == cudaSuccess)
+      e = launch_dependent(kern, p.ctas, kThreads, smem, s, tmK, tmV, (const __nv_bfloat16*)q, q_stride, k_scale, v_scale, block_tables, max_blocks, work,
+                           partial, (__nv_bfloat16*)out, blocks, block_size, FastDiv(static_cast<uint32_t>(block_size)), box_rows, kv_heads, group, stages,
+                           scale * kLog2e, wait_byte);
+    if (e == cudaSuccess && !p.whole)
+      e = launch_dependent(merge, dim3(work.per_sequence * p.GP, batch), head_dim, 0, s, partial, (__nv_bfloat16*)out, work, p.ctas, kv_heads, group);
+    return static_cast<int>(e);
   };
-  if (head_dim == 128)
-    return static_cast<int>(group <= 4 ? launch(paged_attn_decode_fp8_t5_kernel<128, 16>, 16)
-                                       : group <= 8 ? launch(paged_attn_decode_fp8_t5_kernel<128, 32>, 32) : launch(paged_attn_decode_fp8_t5_kernel<128, 64>, 64));
-  return static_cast<int>(group <= 4 ? launch(paged_attn_decode_fp8_t5_kernel<64, 16>, 16)
-                                     : group <= 8 ? launch(paged_attn_decode_fp8_t5_kernel<64, 32>, 32) : launch(paged_attn_decode_fp8_t5_kernel<64, 64>, 64));
+#define LLMCTL_DECODE8(D, GP) launch(paged_attn_decode_fp8_t5_kernel<D, GP>, paged_attn_merge_fp8_t5_kernel<D, GP>)
+#define LLMCTL_DECODE8_OF(D) \
+  (p.GP == 1 ? LLMCTL_DECODE8(D, 1) : p.GP == 2 ? LLMCTL_DECODE8(D, 2) : p.GP == 4 ? LLMCTL_DECODE8(D, 4) : p.GP == 8 ? LLMCTL_DECODE8(D, 8) : LLMCTL_DECODE8(D, 16))
+  return head_dim == 128 ? LLMCTL_DECODE8_OF(128) : LLMCTL_DECODE8_OF(64);
+#undef LLMCTL_DECODE8_OF
+#undef LLMCTL_DECODE8
 }
 
 }  // namespace llmctl
