@@ -13,7 +13,7 @@
 //     O = 2^(M - m) sum_j w_j cv_j / l,    w_j = 2^(s_j + log2 sv_j - M),    l = sum_j 2^(s_j - m)
 // O of a tile is read from tensor memory and added up in registers, where the reference of the tiles before is caught up with.
 //
-//   warp 0      TMA producer: 128 tokens of keys and of values, a box for each block that they stand in, a ring of stages; their scales beside them
+//   warps 0, 7  TMA producers of keys and of values: 128 tokens, a box for each block that they stand in, a ring of stages; their scales beside them
 //   warps 1, 6  MMA issuers, of scores and of values
 //   warps 2-5   the columns of Q, then a token per thread: S^T -> P^T; a dimension per thread: O^T
 //
@@ -36,9 +36,9 @@ using namespace ptx;
 
 namespace dec8 {
 constexpr int kTile = 128;                   // tokens
-constexpr int kThreads = 224;
+constexpr int kThreads = 256;
 constexpr int kPieces = 4, kMaxStages = 8, kMaxBoxes = 16;
-constexpr int kWholeTokens = 512, kLeast = 2;
+constexpr int kWholeTokens = 768, kLeast = 2;
 constexpr float kStep = 16.f;                // between the columns of a number
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int columns(int GP) { return GP < 4 ? 16 : kPieces * GP; }     // of a product: 16 at least, of which those past 4 GP are nobody's
@@ -207,7 +207,7 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
   __shared__ float top[2][4][2 * GP];                                      // per softmax warp: the tile's largest s and s + log2 sv
-  __shared__ float2 box_scale[kMaxStages][kMaxBoxes];                      // of a stage's boxes: sk, log2 sv
+  __shared__ float box_scale[kMaxStages][2][kMaxBoxes];                    // of a stage's boxes: sk, log2 sv
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -217,7 +217,7 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
   if (threadIdx.x == 0) {
     mbar_init(&bar_q, 4);
     for (int i = 0; i < stages; ++i) {
-      mbar_init(&bar_full[i], 1);
+      mbar_init(&bar_full[i], 2);
       mbar_init(&bar_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -241,8 +241,8 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
   const int heads = kv_heads * group;
   const Run run = run_of(work, blockIdx.x, gridDim.x);                     // every warp finds it for itself
 
-  if (warp == 0) {
-    // ------------------------------------ TMA producer: a lane per box ------------------------------------
+  if (warp == 0 || warp == 7) {
+    // ------------------------------------ TMA producers, of keys and of values: a lane per box ------------------------------------
     const int boxes = kTile / box_rows, all_rows = blocks * kv_heads * block_size;
     // Three tiles are under way: the block of the one after next is asked for, the scales of the next, and this one is copied: the producer waits for
     // no load that it has just asked for.  A block outside of the cache is filled with zeros, its scales are no numbers.
@@ -262,6 +262,9 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
     auto scale_of = [&](const float* s, const Box& box) {
       return box.row < 0 ? 0.f : box.block >= 0 && box.block < blocks ? s[static_cast<long long>(box.block) * kv_heads + box.head] : NAN;
     };
+    const bool keys = warp == 0;
+    const CUtensorMap* tm = keys ? &tmK : &tmV;
+    const float* scales = keys ? k_scale : v_scale;
     Items it(run, work);
     int tile = 0, loaded = 0;                             // within the item's part; so far
     auto advance = [&] {
@@ -273,30 +276,27 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
     Box box = find(it, 0);
     advance();
     Box next = find(it, tile);
-    float sk = scale_of(k_scale, box), sv = scale_of(v_scale, box);
+    float scale = scale_of(scales, box);
     Place at;
     for (; loaded < run.left; ++loaded, at.next(stages)) {
       const int st = at.st;
       advance();
       const Box after = find(it, tile);
-      const float next_sk = scale_of(k_scale, next), next_sv = scale_of(v_scale, next);
+      const float next_scale = scale_of(scales, next);
       const bool given = loaded < stages || mbar_wait_bounded(&bar_empty[st], at.phase ^ 1u, abort);
       if (!__all_sync(0xffffffffu, given)) break;
-      if (lane < kMaxBoxes) box_scale[st][lane] = make_float2(sk, __log2f(sv));
+      if (lane < kMaxBoxes) box_scale[st][keys ? 0 : 1][lane] = keys ? scale : __log2f(scale);
       const int count = __popc(__ballot_sync(0xffffffffu, box.row >= 0));
       __syncwarp();                                       // the scales are there for whom the barrier lets through
-      if (lane == 0) mbar_expect_tx(&bar_full[st], count * box_rows * D * 2);
+      if (lane == 0) mbar_expect_tx(&bar_full[st], count * box_rows * D);
       __syncwarp();
       if (box.row >= 0) {
         const int row = box.block >= 0 && box.block < blocks ? (box.block * kv_heads + box.head) * block_size + box.row : all_rows;
-        uint8_t* dst = smem + st * kStage + lane * box_rows * D;
-        tma_load_2d(dst, &tmK, &bar_full[st], 0, row);
-        tma_load_2d(dst + kHalf, &tmV, &bar_full[st], 0, row);
+        tma_load_2d(smem + st * kStage + (keys ? 0 : kHalf) + lane * box_rows * D, tm, &bar_full[st], 0, row);
       }
       box = next;
       next = after;
-      sk = next_sk;
-      sv = next_sv;
+      scale = next_scale;
     }
     // Copies still in flight when a wait ran out land before the CTA's shared memory is given back.
     if (*abort && lane == 0)
@@ -436,15 +436,14 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
         mbar_wait_or_abort(&bar_full[st], at.phase, abort);                // it is: the scales, and values that are written below
         __syncwarp();
         tc_fence_after();
-        const float2 scale = box_scale[st][box];
-        const float lv = seen ? scale.y : 0.f;
+        const float sk = box_scale[st][0][box], lv = seen ? box_scale[st][1][box] : 0.f;
         float s[GP];
         {
           uint32_t c[C];
           tmem_ld<C>(tmem_base + (n & 1) * N + lane_off, c);
           tmem_ld_wait();
 #pragma unroll
-          for (int g = 0; g < GP; ++g) s[g] = seen ? joined<GP>(c, g) * (scale.x * factor[g]) : -INFINITY;
+          for (int g = 0; g < GP; ++g) s[g] = seen ? joined<GP>(c, g) * (sk * factor[g]) : -INFINITY;
         }
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
@@ -557,12 +556,28 @@ paged_attn_merge_fp8_t5_kernel(const float* __restrict__ partial, __nv_bfloat16*
   const int c0 = start / length, c1 = (start + nt - 1) / length;
   if (c0 == c1) return;
   float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int c = c0; c <= c1; ++c) {
-    const float* p = partial + ((2LL * c + (c * length > start ? 0 : 1)) * GP + g) * (D + 2);
-    const float pm = p[D], pl = p[D + 1], po = p[threadIdx.x], to = fmaxf(m, pm), ref = to == -INFINITY ? 0.f : to;
-    const float u = exp2f(m - ref), w = exp2f(pm - ref);
-    l = l * u + pl * w;
-    o = o * u + po * w;
+  constexpr int kAhead = 8;                               // parts that are asked for before the first is there
+  for (int c = c0; c <= c1; c += kAhead) {
+    float pm[kAhead], pl[kAhead], po[kAhead], to = m;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float* p = partial + ((2LL * (c + i) + ((c + i) * length > start ? 0 : 1)) * GP + g) * (D + 2);
+      const bool there = c + i <= c1;
+      pm[i] = there ? p[D] : -INFINITY;
+      pl[i] = there ? p[D + 1] : 0.f;
+      po[i] = there ? p[threadIdx.x] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) to = fmaxf(to, pm[i]);
+    const float ref = to == -INFINITY ? 0.f : to, u = exp2f(m - ref);
+    l *= u;
+    o *= u;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float w = exp2f(pm[i] - ref);
+      l += pl[i] * w;
+      o += po[i] * w;
+    }
     m = to;
   }
   out[row * D + threadIdx.x] = __float2bfloat16(o / l);
