@@ -193,7 +193,7 @@ struct Items {
 // Grid: as many CTAs as there are runs.  GP: query heads of an item.  partial: two rows of items [2 ctas, GP, D + 2] = {sum of w cv at the reference m, m (log2), sum of p}: of the
 // item that the run begins inside of, and of the one that it ends inside of.
 template <int D, int GP>
-__global__ void __launch_bounds__(dec8::kThreads, GP == 16 ? 1 : 2)
+__global__ void __launch_bounds__(dec8::kThreads, GP == 16 ? 1 : D == 64 && GP <= 2 ? 3 : 2)
 paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __nv_bfloat16* __restrict__ q,
                                 long long q_stride, const float* __restrict__ k_scale, const float* __restrict__ v_scale,
                                 const int* __restrict__ block_tables, int max_blocks, dec8::Work work, float* __restrict__ partial,
@@ -416,8 +416,8 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
           for (int i = t; i < heads * D; i += 128) out[static_cast<long long>(b) * heads * D + i] = __float2bfloat16(0.f);
     Place at;
     int n = 0, part = 0;                                  // tiles so far; use of top: items and tiles so far
+    if (it.more()) write_q(x, factor, part++ & 1);
     while (it.more()) {
-      write_q(x, factor, part++ & 1);
       const int first = n, end = n + it.n, b = it.r.b, g0 = it.r.x / kv_heads * GP, kv_head = it.r.x % kv_heads;
       const int t0 = it.r.t * kTile, t1 = it.tokens;
       const bool whole_item = it.n == it.nt, begins_inside = it.r.t > 0;
@@ -483,16 +483,15 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
 #pragma unroll
           for (int i = 0; i < C / 16; ++i) *reinterpret_cast<uint4*>(dst + i * kTile * 16) = make_uint4(codes[4 * i], codes[4 * i + 1], codes[4 * i + 2], codes[4 * i + 3]);
         }
-        // Values past the last token: nothing that the cache holds there may meet a weight of zero.
-        if (!seen) {
-          uint8_t* row = smem + st * kStage + kHalf + t * D;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) *reinterpret_cast<uint4*>(row + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-        }
+        // Values past the last token: nothing that the cache holds there may meet a weight of zero.  A row to eight lanes (a lane to its row has all in
+        // the same banks: 900 clocks in the way of every short context).
+        for (int i = max(t1 - t0 - (n - first) * kTile - quad * 32, 0) + lane / (D / 16); i < 32; i += 512 / D)
+          *reinterpret_cast<uint4*>(smem + st * kStage + kHalf + (quad * 32 + i) * D + lane % (D / 16) * 16) = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar_p[n & 1]);
+        if (n == end - 1 && it.more()) write_q(x, factor, ++part & 1);      // of the next item: its first scores run beside what is left of this one
         if (n > first) add_tile(n - 1);
 #pragma unroll
         for (int g = 0; g < GP; ++g) catch_up[g] = from[g];
@@ -595,10 +594,13 @@ static Plan plan_of(int batch, int heads, int kv_heads, int head_dim, int limit,
   const int group = heads / kv_heads;
   for (p.GP = 1; p.GP < group && p.GP < 16;) p.GP *= 2;
   p.parts = (group + p.GP - 1) / p.GP;
-  p.per_sm = p.GP == 16 ? 1 : 2;
+  p.per_sm = p.GP == 16 ? 1 : head_dim == 64 && p.GP <= 2 ? 3 : 2;        // registers; stages of 192 KB an SM in all
   p.items = static_cast<long long>(batch) * kv_heads * p.parts;
   const long long tiles = p.items * ((limit + kTile - 1) / kTile);
-  p.whole = runs == 1 || limit <= kWholeTokens;
+  // Nothing is split where contexts are short: the second kernel is 2 to 3 us, a tile of a longer chain 0.65.  us, whole / split: 16 contexts of up to 600,
+  // 32 heads of 128 15.4 / 18.3, of 1000 21.1 / 21.8, 32 heads over 8 10.5 / 13.7; one of 1000, 32 heads 9.3 / 7.6, 64 of 1000 64.7 / 61.3; 16 of 2000
+  // 35.5 / 33.8.
+  p.whole = runs == 1 || limit <= kWholeTokens || (limit <= 1024 && p.items >= 128 && p.items <= 1024);
   const long long most = p.whole ? p.items : runs > 1 ? runs : (tiles + kLeast - 1) / kLeast;
   p.ctas = static_cast<int>(most < p.per_sm * kNumSMs ? (most > 1 ? most : 1) : p.per_sm * kNumSMs);
   p.partial = p.whole ? 0 : 2LL * p.ctas * p.GP * (head_dim + 2);
@@ -631,7 +633,7 @@ int launch_paged_attn_fp8_t5(const void* q, long long q_stride, const void* k_ca
   const int items = static_cast<int>(p.items);
   const Work work{context_lens, batch, kv_heads * p.parts, limit, kLeast, p.whole, items / p.ctas, items % p.ctas, FastDiv(static_cast<uint32_t>(kv_heads * p.parts))};
   auto launch = [&](auto kern, auto merge) {
-    const int room = (p.per_sm == 1 ? 225 : 110) * 1024, fit = (room - fixed_smem(head_dim, columns(p.GP))) / stage_bytes(head_dim);
+    const int room = (p.per_sm == 1 ? 225 : p.per_sm == 2 ? 110 : 72) * 1024, fit = (room - fixed_smem(head_dim, columns(p.GP))) / stage_bytes(head_dim);
     const int stages = fit < kMaxStages ? fit : kMaxStages, smem = fixed_smem(head_dim, columns(p.GP)) + stages * stage_bytes(head_dim);
     cudaError_t e = allow_smem(kern, smem);
     if (e == cudaSuccess)
