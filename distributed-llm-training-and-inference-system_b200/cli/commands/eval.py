@@ -22,6 +22,7 @@ app = typer.Typer(help="Evaluate trained checkpoints")
 def evaluate_checkpoint(ckpt: Path, tasks, suite=None, batches: int = 8, batch_size: int = 4, seq_len: int = 512,
                         device: Optional[str] = None) -> dict:
     import torch
+    from ...ops.functional import token_logprobs
     from ...serve.engine import load_model_for_inference
     model, mcfg, tok, dev = load_model_for_inference(ckpt, device)
     seq_len = min(seq_len, mcfg.max_position_embeddings)
@@ -38,13 +39,13 @@ def evaluate_checkpoint(ckpt: Path, tasks, suite=None, batches: int = 8, batch_s
             arr = torch.stack([torch.from_numpy(ds[b * batch_size + i]) for i in range(batch_size)]).to(dev)
             tokens, targets = arr[:, :-1].contiguous(), arr[:, 1:].contiguous()
             t0 = time.perf_counter()
-            logits = model(tokens).float()[:, :mcfg.vocab_size]
+            logits = model(tokens)[:, :mcfg.vocab_size]
             if dev.type == "cuda":
                 torch.cuda.synchronize()
             lat.append(time.perf_counter() - t0)
-            lp = torch.log_softmax(logits, -1)
-            nll += float(-lp.gather(-1, targets.reshape(-1, 1)).sum())
-            correct += int((logits.argmax(-1) == targets.reshape(-1)).sum())
+            said = token_logprobs(logits, targets.reshape(-1), top=1)
+            nll -= float(said.logprobs.double().sum())
+            correct += int((said.top_ids[:, 0] == targets.reshape(-1)).sum())
             count += targets.numel()
     for t in tasks:
         if t == "perplexity":

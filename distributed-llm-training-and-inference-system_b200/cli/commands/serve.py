@@ -25,6 +25,7 @@ def start(
     max_batch_tokens: int = typer.Option(8192, "--max-batch-tokens"),
     max_concurrent: int = typer.Option(128, "--max-concurrent"),
     device: str = typer.Option("auto", "--device", help="auto | cuda | cpu"),
+    kv_cache_dtype: str = typer.Option("auto", "--kv-cache-dtype", help="auto (the model's type) | fp8 (8 bits, a scale for each block and head)"),
     tensor_parallel: int = typer.Option(1, "--tensor-parallel", "--tp", help="Shard the model over this many GPUs (one process per GPU, rank 0 serves HTTP)"),
     dry_run: bool = typer.Option(False, "--dry-run", help="Validate and print the configuration, do not serve"),
 ):
@@ -36,7 +37,7 @@ def start(
         fail(f"artifact not found: {artifact}", 2)
     try:
         cfg = ServeConfig(artifact=artifact, host=host, port=port, scheduler=scheduler, max_batch_size=max_batch_size,
-                          max_batch_tokens=max_batch_tokens, max_concurrent=max_concurrent, device=device)
+                          max_batch_tokens=max_batch_tokens, max_concurrent=max_concurrent, device=device, kv_cache_dtype=kv_cache_dtype)
     except Exception as e:  # noqa: BLE001 - pydantic validation error
         fail(str(e), 2)
     console.print(f"[bold blue]Starting inference server[/bold blue]  artifact={artifact} {host}:{port} "
@@ -51,7 +52,7 @@ def start(
         cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", f"--nproc-per-node={tensor_parallel}",
                "--master-addr", "127.0.0.1", "--master-port", str(free_port()), worker, "--artifact", str(artifact),
                "--host", host, "--port", str(port), "--scheduler", scheduler, "--max-batch-size", str(max_batch_size),
-               "--max-batch-tokens", str(max_batch_tokens), "--max-concurrent", str(max_concurrent), "--device", device]
+               "--max-batch-tokens", str(max_batch_tokens), "--max-concurrent", str(max_concurrent), "--device", device, "--kv-cache-dtype", kv_cache_dtype]
         if dry_run:
             console.print("[yellow]Dry run: configuration valid.[/yellow] " + " ".join(cmd))
             return cfg
@@ -66,7 +67,7 @@ def start(
     from ...serve.server import create_inference_server
     server = create_inference_server(artifact, host=host, port=port, max_batch_size=max_batch_size,
                                      max_batch_tokens=max_batch_tokens, max_concurrent_requests=max_concurrent,
-                                     scheduler=scheduler, device=None if device == "auto" else device)
+                                     scheduler=scheduler, device=None if device == "auto" else device, kv_cache_dtype=kv_cache_dtype)
     try:
         asyncio.run(server.start_server())
     except KeyboardInterrupt:

@@ -238,7 +238,15 @@ class ServeConfig(_Base):
     max_concurrent: int = Field(128, ge=1)
     device: str = "auto"
     kv_block_size: int = 16
+    kv_cache_dtype: str = "auto"          # auto (the model's type) | fp8 (a scale for each block and head)
     tensor_parallel: int = 1
+
+    @field_validator("kv_cache_dtype")
+    @classmethod
+    def _cache(cls, v):
+        if v not in ("auto", "fp8"):
+            raise ValueError("kv_cache_dtype must be auto | fp8")
+        return v
 
     @field_validator("scheduler")
     @classmethod

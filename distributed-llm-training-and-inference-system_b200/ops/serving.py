@@ -22,7 +22,7 @@ native.register_signature("llmctl_paged_attn_decode",
 native.register_signature("llmctl_paged_attn_scratch_elems", [c_int, c_int, c_int, c_int], restype=c_ll)
 native.register_signature("llmctl_rope_kv_append", [c_void_p, c_ll] + [c_int] * 4 + [c_void_p, c_void_p, c_int] + [c_void_p] * 4 + [c_ll, c_void_p])
 native.register_signature("llmctl_rope_kv_append_fp8", [c_void_p, c_ll] + [c_int] * 4 + [c_void_p, c_void_p, c_int] + [c_void_p] * 6 + [c_int, c_int, c_void_p])
-native.register_signature("llmctl_paged_attn_fp8_scratch_elems", [c_int] * 4, restype=c_ll)
+native.register_signature("llmctl_paged_attn_fp8_scratch_elems", [c_int] * 8, restype=c_ll)
 native.register_signature("llmctl_paged_attn_decode_fp8", [c_void_p, c_ll] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 8 + [c_float, c_void_p])
 native.register_signature("llmctl_sample", [c_void_p, c_int, c_ll, c_int, c_int] + [c_void_p] * 6 + [c_void_p])
 
@@ -254,13 +254,6 @@ def _aligned_rows(x: torch.Tensor, width: int) -> torch.Tensor:
     return x[:, :width].clone(memory_format=torch.contiguous_format)
 
 
-def _fp8_splits(batch: int, heads: int, kv_heads: int, max_context: int, block_size: int, sms: int = 148) -> int:
-    if block_size % 8:
-        return choose_splits(batch, heads, max_context, block_size, sms)
-    pairs = batch * kv_heads * -(-heads // kv_heads // 16)
-    return max(1, min(-(-4 * sms // pairs), max_context // 256, 64))
-
-
 def paged_attention_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                                block_tables: torch.Tensor, context_lens: torch.Tensor, max_context: int, scale: Optional[float] = None,
                                num_splits: Optional[int] = None) -> torch.Tensor:
@@ -282,11 +275,11 @@ def paged_attention_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         out = torch.empty(B, H, D, dtype=q.dtype, device=q.device)
         if B == 0:
             return out
-        ns = num_splits or _fp8_splits(B, H, kv_heads, max_context, block_size)
+        ns = num_splits or 0
         block_tables, context_lens = block_tables.contiguous(), context_lens.contiguous()
         if q.stride(2) != 1 or q.stride(1) != D or q.data_ptr() % 16 or q.stride(0) % 8:
             q = q.clone(memory_format=torch.contiguous_format)
-        need = native.lib().llmctl_paged_attn_fp8_scratch_elems(B, H, D, ns)
+        need = native.lib().llmctl_paged_attn_fp8_scratch_elems(B, H, kv_heads, D, block_tables.shape[1], block_size, max_context, ns)
         scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
         with _on_device(q):
             native.call("llmctl_paged_attn_decode_fp8", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),

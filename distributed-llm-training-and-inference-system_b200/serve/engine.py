@@ -8,8 +8,9 @@ themselves (``allocate_caches``); ``forward_portions`` is that step function, us
 
 One ``step()`` = one scheduler step: newly admitted sequences are prefilled (dense causal attention over the
 prompt, K/V scattered into their cache blocks — kernel K13), all running sequences then decode one token
-together (packed qkv GEMM, RoPE at each sequence's own position, K13 append, K12 paged attention over the
-block tables, K14 batched sampling) and finished sequences free their blocks.  Nothing in the step reads
+together (packed qkv GEMM, rotation to each sequence's own position and append in one kernel, K12 paged attention over the
+block tables, K14 batched sampling) and finished sequences free their blocks.  ``kv_cache_dtype="fp8"`` keeps the cache in 8 bits with a
+scale for each block and head.  Nothing in the step reads
 a value back to the host except the sampled token ids (one small D2H copy per step).
 
 Reference: reference llmctl/serve/server.py:127-251 ``InferenceEngine.generate_batch`` right-pads the batch,
@@ -94,6 +95,9 @@ class Sequence:
     cancel_requested: bool = False         # set from any thread (client went away); honoured at the next token
     cancel_applied: bool = False           # lockstep (TP) serving: the cancellation has reached every rank
     done_event: threading.Event = field(default_factory=threading.Event)
+    logprobs: Optional[int] = None         # how many alternatives to each token's log probability; None: no log probabilities
+    token_logprobs: List[dict] = field(default_factory=list)       # of each generated token: token, logprob, entropy, top [(token, logprob)]
+    last_logprob: Optional[dict] = None    # of the token that was sampled last
 
     @property
     def all_ids(self) -> List[int]:
@@ -222,7 +226,7 @@ class InferenceEngine:
                  scheduler: str = "dynamic", device: Optional[str] = None, kv_block_size: int = 16,
                  kv_memory_fraction: float = 0.5, num_kv_blocks: Optional[int] = None, seed: int = 0,
                  cuda_graphs: Optional[bool] = None, fused_tp_decode: Optional[bool] = None,
-                 dtype: Optional[torch.dtype] = None, kv_watermark: float = 0.01):
+                 dtype: Optional[torch.dtype] = None, kv_watermark: float = 0.01, kv_cache_dtype: str = "auto"):
         self.model, self.cfg, self.tokenizer, self.device = load_model_for_inference(artifact, device, dtype)
         self.st = get_state()
         self.lockstep = False       # True under serve/lockstep.py: cancellations take effect on all TP ranks at once
@@ -233,11 +237,21 @@ class InferenceEngine:
             self.head_dim = self.cfg.head_dim
         self.block_size = kv_block_size
         self.dtype = m.dtype if self.ragged else next(m.parameters()).dtype
+        if kv_cache_dtype not in ("auto", "fp8"):
+            raise ValueError(f"kv_cache_dtype {kv_cache_dtype!r}: auto (the model's type) or fp8")
+        self.fp8_cache = kv_cache_dtype == "fp8"
+        if self.fp8_cache and self.ragged:
+            raise ValueError("kv_cache_dtype fp8: this model lays out its own caches")
+        if self.fp8_cache and self.device.type == "cuda" and (self.head_dim not in (64, 128) or self.dtype != torch.bfloat16):
+            raise ValueError(f"kv_cache_dtype fp8: bfloat16 models with heads of 64 or 128, not {self.dtype} with heads of {self.head_dim}")
+        if self.fp8_cache and (self.head_dim % 16 or not 1 <= kv_block_size <= 4096):
+            raise ValueError("kv_cache_dtype fp8: heads of a multiple of 16, blocks of at most 4096 tokens")
         if num_kv_blocks is None:
             if self.ragged:
                 per_block = max(m.cache_bytes_per_block(kv_block_size), 1)
             else:
-                per_block = 2 * len(m.blocks) * kv_block_size * self.heads_local * self.head_dim * self.dtype.itemsize
+                row = self.head_dim if self.fp8_cache else self.head_dim * self.dtype.itemsize
+                per_block = 2 * len(m.blocks) * self.heads_local * (kv_block_size * row + (4 if self.fp8_cache else 0))
             if self.device.type == "cuda":
                 free, _ = torch.cuda.mem_get_info(self.device)
                 num_kv_blocks = int(free * kv_memory_fraction // per_block)
@@ -270,6 +284,9 @@ class InferenceEngine:
         elif self.ragged:
             self.caches = m.allocate_caches(num_kv_blocks, kv_block_size, self.device)
             self.k_caches, self.v_caches = [], []
+        elif self.fp8_cache:
+            k, v = ([sops.allocate_fp8_cache(num_kv_blocks, kv_block_size, self.heads_local, self.head_dim, self.device) for _ in m.blocks] for _ in range(2))
+            (self.k_caches, self.k_scales), (self.v_caches, self.v_scales) = (map(list, zip(*c)) for c in (k, v))
         else:
             shape = (num_kv_blocks, kv_block_size, self.heads_local, self.head_dim)
             self.k_caches = [torch.zeros(shape, dtype=self.dtype, device=self.device) for _ in m.blocks]
@@ -305,7 +322,11 @@ class InferenceEngine:
 
     # ---- request API ---------------------------------------------------------------------------------
     def add_request(self, prompt_ids: List[int], max_tokens: int = 100, temperature: float = 1.0, top_p: float = 1.0,
-                    top_k: int = -1, on_token=None) -> Sequence:
+                    top_k: int = -1, on_token=None, logprobs: Optional[int] = None) -> Sequence:
+        """``logprobs``: the sequence's ``token_logprobs`` get each generated token's log probability under the model (before temperature, top_k and top_p), the
+        entropy and that many of the most probable tokens."""
+        if logprobs is not None and not 0 <= logprobs <= min(ops.MAX_TOP_LOGPROBS, self.cfg.vocab_size):
+            raise ValueError(f"logprobs: 0 to {min(ops.MAX_TOP_LOGPROBS, self.cfg.vocab_size)} alternatives, not {logprobs}")
         if not prompt_ids:
             prompt_ids = [self.tokenizer.bos_token_id if getattr(self.tokenizer, "bos_token_id", None) is not None else 0]
         limit = self.cfg.max_position_embeddings
@@ -314,7 +335,7 @@ class InferenceEngine:
         with self._lock:
             rid = self._next_id
             self._next_id += 1
-            seq = Sequence(rid, list(prompt_ids), max_tokens, temperature, top_p, top_k, on_token=on_token)
+            seq = Sequence(rid, list(prompt_ids), max_tokens, temperature, top_p, top_k, on_token=on_token, logprobs=logprobs)
             if self._plugin_sched is not None and max_tokens > 0:
                 self._staged.append(_StagedRequest(rid, len(prompt_ids), max_tokens, time.time()))
                 self.seqs[rid] = seq
@@ -428,15 +449,21 @@ class InferenceEngine:
         bt = torch.tensor(table, dtype=torch.int64)
         return (bt[idx // self.block_size] * self.block_size + idx % self.block_size).to(self.device)
 
-    def _rope(self, qkv: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+    def _append(self, i: int, qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+        """Rotate q and k of a layer's packed rows to their positions and write k and v to its cache; returns the rows with q and k rotated."""
         cos, sin = self.model.rope_tables(self.device)
-        return ops.rope_packed(qkv.clone() if not qkv.is_cuda else qkv, cos, sin, 2 * self.heads_local, self.head_dim,
-                               self.cfg.max_position_embeddings, positions)
+        H, D = self.heads_local, self.head_dim
+        if self.fp8_cache:
+            return sops.rope_kv_append(qkv, cos, sin, positions, self.k_caches[i], self.v_caches[i], slots, H, D, k_scale=self.k_scales[i], v_scale=self.v_scales[i])
+        if not qkv.is_cuda or (qkv.dtype == torch.bfloat16 and ops.kernel_config().elementwise == "native"):
+            return sops.rope_kv_append(qkv, cos, sin, positions, self.k_caches[i], self.v_caches[i], slots, H, D)
+        qkv = ops.rope_packed(qkv, cos, sin, 2 * H, D, self.cfg.max_position_embeddings, positions)
+        sops.kv_append(qkv, self.k_caches[i], self.v_caches[i], slots, H, D)
+        return qkv
 
     def _layer(self, i: int, blk, x, residual, positions, attn_fn):
         y, residual = blk.norm1(x, residual)
-        qkv = self._rope(blk.attn.qkv(y), positions)
-        a = attn_fn(i, qkv)
+        a = attn_fn(i, blk.attn.qkv(y), positions)
         y, residual = blk.norm2(blk.attn.out(a), residual)
         return blk.mlp(y), residual
 
@@ -452,9 +479,8 @@ class InferenceEngine:
         slots = self._slots(seq.req_id, 0, n)
         m = self.model
 
-        def attn(i, qkv):
-            sops.kv_append(qkv, self.k_caches[i], self.v_caches[i], slots, H, D)
-            v5 = qkv.view(1, n, 3, H, D)
+        def attn(i, qkv, positions):
+            v5 = self._append(i, qkv, positions, slots).view(1, n, 3, H, D)
             o = ops.attention(v5[:, :, 0], v5[:, :, 1], v5[:, :, 2], causal=True)
             return o.reshape(n, H * D)
 
@@ -471,10 +497,12 @@ class InferenceEngine:
         H, D = self.heads_local, self.head_dim
         m = self.model
 
-        def attn(i, qkv):
-            sops.kv_append(qkv, self.k_caches[i], self.v_caches[i], inp.slots, H, D)
-            q = qkv[:, :H * D].reshape(B, H, D)
-            o = sops.paged_attention_decode(q, self.k_caches[i], self.v_caches[i], inp.block_tables, inp.ctx, max_ctx)
+        def attn(i, qkv, positions):
+            q = self._append(i, qkv, positions, inp.slots)[:, :H * D].reshape(B, H, D)
+            if self.fp8_cache:
+                o = sops.paged_attention_decode_fp8(q, self.k_caches[i], self.v_caches[i], self.k_scales[i], self.v_scales[i], inp.block_tables, inp.ctx, max_ctx)
+            else:
+                o = sops.paged_attention_decode(q, self.k_caches[i], self.v_caches[i], inp.block_tables, inp.ctx, max_ctx)
             return o.reshape(B, H * D)
 
         x, residual = m.embed_tokens(inp.tokens), None
@@ -495,8 +523,7 @@ class InferenceEngine:
             x = x.reshape(B, -1)
             y, residual = m.blocks[0].norm1(x, None)
             for i, blk in enumerate(m.blocks):
-                qkv = self._rope(blk.attn.qkv(y), inp.positions)
-                a = attn(i, qkv)
+                a = attn(i, blk.attn.qkv(y), inp.positions)
                 rowpar(a, blk.attn.out.weight, ar.partial_out(B))
                 y, residual = ar.reduce_norm(B, residual, blk.norm2.weight, eps)
                 gu = blk.mlp.up(y)
@@ -581,9 +608,19 @@ class InferenceEngine:
         if self.st.tp > 1:
             import torch.distributed as dist
             dist.broadcast(u, src=self.st.tp_ranks[0], group=self.st.tp_group)   # same draw on every TP rank
-        tokens = sops.sample(logits, t, k, p, u).tolist()  # the step's only D2H copy
+        sampled = sops.sample(logits, t, k, p, u)
+        if any(s.logprobs is not None for s in seqs):
+            self._take_logprobs(logits, sampled, seqs)
+        tokens = sampled.tolist()  # the step's only D2H copy but for log probabilities
         native.check_waits("the step of these tokens")
         return tokens
+
+    def _take_logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, seqs: List[Sequence]) -> None:
+        out = ops.token_logprobs(logits, tokens, max(s.logprobs or 0 for s in seqs))
+        chosen, entropy, ids = out.logprobs.tolist(), out.entropy.tolist(), tokens.tolist()
+        top = [[] for _ in seqs] if out.top_ids is None else [list(zip(i, v)) for i, v in zip(out.top_ids.tolist(), out.top_logprobs.tolist())]
+        for r, s in enumerate(seqs):
+            s.last_logprob = None if s.logprobs is None else {"token": ids[r], "logprob": chosen[r], "entropy": entropy[r], "top": top[r][:s.logprobs]}
 
     # ---- one engine step ---------------------------------------------------------------------------------
     def step(self) -> List[Sequence]:
@@ -630,6 +667,8 @@ class InferenceEngine:
         if s.first_token_time is None:
             s.first_token_time = time.time()
         s.generated.append(int(tok))
+        if s.logprobs is not None:
+            s.token_logprobs.append(s.last_logprob)
         if s.on_token is not None:
             try:
                 s.on_token(s, int(tok))

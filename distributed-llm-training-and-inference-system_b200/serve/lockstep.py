@@ -55,12 +55,12 @@ class LockstepEngine:
 
     # ---- leader API (HTTP threads) -------------------------------------------------------------------------
     def add_request(self, prompt_ids: List[int], max_tokens: int = 100, temperature: float = 1.0, top_p: float = 1.0,
-                    top_k: int = -1, on_token=None) -> Sequence:
+                    top_k: int = -1, on_token=None, logprobs: Optional[int] = None) -> Sequence:
         """Queue a request; it is admitted on every rank at the start of the next step.  Blocks the calling (HTTP
         worker) thread until then, i.e. for at most one engine step."""
         holder: Dict[str, Any] = {"event": threading.Event(), "seq": None, "on_token": on_token}
         with self._lock:
-            self._pending.append(((list(prompt_ids), int(max_tokens), float(temperature), float(top_p), int(top_k)), holder))
+            self._pending.append(((list(prompt_ids), int(max_tokens), float(temperature), float(top_p), int(top_k), logprobs), holder))
         if self.on_pending is not None:
             self.on_pending()
         holder["event"].wait()
@@ -99,7 +99,7 @@ class LockstepEngine:
             return
         for i, args in enumerate(payload.get("adds", [])):
             on_token = holders[i]["on_token"] if i < len(holders) else None
-            seq = self.engine.add_request(*args, on_token=on_token)
+            seq = self.engine.add_request(*args[:5], on_token=on_token, logprobs=args[5])
             if i < len(holders):
                 holders[i]["seq"] = seq
                 holders[i]["event"].set()

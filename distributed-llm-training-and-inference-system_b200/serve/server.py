@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import asyncio
 import json
+import math
 import threading
 import time
 import uuid
@@ -26,6 +27,7 @@ class GenerationRequest(BaseModel):
     top_p: float = Field(1.0, gt=0.0, le=1.0)
     top_k: int = -1
     stream: bool = False
+    logprobs: Optional[int] = Field(None, ge=0, le=20)      # log probabilities of the generated tokens, with so many alternatives to each
 
 
 class GenerationResponse(BaseModel):
@@ -33,6 +35,16 @@ class GenerationResponse(BaseModel):
     text: str
     finish_reason: str
     usage: Dict[str, int]
+
+
+class GenerationLogprobsResponse(GenerationResponse):
+    """The response to a request with ``logprobs``: of each token its text, its id, its log probability, the entropy of the distribution it was drawn
+    from and the most probable tokens; null where a number is not finite."""
+    logprobs: Dict[str, list]
+
+
+def _finite(x: float) -> Optional[float]:
+    return x if math.isfinite(x) else None
 
 
 class RequestState:
@@ -86,7 +98,7 @@ class EngineLoop(threading.Thread):
 class InferenceServer:
     def __init__(self, model_path: str, host: str = "0.0.0.0", port: int = 8080, max_batch_size: int = 8,
                  max_batch_tokens: int = 8192, max_concurrent_requests: int = 128, scheduler: str = "dynamic",
-                 device: Optional[str] = None, engine: Optional[InferenceEngine] = None):
+                 device: Optional[str] = None, engine: Optional[InferenceEngine] = None, kv_cache_dtype: str = "auto"):
         from fastapi import FastAPI, HTTPException
         from fastapi.middleware.cors import CORSMiddleware
         from fastapi.responses import PlainTextResponse, StreamingResponse
@@ -94,7 +106,8 @@ class InferenceServer:
         self.model_path, self.host, self.port = str(model_path), host, port
         self.max_concurrent_requests = max_concurrent_requests
         self.engine = engine or InferenceEngine(model_path, max_batch_size=max_batch_size,
-                                                max_batch_tokens=max_batch_tokens, scheduler=scheduler, device=device)
+                                                max_batch_tokens=max_batch_tokens, scheduler=scheduler, device=device,
+                                                kv_cache_dtype=kv_cache_dtype)
         self.scheduler = self.engine.sched
         self.active_requests: Dict[str, RequestState] = {}
         self.completed = 0
@@ -160,7 +173,8 @@ class InferenceServer:
 
     def _submit(self, req: GenerationRequest, on_token=None):
         ids = self.engine.tokenizer.encode(req.prompt)
-        seq = self.engine.add_request(ids, req.max_tokens, req.temperature, req.top_p, req.top_k, on_token=on_token)
+        more = {} if req.logprobs is None else {"logprobs": req.logprobs}
+        seq = self.engine.add_request(ids, req.max_tokens, req.temperature, req.top_p, req.top_k, on_token=on_token, **more)
         rid = str(uuid.uuid4())
         self.active_requests[rid] = RequestState(rid, seq)
         self.loop_thread.wake.set()
@@ -169,9 +183,18 @@ class InferenceServer:
     def _response(self, rid: str, seq: Sequence, n_prompt: int) -> GenerationResponse:
         gen = [t for t in seq.generated if t != getattr(self.engine.tokenizer, "eos_token_id", -1)]
         text = self.engine.tokenizer.decode(gen)
-        return GenerationResponse(id=rid, text=text, finish_reason=seq.finish_reason or "error",
-                                  usage={"prompt_tokens": n_prompt, "completion_tokens": len(seq.generated),
-                                         "total_tokens": n_prompt + len(seq.generated)})
+        fields = {"id": rid, "text": text, "finish_reason": seq.finish_reason or "error",
+                  "usage": {"prompt_tokens": n_prompt, "completion_tokens": len(seq.generated), "total_tokens": n_prompt + len(seq.generated)}}
+        if seq.logprobs is None:
+            return GenerationResponse(**fields)
+        of = [self._token_logprob(r) for r in seq.token_logprobs if r["token"] != getattr(self.engine.tokenizer, "eos_token_id", -1)]
+        return GenerationLogprobsResponse(**fields, logprobs={n: [r[n] for r in of] for n in ("tokens", "token_ids", "token_logprobs", "entropy", "top_logprobs")})
+
+    def _token_logprob(self, r: dict) -> dict:
+        def text(token):
+            return self.engine.tokenizer.decode([token])
+        return {"tokens": text(r["token"]), "token_ids": r["token"], "token_logprobs": _finite(r["logprob"]), "entropy": _finite(r["entropy"]),
+                "top_logprobs": [{"token": text(i), "token_id": i, "logprob": _finite(v)} for i, v in r["top"]]}
 
     async def handle_generation_request(self, req: GenerationRequest) -> GenerationResponse:
         loop = asyncio.get_running_loop()
@@ -193,7 +216,7 @@ class InferenceServer:
         q: asyncio.Queue = asyncio.Queue()
 
         def on_token(seq, tok):
-            loop.call_soon_threadsafe(q.put_nowait, tok)
+            loop.call_soon_threadsafe(q.put_nowait, (tok, seq.token_logprobs[-1] if seq.logprobs is not None else None))
 
         rid, seq, n_prompt = await loop.run_in_executor(None, self._submit, req, on_token)
         try:
@@ -202,12 +225,15 @@ class InferenceServer:
                 if seq.finished and q.empty():
                     break
                 try:
-                    tok = await asyncio.wait_for(q.get(), timeout=0.1)
+                    tok, said = await asyncio.wait_for(q.get(), timeout=0.1)
                 except asyncio.TimeoutError:
                     continue
                 sent += 1
                 piece = self.engine.tokenizer.decode([tok])
-                yield f"data: {json.dumps({'id': rid, 'text': piece, 'index': sent - 1})}\n\n"
+                event = {"id": rid, "text": piece, "index": sent - 1}
+                if said is not None:
+                    event["logprobs"] = self._token_logprob(said)
+                yield f"data: {json.dumps(event)}\n\n"
             yield f"data: {json.dumps({'id': rid, 'finish_reason': seq.finish_reason, 'usage': self._response(rid, seq, n_prompt).usage})}\n\n"
             yield "data: [DONE]\n\n"
             self.completed += 1

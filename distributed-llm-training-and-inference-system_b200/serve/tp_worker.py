@@ -25,6 +25,7 @@ def main(argv=None) -> int:
     ap.add_argument("--max-concurrent", type=int, default=128)
     ap.add_argument("--device", default="auto")
     ap.add_argument("--num-kv-blocks", type=int, default=None)
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"])
     a = ap.parse_args(argv)
     import torch
     from llmctl_b200.comms import mesh
@@ -36,7 +37,7 @@ def main(argv=None) -> int:
     torch.manual_seed(1234 + st.rank)
     kw = {} if a.num_kv_blocks is None else {"num_kv_blocks": a.num_kv_blocks}
     eng = InferenceEngine(a.artifact, max_batch_size=a.max_batch_size, max_batch_tokens=a.max_batch_tokens,
-                          scheduler=a.scheduler, device=None if use_cuda else "cpu", **kw)
+                          scheduler=a.scheduler, device=None if use_cuda else "cpu", kv_cache_dtype=a.kv_cache_dtype, **kw)
     lock = LockstepEngine(eng)
     if st.tp_rank != 0:
         lock.serve_forever()

@@ -133,7 +133,8 @@ int llmctl_rope_kv_append(void* qkv, long long row_stride, int tokens, int heads
 int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int tokens, int heads, int kv_heads, int head_dim, const float* cos_t,
                               const float* sin_t, int table_rows, const int* positions, const long long* slots, void* k_cache, void* v_cache,
                               float* k_scale, float* v_scale, int blocks, int block_size, void* stream);
-long long llmctl_paged_attn_fp8_scratch_elems(int batch, int heads, int head_dim, int num_splits);
+long long llmctl_paged_attn_fp8_scratch_elems(int batch, int heads, int kv_heads, int head_dim, int max_blocks, int block_size, int max_context,
+                                              int num_splits);
 int llmctl_paged_attn_decode_fp8(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const float* k_scale,
                                  const float* v_scale, const int* block_tables, int max_blocks, const int* context_lens, void* out, float* scratch,
                                  int batch, int heads, int kv_heads, int head_dim, int blocks, int block_size, int max_context, int num_splits,

@@ -143,3 +143,46 @@ def test_refusals(sops):
                    (5, torch.zeros(2, 2, dtype=torch.int64)), (6, torch.ones(1, dtype=torch.int32)), (6, torch.ones(2, dtype=torch.int64))):
         with pytest.raises(ValueError):
             sops.paged_attention_decode_fp8(*fine[:i], bad, *fine[i + 1:])
+
+
+def _engine(**kw):
+    from llmctl_b200.comms import mesh
+    from llmctl_b200.serve.engine import InferenceEngine
+    mesh.reset_state()
+    return InferenceEngine("gpt-tiny", device="cpu", kv_block_size=4, num_kv_blocks=64, **kw)
+
+
+def test_engine_with_a_cache_of_8_bits():
+    """Greedy tokens of a served model are its best or next to it: the logits of a full recomputation differ by what e4m3 rounds (half a step of 2^-4 of
+    a key or value, in a model whose logits spread by about 1)."""
+    eng = _engine(max_batch_size=3, max_batch_tokens=256, kv_cache_dtype="fp8")
+    assert all(c.dtype == torch.float8_e4m3fn for c in eng.k_caches + eng.v_caches) and len(eng.k_scales) == len(eng.v_scales) == 2
+    g = torch.Generator().manual_seed(0)
+    prompts = [torch.randint(3, 500, (n,), generator=g).tolist() for n in (1, 9, 30)]
+    outs = eng.generate(prompts, max_tokens=7, temperature=0.0)
+    assert eng.kv.free_blocks == 64 and all(s.any() for s in eng.k_scales + eng.v_scales)
+    for p, o in zip(prompts, outs):
+        assert len(o) == 7
+        for i, t in enumerate(o):
+            logits = eng.model(torch.tensor([p + o[:i]])).float()[-1, :512]
+            assert logits.max() - logits[t] <= 0.1 * logits.std()
+    plain = _engine(max_batch_size=3, max_batch_tokens=256)
+    bytes_of = [sum(t.numel() * t.element_size() for t in e.k_caches + getattr(e, "k_scales", [])) for e in (plain, eng)]
+    assert bytes_of[1] < 0.3 * bytes_of[0]                     # of 32 bits here
+
+
+def test_engine_refuses_what_has_no_cache_of_8_bits():
+    with pytest.raises(ValueError, match="kv_cache_dtype"):
+        _engine(kv_cache_dtype="int3")
+    from llmctl_b200.config.schemas import ServeConfig
+    assert ServeConfig(artifact="x", kv_cache_dtype="fp8").kv_cache_dtype == "fp8"
+    with pytest.raises(ValueError):
+        ServeConfig(artifact="x", kv_cache_dtype="fp9")
+
+
+def test_serve_command_takes_the_cache_type():
+    from typer.testing import CliRunner
+    from llmctl_b200.cli.main import app
+    r = CliRunner().invoke(app, ["serve", "start", "--artifact", "gpt-tiny", "--kv-cache-dtype", "fp8", "--dry-run"])
+    assert r.exit_code == 0, r.output
+    assert CliRunner().invoke(app, ["serve", "start", "--artifact", "gpt-tiny", "--kv-cache-dtype", "fp4", "--dry-run"]).exit_code != 0

@@ -288,3 +288,74 @@ def test_gpu_refusals(sops):
     from llmctl_b200.ops import native
     assert native.lib().llmctl_paged_attn_decode_fp8(q.data_ptr(), H * D, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), tables.data_ptr(), 2, n.data_ptr(), q.data_ptr(), None, 1, H, H, 32, 2,
                                                      8, 8, 1, 1.0, native.stream_ptr()) == 1
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_and_keys_that_are_no_numbers(sops, D):
+    """A NaN among the values reaches its dimension of its head's output and no other, one among the keys or the queries the whole of its head."""
+    H, size, n = 2, 16, 100
+    tables, lens, blocks = _batch([n] * 4, size)
+    (k, ks), (v, vs) = _state(blocks, H, size, D), _state(blocks, H, size, D, seed=2)
+    q = _randn(4, H, D, std=0.1)
+    plain = sops.paged_attention_decode_fp8(q, k, v, ks, vs, tables, lens, n)
+    v.view(torch.uint8)[int(tables[0, 2]), 1, 3, 5] = 0x7f
+    k.view(torch.uint8)[int(tables[1, 6]), 0, 3, 7] = 0xff
+    q[2, 1, 3], q[3, 0, 0] = float("inf"), float("nan")
+    for splits in (None, 1, 3):
+        out = sops.paged_attention_decode_fp8(q, k, v, ks, vs, tables, lens, n, num_splits=splits)
+        bad = torch.zeros_like(out, dtype=torch.bool)
+        bad[0, 1, 5], bad[1, 0], bad[2, 1], bad[3, 0] = True, True, True, True
+        assert torch.equal(out.isnan(), bad)
+        assert torch.allclose(out[~bad].float(), plain[~bad].float(), rtol=2.0 ** -6, atol=1e-3)
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("heads,hidden", [(4, 512), (4, 256)])
+def test_engine_with_a_cache_of_8_bits(sops, graphs, heads, hidden):
+    """Greedy tokens against a full recomputation in bf16: the best one or next to it, prompts and decoding steps past the ends of blocks, graphs or not."""
+    from llmctl_b200.comms import mesh
+    from llmctl_b200.models.config import ModelConfig
+    from llmctl_b200.serve.engine import InferenceEngine
+    mesh.reset_state()
+    torch.manual_seed(0)
+    cfg = ModelConfig(name="fp8-test", layers=2, hidden=hidden, ffn=704, heads=heads, vocab_size=4096, max_position_embeddings=512)
+    eng = InferenceEngine(cfg, max_batch_size=4, max_batch_tokens=2048, num_kv_blocks=256, kv_cache_dtype="fp8", cuda_graphs=graphs)
+    prompts = [torch.randint(3, 4000, (n,)).tolist() for n in (17, 64, 5, 130)]
+    outs = eng.generate(prompts, max_tokens=20, temperature=0.0)
+    for p, o in zip(prompts, outs):
+        for i, t in enumerate(o):
+            logits = eng.model(torch.tensor([p + o[:i]], device="cuda")).float()[-1, :4096]
+            assert logits.max() - logits[t] <= 0.15 * logits.std()
+    assert eng.kv.free_blocks == 256
+
+
+def test_engine_refuses_heads_that_the_kernel_has_not(sops):
+    from llmctl_b200.comms import mesh
+    from llmctl_b200.serve.engine import InferenceEngine
+    mesh.reset_state()
+    with pytest.raises(ValueError, match="heads of 32"):
+        InferenceEngine("gpt-tiny", num_kv_blocks=16, kv_cache_dtype="fp8")
+
+
+def test_engine_of_16_bits_gives_the_bits_of_rotation_and_append(sops, monkeypatch):
+    """The engine's one kernel for rotation and append against the two that it had: the same logits and caches bit for bit."""
+    from llmctl_b200.comms import mesh
+    from llmctl_b200.models.config import ModelConfig
+    from llmctl_b200.ops import functional
+    from llmctl_b200.serve.engine import InferenceEngine
+    cfg = ModelConfig(name="append-test", layers=2, hidden=256, ffn=704, heads=4, vocab_size=4096, max_position_embeddings=512)
+    prompts = [list(range(3, 3 + n)) for n in (17, 40)]
+
+    def run(old):
+        mesh.reset_state()
+        eng = InferenceEngine(cfg, max_batch_size=2, max_batch_tokens=1024, num_kv_blocks=64, cuda_graphs=False)
+        if old:
+            def append(i, qkv, positions, slots):
+                cos, sin = eng.model.rope_tables(eng.device)
+                qkv = functional.rope_packed(qkv, cos, sin, 8, 64, 512, positions)
+                sops.kv_append(qkv, eng.k_caches[i], eng.v_caches[i], slots, 4, 64)
+                return qkv
+            eng._append = append
+        return eng.generate(prompts, max_tokens=9, temperature=0.0), eng.k_caches + eng.v_caches
+    (a, ca), (b, cb) = run(True), run(False)
+    assert a == b and all(torch.equal(x, y) for x, y in zip(ca, cb))

@@ -59,3 +59,91 @@ def test_refusals(ops):
     for bad in ((x, tokens.int(), 0), (x, tokens[:1], 0), (x, tokens[:, None], 0), (x, tokens, 10), (x, tokens, -1), (_logits(2, 100), tokens, 65), (x.long(), tokens, 0)):
         with pytest.raises(ValueError):
             ops.token_logprobs(*bad)
+
+
+def _engine(**kw):
+    from llmctl_b200.comms import mesh
+    from llmctl_b200.serve.engine import InferenceEngine
+    mesh.reset_state()
+    return InferenceEngine("gpt-tiny", device="cpu", kv_block_size=4, num_kv_blocks=64, **kw)
+
+
+def test_engine_gives_log_probabilities_with_its_tokens():
+    eng = _engine(max_batch_size=3, max_batch_tokens=256)
+    prompts = [[5, 6, 7], [9, 8], [3]]
+    seqs = [eng.add_request(p, 4, temperature=t, logprobs=n) for p, t, n in zip(prompts, (0.0, 1.3, 0.0), (3, 0, None))]
+    while eng.has_work():
+        eng.step()
+    assert seqs[2].token_logprobs == [] and len(seqs[2].generated) == 4
+    for s, n in zip(seqs[:2], (3, 0)):
+        assert [r["token"] for r in s.token_logprobs] == s.generated
+        for i, r in enumerate(s.token_logprobs):
+            lp = torch.log_softmax(eng.model(torch.tensor([s.prompt_ids + s.generated[:i]]))[-1, :512].double(), -1)
+            best = torch.topk(lp, 3)
+            assert abs(r["logprob"] - float(lp[r["token"]])) < 1e-3 and abs(r["entropy"] + float((lp.exp() * lp).sum())) < 1e-3
+            assert len(r["top"]) == n
+            if n:
+                assert [t for t, _ in r["top"]] == best.indices.tolist() and r["top"][0][0] == r["token"]
+                assert all(abs(v - float(w)) < 1e-3 for (_, v), w in zip(r["top"], best.values))
+    for bad in (-1, 65):
+        with pytest.raises(ValueError, match="logprobs"):
+            eng.add_request([5], 4, logprobs=bad)
+
+
+def test_http_log_probabilities():
+    import json
+
+    from fastapi.testclient import TestClient
+    from llmctl_b200.serve.server import InferenceServer
+    srv = InferenceServer("gpt-tiny", engine=_engine(max_batch_size=4, max_batch_tokens=512))
+    srv.start_background()
+    try:
+        c = TestClient(srv.app)
+        ask = {"prompt": "hello", "max_tokens": 5, "temperature": 0.0}
+        plain, body = c.post("/v1/completions", json=ask).json(), c.post("/v1/completions", json={**ask, "logprobs": 2}).json()
+        assert "logprobs" not in plain and body["text"] == plain["text"]
+        said = body["logprobs"]
+        assert set(said) == {"tokens", "token_ids", "token_logprobs", "entropy", "top_logprobs"} and len({len(v) for v in said.values()}) == 1
+        assert all(v <= 0 for v in said["token_logprobs"]) and all(len(t) == 2 and t[0]["token_id"] == i for t, i in zip(said["top_logprobs"], said["token_ids"]))
+        with c.stream("POST", "/v1/completions", json={**ask, "logprobs": 0, "stream": True}) as s:
+            events = [json.loads(x[6:]) for x in s.iter_lines() if x.startswith("data: {")]
+        assert [e["logprobs"]["token_logprobs"] for e in events if "text" in e][:len(said["token_ids"])] == said["token_logprobs"]
+        assert c.post("/v1/completions", json={**ask, "logprobs": 21}).status_code == 422
+    finally:
+        srv.shutdown()
+
+
+def test_lockstep_engine_passes_log_probabilities_on():
+    """The leader's queue carries the number of alternatives to the engine of every rank."""
+    import threading
+
+    from llmctl_b200.serve import lockstep
+    eng = _engine(max_batch_size=2, max_batch_tokens=256)
+    lock = lockstep.LockstepEngine.__new__(lockstep.LockstepEngine)
+    lock.engine, lock._lock, lock._pending, lock.on_pending = eng, threading.Lock(), [], None
+    got = []
+    t = threading.Thread(target=lambda: got.append(lock.add_request([5, 6], 3, 0.0, logprobs=1)))
+    t.start()
+    while not lock._pending:
+        pass
+    (args, holder), = lock._pending
+    lock._apply({"adds": [args], "cancels": []}, [holder])
+    t.join(10)
+    assert got[0].logprobs == 1 and got[0].max_tokens == 3 and got[0].temperature == 0.0
+
+
+def test_eval_reads_likelihood_and_best_guess_from_one_call(tmp_path):
+    import math
+
+    from llmctl_b200.cli.commands.eval import evaluate_checkpoint
+    from llmctl_b200.io.dataset import build_dataset
+    from llmctl_b200.serve.engine import load_model_for_inference
+    res = evaluate_checkpoint("gpt-tiny", ["perplexity", "accuracy"], batches=2, batch_size=2, seq_len=32, device="cpu")
+    model, cfg, _, _ = load_model_for_inference("gpt-tiny", "cpu")
+    ds = build_dataset(None, cfg.vocab_size, 32, seed=4242)
+    rows = torch.stack([torch.from_numpy(ds[i]) for i in range(4)])
+    logits = model(rows[:, :-1].contiguous()).double()[:, :cfg.vocab_size]
+    lp = torch.log_softmax(logits, -1).gather(1, rows[:, 1:].reshape(-1, 1))
+    task = res["tasks"]["perplexity"]
+    assert task["tokens"] == lp.numel() and abs(task["loss"] + float(lp.mean())) < 1e-5 and abs(task["perplexity"] - math.exp(-float(lp.mean()))) < 1e-2
+    assert res["tasks"]["accuracy"]["next_token_accuracy"] == float((logits.argmax(-1) == rows[:, 1:].reshape(-1)).double().mean())

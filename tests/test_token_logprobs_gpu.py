@@ -208,3 +208,23 @@ def test_saved_logits_that_a_hook_changes_are_refused(ops):
         out = ops.token_logprobs(x, tokens, 2)
         dx, = torch.autograd.grad(out.logprobs.sum(), x)
     assert torch.equal(dx, torch.autograd.grad(ops.token_logprobs(x, tokens, 2).logprobs.sum(), x)[0])
+
+
+def test_engine_log_probabilities(ops):
+    from llmctl_b200.comms import mesh
+    from llmctl_b200.models.config import ModelConfig
+    from llmctl_b200.serve.engine import InferenceEngine
+    mesh.reset_state()
+    cfg = ModelConfig(name="logprob-test", layers=2, hidden=256, ffn=704, heads=4, vocab_size=4001, max_position_embeddings=256)
+    eng = InferenceEngine(cfg, max_batch_size=4, max_batch_tokens=1024, num_kv_blocks=64)
+    seqs = [eng.add_request(list(range(3, 3 + n)), 6, temperature=0.0, logprobs=4) for n in (5, 33)]
+    while eng.has_work():
+        eng.step()
+    for s in seqs:
+        assert [r["token"] for r in s.token_logprobs] == s.generated
+        for i, r in enumerate(s.token_logprobs):
+            logits = eng.model(torch.tensor([s.prompt_ids + s.generated[:i]], device="cuda"))[-1, :4001].double()
+            lp = torch.log_softmax(logits, -1)
+            # the decoding step's logits are rounded to bf16 and come by other kernels than the prompt's
+            assert abs(r["logprob"] - float(lp[r["token"]])) < 0.1 and len(r["top"]) == 4 and r["top"][0] == (r["token"], r["logprob"])
+            assert abs(r["entropy"] + float((lp.exp() * lp).sum())) < 0.05
