@@ -94,18 +94,21 @@ rope_kv_append_kernel(RopeRows r, uint32_t total, FastDiv per_token, FastDiv per
 }
 
 // ---------------------------------------------------------------------------------------------
-// 8 bits.  A block of the cache is written by one CTA part alone, which finds all tokens of the call that go to it, wherever they stand and however
-// often a slot is named (the last token of a slot is the one that is kept): no atomics on results, and the same bytes every time.
+// 8 bits.  A block of the cache is written by one CTA alone (for its share of the heads), which finds all tokens of the call that go to it, wherever they
+// stand and however often a slot is named (the last token of a slot is the one that is kept): no atomics on results, and the same bytes every
+// time.
 //
-// Grid: (windows of `window` tokens, parts of the heads).  A CTA rotates q of its window; of the tokens in it, one that is the first of the call in
-// its block takes the block: a scan over the slots tells, and it is left out where the token before goes to the same block (in a prompt,
-// 15 of 16).  A warp then writes a head's block: the rows into registers (or twice, where a block is longer than they hold), the largest
-// number, the scale, the codes.
+// CTAs 0 .. windows * parts - 1: of the tokens of a window, one that is the first of the call in its block takes the block.  A scan over the slots tells,
+// which is left out where the token before goes to the same block (in a prompt, 15 of 16).  A warp then writes a head's block: the rows as they
+// are into registers (again, where a block is longer than they hold), the largest rotated number, the scale, the codes.  The others rotate q, four
+// units to a thread.
 // ---------------------------------------------------------------------------------------------
 namespace append8 {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kRows = 4;                     // rows that a lane holds of its place in them
+constexpr int kUnits = 4;                    // of q, to a thread
 constexpr int kMaxBlock = 4096;
+constexpr int kParts = 1000;                 // CTAs of a call that write blocks, or as many as have work
 
 // |x| as an integer that grows with it, 0 for what is no finite number
 __device__ __forceinline__ uint32_t magnitude(float x) {
@@ -120,11 +123,12 @@ __device__ __forceinline__ float scale_for(uint32_t most) {
 }
 }  // namespace append8
 
-__global__ void __launch_bounds__(append8::kThreads)
+__global__ void __launch_bounds__(append8::kThreads, 3)
 rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
-                          float* __restrict__ k_scale, float* __restrict__ v_scale, int blocks, int block_size, int window) {
+                          float* __restrict__ k_scale, float* __restrict__ v_scale, int blocks, int block_size, int window, int windows, int parts,
+                          uint32_t q_units, FastDiv per_token, FastDiv per_head) {
   using namespace append8;
-  extern __shared__ int row_token[];          // [block_size]: the token that a row of the block at hand is written from, or -1
+  extern __shared__ int2 row_of[];            // [block_size]: the token that a row of the block at hand is written from, or -1, and its row in the tables
   __shared__ int first_token, twice;
   __nv_bfloat16* qkv = r.qkv;
   const float *cos_t = r.cos_t, *sin_t = r.sin_t;
@@ -132,118 +136,154 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
   wait_for_previous(qkv, cos_t, sin_t, positions, slots, k_cache, v_cache, k_scale, v_scale);
   release_dependents();
   const int half = r.head_dim >> 1, per_row = r.head_dim >> 4;      // lanes to a row: eight pairs, or 16 neighbours, each
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int parts = gridDim.y, part = blockIdx.y;
-  const int t0 = blockIdx.x * window, t1 = min(r.tokens, t0 + window);
-  const long long rows = static_cast<long long>(blocks) * block_size;
+  const int work = static_cast<int>(blockIdx.x);
 
-  auto rotate_in_place = [&](int tok, int head, int at) {
-    __nv_bfloat16* p = qkv + tok * r.row_stride + static_cast<long long>(head) * r.head_dim + at * 8;
-    float a[8], b[8];
-    unpack8(load8(p), a);
-    unpack8(load8(p + half), b);
-    const long long row = table_row(r, positions, tok) + at * 8;
-    rotate8(a, b, cos_t + row, sin_t + row);
-    store8(p, pack8(a));
-    store8(p + half, pack8(b));
-  };
+  if (work >= windows * parts) {              // q
+    const uint32_t first = static_cast<uint32_t>(work - windows * parts) * (kThreads * kUnits) + threadIdx.x;
+    bf16x8 x[kUnits], y[kUnits];
+    __nv_bfloat16* at[kUnits];
+    long long row[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      const uint32_t idx = first + i * kThreads;
+      at[i] = nullptr;
+      if (idx < q_units) {
+        uint32_t unit, pair;
+        const int tok = static_cast<int>(per_token.divide(idx, unit)), head = static_cast<int>(per_head.divide(unit, pair));
+        at[i] = qkv + tok * r.row_stride + head * r.head_dim + pair * 8;
+        row[i] = table_row(r, positions, tok) + pair * 8;
+        x[i] = load8(at[i]);
+        y[i] = load8(at[i] + half);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i)
+      if (at[i] != nullptr) {
+        float a[8], b[8];
+        unpack8(x[i], a);
+        unpack8(y[i], b);
+        rotate8(a, b, cos_t + row[i], sin_t + row[i]);
+        store8(at[i], pack8(a));
+        store8(at[i] + half, pack8(b));
+      }
+    return;
+  }
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = work / windows, t0 = (work - part * windows) * window, t1 = min(r.tokens, t0 + window);
+  const long long rows = static_cast<long long>(blocks) * block_size;
   // heads of keys that no block's writer rotates: all of a token's, this part's share
   auto rotate_keys = [&](int tok) {
     for (int i = threadIdx.x; i < r.kv_heads * per_row; i += kThreads)
-      if ((i / per_row) % parts == part) rotate_in_place(tok, r.heads + i / per_row, i % per_row);
+      if ((i / per_row) % parts == part) {
+        const int at = i % per_row;
+        __nv_bfloat16* p = qkv + tok * r.row_stride + static_cast<long long>(r.heads + i / per_row) * r.head_dim + at * 8;
+        float a[8], b[8];
+        unpack8(load8(p), a);
+        unpack8(load8(p + half), b);
+        const long long row = table_row(r, positions, tok) + at * 8;
+        rotate8(a, b, cos_t + row, sin_t + row);
+        store8(p, pack8(a));
+        store8(p + half, pack8(b));
+      }
   };
 
-  {
-    const int mine = (r.heads - part + parts - 1) / parts;          // query heads part, part + parts, ...
-    for (int i = threadIdx.x; i < (t1 - t0) * mine * per_row; i += kThreads) {
-      const int unit = i / per_row;
-      rotate_in_place(t0 + unit / mine, part + unit % mine * parts, i % per_row);
-    }
-  }
-
   const int sub = lane / per_row, at = lane - sub * per_row, step = 32 / per_row;      // rows of a warp at a time; lanes past them idle
-  for (int t = t0; t < t1; ++t) {
-    const long long slot = slots[t];
-    if (slot < 0 || slot >= rows) {           // a padded token
-      rotate_keys(t);
-      continue;
-    }
-    const int block = static_cast<int>(slot / block_size);
+  // Of the window's tokens (16 at most, a lane each): those without a row, and those that may be the first in their block.
+  long long slot = -1, before = -1;
+  if (t0 + lane < t1) {
+    slot = slots[t0 + lane];
+    if (t0 + lane > 0) before = slots[t0 + lane - 1];
+  }
+  const bool padded = slot < 0 || slot >= rows, behind = !padded && before >= 0 && before < rows && before / block_size == slot / block_size;
+  const unsigned window_mask = t1 - t0 >= 32 ? ~0u : (1u << (t1 - t0)) - 1u;
+  for (unsigned left = __ballot_sync(0xffffffffu, padded) & window_mask; left != 0u; left &= left - 1u) rotate_keys(t0 + __ffs(left) - 1);
+  for (unsigned left = __ballot_sync(0xffffffffu, !padded && !behind) & window_mask; left != 0u; left &= left - 1u) {
+    const int t = t0 + __ffs(left) - 1, block = static_cast<int>(__shfl_sync(0xffffffffu, slot, t - t0) / block_size);
     const long long lo = static_cast<long long>(block) * block_size, hi = lo + block_size;
-    if (t > 0) {
-      const long long before = slots[t - 1];
-      if (before >= lo && before < hi) continue;                   // that token or one before it takes the block
-    }
     __syncthreads();                          // the rows of the block before have been read
-    for (int i = threadIdx.x; i < block_size; i += kThreads) row_token[i] = -1;
+    for (int i = threadIdx.x; i < block_size; i += kThreads) row_of[i].x = -1;
     if (threadIdx.x == 0) {
       first_token = t;
       twice = 0;
     }
     __syncthreads();
+#pragma unroll 4
     for (int i = threadIdx.x; i < r.tokens; i += kThreads) {
       const long long s = slots[i];
       if (s >= lo && s < hi) {
         if (i < t) atomicMin(&first_token, i);
-        if (atomicMax(&row_token[s - lo], i) >= 0) twice = 1;
+        if (atomicMax(&row_of[s - lo].x, i) >= 0) twice = 1;
       }
     }
     __syncthreads();
     if (first_token != t) continue;
+    for (int i = threadIdx.x; i < block_size; i += kThreads)
+      if (row_of[i].x >= 0) row_of[i].y = min(max(positions[row_of[i].x], 0), r.table_rows - 1);
     if (twice)
       for (int i = 0; i < r.tokens; ++i) {
         const long long s = slots[i];
-        if (s >= lo && s < hi && row_token[s - lo] != i) rotate_keys(i);
+        if (s >= lo && s < hi && row_of[s - lo].x != i) rotate_keys(i);
       }
-    const bool begun = row_token[0] >= 0;
+    __syncthreads();
+    const bool begun = row_of[0].x >= 0;
 
     for (int task = part + warp * parts; task < 2 * r.kv_heads; task += kWarps * parts) {
       const bool key = task < r.kv_heads;
       const int head = key ? task : task - r.kv_heads;
       uint8_t* codes = (key ? k_cache : v_cache) + (static_cast<long long>(block) * r.kv_heads + head) * block_size * r.head_dim;
       float* scale_at = (key ? k_scale : v_scale) + static_cast<long long>(block) * r.kv_heads + head;
-      const float old = begun ? 0.f : fmaxf(*scale_at, 0.f);
       __nv_bfloat16* src = qkv + static_cast<long long>(r.heads + task) * r.head_dim + (key ? at * 8 : at * 16);
       const int second = key ? half : 8;
-      float a[kRows][8], b[kRows][8];
+      bf16x8 x[kRows], y[kRows];              // as they stand: rotated again for the codes, which costs less than the registers
+      auto row_at = [&](int row0, int i) {
+        const int row = row0 + i * step + sub;
+        return sub < step && row < block_size ? row : -1;
+      };
       auto load = [&](int row0) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-          const int row = row0 + i * step + sub;
-          const int tok = sub < step && row < block_size ? row_token[row] : -1;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) a[i][j] = b[i][j] = 0.f;
+          const int row = row_at(row0, i), tok = row >= 0 ? row_of[row].x : -1;
           if (tok >= 0) {
-            unpack8(load8(src + tok * r.row_stride), a[i]);
-            unpack8(load8(src + tok * r.row_stride + second), b[i]);
-          }
-        }
-        if (key) {
-#pragma unroll
-          for (int i = 0; i < kRows; ++i) {
-            const int row = row0 + i * step + sub;
-            const int tok = sub < step && row < block_size ? row_token[row] : -1;
-            if (tok >= 0) {
-              const long long row_at = table_row(r, positions, tok) + at * 8;
-              rotate8(a[i], b[i], cos_t + row_at, sin_t + row_at);
-            }
+            x[i] = load8(src + tok * r.row_stride);
+            y[i] = load8(src + tok * r.row_stride + second);
           }
         }
       };
+      // f(row, its token, the numbers in 32 bits) for each row that is written
+      auto each = [&](int row0, auto&& f) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const int row = row_at(row0, i);
+          if (row < 0) continue;
+          const int2 of = row_of[row];
+          if (of.x < 0) continue;
+          float a[8], b[8];
+          unpack8(x[i], a);
+          unpack8(y[i], b);
+          if (key) {
+            const long long table = static_cast<long long>(of.y) * half + at * 8;
+            rotate8(a, b, cos_t + table, sin_t + table);
+          }
+          f(row, of.x, a, b);
+        }
+      };
+      const bool once = block_size <= kRows * step;
+      const float old = begun ? 0.f : fmaxf(*scale_at, 0.f);
       uint32_t most = 0u;
       for (int row0 = 0; row0 < block_size; row0 += kRows * step) {
         load(row0);
+        each(row0, [&](int, int, const float (&a)[8], const float (&b)[8]) {
 #pragma unroll
-        for (int i = 0; i < kRows; ++i)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) most = max(most, max(magnitude(a[i][j]), magnitude(b[i][j])));
+          for (int j = 0; j < 8; ++j) most = max(most, max(magnitude(a[j]), magnitude(b[j])));
+        });
       }
       most = __reduce_max_sync(0xffffffffu, most);
       const float need = scale_for(most), scale = fmaxf(need, old);
       if (!begun && scale > old) {            // what stands in the block, in the new scale
         const float factor = old / scale;
         for (int i = lane * 8; i < block_size * r.head_dim; i += 256) {
-          if (row_token[i / r.head_dim] >= 0) continue;
+          if (row_of[i / r.head_dim].x >= 0) continue;
           uint2 c = *reinterpret_cast<const uint2*>(codes + i);
           float f[8];
           unpack_e4m3x8(c, f);
@@ -254,31 +294,27 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
       }
       const float inv = scale > 0.f ? 1.f / scale : 0.f;
       for (int row0 = 0; row0 < block_size; row0 += kRows * step) {
-        if (block_size > kRows * step) load(row0);
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          const int row = row0 + i * step + sub;
-          const int tok = sub < step && row < block_size ? row_token[row] : -1;
-          if (tok < 0) continue;
+        if (!once) load(row0);
+        each(row0, [&](int row, int tok, float (&a)[8], float (&b)[8]) {
           if (key) {
             __nv_bfloat16* dst = src + tok * r.row_stride;
-            store8(dst, pack8(a[i]));
-            store8(dst + half, pack8(b[i]));
+            store8(dst, pack8(a));
+            store8(dst + half, pack8(b));
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {       // (what is not finite has no code but NaN)
-            a[i][j] = isfinite(a[i][j]) ? a[i][j] * inv : NAN;
-            b[i][j] = isfinite(b[i][j]) ? b[i][j] * inv : NAN;
+            a[j] = isfinite(a[j]) ? a[j] * inv : NAN;
+            b[j] = isfinite(b[j]) ? b[j] * inv : NAN;
           }
           uint8_t* dst = codes + row * r.head_dim + (key ? at * 8 : at * 16);
-          const uint2 x = pack_e4m3x8(a[i]), y = pack_e4m3x8(b[i]);
+          const uint2 c = pack_e4m3x8(a), d = pack_e4m3x8(b);
           if (key) {
-            *reinterpret_cast<uint2*>(dst) = x;
-            *reinterpret_cast<uint2*>(dst + half) = y;
+            *reinterpret_cast<uint2*>(dst) = c;
+            *reinterpret_cast<uint2*>(dst + half) = d;
           } else {
-            *reinterpret_cast<uint4*>(dst) = make_uint4(x.x, x.y, y.x, y.y);
+            *reinterpret_cast<uint4*>(dst) = make_uint4(c.x, c.y, d.x, d.y);
           }
-        }
+        });
       }
       if (lane == 0) *scale_at = scale;
       __syncwarp();
@@ -327,12 +363,14 @@ LLMCTL_API int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int to
   const RopeRows r{static_cast<__nv_bfloat16*>(qkv), row_stride, tokens, heads, kv_heads, head_dim, cos_t, sin_t, table_rows, positions};
   LLMCTL_REQUIRE(rope_rows_ok(r) && head_dim <= 512 && blocks >= 0 && block_size >= 1 && block_size <= kMaxBlock && aligned16(k_cache, v_cache));
   if (tokens == 0) return 0;
-  const int window = tokens > 256 ? 16 : 1;
-  const int windows = (tokens + window - 1) / window;
-  int parts = (4 * kNumSMs + windows - 1) / windows;
-  const int most = (2 * kv_heads + kWarps - 1) / kWarps;
+  const int window = tokens > 256 ? 16 : 1, windows = (tokens + window - 1) / window, most = (2 * kv_heads + kWarps - 1) / kWarps;
+  int parts = (kParts + windows - 1) / windows;
   if (parts > most) parts = most;
-  LLMCTL_CHECK(launch_dependent(rope_kv_append_fp8_kernel, dim3(windows, parts), kThreads, block_size * 4, (cudaStream_t)stream, r, slots,
-                                (uint8_t*)k_cache, (uint8_t*)v_cache, k_scale, v_scale, blocks, block_size, window));
+  const long long per_token = static_cast<long long>(heads) * (head_dim / 16), units = per_token * tokens;
+  LLMCTL_REQUIRE(units < (1LL << 30));
+  const int q_ctas = static_cast<int>((units + kThreads * kUnits - 1) / (kThreads * kUnits));
+  LLMCTL_CHECK(launch_dependent(rope_kv_append_fp8_kernel, windows * parts + q_ctas, kThreads, block_size * sizeof(int2), (cudaStream_t)stream, r, slots,
+                                (uint8_t*)k_cache, (uint8_t*)v_cache, k_scale, v_scale, blocks, block_size, window, windows, parts,
+                                static_cast<uint32_t>(units), FastDiv(static_cast<uint32_t>(per_token)), FastDiv(head_dim / 16)));
   LLMCTL_RETURN_LAST();
 }

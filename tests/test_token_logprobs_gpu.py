@@ -31,14 +31,14 @@ def _want(x, tokens, top):
 
 
 def _slack(lp, V):
-    """Errors of 32 bits: a thread adds up to V / 512 + 40 terms one by one (2^-24 each), each exponential is off by its argument's rounding and its
+    """Errors of 32 bits: a thread adds up to V / 256 + 40 terms one by one (2^-24 each), each exponential is off by its argument's rounding and its
     own (|x - m| 2^-23 + 2^-22 of it, of which x - m weighted by the exponential is at most 1) -> relative error of the sum, which is the logarithm's."""
-    return (V / 512 + 40) * 2.0 ** -24 + 2.0 ** -21
+    return (V / 256 + 40) * 2.0 ** -24 + 2.0 ** -21
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,V,top,shift,pad", [(1, 1, 1, 0, 0), (3, 7, 7, 1, 0), (5, 50, 20, 0, 14), (2, 511, 64, 3, 0), (33, 1000, 5, 0, 24), (4, 4097, 64, 1, 2), (7, 32000, 20, 0, 0),
-                                                  (300, 32001, 1, 0, 127), (2, 50257, 3, 0, 0), (2, 200000, 20, 2, 1), (9, 777, 0, 5, 3)])
+                                                  (300, 32001, 1, 0, 127), (2, 50257, 3, 0, 0), (2, 200000, 20, 2, 1), (9, 777, 0, 5, 3), (40, 128000, 64, 0, 0), (150, 8200, 5, 1, 1), (1200, 5000, 20, 0, 0), (1, 131072, 1, 0, 0)])
 def test_forward(ops, rows, V, top, shift, pad, dtype):
     x, tokens = _logits(rows, V, dtype, shift=shift, pad=pad), _tokens(rows, V)
     kept = x.clone()
@@ -69,17 +69,20 @@ def test_ties_and_order(ops, V, top):
 
 
 @pytest.mark.parametrize("dtype,unit", [(torch.bfloat16, 8), (torch.float32, 4)])
-@pytest.mark.parametrize("many", [400, 3000])
-def test_many_candidates(ops, dtype, unit, many):
-    """The units of a few threads (every 512th) hold all of the row's larger numbers: more than the list of candidates has room for."""
-    top, V = 24, 512 * unit * 40
-    x = torch.full((2, V), -5.0, device="cuda")
-    place = (torch.arange(40, device="cuda")[:, None, None] * 512 + torch.arange(24, device="cuda")[None, :, None] * 8) * unit + torch.arange(unit, device="cuda")
-    place = place.reshape(-1)[torch.randperm(40 * 24 * unit, device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))][:many]
+@pytest.mark.parametrize("rows", [2, 700])
+@pytest.mark.parametrize("many", [40, 300])
+def test_many_candidates(ops, dtype, unit, rows, many):
+    """The units of four neighbouring threads hold all of the row's larger numbers: up to 9600, more than the list of candidates has room for."""
+    top, V = 24, 256 * unit * many
+    x = torch.full((1, V), -5.0, device="cuda")
+    place = (torch.arange(many, device="cuda")[:, None, None] * 256 + torch.arange(4, device="cuda")[None, :, None]) * unit + torch.arange(unit, device="cuda")
+    place = place.reshape(-1)[torch.randperm(place.numel(), device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))]
     x[:, place] = (torch.arange(place.numel(), device="cuda") % 200).float() * 0.25
     x = x.to(dtype)
-    tokens = place[:2].clone()
-    assert torch.equal(ops.token_logprobs(x, tokens, top).top_ids, _want(x, tokens, top)[3])
+    tokens = place[:1].clone()
+    want = _want(x, tokens, top)
+    got = ops.token_logprobs(x.expand(rows, V), tokens.expand(rows), top)
+    assert torch.equal(got.top_ids, want[3].expand(rows, top)) and torch.equal(got.logprobs, got.logprobs[:1].expand(rows))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -128,7 +131,7 @@ def _gradient(x, tokens, top, order, g, gh, gt):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("rows,V,top,shift,pad", [(1, 5, 5, 0, 0), (3, 777, 0, 1, 0), (4, 4000, 3, 0, 96), (130, 32000, 0, 0, 0), (3, 50257, 20, 3, 0)])
+@pytest.mark.parametrize("rows,V,top,shift,pad", [(1, 5, 5, 0, 0), (3, 777, 0, 1, 0), (4, 4000, 3, 0, 96), (130, 32000, 0, 0, 0), (3, 50257, 20, 3, 0), (700, 3000, 2, 0, 8)])
 def test_backward(ops, rows, V, top, shift, pad, dtype):
     x, tokens = _logits(rows, V, dtype, shift=shift, pad=pad), _tokens(rows, V)
     x[:, V // 2] = float("-inf")
