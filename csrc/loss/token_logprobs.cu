@@ -39,6 +39,9 @@ __device__ __forceinline__ void unpack(const uint4& raw, float (&f)[8]) { unpack
 __device__ __forceinline__ void unpack(const uint4& raw, float (&f)[4]) {
   f[0] = __uint_as_float(raw.x), f[1] = __uint_as_float(raw.y), f[2] = __uint_as_float(raw.z), f[3] = __uint_as_float(raw.w);
 }
+// A unit of -inf
+__device__ __forceinline__ uint4 nothing(const __nv_bfloat16*) { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+__device__ __forceinline__ uint4 nothing(const float*) { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
 // The same, but no number below kLow; NaN stays.
 __device__ __forceinline__ void unpack_clamped(const uint4& raw, float (&f)[8]) {
   bf16x8 v = *reinterpret_cast<const bf16x8*>(&raw);
@@ -184,14 +187,18 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long lon
   if (tid == 0 && part == 0 && given) x_token = as_f32(r.p[token]);
   auto unit = [&](int i) { return r.p + r.head + static_cast<long long>(i) * U; };
 
-  // Numbers are met in the order of their indices: before the first 16-byte boundary, units, the rest.
+  // Numbers are met in the order of their indices: before the first 16-byte boundary, units, the rest.  The reference moves once in kAhead units (some lane of a
+  // warp has a new maximum in nearly each of a row's first, and the others wait: 4096 x 32000 76 us with a look at every unit, XX so); the unit of the
+  // maximum is kept, its place in it is looked up at the end.
   Sums a;
-  int best = tid < head ? tid : lo + tid < hi ? r.head + (lo + tid) * U : tail + tid;      // where the maximum stands; >= V: no numbers
+  int best = tid < head ? tid : -1, best_unit = tid >= head && lo + tid < hi ? lo + tid : -1;      // where the maximum stands, one of the two
+  if (best < 0 && best_unit < 0 && tail + tid < V) best = tail + tid;
   auto one = [&](int at) {
     const float x = as_f32(r.p[at]);
     if (x > a.m) {
       a.move_to(x);
       best = at;
+      best_unit = -1;
     }
     a.add(x);
   };
@@ -199,24 +206,26 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long lon
   for (int i0 = lo + tid; i0 < hi; i0 += kAhead * kThreads) {
     uint4 raw[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (i0 + k * kThreads < hi) raw[k] = load_raw(unit(i0 + k * kThreads));
+    for (int k = 0; k < kAhead; ++k) raw[k] = i0 + k * kThreads < hi ? load_raw(unit(i0 + k * kThreads)) : nothing(r.p);
+    float of[kAhead], most = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int i = i0 + k * kThreads;
-      if (i >= hi) break;
-      const float most = largest(raw[k], r.p);
-      float x[U];
-      if (most > a.m) {
-        a.move_to(most);
-        unpack(raw[k], x);
-        int j = 0;
+      of[k] = largest(raw[k], r.p);
+      most = fmaxf(most, of[k]);
+    }
+    if (most > a.m) {
+      a.move_to(most);
+      int k = 0;
 #pragma unroll
-        for (int e = U - 1; e >= 0; --e)
-          if (x[e] == most) j = e;
-        best = r.head + i * U + j;
-      }
-      if (a.m > kUsual && a.m < INFINITY) {
+      for (int e = kAhead - 1; e >= 0; --e)
+        if (of[e] == most) k = e;
+      best_unit = i0 + k * kThreads;
+    }
+    const bool usual = a.m > kUsual && a.m < INFINITY;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      float x[U];
+      if (usual) {
         unpack_clamped(raw[k], x);
         a.add_usual(x);
       } else {
@@ -227,7 +236,17 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long lon
     }
   }
   if (tail + tid < V) one(tail + tid);
-  const unsigned long long key = best < V ? make_key(a.m, best) : 0ull;
+  unsigned long long key = 0ull;              // of this thread's maximum
+  if (top > 0 && best_unit >= 0) {
+    float x[U];
+    unpack(load_raw(unit(best_unit)), x);
+    int j = 0;
+#pragma unroll
+    for (int e = U - 1; e >= 0; --e)
+      if (x[e] == a.m) j = e;
+    best = r.head + best_unit * U + j;
+  }
+  if (top > 0 && best >= 0) key = make_key(a.m, best);
 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)

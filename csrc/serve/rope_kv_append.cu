@@ -17,9 +17,20 @@
 #include "../common/dependent.cuh"
 #include "../common/fast_div.h"
 #include "../common/fp8.cuh"
+#include "../common/ptx.cuh"
 #include "../common/util.cuh"
 
 namespace llmctl {
+
+// (a0, a1) = (a0, a1) * (b0, b1) + (c0, c1)
+__device__ __forceinline__ void fma2vv(float& a0, float& a1, float b0, float b1, float c0, float c1) {
+  asm("{\n\t.reg .b64 ra, rb, rc;\n\t"
+      "mov.b64 ra, {%0, %1};\n\tmov.b64 rb, {%2, %3};\n\tmov.b64 rc, {%4, %5};\n\t"
+      "fma.rn.f32x2 ra, ra, rb, rc;\n\t"
+      "mov.b64 {%0, %1}, ra;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
 
 // Eight pairs (a: from the first half, b: from the second) of one row, rotated.
 __device__ __forceinline__ void rotate8(float (&a)[8], float (&b)[8], const float* __restrict__ cos_row, const float* __restrict__ sin_row) {
@@ -29,10 +40,12 @@ __device__ __forceinline__ void rotate8(float (&a)[8], float (&b)[8], const floa
   *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sin_row);
   *reinterpret_cast<float4*>(s + 4) = *reinterpret_cast<const float4*>(sin_row + 4);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float x = a[j], y = b[j];
-    a[j] = __fmaf_rn(x, c[j], -__fmul_rn(y, s[j]));
-    b[j] = __fmaf_rn(y, c[j], __fmul_rn(x, s[j]));
+  for (int j = 0; j < 8; j += 2) {            // a c - b s and b c + a s, the products with s rounded by themselves
+    float t0, t1, u0, u1;
+    ptx::mul2v(t0, t1, b[j], b[j + 1], s[j], s[j + 1]);
+    ptx::mul2v(u0, u1, a[j], a[j + 1], s[j], s[j + 1]);
+    fma2vv(a[j], a[j + 1], c[j], c[j + 1], -t0, -t1);
+    fma2vv(b[j], b[j + 1], c[j], c[j + 1], u0, u1);
   }
 }
 
@@ -110,10 +123,15 @@ constexpr int kUnits = 4;                    // of q, to a thread
 constexpr int kMaxBlock = 4096;
 constexpr int kParts = 1000;                 // CTAs of a call that write blocks, or as many as have work
 
-// |x| as an integer that grows with it, 0 for what is no finite number
-__device__ __forceinline__ uint32_t magnitude(float x) {
-  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
-  return u < 0x7f800000u ? u : 0u;
+// |x| as an integer that grows with it: kInfinite and more for what is no finite number
+constexpr uint32_t kInfinite = 0x7f800000u;
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t finite_magnitude(float x) { return magnitude(x) < kInfinite ? magnitude(x) : 0u; }
+// The largest |x| of eight, NaN if there is one.
+__device__ __forceinline__ float most_of(const bf16x8& v) {
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(v.v[0]), __habs2(v.v[1])), __hmax2_nan(__habs2(v.v[2]), __habs2(v.v[3])));
+  const float2 f = __bfloat1622float2(m);
+  return f.x != f.x ? f.x : f.y != f.y ? f.y : fmaxf(f.x, f.y);
 }
 // The smallest power of two (of 2^-126 and up) under which a number of this magnitude is at most 448; 0 for zero.
 __device__ __forceinline__ float scale_for(uint32_t most) {
@@ -273,12 +291,31 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
       uint32_t most = 0u;
       for (int row0 = 0; row0 < block_size; row0 += kRows * step) {
         load(row0);
-        each(row0, [&](int, int, const float (&a)[8], const float (&b)[8]) {
+        if (key)
+          each(row0, [&](int, int, const float (&a)[8], const float (&b)[8]) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) most = max(most, max(magnitude(a[j]), magnitude(b[j])));
-        });
+            for (int j = 0; j < 8; ++j) most = max(most, max(magnitude(a[j]), magnitude(b[j])));
+          });
+        else
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) {
+            const int row = row_at(row0, i);
+            if (row >= 0 && row_of[row].x >= 0) most = max(most, max(magnitude(most_of(x[i])), magnitude(most_of(y[i]))));
+          }
       }
       most = __reduce_max_sync(0xffffffffu, most);
+      const bool finite = most < kInfinite;
+      if (!finite) {                          // rare: once more without them
+        most = 0u;
+        for (int row0 = 0; row0 < block_size; row0 += kRows * step) {
+          if (!once) load(row0);
+          each(row0, [&](int, int, const float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = max(most, max(finite_magnitude(a[j]), finite_magnitude(b[j])));
+          });
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+      }
       const float need = scale_for(most), scale = fmaxf(need, old);
       if (!begun && scale > old) {            // what stands in the block, in the new scale
         const float factor = old / scale;
@@ -302,10 +339,16 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
             store8(dst + half, pack8(b));
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {       // (what is not finite has no code but NaN)
-            a[j] = isfinite(a[j]) ? a[j] * inv : NAN;
-            b[j] = isfinite(b[j]) ? b[j] * inv : NAN;
+          for (int j = 0; j < 8; j += 2) {
+            ptx::mul2(a[j], a[j + 1], a[j], a[j + 1], inv);
+            ptx::mul2(b[j], b[j + 1], b[j], b[j + 1], inv);
           }
+          if (!finite)                        // an infinity has no code, and no other number becomes one: inv is at most 2^126, and 0 beside zeros alone
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if (!isfinite(a[j])) a[j] = NAN;
+              if (!isfinite(b[j])) b[j] = NAN;
+            }
           uint8_t* dst = codes + row * r.head_dim + (key ? at * 8 : at * 16);
           const uint2 c = pack_e4m3x8(a), d = pack_e4m3x8(b);
           if (key) {
