@@ -10,6 +10,8 @@
 // larger ones.  All sums in fp32.
 //
 // Reference: none — the reference offers neither (its server returns text alone, reference llmctl/serve/server.py:57-75).
+#include <type_traits>
+
 #include "../common/dependent.cuh"
 #include "../common/ptx.cuh"
 #include "../common/util.cuh"
@@ -203,10 +205,10 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long lon
     a.add(x);
   };
   if (tid < head) one(tid);
-  for (int i0 = lo + tid; i0 < hi; i0 += kAhead * kThreads) {
+  auto turn = [&](int i0, auto whole) {       // kAhead units; not whole: those behind the last count as -inf
     uint4 raw[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) raw[k] = i0 + k * kThreads < hi ? load_raw(unit(i0 + k * kThreads)) : nothing(r.p);
+    for (int k = 0; k < kAhead; ++k) raw[k] = whole.value || i0 + k * kThreads < hi ? load_raw(unit(i0 + k * kThreads)) : nothing(r.p);
     float of[kAhead], most = -INFINITY;
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
@@ -234,7 +236,10 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long lon
         for (int j = 0; j < U; ++j) a.add(x[j]);
       }
     }
-  }
+  };
+  int i0 = lo + tid;
+  for (; i0 + (kAhead - 1) * kThreads < hi; i0 += kAhead * kThreads) turn(i0, std::true_type());
+  if (i0 < hi) turn(i0, std::false_type());
   if (tail + tid < V) one(tail + tid);
   unsigned long long key = 0ull;              // of this thread's maximum
   if (top > 0 && best_unit >= 0) {
@@ -248,10 +253,11 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long lon
   }
   if (top > 0 && best >= 0) key = make_key(a.m, best);
 
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a.join(__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.t, o));
-  if (lane == 0) red[0][warp] = a.m, red[1][warp] = a.s, red[2][warp] = a.t;
+  // One reference for the CTA, then plain sums (joining pairs of sums at each step of a tree was a third of the instructions at 32000 numbers).
+  {
+    const float m = ptx::warp_max_all(a.m);   // NaN has no part in it: it is in the sums
+    if (lane == 0) red[0][warp] = m;
+  }
   const int groups = kGroups / parts;         // of this CTA
   if (top > 0) {
     const unsigned long long k = reduce_key(key, kThreads / groups);
@@ -264,7 +270,17 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long lon
   __syncthreads();
   Sums all;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) all.join(red[0][w], red[1][w], red[2][w]);
+  for (int w = 0; w < kWarps; ++w) all.m = fmaxf(all.m, red[0][w]);
+  if (all.m > a.m) a.move_to(all.m);
+  a.s = warp_sum(a.s);
+  a.t = warp_sum(a.t);
+  if (lane == 0) red[1][warp] = a.s, red[2][warp] = a.t;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    all.s += red[1][w];
+    all.t += red[2][w];
+  }
   if (kCluster) {
     if (tid == 0) sums[0] = all.m, sums[1] = all.s, sums[2] = all.t;
     ptx::cluster_sync();
