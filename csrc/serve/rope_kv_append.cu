@@ -17,6 +17,7 @@
 #include "../common/dependent.cuh"
 #include "../common/fast_div.h"
 #include "../common/fp8.cuh"
+#include "../common/mma_sync.cuh"
 #include "../common/ptx.cuh"
 #include "../common/util.cuh"
 
@@ -32,13 +33,15 @@ __device__ __forceinline__ void fma2vv(float& a0, float& a1, float b0, float b1,
       : "f"(b0), "f"(b1), "f"(c0), "f"(c1));
 }
 
-// Eight pairs (a: from the first half, b: from the second) of one row, rotated.
-__device__ __forceinline__ void rotate8(float (&a)[8], float (&b)[8], const float* __restrict__ cos_row, const float* __restrict__ sin_row) {
-  float c[8], s[8];
+// The angles of eight pairs.
+__device__ __forceinline__ void load_angles(float (&c)[8], float (&s)[8], const float* __restrict__ cos_row, const float* __restrict__ sin_row) {
   *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cos_row);
   *reinterpret_cast<float4*>(c + 4) = *reinterpret_cast<const float4*>(cos_row + 4);
   *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sin_row);
   *reinterpret_cast<float4*>(s + 4) = *reinterpret_cast<const float4*>(sin_row + 4);
+}
+// Eight pairs (a: from the first half, b: from the second) of one row, rotated.
+__device__ __forceinline__ void rotate8(float (&a)[8], float (&b)[8], const float (&c)[8], const float (&s)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {            // a c - b s and b c + a s, the products with s rounded by themselves
     float t0, t1, u0, u1;
@@ -47,6 +50,11 @@ __device__ __forceinline__ void rotate8(float (&a)[8], float (&b)[8], const floa
     fma2vv(a[j], a[j + 1], c[j], c[j + 1], -t0, -t1);
     fma2vv(b[j], b[j + 1], c[j], c[j + 1], u0, u1);
   }
+}
+__device__ __forceinline__ void rotate8(float (&a)[8], float (&b)[8], const float* __restrict__ cos_row, const float* __restrict__ sin_row) {
+  float c[8], s[8];
+  load_angles(c, s, cos_row, sin_row);
+  rotate8(a, b, c, s);
 }
 
 struct RopeRows {
@@ -112,26 +120,24 @@ rope_kv_append_kernel(RopeRows r, uint32_t total, FastDiv per_token, FastDiv per
 // time.
 //
 // CTAs 0 .. windows * parts - 1: of the tokens of a window, one that is the first of the call in its block takes the block.  A scan over the slots tells,
-// which is left out where the token before goes to the same block (in a prompt, 15 of 16).  A warp then writes a head's block: the rows as they
-// are into registers (again, where a block is longer than they hold), the largest rotated number, the scale, the codes.  The others rotate q, four
-// units to a thread.
+// which is left out where the token before goes to the same block (in a prompt, 15 of 16).  Then a lane has one place in one row of the block for
+// all heads, and keeps its token's angles; as many warps as the block's rows need write a head after the other: the largest rotated number, by
+// all of them, the scale, the codes.  The next head's numbers are asked for beside that.  (A warp to a head's block had to read the angles anew for each
+// row and head and rotate twice, for want of registers: 8000 tokens, 40 heads of 128 130 us, so XX.)  Blocks of more rows than 8 warps hold are
+// read twice.  The other CTAs rotate q, four units to a thread.
 // ---------------------------------------------------------------------------------------------
 namespace append8 {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kRows = 4;                     // rows that a lane holds of its place in them
 constexpr int kUnits = 4;                    // of q, to a thread
 constexpr int kMaxBlock = 4096;
+constexpr int kStages = 4;                   // heads under way (1: 8000 tokens, 40 heads of 128 142 us)
+constexpr uint32_t kInfinite = 0x7f800000u;
 constexpr int kParts = 1000;                 // CTAs of a call that write blocks, or as many as have work
 
-// |x| as an integer that grows with it: kInfinite and more for what is no finite number
-constexpr uint32_t kInfinite = 0x7f800000u;
-__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-__device__ __forceinline__ uint32_t finite_magnitude(float x) { return magnitude(x) < kInfinite ? magnitude(x) : 0u; }
-// The largest |x| of eight, NaN if there is one.
-__device__ __forceinline__ float most_of(const bf16x8& v) {
-  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(v.v[0]), __habs2(v.v[1])), __hmax2_nan(__habs2(v.v[2]), __habs2(v.v[3])));
-  const float2 f = __bfloat1622float2(m);
-  return f.x != f.x ? f.x : f.y != f.y ? f.y : fmaxf(f.x, f.y);
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 // The smallest power of two (of 2^-126 and up) under which a number of this magnitude is at most 448; 0 for zero.
 __device__ __forceinline__ float scale_for(uint32_t most) {
@@ -139,15 +145,127 @@ __device__ __forceinline__ float scale_for(uint32_t most) {
   const int e = static_cast<int>(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);
   return __uint_as_float(static_cast<uint32_t>(max(e, 1)) << 23);
 }
+// 1 / scale, 0 for 0: exact for the powers of two that this file writes
+__device__ __forceinline__ float inverse(float scale) {
+  const uint32_t u = __float_as_uint(scale);
+  if ((u & 0x7fffffu) == 0u && u >= 1u << 23 && u < 253u << 23) return __uint_as_float((254u << 23) - u);
+  return scale > 0.f ? 1.f / scale : 0.f;
+}
+// Warps that write a block together: as many as the rows that are written need, a power of two.
+__device__ __forceinline__ int warps_together(int rows, int step) {
+  int w = 1;
+  while (w < kWarps && w * step < rows) w *= 2;
+  return w;
+}
 }  // namespace append8
 
+namespace append8 {
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// A block of the cache and what is written to it.
+struct Block {
+  const RopeRows& r;
+  const float *cos_t, *sin_t;
+  const int* positions;
+  uint8_t *k, *v;                             // codes and scales of its heads
+  float *ks, *vs;
+  const int *row_token, *row_list;            // as in the kernel
+  int n, block_size;
+  bool begun;
+  // tasks: heads of keys, then of values
+  __device__ __forceinline__ uint8_t* codes_of(int task) const {
+    const int size = block_size * r.head_dim;
+    return task < r.kv_heads ? k + task * size : v + (task - r.kv_heads) * size;
+  }
+  __device__ __forceinline__ float* scale_of(int task) const { return task < r.kv_heads ? ks + task : vs + (task - r.kv_heads); }
+};
+__device__ __forceinline__ void write_codes(uint8_t* dst, bool key, int at, int half, float (&a)[8], float (&b)[8], float inv) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    ptx::mul2(a[j], a[j + 1], a[j], a[j + 1], inv);
+    ptx::mul2(b[j], b[j + 1], b[j], b[j + 1], inv);
+  }
+  const uint2 u = pack_e4m3x8(a), v = pack_e4m3x8(b);
+  if (key) {
+    *reinterpret_cast<uint2*>(dst + at * 8) = u;
+    *reinterpret_cast<uint2*>(dst + at * 8 + half) = v;
+  } else {
+    *reinterpret_cast<uint4*>(dst + at * 16) = make_uint4(u.x, u.y, v.x, v.y);
+  }
+}
+// What stands in the block, in its larger scale; by `threads` threads.
+__device__ __forceinline__ void grow(const Block& b, uint8_t* codes, float factor, int thread, int threads) {
+  for (int i = thread * 8; i < b.block_size * b.r.head_dim; i += threads * 8) {
+    if (b.row_token[i / b.r.head_dim] >= 0) continue;
+    float f[8];
+    unpack_e4m3x8(*reinterpret_cast<const uint2*>(codes + i), f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] *= factor;
+    *reinterpret_cast<uint2*>(codes + i) = pack_e4m3x8(f);
+  }
+}
+// A head's block by one warp, in two passes over its rows, of any number of them.
+__device__ __forceinline__ void write_alone(const Block& bk, int task) {
+  const RopeRows& r = bk.r;
+  const int lane = threadIdx.x & 31, per_row = r.head_dim >> 4, step = 32 / per_row, sub = lane / per_row, at = lane - sub * per_row, half = r.head_dim >> 1;
+  const bool key = task < r.kv_heads;
+  float* const scale_at = bk.scale_of(task);
+  uint8_t* const codes = bk.codes_of(task);
+  const float old = bk.begun ? 0.f : fmaxf(*scale_at, 0.f);
+  auto each = [&](auto&& f) {                 // f(row, where the token's numbers stand, the numbers)
+#pragma unroll 2
+    for (int i = sub; i < bk.n; i += step) {
+      if (sub >= step) break;
+      const int row = bk.row_list[i], tok = bk.row_token[row];
+      __nv_bfloat16* p = r.qkv + tok * r.row_stride + static_cast<long long>(r.heads + task) * r.head_dim + (key ? at * 8 : at * 16);
+      float a[8], b[8];
+      unpack8(load8(p), a);
+      unpack8(load8(p + (key ? half : 8)), b);
+      if (key) {
+        const long long table = table_row(r, bk.positions, tok) + at * 8;
+        rotate8(a, b, bk.cos_t + table, bk.sin_t + table);
+      }
+      f(row, p, a, b);
+    }
+  };
+  uint32_t most = 0u;
+  each([&](int, __nv_bfloat16*, float (&a)[8], float (&b)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (isfinite(a[j])) most = max(most, __float_as_uint(fabsf(a[j])));
+      if (isfinite(b[j])) most = max(most, __float_as_uint(fabsf(b[j])));
+    }
+  });
+  const float scale = fmaxf(scale_for(__reduce_max_sync(0xffffffffu, most)), old), inv = inverse(scale);
+  if (!bk.begun && scale > old) grow(bk, codes, old / scale, lane, 32);
+  each([&](int row, __nv_bfloat16* p, float (&a)[8], float (&b)[8]) {
+    if (key) {
+      store8(p, pack8(a));
+      store8(p + half, pack8(b));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {             // (no finite number becomes an infinity: inv is at most 2^126, and 0 beside zeros alone)
+      if (!isfinite(a[j])) a[j] = NAN;
+      if (!isfinite(b[j])) b[j] = NAN;
+    }
+    write_codes(codes + row * r.head_dim, key, at, half, a, b, inv);
+  });
+  if (lane == 0) *scale_at = scale;
+  __syncwarp();
+}
+}  // namespace append8
+
+// kOnce: a block is of no more rows than 8 warps hold.
+template <bool kOnce>
 __global__ void __launch_bounds__(append8::kThreads, 3)
 rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
                           float* __restrict__ k_scale, float* __restrict__ v_scale, int blocks, int block_size, int window, int windows, int parts,
                           uint32_t q_units, FastDiv per_token, FastDiv per_head) {
   using namespace append8;
-  extern __shared__ int2 row_of[];            // [block_size]: the token that a row of the block at hand is written from, or -1, and its row in the tables
-  __shared__ int first_token, twice;
+  extern __shared__ __align__(16) int row_token[];          // [block_size]: the token that a row of the block at hand is written from, or -1; then those rows
+  __shared__ int first_token, twice, written;
+  int* const row_list = row_token + (block_size + 3) / 4 * 4;          // (what follows both lies on a 16-byte boundary)
+  __shared__ __align__(16) uint32_t warp_most[2][kWarps];
   __nv_bfloat16* qkv = r.qkv;
   const float *cos_t = r.cos_t, *sin_t = r.sin_t;
   const int* positions = r.positions;
@@ -206,7 +324,7 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
       }
   };
 
-  const int sub = lane / per_row, at = lane - sub * per_row, step = 32 / per_row;      // rows of a warp at a time; lanes past them idle
+  const int sub = lane / per_row, at = lane - sub * per_row, step = 32 / per_row;      // rows of a warp; lanes past them idle
   // Of the window's tokens (16 at most, a lane each): those without a row, and those that may be the first in their block.
   long long slot = -1, before = -1;
   if (t0 + lane < t1) {
@@ -220,148 +338,141 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
     const int t = t0 + __ffs(left) - 1, block = static_cast<int>(__shfl_sync(0xffffffffu, slot, t - t0) / block_size);
     const long long lo = static_cast<long long>(block) * block_size, hi = lo + block_size;
     __syncthreads();                          // the rows of the block before have been read
-    for (int i = threadIdx.x; i < block_size; i += kThreads) row_of[i].x = -1;
+    for (int i = threadIdx.x; i < block_size; i += kThreads) row_token[i] = -1;
     if (threadIdx.x == 0) {
       first_token = t;
-      twice = 0;
+      twice = written = 0;
     }
     __syncthreads();
-#pragma unroll 4
-    for (int i = threadIdx.x; i < r.tokens; i += kThreads) {
-      const long long s = slots[i];
+    auto meet = [&](int i, long long s) {
       if (s >= lo && s < hi) {
         if (i < t) atomicMin(&first_token, i);
-        if (atomicMax(&row_of[s - lo].x, i) >= 0) twice = 1;
+        if (atomicMax(&row_token[s - lo], i) >= 0) twice = 1;
       }
+    };
+    const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(slots) >> 3 & 1u);      // a slot before the first 16-byte boundary
+    if (threadIdx.x == 0 && odd != 0) meet(0, slots[0]);
+    const longlong2* two = reinterpret_cast<const longlong2*>(slots + odd);
+    const int pairs = (r.tokens - odd) >> 1;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < pairs; i += kThreads) {
+      const longlong2 s = two[i];
+      meet(odd + 2 * i, s.x);
+      meet(odd + 2 * i + 1, s.y);
     }
+    if (threadIdx.x == 0 && (r.tokens - odd) % 2 != 0) meet(r.tokens - 1, slots[r.tokens - 1]);
     __syncthreads();
     if (first_token != t) continue;
     for (int i = threadIdx.x; i < block_size; i += kThreads)
-      if (row_of[i].x >= 0) row_of[i].y = min(max(positions[row_of[i].x], 0), r.table_rows - 1);
+      if (row_token[i] >= 0) row_list[atomicAdd(&written, 1)] = i;          // in whatever order: rows do not depend on each other
     if (twice)
       for (int i = 0; i < r.tokens; ++i) {
         const long long s = slots[i];
-        if (s >= lo && s < hi && row_of[s - lo].x != i) rotate_keys(i);
+        if (s >= lo && s < hi && row_token[s - lo] != i) rotate_keys(i);
       }
     __syncthreads();
-    const bool begun = row_of[0].x >= 0;
+    const int n = written, together = warps_together(n, step), groups = kWarps / together, group = warp / together, mine = warp - group * together;
+    const bool begun = row_token[0] >= 0;
 
-    for (int task = part + warp * parts; task < 2 * r.kv_heads; task += kWarps * parts) {
-      const bool key = task < r.kv_heads;
-      const int head = key ? task : task - r.kv_heads;
-      uint8_t* codes = (key ? k_cache : v_cache) + (static_cast<long long>(block) * r.kv_heads + head) * block_size * r.head_dim;
-      float* scale_at = (key ? k_scale : v_scale) + static_cast<long long>(block) * r.kv_heads + head;
-      __nv_bfloat16* src = qkv + static_cast<long long>(r.heads + task) * r.head_dim + (key ? at * 8 : at * 16);
-      const int second = key ? half : 8;
-      bf16x8 x[kRows], y[kRows];              // as they stand: rotated again for the codes, which costs less than the registers
-      auto row_at = [&](int row0, int i) {
-        const int row = row0 + i * step + sub;
-        return sub < step && row < block_size ? row : -1;
-      };
-      auto load = [&](int row0) {
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          const int row = row_at(row0, i), tok = row >= 0 ? row_of[row].x : -1;
-          if (tok >= 0) {
-            x[i] = load8(src + tok * r.row_stride);
-            y[i] = load8(src + tok * r.row_stride + second);
-          }
-        }
-      };
-      // f(row, its token, the numbers in 32 bits) for each row that is written
-      auto each = [&](int row0, auto&& f) {
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          const int row = row_at(row0, i);
-          if (row < 0) continue;
-          const int2 of = row_of[row];
-          if (of.x < 0) continue;
-          float a[8], b[8];
-          unpack8(x[i], a);
-          unpack8(y[i], b);
-          if (key) {
-            const long long table = static_cast<long long>(of.y) * half + at * 8;
-            rotate8(a, b, cos_t + table, sin_t + table);
-          }
-          f(row, of.x, a, b);
-        }
-      };
-      const bool once = block_size <= kRows * step;
-      const float old = begun ? 0.f : fmaxf(*scale_at, 0.f);
-      uint32_t most = 0u;
-      for (int row0 = 0; row0 < block_size; row0 += kRows * step) {
-        load(row0);
-        if (key)
-          each(row0, [&](int, int, const float (&a)[8], const float (&b)[8]) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) most = max(most, max(magnitude(a[j]), magnitude(b[j])));
-          });
-        else
-#pragma unroll
-          for (int i = 0; i < kRows; ++i) {
-            const int row = row_at(row0, i);
-            if (row >= 0 && row_of[row].x >= 0) most = max(most, max(magnitude(most_of(x[i])), magnitude(most_of(y[i]))));
-          }
-      }
-      most = __reduce_max_sync(0xffffffffu, most);
-      const bool finite = most < kInfinite;
-      if (!finite) {                          // rare: once more without them
-        most = 0u;
-        for (int row0 = 0; row0 < block_size; row0 += kRows * step) {
-          if (!once) load(row0);
-          each(row0, [&](int, int, const float (&a)[8], const float (&b)[8]) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) most = max(most, max(finite_magnitude(a[j]), finite_magnitude(b[j])));
-          });
-        }
-        most = __reduce_max_sync(0xffffffffu, most);
-      }
-      const float need = scale_for(most), scale = fmaxf(need, old);
-      if (!begun && scale > old) {            // what stands in the block, in the new scale
-        const float factor = old / scale;
-        for (int i = lane * 8; i < block_size * r.head_dim; i += 256) {
-          if (row_of[i / r.head_dim].x >= 0) continue;
-          uint2 c = *reinterpret_cast<const uint2*>(codes + i);
-          float f[8];
-          unpack_e4m3x8(c, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] *= factor;
-          *reinterpret_cast<uint2*>(codes + i) = pack_e4m3x8(f);
-        }
-      }
-      const float inv = scale > 0.f ? 1.f / scale : 0.f;
-      for (int row0 = 0; row0 < block_size; row0 += kRows * step) {
-        if (!once) load(row0);
-        each(row0, [&](int row, int tok, float (&a)[8], float (&b)[8]) {
-          if (key) {
-            __nv_bfloat16* dst = src + tok * r.row_stride;
-            store8(dst, pack8(a));
-            store8(dst + half, pack8(b));
-          }
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            ptx::mul2(a[j], a[j + 1], a[j], a[j + 1], inv);
-            ptx::mul2(b[j], b[j + 1], b[j], b[j + 1], inv);
-          }
-          if (!finite)                        // an infinity has no code, and no other number becomes one: inv is at most 2^126, and 0 beside zeros alone
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              if (!isfinite(a[j])) a[j] = NAN;
-              if (!isfinite(b[j])) b[j] = NAN;
-            }
-          uint8_t* dst = codes + row * r.head_dim + (key ? at * 8 : at * 16);
-          const uint2 c = pack_e4m3x8(a), d = pack_e4m3x8(b);
-          if (key) {
-            *reinterpret_cast<uint2*>(dst) = c;
-            *reinterpret_cast<uint2*>(dst + half) = d;
-          } else {
-            *reinterpret_cast<uint4*>(dst) = make_uint4(c.x, c.y, d.x, d.y);
-          }
-        });
-      }
-      if (lane == 0) *scale_at = scale;
-      __syncwarp();
+    const long long at_block = static_cast<long long>(block) * r.kv_heads;
+    Block bk{r, cos_t, sin_t, positions, k_cache + at_block * block_size * r.head_dim, v_cache + at_block * block_size * r.head_dim, k_scale + at_block,
+             v_scale + at_block, row_token, row_list, n, block_size, begun};
+    const int tasks = 2 * r.kv_heads;
+    if constexpr (!kOnce) {
+      for (int task = part + warp * parts; task < tasks; task += kWarps * parts) write_alone(bk, task);
+      continue;
     }
+
+    // the lane's place: one of the rows that are written and the token that it is written from, or -1
+    const int i = mine * step + sub;
+    const int row = sub < step && i < n ? row_list[i] : 0, tok = sub < step && i < n ? row_token[row] : -1;
+    __nv_bfloat16* const base = qkv + max(tok, 0) * r.row_stride + static_cast<long long>(r.heads) * r.head_dim;
+    float c[8] = {}, s[8] = {};
+    if (tok >= 0) {
+      const long long table = table_row(r, positions, tok) + at * 8;
+      load_angles(c, s, cos_t + table, sin_t + table);
+    }
+    // The numbers of the heads to come, kStages - 1 of them, on their way into places that only the lane itself reads.
+    uint8_t* const ring = reinterpret_cast<uint8_t*>(row_list + (block_size + 3) / 4 * 4) + warp * (kStages * 1024) + lane * 16;
+    auto ask = [&](int task, int stage) {
+      if (task < tasks && tok >= 0) {
+        const __nv_bfloat16* p = base + task * r.head_dim + (task < r.kv_heads ? at * 8 : at * 16);
+        cp_async_16(ring + stage * 1024, p);
+        cp_async_16(ring + stage * 1024 + 512, p + (task < r.kv_heads ? half : 8));
+      }
+      cp_async_commit();
+    };
+    const int first = part + group * parts, by = groups * parts;
+    int turn = 0;
+    auto largest = [&](uint32_t most) {       // over the warps that write the block together
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (together > 1) {
+        uint32_t* const of = warp_most[turn++ & 1] + group * together;
+        if (lane == 0) of[mine] = most;
+        ptx::named_bar_sync(1 + group, together * 32);
+        if (together == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(of);
+          most = max(v.x, v.y);
+        } else {
+          for (int w = 0; w < together; w += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(of + w);
+            most = max(most, max(max(v.x, v.y), max(v.z, v.w)));
+          }
+        }
+      }
+      return most;
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) ask(first + i * by, i);
+    int stage = 0;
+    for (int task = first; task < tasks; task += by) {
+      const bool key = task < r.kv_heads;
+      float* const scale_at = bk.scale_of(task);
+      const float old = begun ? 0.f : fmaxf(*scale_at, 0.f);
+      float a[8] = {}, b[8] = {};
+      ask(task + (kStages - 1) * by, (stage + kStages - 1) % kStages);
+      cp_async_wait<kStages - 1>();
+      if (tok >= 0) {
+        unpack8(*reinterpret_cast<const bf16x8*>(ring + stage * 1024), a);
+        unpack8(*reinterpret_cast<const bf16x8*>(ring + stage * 1024 + 512), b);
+      }
+      stage = (stage + 1) % kStages;
+      if (key) rotate8(a, b, c, s);
+      float x8 = 0.f;                         // rows that are not there hold zeros
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x8 = max_nan(x8, max_nan(fabsf(a[j]), fabsf(b[j])));
+      uint32_t most = largest(__float_as_uint(x8) & 0x7fffffffu);
+      const bool finite = most < kInfinite;
+      if (!finite) {                          // rare: once more without what has no code but NaN
+        most = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          most = isfinite(a[j]) ? max(most, __float_as_uint(fabsf(a[j]))) : most;
+          most = isfinite(b[j]) ? max(most, __float_as_uint(fabsf(b[j]))) : most;
+        }
+        most = largest(most);
+      }
+      const float need = scale_for(most), scale = fmaxf(need, old), inv = inverse(scale);
+      uint8_t* const codes = bk.codes_of(task);
+      if (!begun && scale > old) grow(bk, codes, old / scale, mine * 32 + lane, together * 32);
+      if (tok >= 0) {
+        if (key) {
+          __nv_bfloat16* dst = base + task * r.head_dim + at * 8;
+          store8(dst, pack8(a));
+          store8(dst + half, pack8(b));
+        }
+        if (!finite)                          // (no finite number becomes an infinity: inv is at most 2^126, and 0 beside zeros alone)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (!isfinite(a[j])) a[j] = NAN;
+            if (!isfinite(b[j])) b[j] = NAN;
+          }
+        write_codes(codes + row * r.head_dim, key, at, half, a, b, inv);
+      }
+      if (together == 1) __syncwarp();        // else they have met since they read it
+      if (lane == 0 && mine == 0) *scale_at = scale;
+    }
+    cp_async_wait<0>();
   }
 }
 
@@ -405,14 +516,19 @@ LLMCTL_API int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int to
   using namespace append8;
   const RopeRows r{static_cast<__nv_bfloat16*>(qkv), row_stride, tokens, heads, kv_heads, head_dim, cos_t, sin_t, table_rows, positions};
   LLMCTL_REQUIRE(rope_rows_ok(r) && head_dim <= 512 && blocks >= 0 && block_size >= 1 && block_size <= kMaxBlock && aligned16(k_cache, v_cache));
+  LLMCTL_REQUIRE(static_cast<long long>(blocks) * kv_heads < (1LL << 31) && static_cast<long long>(kv_heads) * block_size * head_dim < (1LL << 31));
   if (tokens == 0) return 0;
-  const int window = tokens > 256 ? 16 : 1, windows = (tokens + window - 1) / window, most = (2 * kv_heads + kWarps - 1) / kWarps;
-  int parts = (kParts + windows - 1) / windows;
+  const int window = tokens > 256 ? 16 : 1, windows = (tokens + window - 1) / window;
+  // A block to each token where they may all be of other sequences, else to each block_size of them.
+  const int writers = tokens > 256 ? (tokens + block_size - 1) / block_size : tokens, most = tokens > 256 ? kv_heads : (2 * kv_heads + kWarps - 1) / kWarps;
+  int parts = (kParts + writers - 1) / writers;
   if (parts > most) parts = most;
   const long long per_token = static_cast<long long>(heads) * (head_dim / 16), units = per_token * tokens;
   LLMCTL_REQUIRE(units < (1LL << 30));
   const int q_ctas = static_cast<int>((units + kThreads * kUnits - 1) / (kThreads * kUnits));
-  LLMCTL_CHECK(launch_dependent(rope_kv_append_fp8_kernel, windows * parts + q_ctas, kThreads, block_size * sizeof(int2), (cudaStream_t)stream, r, slots,
+  const bool once = block_size <= kWarps * (32 / (head_dim / 16));
+  const int smem = (block_size + 3) / 4 * 4 * 2 * static_cast<int>(sizeof(int)) + (once ? kWarps * kStages * 1024 : 0);
+  LLMCTL_CHECK(launch_dependent(once ? rope_kv_append_fp8_kernel<true> : rope_kv_append_fp8_kernel<false>, windows * parts + q_ctas, kThreads, smem, (cudaStream_t)stream, r, slots,
                                 (uint8_t*)k_cache, (uint8_t*)v_cache, k_scale, v_scale, blocks, block_size, window, windows, parts,
                                 static_cast<uint32_t>(units), FastDiv(static_cast<uint32_t>(per_token)), FastDiv(head_dim / 16)));
   LLMCTL_RETURN_LAST();
