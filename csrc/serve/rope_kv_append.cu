@@ -14,6 +14,8 @@
 // The first row of a block begins it anew.  Keys are rounded once, from the rotated value in 32 bits.
 //
 // Reference: none — the reference keeps no cache (reference llmctl/serve/server.py:199-204).
+#include <type_traits>
+
 #include "../common/dependent.cuh"
 #include "../common/fast_div.h"
 #include "../common/fp8.cuh"
@@ -204,7 +206,7 @@ __device__ __forceinline__ void grow(const Block& b, uint8_t* codes, float facto
     *reinterpret_cast<uint2*>(codes + i) = pack_e4m3x8(f);
   }
 }
-// A head's block by one warp, in two passes over its rows, of any number of them.
+// A head's block by one warp, in two passes over its rows, of any number of them; what is not finite has no code but NaN.
 __device__ __forceinline__ void write_alone(const Block& bk, int task) {
   const RopeRows& r = bk.r;
   const int lane = threadIdx.x & 31, per_row = r.head_dim >> 4, step = 32 / per_row, sub = lane / per_row, at = lane - sub * per_row, half = r.head_dim >> 1;
@@ -265,7 +267,7 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
   extern __shared__ __align__(16) int row_token[];          // [block_size]: the token that a row of the block at hand is written from, or -1; then those rows
   __shared__ int first_token, twice, written;
   int* const row_list = row_token + (block_size + 3) / 4 * 4;          // (what follows both lies on a 16-byte boundary)
-  __shared__ __align__(16) uint32_t warp_most[2][kWarps];
+  __shared__ uint32_t warp_most[2][kWarps];
   __nv_bfloat16* qkv = r.qkv;
   const float *cos_t = r.cos_t, *sin_t = r.sin_t;
   const int* positions = r.positions;
@@ -403,30 +405,23 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
       cp_async_commit();
     };
     const int first = part + group * parts, by = groups * parts;
-    int turn = 0;
+    int turn = 0, turns = 0;
+    uint32_t later = 0u;                      // a bit for each of the turns, 32 to a lane
     auto largest = [&](uint32_t most) {       // over the warps that write the block together
       most = __reduce_max_sync(0xffffffffu, most);
       if (together > 1) {
         uint32_t* const of = warp_most[turn++ & 1] + group * together;
         if (lane == 0) of[mine] = most;
         ptx::named_bar_sync(1 + group, together * 32);
-        if (together == 2) {
-          const uint2 v = *reinterpret_cast<const uint2*>(of);
-          most = max(v.x, v.y);
-        } else {
-          for (int w = 0; w < together; w += 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(of + w);
-            most = max(most, max(max(v.x, v.y), max(v.z, v.w)));
-          }
-        }
+        most = __reduce_max_sync(0xffffffffu, of[lane & (together - 1)]);
       }
       return most;
     };
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) ask(first + i * by, i);
     int stage = 0;
-    for (int task = first; task < tasks; task += by) {
-      const bool key = task < r.kv_heads;
+    auto one = [&](int task, auto of_keys) {
+      constexpr bool key = of_keys.value;     // (known at compile time: what only keys need would be stepped over one by one for values)
       float* const scale_at = bk.scale_of(task);
       const float old = begun ? 0.f : fmaxf(*scale_at, 0.f);
       float a[8] = {}, b[8] = {};
@@ -441,16 +436,10 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
       float x8 = 0.f;                         // rows that are not there hold zeros
 #pragma unroll
       for (int j = 0; j < 8; ++j) x8 = max_nan(x8, max_nan(fabsf(a[j]), fabsf(b[j])));
-      uint32_t most = largest(__float_as_uint(x8) & 0x7fffffffu);
-      const bool finite = most < kInfinite;
-      if (!finite) {                          // rare: once more without what has no code but NaN
-        most = 0u;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          most = isfinite(a[j]) ? max(most, __float_as_uint(fabsf(a[j]))) : most;
-          most = isfinite(b[j]) ? max(most, __float_as_uint(fabsf(b[j]))) : most;
-        }
-        most = largest(most);
+      const uint32_t most = largest(__float_as_uint(x8) & 0x7fffffffu);
+      if (most >= kInfinite) {                // rare, and written behind the others
+        if (lane == turns >> 5) later |= 1u << (turns & 31);
+        return;
       }
       const float need = scale_for(most), scale = fmaxf(need, old), inv = inverse(scale);
       uint8_t* const codes = bk.codes_of(task);
@@ -461,18 +450,18 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
           store8(dst, pack8(a));
           store8(dst + half, pack8(b));
         }
-        if (!finite)                          // (no finite number becomes an infinity: inv is at most 2^126, and 0 beside zeros alone)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (!isfinite(a[j])) a[j] = NAN;
-            if (!isfinite(b[j])) b[j] = NAN;
-          }
         write_codes(codes + row * r.head_dim, key, at, half, a, b, inv);
       }
       if (together == 1) __syncwarp();        // else they have met since they read it
       if (lane == 0 && mine == 0) *scale_at = scale;
-    }
+    };
+    int task = first;
+    for (; task < r.kv_heads; task += by, ++turns) one(task, std::true_type());
+    for (; task < tasks; task += by, ++turns) one(task, std::false_type());
     cp_async_wait<0>();
+    if (mine == 0 && __any_sync(0xffffffffu, later != 0u))                 // heads with a number that is not finite
+      for (int i = 0; i < turns; ++i)
+        if (__shfl_sync(0xffffffffu, later, i >> 5) >> (i & 31) & 1u) write_alone(bk, first + i * by);
   }
 }
 
@@ -515,7 +504,7 @@ LLMCTL_API int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int to
   LLMCTL_BEGIN();
   using namespace append8;
   const RopeRows r{static_cast<__nv_bfloat16*>(qkv), row_stride, tokens, heads, kv_heads, head_dim, cos_t, sin_t, table_rows, positions};
-  LLMCTL_REQUIRE(rope_rows_ok(r) && head_dim <= 512 && blocks >= 0 && block_size >= 1 && block_size <= kMaxBlock && aligned16(k_cache, v_cache));
+  LLMCTL_REQUIRE(rope_rows_ok(r) && head_dim <= 512 && kv_heads <= 512 && blocks >= 0 && block_size >= 1 && block_size <= kMaxBlock && aligned16(k_cache, v_cache));
   LLMCTL_REQUIRE(static_cast<long long>(blocks) * kv_heads < (1LL << 31) && static_cast<long long>(kv_heads) * block_size * head_dim < (1LL << 31));
   if (tokens == 0) return 0;
   const int window = tokens > 256 ? 16 : 1, windows = (tokens + window - 1) / window;

@@ -208,7 +208,8 @@ def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
     _check(slot_mapping.shape == (T,) and slot_mapping.dtype == torch.int64 and slot_mapping.device == qkv.device, "slot_mapping: int64 beside the rows, one per row")
     if fp8:
         _check_fp8_caches(k_cache, v_cache, k_scale, v_scale, head_dim, qkv.device)
-        _check(k_cache.shape[1] == kv_heads and 1 <= k_cache.shape[2] <= 4096 and head_dim <= 512, f"a cache of 8 bits of {kv_heads} heads, blocks of at most 4096 rows, heads of at most 512")
+        _check(k_cache.shape[1] == kv_heads and 1 <= k_cache.shape[2] <= 4096 and head_dim <= 512 and kv_heads <= 512,
+               f"a cache of 8 bits of {kv_heads} heads, at most 512 of them and of at most 512 numbers, in blocks of at most 4096 rows")
     else:
         _check(k_scale is None and v_scale is None, "scales belong to caches of 8 bits")
         for c in (k_cache, v_cache):
