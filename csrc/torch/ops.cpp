@@ -15,16 +15,19 @@
 #include <ATen/autocast_mode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/dynamo/compiled_autograd.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
 #include <array>
 #include <atomic>
 #include <cstdio>
@@ -42,7 +45,8 @@ using at::Tensor;
 #define LLMCTL_ENTRIES(X)                                                                                                         \
   X(llmctl_rmsnorm_fwd) X(llmctl_rmsnorm_bwd_bf16w) X(llmctl_rope_inplace) X(llmctl_gemm_rope_bf16) X(llmctl_gemm_bf16) X(llmctl_gemm_swiglu_bf16)               \
   X(llmctl_gemm_swiglu_bwd_bf16) X(llmctl_swiglu_bwd) X(llmctl_gemm_skinny_bf16) X(llmctl_gemm_skinny_scratch_elems) X(llmctl_flash_attn_fwd) X(llmctl_flash_attn_bwd) X(llmctl_kv_append) \
-  X(llmctl_paged_attn_decode) X(llmctl_paged_attn_scratch_elems) X(llmctl_latent_kv_write) X(llmctl_latent_decode)
+  X(llmctl_paged_attn_decode) X(llmctl_paged_attn_scratch_elems) X(llmctl_latent_kv_write) X(llmctl_latent_decode) \
+  X(llmctl_rope_kv_append) X(llmctl_rope_kv_append_fp8) X(llmctl_paged_attn_decode_fp8) X(llmctl_paged_attn_fp8_scratch_elems) X(llmctl_token_logprobs) X(llmctl_token_logprobs_bwd)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
   LLMCTL_ENTRIES(X)
@@ -918,6 +922,211 @@ PyObject* py_paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// All on the device whose stream launches go to; others go through the Python operator, which makes theirs the current one.
+bool here(std::initializer_list<const Tensor*> ts) {
+  const auto device = c10::cuda::current_device();
+  for (const Tensor* x : ts)
+    if (x->get_device() != device) return false;
+  return true;
+}
+// a cache of 8 bits [blocks, heads, block_size, D] and its scales
+bool is_fp8_cache(const Tensor& c, const Tensor& s, int64_t D) {
+  return c.scalar_type() == at::kFloat8_e4m3fn && c.dim() == 4 && c.is_contiguous() && unit16(c) && c.size(3) == D && s.scalar_type() == at::kFloat && s.is_contiguous() &&
+         s.dim() == 2 && s.size(0) == c.size(0) && s.size(1) == c.size(1) && c.size(0) < (1LL << 31) && c.size(2) < (1LL << 31);
+}
+
+// rope_kv_append(qkv, cos, sin, positions, k_cache, v_cache, slots, heads, kv_heads, head_dim, k_scale or None, v_scale or None) -> True
+PyObject* py_rope_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return call(a, n, 12, [&](Args& args) -> PyObject* {
+    const Tensor qkv = args.tensor(0), cos = args.tensor(1), sin = args.tensor(2), positions = args.tensor(3), k = args.tensor(4), v = args.tensor(5), slots = args.tensor(6),
+                 ks = args.optional(10), vs = args.optional(11);
+    const int64_t H = args.integer(7), Hk = args.integer(8), D = args.integer(9), width = (H + 2 * Hk) * D;
+    if (!args.ok || !quiet() || H < 1 || Hk < 1 || H % Hk || D < 16 || D % 16 || !here({&qkv, &cos, &sin, &positions, &k, &v, &slots}) || !is_matrix(qkv) || qkv.size(1) < width ||
+        qkv.stride(0) < width || recorded({&qkv}) || qkv.size(0) >= (1LL << 31))
+      return none();
+    const int64_t T = qkv.size(0);
+    for (const Tensor* t : {&cos, &sin})
+      if (t->scalar_type() != at::kFloat || t->dim() != 2 || t->size(0) != cos.size(0) || t->size(0) < 1 || t->size(1) != D / 2 || !t->is_contiguous() || !unit16(*t)) return none();
+    if (positions.scalar_type() != at::kInt || positions.dim() != 1 || positions.size(0) != T || !positions.is_contiguous() || slots.scalar_type() != at::kLong || slots.dim() != 1 ||
+        slots.size(0) != T || !slots.is_contiguous() || k.dim() != 4 || v.sizes() != k.sizes())
+      return none();
+    const auto f32 = [](const Tensor& x) { return static_cast<const float*>(cdata(x)); };
+    const bool fp8 = ks.defined() && vs.defined();
+    if (fp8) {
+      if (!ready(lib.llmctl_rope_kv_append_fp8) || !here({&ks, &vs}) || !is_fp8_cache(k, ks, D) || !is_fp8_cache(v, vs, D) || k.size(1) != Hk || k.size(2) < 1 || k.size(2) > 4096 || D > 512 ||
+          Hk > 512)
+        return none();
+    } else if (ks.defined() || vs.defined() || !ready(lib.llmctl_rope_kv_append) || !bf16(k) || !bf16(v) || !k.is_contiguous() || !v.is_contiguous() || !unit16(k) || !unit16(v) ||
+               k.size(2) != Hk || k.size(3) != D) {
+      return none();
+    }
+    without_gil([&] {
+      if (fp8)
+        done("llmctl_rope_kv_append_fp8", lib.llmctl_rope_kv_append_fp8(data(qkv), qkv.stride(0), static_cast<int>(T), static_cast<int>(H), static_cast<int>(Hk), static_cast<int>(D), f32(cos),
+                                                                        f32(sin), static_cast<int>(cos.size(0)), static_cast<const int*>(cdata(positions)),
+                                                                        static_cast<const long long*>(cdata(slots)), data(k), data(v), static_cast<float*>(data(ks)), static_cast<float*>(data(vs)),
+                                                                        static_cast<int>(k.size(0)), static_cast<int>(k.size(2)), stream()));
+      else
+        done("llmctl_rope_kv_append", lib.llmctl_rope_kv_append(data(qkv), qkv.stride(0), static_cast<int>(T), static_cast<int>(H), static_cast<int>(Hk), static_cast<int>(D), f32(cos), f32(sin),
+                                                                static_cast<int>(cos.size(0)), static_cast<const int*>(cdata(positions)), static_cast<const long long*>(cdata(slots)), data(k),
+                                                                data(v), k.size(0) * k.size(1), stream()));
+    });
+    if (!qkv.is_inference()) qkv.unsafeGetTensorImpl()->bump_version();
+    Py_RETURN_TRUE;
+  });
+}
+
+// paged_decode_fp8(q, k_cache, v_cache, k_scale, v_scale, tables, lens, max_context, splits, scale) -> out
+PyObject* py_paged_decode_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return call(a, n, 10, [&](Args& args) -> PyObject* {
+    const Tensor q = args.tensor(0), k = args.tensor(1), v = args.tensor(2), ks = args.tensor(3), vs = args.tensor(4), tables = args.tensor(5), lens = args.tensor(6);
+    const int64_t most = args.integer(7), splits = args.integer(8);
+    const double scale = args.number(9);
+    if (!args.ok || !quiet() || !ready(lib.llmctl_paged_attn_decode_fp8) || !lib.llmctl_paged_attn_fp8_scratch_elems || !here({&q, &k, &v, &ks, &vs, &tables, &lens}) || !bf16(q) || q.dim() != 3 ||
+        q.numel() == 0 || q.stride(2) != 1 || q.stride(1) != q.size(2) || q.stride(0) % 8 || !unit16(q) || recorded({&q}))
+      return none();
+    const int64_t B = q.size(0), H = q.size(1), D = q.size(2);
+    if ((D != 64 && D != 128) || B >= 65536 || !is_fp8_cache(k, ks, D) || !is_fp8_cache(v, vs, D) || v.sizes() != k.sizes() || k.numel() == 0 || H % k.size(1) || splits < 0 || splits > 256 ||
+        tables.dim() != 2 || tables.scalar_type() != at::kInt || !tables.is_contiguous() || tables.size(0) < B || lens.dim() != 1 || lens.scalar_type() != at::kInt || !lens.is_contiguous() ||
+        lens.size(0) < B)
+      return none();
+    const int64_t room = tables.size(1) * k.size(2);
+    const int context = static_cast<int>(std::max<int64_t>(0, std::min<int64_t>({most, room, (1LL << 31) - 1})));
+    Tensor o = without_gil([&] {
+      const long long need = lib.llmctl_paged_attn_fp8_scratch_elems(static_cast<int>(B), static_cast<int>(H), static_cast<int>(k.size(1)), static_cast<int>(D), static_cast<int>(tables.size(1)),
+                                                                     static_cast<int>(k.size(2)), context, static_cast<int>(splits));
+      Tensor scratch = need ? new_f32(q, {need}) : Tensor(), out = new_bf16(q, q.sizes());
+      const auto f32 = [](const Tensor& x) { return static_cast<const float*>(cdata(x)); };
+      done("llmctl_paged_attn_decode_fp8",
+           lib.llmctl_paged_attn_decode_fp8(cdata(q), q.stride(0), cdata(k), cdata(v), f32(ks), f32(vs), static_cast<const int*>(cdata(tables)), static_cast<int>(tables.size(1)),
+                                            static_cast<const int*>(cdata(lens)), data(out), need ? static_cast<float*>(data(scratch)) : nullptr, static_cast<int>(B), static_cast<int>(H),
+                                            static_cast<int>(k.size(1)), static_cast<int>(D), static_cast<int>(k.size(0)), static_cast<int>(k.size(2)), context, static_cast<int>(splits),
+                                            static_cast<float>(scale), stream()),
+           need ? 2 : 1);
+      return out;
+    });
+    return THPVariable_Wrap(o);
+  });
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// log probabilities of tokens
+// ---------------------------------------------------------------------------------------------------------------------------------
+struct LogprobsOut {
+  Tensor logprobs, entropy, ids, top, stats;
+};
+LogprobsOut logprobs_fwd(const Tensor& logits, const Tensor& tokens, int64_t top, bool keep) {
+  const int64_t rows = logits.size(0), V = logits.size(1);
+  LogprobsOut r{new_f32(logits, {rows}), new_f32(logits, {rows}), top ? empty_like_on(logits, {rows, top}, at::kLong) : Tensor(), top ? new_f32(logits, {rows, top}) : Tensor(),
+                keep ? new_f32(logits, {rows, 2}) : Tensor()};
+  const auto f32 = [](const Tensor& x) { return x.defined() ? static_cast<float*>(data(x)) : nullptr; };
+  done("llmctl_token_logprobs",
+       lib.llmctl_token_logprobs(cdata(logits), logits.scalar_type() == at::kFloat, logits.stride(0), static_cast<const long long*>(cdata(tokens)), static_cast<int>(rows), static_cast<int>(V),
+                                 static_cast<int>(top), f32(r.logprobs), f32(r.entropy), f32(r.stats), top ? static_cast<long long*>(data(r.ids)) : nullptr, f32(r.top), stream()));
+  return r;
+}
+// Uninitialised rows that lie to 16-byte boundaries as those of `x` do.
+Tensor rows_like(const Tensor& x) {
+  const int64_t size = x.element_size(), units = 16 / size, shift = reinterpret_cast<uintptr_t>(x.const_data_ptr()) % 16 / size, rows = x.size(0), V = x.size(1);
+  const int64_t ld = rows > 1 ? V + ((x.stride(0) - V) % units + units) % units : V;
+  return empty_like_on(x, {shift + rows * ld}, x.scalar_type()).as_strided({rows, V}, {ld, 1}, shift);
+}
+
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, int64_t top) {
+    LogprobsOut r = logprobs_fwd(logits, tokens, top, true);
+    ctx->saved_data["top"] = top;
+    ctx->saved_data["rows"] = logits.size(0);
+    ctx->saved_data["vocabulary"] = logits.size(1);
+    ctx->saved_data["fp32"] = logits.scalar_type() == at::kFloat;
+    ctx->set_materialize_grads(false);
+    if (top == 0) {
+      ctx->save_for_backward({logits, tokens, r.stats, r.entropy});
+      return {r.logprobs, r.entropy};
+    }
+    ctx->save_for_backward({logits, tokens, r.stats, r.entropy, r.ids});
+    ctx->mark_non_differentiable({r.ids});
+    return {r.logprobs, r.entropy, r.ids, r.top};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    return node_body("llmctl_token_logprobs_bwd", ready(lib.llmctl_token_logprobs_bwd), [&]() -> torch::autograd::variable_list {
+      const auto saved = ctx->get_saved_variables();
+      const int64_t top = ctx->saved_data["top"].toInt(), rows = ctx->saved_data["rows"].toInt(), V = ctx->saved_data["vocabulary"].toInt();
+      const bool fp32 = ctx->saved_data["fp32"].toBool();
+      const Tensor dlp = grads[0], dh = grads[1], dtop = top ? grads[3] : Tensor();
+      const Tensor& some = dlp.defined() ? dlp : dh.defined() ? dh : dtop;
+      if (!some.defined()) return {Tensor(), Tensor(), Tensor()};
+      constexpr const char* kNode = "TokenLogprobsBackward";
+      came_back(kNode, saved[0], fp32 ? at::kFloat : at::kBFloat16, {rows, V}, some);
+      came_back(kNode, saved[1], at::kLong, {rows}, some);
+      came_back(kNode, saved[2], at::kFloat, {rows, 2}, some);
+      came_back(kNode, saved[3], at::kFloat, {rows}, some);
+      if (top) came_back(kNode, saved[4], at::kLong, {rows, top}, some);
+      Tensor dx;
+      {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const c10::cuda::CUDAGuard guard(some.device());
+        const Tensor x = saved[0].stride(1) == 1 ? saved[0] : saved[0].contiguous(), tokens = saved[1].contiguous(), stats = saved[2].contiguous(), h = saved[3].contiguous(),
+                     ids = top ? saved[4].contiguous() : Tensor();
+        const auto given = [](const Tensor& g) { return g.defined() ? g.to(at::kFloat).contiguous() : Tensor(); };
+        const Tensor g = given(dlp), gh = given(dh), gt = given(dtop);
+        const auto f32 = [](const Tensor& t) { return t.defined() ? static_cast<const float*>(cdata(t)) : nullptr; };
+        dx = rows_like(x);
+        done("llmctl_token_logprobs_bwd",
+             lib.llmctl_token_logprobs_bwd(cdata(x), fp32, x.stride(0), static_cast<const long long*>(cdata(tokens)), static_cast<int>(rows), static_cast<int>(V), static_cast<int>(top), f32(stats),
+                                           f32(h), top ? static_cast<const long long*>(cdata(ids)) : nullptr, f32(g), f32(gh), f32(gt), data(dx), dx.stride(0), stream()));
+      }
+      if (at::GradMode::is_enabled()) {            // asked for with a graph of its own: that one says so if it is walked
+        auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", 1);
+        dx = (*error)({dx.requires_grad_(true)})[0];
+      }
+      return {dx, Tensor(), Tensor()};
+    });
+  }
+};
+
+// token_logprobs(logits, tokens, top) -> (logprobs, entropy, top ids or None, top log probabilities or None)
+PyObject* py_token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return call(a, n, 3, [&](Args& args) -> PyObject* {
+    const Tensor logits = args.tensor(0), tokens = args.tensor(1);
+    const int64_t top = args.integer(2);
+    if (!args.ok || !quiet() || !ready(lib.llmctl_token_logprobs) || (!bf16(logits) && logits.scalar_type() != at::kFloat) || logits.dim() < 1 || logits.numel() == 0 ||
+        logits.stride(-1) != 1 || !here({&logits, &tokens}) || tokens.scalar_type() != at::kLong || !tokens.is_contiguous() || tokens.sizes() != logits.sizes().slice(0, logits.dim() - 1))
+      return none();
+    const int64_t V = logits.size(-1), rows = logits.numel() / V;
+    if (top < 0 || top > 64 || top > V || V >= (1LL << 31) || rows >= (1LL << 31) || (logits.dim() != 2 && !logits.is_contiguous())) return none();
+    LogprobsOut r;
+    without_gil([&] {
+      const bool flat = logits.dim() == 2;
+      const Tensor x = flat ? logits : logits.view({rows, V}), t = flat ? tokens : tokens.view({rows});
+      if (recorded({&logits})) {
+        const auto out = TokenLogprobs::apply(x, t, top);
+        r.logprobs = out[0];
+        r.entropy = out[1];
+        if (top) r.ids = out[2], r.top = out[3];
+      } else {
+        r = logprobs_fwd(x, t, top, false);
+      }
+      if (!flat) {
+        auto lead = tokens.sizes().vec();
+        r.logprobs = r.logprobs.view(lead);
+        r.entropy = r.entropy.view(lead);
+        lead.push_back(top);
+        if (top) r.ids = r.ids.view(lead), r.top = r.top.view(lead);
+      }
+    });
+    PyObject* items[4] = {THPVariable_Wrap(r.logprobs), THPVariable_Wrap(r.entropy), top ? THPVariable_Wrap(r.ids) : nullptr, top ? THPVariable_Wrap(r.top) : nullptr};
+    for (int i = 2; i < 4; ++i)
+      if (!top) {
+        Py_INCREF(Py_None);
+        items[i] = Py_None;
+      }
+    PyObject* tuple = PyTuple_Pack(4, items[0], items[1], items[2], items[3]);
+    for (PyObject* o : items) Py_XDECREF(o);
+    return tuple;
+  });
+}
+
 // ---------------------------------------------------------------------------------------------------------------------------------
 // latent attention
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -1019,7 +1228,8 @@ PyObject* py_launches(PyObject*, PyObject*) { return PyLong_FromLongLong(launche
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"bind", py_bind, METH_VARARGS, nullptr}, {"launches", py_launches, METH_NOARGS, nullptr}, FAST(rmsnorm), FAST(gemm), FAST(linear), FAST(gemm_swiglu),
-                         FAST(mlp), FAST(attention), FAST(rope_attention), FAST(block), FAST(kv_append), FAST(paged_decode), FAST(latent_kv_write), FAST(latent_decode), {nullptr, nullptr, 0, nullptr}};
+                         FAST(mlp), FAST(attention), FAST(rope_attention), FAST(block), FAST(kv_append), FAST(paged_decode), FAST(latent_kv_write), FAST(latent_decode), FAST(rope_kv_append),
+                         FAST(paged_decode_fp8), FAST(token_logprobs), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "llmctl_ops", "Host side of the operators (csrc/torch/ops.cpp)", -1, methods};
 
 }  // namespace

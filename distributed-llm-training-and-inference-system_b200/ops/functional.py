@@ -776,8 +776,15 @@ class _TokenLogprobsFn(torch.autograd.Function):
         return logprobs, entropy, top_ids, top_logprobs
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_logprobs, d_entropy, _, d_top):
+        with torch.no_grad():
+            dx = _TokenLogprobsFn._gradient(ctx, d_logprobs, d_entropy, d_top)
+        if torch.is_grad_enabled():         # asked for with a graph of its own: that one says so if it is walked
+            dx = torch._C._functions.DelayedError("trying to differentiate twice a function that was marked with @once_differentiable", 1)(dx.requires_grad_(True))
+        return dx, None, None
+
+    @staticmethod
+    def _gradient(ctx, d_logprobs, d_entropy, d_top):
         logits, tokens, stats, entropy, top_ids = native.kept(ctx)
         if logits.stride(1) != 1:
             logits = logits.contiguous()
@@ -789,7 +796,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
             native.call("llmctl_token_logprobs_bwd", logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), tokens.data_ptr(), *logits.shape,
                         ctx.top, stats.data_ptr(), entropy.data_ptr(), native.ptr(top_ids), native.ptr(d_logprobs), native.ptr(d_entropy), native.ptr(d_top),
                         dx.data_ptr(), dx.stride(0), native.stream_ptr())
-        return dx, None, None
+        return dx
 
 
 def _token_logprobs_torch(x: torch.Tensor, tokens: torch.Tensor, top: int) -> TokenLogprobs:
@@ -809,6 +816,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     """Log probabilities of ``tokens`` (int64 [...]; a number that is no token of the vocabulary has 0 and no gradient) under ``logits`` [..., vocabulary], the
     entropy of each row and its ``top`` most probable tokens.  ``logits`` are left as they are; gradients of the log probabilities (``top_logprobs`` among
     them) and of the entropy flow back to them.  A row that holds a NaN or +inf, or nothing but -inf, has NaN for each."""
+    if logits.is_cuda and _cfg.elementwise == "native":
+        out = native.fast.token_logprobs(logits, tokens, top)
+        if out is not None:
+            return TokenLogprobs(*out)
     V = logits.shape[-1]
     if tokens.shape != logits.shape[:-1] or tokens.dtype != torch.int64 or tokens.device != logits.device:
         raise ValueError(f"token_logprobs: int64 tokens of sizes {list(logits.shape[:-1])} beside the logits, not {tokens.dtype} {list(tokens.shape)} on {tokens.device}")

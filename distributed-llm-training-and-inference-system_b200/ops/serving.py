@@ -196,6 +196,8 @@ def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
     stand anywhere in the call; where it names a slot more than once the last is kept.  A block whose first row is written begins anew; in any
     other the rows that the call does not write keep what they stand for, in codes of the larger scale where it grows.  NaN and infinities become NaN."""
     kv_heads = heads if kv_heads is None else kv_heads
+    if qkv.is_cuda and native.fast.rope_kv_append(qkv, cos, sin, positions, k_cache, v_cache, slot_mapping, heads, kv_heads, head_dim, k_scale, v_scale) is not None:
+        return qkv
     fp8 = k_cache.dtype == FP8
     T, width = qkv.shape[0], (heads + 2 * kv_heads) * head_dim
     _check(heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and head_dim > 0 and head_dim % 16 == 0, "heads: a multiple of kv_heads; head_dim: a multiple of 16")
@@ -262,8 +264,12 @@ def paged_attention_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     [B], at most ``max_context`` (tokens beyond it, or beyond the table, are left out) -> [B, heads, head_dim].  heads may be a multiple of the cache's heads:
     query head h reads head h // (heads / kv_heads).  A sequence without tokens gets zeros.  What the cache holds behind a sequence's last token does not matter."""
     B, H, D = q.shape
-    blocks, kv_heads, block_size = k_cache.shape[:3]
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    if q.is_cuda and num_splits != 0:
+        out = native.fast.paged_decode_fp8(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, max_context, num_splits or 0, scale)
+        if out is not None:
+            return out
+    blocks, kv_heads, block_size = k_cache.shape[:3]
     _check(not (torch.is_grad_enabled() and q.requires_grad), "paged_attention_decode_fp8 has no backward: call it under no_grad")
     _check_fp8_caches(k_cache, v_cache, k_scale, v_scale, D, q.device)
     _check(H % kv_heads == 0, "heads: a multiple of the cache's")
