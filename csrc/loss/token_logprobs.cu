@@ -90,6 +90,10 @@ __device__ __forceinline__ unsigned long long make_key(float v, int index) {
   return static_cast<unsigned long long>(order) << 32 | (0xffffffffu - static_cast<uint32_t>(index));
 }
 __device__ __forceinline__ int key_index(unsigned long long k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
+__device__ __forceinline__ float key_number(unsigned long long k) {
+  const uint32_t order = static_cast<uint32_t>(k >> 32);
+  return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
+}
 __device__ __forceinline__ unsigned long long key_max(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 __device__ __forceinline__ unsigned long long reduce_key(unsigned long long k, int lanes) {
   for (int o = lanes / 2; o > 0; o >>= 1) k = key_max(k, __shfl_xor_sync(0xffffffffu, k, o));
@@ -305,9 +309,8 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long lon
   }
 
   auto write = [&](int place, unsigned long long k) {
-    const int index = key_index(k);
-    top_ids[row * top + place] = index;
-    top_logprobs[row * top + place] = (as_f32(r.p[index]) - all.m) - log_s;
+    top_ids[row * top + place] = key_index(k);
+    top_logprobs[row * top + place] = (key_number(k) - all.m) - log_s;
   };
   // the top-th largest of the groups' maxima: keys are unlike but for groups without numbers
   if (tid < kGroups) all_keys[tid] = kCluster ? load_cluster_u64(ptx::mapa_u32(ptx::smem_u32(group_key + tid % groups), tid / groups)) : group_key[tid];
@@ -454,10 +457,19 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const long
 }
 
 namespace lp {
-// Rows that are fewer than the CTAs that fit share themselves between CTAs of at least two turns of loads each.
+// CTAs to a row of the forward: its rounds between them (two or three, 0.5 us each) pay where a thread would have 24 units and more.  us by CTAs to a row, 20
+// alternatives: one row of 32000 in 16 bits 1: 7.1, 4: 7.2; 50257 1: 9.5, 2: 8.2, 4: 7.3, 8: 8.0; 130000 1: 17.4, 4: 8.9, 8: 8.7; 256 rows of 32000 1: 8.9,
+// 2: 11.5, of 50257 1: 12.9, 2: 14.0, of 130000 1: 28.5, 2: 24.0.
 static int cluster_of(int rows, int V, int unit) {
+  const int turns = V / unit / kThreads;
+  int c = turns >= 48 ? kMaxCluster : turns >= 24 ? 4 : 1;
+  while (c > 1 && static_cast<long long>(rows) * c > kResident) c /= 2;
+  return c == 2 && turns < 48 ? 1 : c;
+}
+// CTAs to a row of the backward, which share nothing: as many as fit, of two turns of loads each.
+static int parts_of(int rows, int V, int unit) {
   int c = 1;
-  while (c < kMaxCluster && rows * 2 * c <= kResident && V / unit >= 2 * c * kThreads * 2) c *= 2;
+  while (c < kMaxCluster && static_cast<long long>(rows) * 2 * c <= kResident && V / unit >= 2 * c * kThreads * 2) c *= 2;
   return c;
 }
 template <typename T>
@@ -512,7 +524,7 @@ LLMCTL_API int llmctl_token_logprobs_bwd(const void* logits, int is_fp32, long l
                  (rows <= 1 || ((ld - ldd) * size & 15) == 0));
   if (rows == 0) return 0;
   if (top == 0) d_top = nullptr;
-  const dim3 grid(rows, lp::cluster_of(rows, V, is_fp32 ? lp::kUnit<float> : lp::kUnit<__nv_bfloat16>));
+  const dim3 grid(rows, lp::parts_of(rows, V, is_fp32 ? lp::kUnit<float> : lp::kUnit<__nv_bfloat16>));
   if (is_fp32)
     LLMCTL_CHECK(launch_dependent(token_logprobs_bwd_kernel<float>, grid, lp::kThreads, 0, (cudaStream_t)stream, (const float*)logits, ld, tokens, V, top,
                                   stats, entropy, top_ids, d_logprobs, d_entropy, d_top, (float*)dx, ldd));
