@@ -169,9 +169,10 @@ struct Sums {
 };
 }  // namespace lp
 
-// Grid: clusters of `cluster` CTAs, one to a row.
+// Grid: clusters of `cluster` CTAs, one to a row.  As many CTAs to an SM as hide the loads of each other's turns, in few registers: 4096 x 32000 in 16 bits
+// 4: 57.3 us, 6: 50.6, 8: 48.4; in 32 bits 4: 82.6, 5: 82.5, 6: 80.1, 8: 86.3, 2000 x 50257 4: 68.0, 5: 68.5, 6: 71.9.
 template <typename T, bool kCluster>
-__global__ void __launch_bounds__(lp::kThreads, 4)
+__global__ void __launch_bounds__(lp::kThreads, sizeof(T) == 2 ? 8 : 5)
 token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ tokens, int V, int top, float* __restrict__ logprobs,
                       float* __restrict__ entropy, float* __restrict__ stats, long long* __restrict__ top_ids, float* __restrict__ top_logprobs, int cluster) {
   using namespace lp;
