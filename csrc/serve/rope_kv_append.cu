@@ -125,8 +125,8 @@ rope_kv_append_kernel(RopeRows r, uint32_t total, FastDiv per_token, FastDiv per
 // which is left out where the token before goes to the same block (in a prompt, 15 of 16).  Then a lane has one place in one row of the block for
 // all heads, and keeps its token's angles; as many warps as the block's rows need write a head after the other: the largest rotated number, by
 // all of them, the scale, the codes.  The next head's numbers are asked for beside that.  (A warp to a head's block had to read the angles anew for each
-// row and head and rotate twice, for want of registers: 8000 tokens, 40 heads of 128 130 us, so XX.)  Blocks of more rows than 8 warps hold are
-// read twice.  The other CTAs rotate q, four units to a thread.
+// row and head and rotate twice, for want of registers: 8000 tokens, 40 heads of 128 130 us, so XX.)  Blocks of more than twice the rows
+// that 8 warps hold are read twice, by a warp to a head.  The other CTAs rotate q, four units to a thread.
 // ---------------------------------------------------------------------------------------------
 namespace append8 {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
@@ -259,9 +259,9 @@ __device__ __forceinline__ void write_alone(const Block& bk, int task) {
 }
 }  // namespace append8
 
-// kOnce: a block is of no more rows than 8 warps hold.
-template <bool kOnce>
-__global__ void __launch_bounds__(append8::kThreads, 3)
+// kHeld: rows of a block that a lane has a place in (so many of 8 warps' are a block's at most), or 0: blocks of more.
+template <int kHeld>
+__global__ void __launch_bounds__(append8::kThreads, kHeld == 2 ? 2 : 3)
 rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
                           float* __restrict__ k_scale, float* __restrict__ v_scale, int blocks, int block_size, int window, int windows, int parts,
                           uint32_t q_units, FastDiv per_token, FastDiv per_head) {
@@ -382,28 +382,37 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
     Block bk{r, cos_t, sin_t, positions, k_cache + at_block * block_size * r.head_dim, v_cache + at_block * block_size * r.head_dim, k_scale + at_block,
              v_scale + at_block, row_token, row_list, n, block_size, begun};
     const int tasks = 2 * r.kv_heads;
-    if constexpr (!kOnce) {
+    if constexpr (kHeld == 0) {
       for (int task = part + warp * parts; task < tasks; task += kWarps * parts) write_alone(bk, task);
       continue;
     }
 
-    // the lane's place: one of the rows that are written and the token that it is written from, or -1
-    const int i = mine * step + sub;
-    const int row = sub < step && i < n ? row_list[i] : 0, tok = sub < step && i < n ? row_token[row] : -1;
-    __nv_bfloat16* const base = qkv + max(tok, 0) * r.row_stride + static_cast<long long>(r.heads) * r.head_dim;
-    float c[8] = {}, s[8] = {};
-    if (tok >= 0) {
-      const long long table = table_row(r, positions, tok) + at * 8;
-      load_angles(c, s, cos_t + table, sin_t + table);
+    // the lane's places: of the rows that are written one, or one of each half, and the tokens that they are written from, or -1
+    constexpr int R = kHeld > 0 ? kHeld : 1;
+    int row[R], tok[R];
+    __nv_bfloat16* base[R];
+    float c[R][8] = {}, s[R][8] = {};
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int i = (k * together + mine) * step + sub;
+      row[k] = sub < step && i < n ? row_list[i] : 0;
+      tok[k] = sub < step && i < n ? row_token[row[k]] : -1;
+      base[k] = qkv + max(tok[k], 0) * r.row_stride + static_cast<long long>(r.heads) * r.head_dim;
+      if (tok[k] >= 0) {
+        const long long table = table_row(r, positions, tok[k]) + at * 8;
+        load_angles(c[k], s[k], cos_t + table, sin_t + table);
+      }
     }
     // The numbers of the heads to come, kStages - 1 of them, on their way into places that only the lane itself reads.
-    uint8_t* const ring = reinterpret_cast<uint8_t*>(row_list + (block_size + 3) / 4 * 4) + warp * (kStages * 1024) + lane * 16;
+    uint8_t* const ring = reinterpret_cast<uint8_t*>(row_list + (block_size + 3) / 4 * 4) + warp * (kStages * R * 1024) + lane * 16;
     auto ask = [&](int task, int stage) {
-      if (task < tasks && tok >= 0) {
-        const __nv_bfloat16* p = base + task * r.head_dim + (task < r.kv_heads ? at * 8 : at * 16);
-        cp_async_16(ring + stage * 1024, p);
-        cp_async_16(ring + stage * 1024 + 512, p + (task < r.kv_heads ? half : 8));
-      }
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+        if (task < tasks && tok[k] >= 0) {
+          const __nv_bfloat16* p = base[k] + task * r.head_dim + (task < r.kv_heads ? at * 8 : at * 16);
+          cp_async_16(ring + (stage * R + k) * 1024, p);
+          cp_async_16(ring + (stage * R + k) * 1024 + 512, p + (task < r.kv_heads ? half : 8));
+        }
       cp_async_commit();
     };
     const int first = part + group * parts, by = groups * parts;
@@ -426,18 +435,20 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
       constexpr bool key = of_keys.value;     // (known at compile time: what only keys need would be stepped over one by one for values)
       float* const scale_at = bk.scale_of(task);
       const float old = begun ? 0.f : fmaxf(*scale_at, 0.f);
-      float a[8] = {}, b[8] = {};
+      float a[R][8] = {}, b[R][8] = {}, x8 = 0.f;          // rows that are not there hold zeros
       ask(task + (kStages - 1) * by, (stage + kStages - 1) % kStages);
       cp_async_wait<kStages - 1>();
-      if (tok >= 0) {
-        unpack8(*reinterpret_cast<const bf16x8*>(ring + stage * 1024), a);
-        unpack8(*reinterpret_cast<const bf16x8*>(ring + stage * 1024 + 512), b);
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        if (tok[k] >= 0) {
+          unpack8(*reinterpret_cast<const bf16x8*>(ring + (stage * R + k) * 1024), a[k]);
+          unpack8(*reinterpret_cast<const bf16x8*>(ring + (stage * R + k) * 1024 + 512), b[k]);
+        }
+        if (key) rotate8(a[k], b[k], c[k], s[k]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x8 = max_nan(x8, max_nan(fabsf(a[k][j]), fabsf(b[k][j])));
       }
       stage = (stage + 1) % kStages;
-      if (key) rotate8(a, b, c, s);
-      float x8 = 0.f;                         // rows that are not there hold zeros
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x8 = max_nan(x8, max_nan(fabsf(a[j]), fabsf(b[j])));
       const uint32_t most = largest(__float_as_uint(x8) & 0x7fffffffu);
       if (most >= kInfinite) {                // rare, and written behind the others
         if (lane == turns >> 5) later |= 1u << (turns & 31);
@@ -446,13 +457,15 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
       const float need = scale_for(most), scale = fmaxf(need, old), inv = inverse(scale);
       uint8_t* const codes = bk.codes_of(task);
       if (!begun && scale > old) grow(bk, codes, old / scale, mine * 32 + lane, together * 32);
-      if (tok >= 0) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        if (tok[k] < 0) continue;
         if (key) {
-          __nv_bfloat16* dst = base + task * r.head_dim + at * 8;
-          store8(dst, pack8(a));
-          store8(dst + half, pack8(b));
+          __nv_bfloat16* dst = base[k] + task * r.head_dim + at * 8;
+          store8(dst, pack8(a[k]));
+          store8(dst + half, pack8(b[k]));
         }
-        write_codes(codes + row * r.head_dim, key, at, half, a, b, inv);
+        write_codes(codes + row[k] * r.head_dim, key, at, half, a[k], b[k], inv);
       }
       if (together == 1) __syncwarp();        // else they have met since they read it
       if (lane == 0 && mine == 0) *scale_at = scale;
@@ -517,9 +530,12 @@ LLMCTL_API int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int to
   const long long per_token = static_cast<long long>(heads) * (head_dim / 16), units = per_token * tokens;
   LLMCTL_REQUIRE(units < (1LL << 30));
   const int q_ctas = static_cast<int>((units + kThreads * kUnits - 1) / (kThreads * kUnits));
-  const bool once = block_size <= kWarps * (32 / (head_dim / 16));
-  const int smem = (block_size + 3) / 4 * 4 * 2 * static_cast<int>(sizeof(int)) + (once ? kWarps * kStages * 1024 : 0);
-  LLMCTL_CHECK(launch_dependent(once ? rope_kv_append_fp8_kernel<true> : rope_kv_append_fp8_kernel<false>, windows * parts + q_ctas, kThreads, smem, (cudaStream_t)stream, r, slots,
+  const int held = (block_size - 1) / (kWarps * (32 / (head_dim / 16))) + 1;          // rows to a lane
+  const int smem = (block_size + 3) / 4 * 4 * 2 * static_cast<int>(sizeof(int)) + (held <= 2 ? kWarps * kStages * held * 1024 : 0);
+  auto kern = held == 1 ? rope_kv_append_fp8_kernel<1> : held == 2 ? rope_kv_append_fp8_kernel<2> : rope_kv_append_fp8_kernel<0>;
+  const cudaError_t e = allow_smem(kern, smem);
+  if (e != cudaSuccess) LLMCTL_FAIL(e, "shared memory");
+  LLMCTL_CHECK(launch_dependent(kern, windows * parts + q_ctas, kThreads, smem, (cudaStream_t)stream, r, slots,
                                 (uint8_t*)k_cache, (uint8_t*)v_cache, k_scale, v_scale, blocks, block_size, window, windows, parts,
                                 static_cast<uint32_t>(units), FastDiv(static_cast<uint32_t>(per_token)), FastDiv(head_dim / 16)));
   LLMCTL_RETURN_LAST();
