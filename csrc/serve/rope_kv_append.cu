@@ -136,7 +136,7 @@ constexpr int kStages = 4;                   // heads under way (1: 8000 tokens,
 constexpr uint32_t kInfinite = 0x7f800000u;
 // CTAs that write blocks: one wave of them, or two to a block.  us by CTAs to a block: 64 decoded tokens, 32 heads of 128 5: 6.6, 8: 8.1; 1000 tokens 5: 14.3, 8:
 // 17.2, 10: 16.3, 16: 18.2; 4000 1: 52.3, 2: 50.7, 3: 49.2; 8000, 40 heads 1: 111, 2: 106.  (Each looks through all slots.)
-constexpr int kResident = 3 * kNumSMs;
+constexpr int resident(int held) { return (held == 2 ? 2 : 3) * kNumSMs; }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -525,12 +525,12 @@ LLMCTL_API int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int to
   const int window = tokens > 256 ? 16 : 1, windows = (tokens + window - 1) / window;
   // A block to each token where they may all be of other sequences, else to each block_size of them.
   const int writers = tokens > 256 ? (tokens + block_size - 1) / block_size : tokens, most = tokens > 256 ? kv_heads : (2 * kv_heads + kWarps - 1) / kWarps;
-  int parts = writers <= kResident / 2 ? kResident / writers : 2;
+  const int held = (block_size - 1) / (kWarps * (32 / (head_dim / 16))) + 1;          // rows to a lane
+  int parts = writers <= resident(held) / 2 ? resident(held) / writers : 2;
   if (parts > most) parts = most;
   const long long per_token = static_cast<long long>(heads) * (head_dim / 16), units = per_token * tokens;
   LLMCTL_REQUIRE(units < (1LL << 30));
   const int q_ctas = static_cast<int>((units + kThreads * kUnits - 1) / (kThreads * kUnits));
-  const int held = (block_size - 1) / (kWarps * (32 / (head_dim / 16))) + 1;          // rows to a lane
   const int smem = (block_size + 3) / 4 * 4 * 2 * static_cast<int>(sizeof(int)) + (held <= 2 ? kWarps * kStages * held * 1024 : 0);
   auto kern = held == 1 ? rope_kv_append_fp8_kernel<1> : held == 2 ? rope_kv_append_fp8_kernel<2> : rope_kv_append_fp8_kernel<0>;
   const cudaError_t e = allow_smem(kern, smem);
