@@ -217,7 +217,7 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
   if (threadIdx.x == 0) {
     mbar_init(&bar_q, 4);
     for (int i = 0; i < stages; ++i) {
-      mbar_init(&bar_full[i], 2);
+      mbar_init(&bar_full[i], 4);                         // copies and scales of keys and of values
       mbar_init(&bar_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -285,15 +285,16 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
       const float next_scale = scale_of(scales, next);
       const bool given = loaded < stages || mbar_wait_bounded(&bar_empty[st], at.phase ^ 1u, abort);
       if (!__all_sync(0xffffffffu, given)) break;
-      if (lane < kMaxBoxes) box_scale[st][keys ? 0 : 1][lane] = keys ? scale : __log2f(scale);
       const int count = __popc(__ballot_sync(0xffffffffu, box.row >= 0));
-      __syncwarp();                                       // the scales are there for whom the barrier lets through
       if (lane == 0) mbar_expect_tx(&bar_full[st], count * box_rows * D);
       __syncwarp();
       if (box.row >= 0) {
         const int row = box.block >= 0 && box.block < blocks ? (box.block * kv_heads + box.head) * block_size + box.row : all_rows;
         tma_load_2d(smem + st * kStage + (keys ? 0 : kHalf) + lane * box_rows * D, tm, &bar_full[st], 0, row);
       }
+      if (lane < kMaxBoxes) box_scale[st][keys ? 0 : 1][lane] = keys ? scale : __log2f(scale);       // (the first copies do not wait for them)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_full[st]);
       box = next;
       next = after;
       scale = next_scale;
