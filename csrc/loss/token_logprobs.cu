@@ -9,6 +9,10 @@
 // reaches it are looked through again (of 32000 numbers some 25 are candidates for 20 places), and a candidate's rank is the number of
 // larger ones.  All sums in fp32.
 //
+// 2000 x 50257 in 32 bits 68 us (5.9 TB/s: the pass over the logits bounds it), 4096 x 32000 bf16 48 us (5.4 TB/s; instructions and exponentials are as near: two
+// thirds of either's rate), 64 x 32000 with 5 alternatives 6.3 us, one row with 20 6.9 us (the chain of a cluster's exchanges).
+// Backward: 4096 x 32000 bf16 86 us (6.1 TB/s over logits and their gradient).
+//
 // Reference: none — the reference offers neither (its server returns text alone, reference llmctl/serve/server.py:57-75).
 #include <type_traits>
 
@@ -195,7 +199,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long lon
   auto unit = [&](int i) { return r.p + r.head + static_cast<long long>(i) * U; };
 
   // Numbers are met in the order of their indices: before the first 16-byte boundary, units, the rest.  The reference moves once in kAhead units (some lane of a
-  // warp has a new maximum in nearly each of a row's first, and the others wait: 4096 x 32000 76 us with a look at every unit, XX so); the unit of the
+  // warp has a new maximum in nearly each of a row's first, and the others wait: 4096 x 32000 76 us with a look at every unit, 64.9 so); the unit of the
   // maximum is kept, its place in it is looked up at the end.
   Sums a;
   int best = tid < head ? tid : -1, best_unit = tid >= head && lo + tid < hi ? lo + tid : -1;      // where the maximum stands, one of the two

@@ -21,6 +21,9 @@
 // batches of unlike contexts end together; a sequence and head that more than one CTA has a part of is merged by a second kernel.
 // Where contexts are of a few tiles only the runs are cut between heads, and nothing is merged.
 //
+// Bound by the pass over the cache, 6.5 - 6.9 TB/s of it once all CTAs are under way, and by 6 - 8 us of start, last tiles and merge.  us: 4 contexts of up to
+// 50001, 32 heads of 128 over 8 180 (6.6 TB/s), 16 of up to 4096, 32 heads 60.6 (5.8), 64 of 1000 to 4000, 32 over 8 63.7 (5.3), one of 300 5.7.
+//
 // Every wait is bounded, as in latent_attention_t5.cu.
 // Reference: none.
 #include "../common/dependent.cuh"
@@ -76,7 +79,7 @@ __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t* r) {
 }
 
 // Place in the ring of stages.  (A quotient and a remainder by a number known at launch are 200 clocks in the issuing warp's way, three of them in
-// each turn of its loop: 2600 clocks a tile, 16 contexts up to 4096, 32 heads 66.1 us instead of XX.)
+// each turn of its loop: 2600 clocks a tile, 16 contexts up to 4096, 32 heads 66.1 us, so 62.2.)
 struct Place {
   int st = 0;
   uint32_t phase = 0;
@@ -169,7 +172,8 @@ struct Items {
     if (r.left > 0) skip(w);
   }
   __device__ __forceinline__ void skip(const Work& w) {          // sequences without tokens
-    while ((tokens = w.tokens(r.b)) == 0) ++r.b, r.x = 0;
+    while (r.b < w.batch && (tokens = w.tokens(r.b)) == 0) ++r.b, r.x = 0;
+    if (r.b >= w.batch) r.left = 0;                      // (lengths that change meanwhile)
     nt = (tokens + kTile - 1) / kTile;
     n = min(nt - r.t, r.left);
   }
