@@ -42,7 +42,7 @@ CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-I",
 #: sub-directories (or single files) of csrc/ per component; None = everything
 _SERVE_COMMON = ["common", "gemm", "activation", "moe", "comm/watchdog.cu"]    # the gated GEMM modes report expired flag waits through the watchdog
 COMPONENTS = {
-    "serve": _SERVE_COMMON + ["norm", "rope", "swiglu", "serve", "attention/latent_attention.cu", "attention/latent_attention_t5.cu", "attention/latent_decode.cu",
+    "serve": _SERVE_COMMON + ["norm", "rope", "swiglu", "serve", "loss/token_logprobs.cu", "attention/latent_attention.cu", "attention/latent_attention_t5.cu", "attention/latent_decode.cu",
                               "attention/latent_prompt.cu", "attention/flash_fwd.cu",
                               "attention/pooled_window_attention.cu", "attention/pooled_window_attention_mma.cu", "attention/qkv_write.cu",
                               "attention/diff_attention.cu", "attention/softcap_window_attention.cu", "recurrent"],
