@@ -189,7 +189,7 @@ def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
                    slot_mapping: torch.Tensor, heads: int, head_dim: int, *, kv_heads: Optional[int] = None, k_scale: Optional[torch.Tensor] = None,
                    v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotates q and k of the packed rows ``qkv`` [T, (heads + 2 kv_heads) * head_dim] in place to their ``positions`` (int32 [T], rows of the tables ``cos`` /
-    ``sin``, fp32 [positions, head_dim / 2]) and writes k and v to the rows ``slot_mapping`` (int64 [T]; outside of the cache = skip) of the caches:
+    ``sin``, fp32 [positions, head_dim / 2]; one outside of them reads the nearest) and writes k and v to the rows ``slot_mapping`` (int64 [T]; outside of the cache = skip) of the caches:
     [blocks, block_size, kv_heads, head_dim] of the rows' type, or caches of 8 bits with their scales.  Returns ``qkv``.
 
     Where the call names a row of a cache of 16 bits more than once any of its tokens is kept.  In a cache of 8 bits a block's scale is the smallest power of two under which the largest number written to it fits.  The tokens of a block may

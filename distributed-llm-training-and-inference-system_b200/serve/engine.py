@@ -320,13 +320,17 @@ class InferenceEngine:
         self._graphs: Dict[Tuple[int, int], "_DecodeGraph"] = {}
         self._staging: Dict[Tuple[int, int], "_DecodeInputs"] = {}
 
+    def check_logprobs(self, logprobs: Optional[int]) -> None:
+        most = min(ops.MAX_TOP_LOGPROBS, self.cfg.vocab_size)
+        if logprobs is not None and not 0 <= logprobs <= most:
+            raise ValueError(f"logprobs: 0 to {most} alternatives, not {logprobs}")
+
     # ---- request API ---------------------------------------------------------------------------------
     def add_request(self, prompt_ids: List[int], max_tokens: int = 100, temperature: float = 1.0, top_p: float = 1.0,
                     top_k: int = -1, on_token=None, logprobs: Optional[int] = None) -> Sequence:
         """``logprobs``: the sequence's ``token_logprobs`` get each generated token's log probability under the model (before temperature, top_k and top_p), the
         entropy and that many of the most probable tokens."""
-        if logprobs is not None and not 0 <= logprobs <= min(ops.MAX_TOP_LOGPROBS, self.cfg.vocab_size):
-            raise ValueError(f"logprobs: 0 to {min(ops.MAX_TOP_LOGPROBS, self.cfg.vocab_size)} alternatives, not {logprobs}")
+        self.check_logprobs(logprobs)
         if not prompt_ids:
             prompt_ids = [self.tokenizer.bos_token_id if getattr(self.tokenizer, "bos_token_id", None) is not None else 0]
         limit = self.cfg.max_position_embeddings

@@ -58,6 +58,7 @@ class LockstepEngine:
                     top_k: int = -1, on_token=None, logprobs: Optional[int] = None) -> Sequence:
         """Queue a request; it is admitted on every rank at the start of the next step.  Blocks the calling (HTTP
         worker) thread until then, i.e. for at most one engine step."""
+        self.engine.check_logprobs(logprobs)                 # here, and not where every rank applies it
         holder: Dict[str, Any] = {"event": threading.Event(), "seq": None, "on_token": on_token}
         with self._lock:
             self._pending.append(((list(prompt_ids), int(max_tokens), float(temperature), float(top_p), int(top_k), logprobs), holder))

@@ -173,7 +173,7 @@ class InferenceServer:
 
     def _submit(self, req: GenerationRequest, on_token=None):
         ids = self.engine.tokenizer.encode(req.prompt)
-        more = {} if req.logprobs is None else {"logprobs": req.logprobs}
+        more = {} if req.logprobs is None else {"logprobs": min(req.logprobs, self.engine.cfg.vocab_size)}
         seq = self.engine.add_request(ids, req.max_tokens, req.temperature, req.top_p, req.top_k, on_token=on_token, **more)
         rid = str(uuid.uuid4())
         self.active_requests[rid] = RequestState(rid, seq)

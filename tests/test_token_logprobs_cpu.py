@@ -122,6 +122,9 @@ def test_lockstep_engine_passes_log_probabilities_on():
     lock = lockstep.LockstepEngine.__new__(lockstep.LockstepEngine)
     lock.engine, lock._lock, lock._pending, lock.on_pending = eng, threading.Lock(), [], None
     got = []
+    with pytest.raises(ValueError, match="logprobs"):
+        lock.add_request([5, 6], 3, 0.0, logprobs=99)
+    assert not lock._pending
     t = threading.Thread(target=lambda: got.append(lock.add_request([5, 6], 3, 0.0, logprobs=1)))
     t.start()
     while not lock._pending:

@@ -201,6 +201,22 @@ def test_leading_dimensions_and_strides(ops):
     assert torch.equal(one.top_ids, flat.top_ids[:1].expand(6, 2))
 
 
+def test_gradients_of_broadcast_and_shared_logits(ops):
+    """One row under six tokens, and a row used twice: its gradient is the sum of theirs."""
+    x, tokens, g = _logits(1, 500, torch.float32).requires_grad_(True), _tokens(6, 500), torch.randn(6, device="cuda")
+    dx, = torch.autograd.grad(ops.token_logprobs(x.expand(6, 500), tokens).logprobs, x, g)
+    rows, = torch.autograd.grad(ops.token_logprobs(x.repeat(6, 1), tokens).logprobs, x, g)
+    assert torch.allclose(dx, rows, rtol=1e-5, atol=1e-7) and dx.shape == (1, 500)
+    y = x * 2
+    both, = torch.autograd.grad(ops.token_logprobs(y, tokens[:1]).logprobs.sum() + ops.token_logprobs(y, tokens[:1], 3).entropy.sum(), x)
+    want = torch.log_softmax(x.detach().double() * 2, -1)
+    p = want.exp()
+    h = -(p * want).sum()
+    ref = -p * (1 + want + h)
+    ref[0, tokens[0]] += 1
+    assert (both.double() - 2 * ref).abs().max() <= 1e-5
+
+
 def test_saved_logits_that_a_hook_changes_are_refused(ops):
     x, tokens = _logits(3, 100, torch.bfloat16).requires_grad_(True), _tokens(3, 100)
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.float() if t.dtype == torch.bfloat16 else t):
