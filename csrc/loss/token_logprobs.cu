@@ -509,7 +509,7 @@ using namespace llmctl;
 LLMCTL_API int llmctl_token_logprobs(const void* logits, int is_fp32, long long ld, const long long* tokens, int rows, int V, int top, float* logprobs,
                                      float* entropy, float* stats, long long* top_ids, float* top_logprobs, void* stream) {
   LLMCTL_BEGIN();
-  LLMCTL_REQUIRE(rows >= 0 && V >= 1 && top >= 0 && top <= lp::kMaxTop && top <= V && (top == 0 || (top_ids != nullptr && top_logprobs != nullptr)));
+  LLMCTL_REQUIRE(rows >= 0 && V >= 1 && V <= 0x7fffffff - 4096 && top >= 0 && top <= lp::kMaxTop && top <= V && (top == 0 || (top_ids != nullptr && top_logprobs != nullptr)));
   LLMCTL_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (is_fp32 ? 4 : 2) == 0);
   if (rows == 0) return 0;
   cudaStream_t s = (cudaStream_t)stream;

@@ -22,7 +22,7 @@
 // Where contexts are of a few tiles only the runs are cut between heads, and nothing is merged.
 //
 // Bound by the pass over the cache, 6.5 - 6.9 TB/s of it once all CTAs are under way, and by 6 - 8 us of start, last tiles and merge.  us: 4 contexts of up to
-// 50001, 32 heads of 128 over 8 180 (6.6 TB/s), 16 of up to 4096, 32 heads 60.6 (5.8), 64 of 1000 to 4000, 32 over 8 63.7 (5.3), one of 300 5.7.
+// 50001, 32 heads of 128 180 (6.6 TB/s), 16 of up to 4096, 32 heads 60.6 (5.8), 64 of 1000 to 4000, 32 over 8 63.7 (5.3), one of 300 5.7.
 //
 // Every wait is bounded, as in latent_attention_t5.cu.
 // Reference: none.

@@ -75,7 +75,7 @@ __device__ __forceinline__ long long table_row(const RopeRows& r, const int* pos
 
 // ---------------------------------------------------------------------------------------------
 // 16 bits: a thread takes 16 numbers of a head, eight pairs of q and k or 16 neighbours of v.  Bound by the pass over the rows:
-// 2000 tokens, 32 heads of 128 19.0 us, 5.4 TB/s.  (Two such pieces to a thread: more registers, fewer threads on the chip, slower.)
+// 1777 tokens, 32 heads of 128 19.0 us, 5.4 TB/s.  (Two such pieces to a thread: more registers, fewer threads on the chip, slower.)
 // ---------------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256)
 rope_kv_append_kernel(RopeRows r, uint32_t total, FastDiv per_token, FastDiv per_head, const long long* __restrict__ slots,

@@ -189,12 +189,13 @@ def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
                    slot_mapping: torch.Tensor, heads: int, head_dim: int, *, kv_heads: Optional[int] = None, k_scale: Optional[torch.Tensor] = None,
                    v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotates q and k of the packed rows ``qkv`` [T, (heads + 2 kv_heads) * head_dim] in place to their ``positions`` (int32 [T], rows of the tables ``cos`` /
-    ``sin``, fp32 [positions, head_dim / 2]; one outside of them reads the nearest) and writes k and v to the rows ``slot_mapping`` (int64 [T]; outside of the cache = skip) of the caches:
-    [blocks, block_size, kv_heads, head_dim] of the rows' type, or caches of 8 bits with their scales.  Returns ``qkv``.
+    ``sin``, fp32 [positions, head_dim / 2]; one outside of them reads the nearest) and writes k and v to the rows ``slot_mapping`` (int64 [T]; outside of the
+    cache = skip) of the caches: [blocks, block_size, kv_heads, head_dim] of the rows' type, or caches of 8 bits with their scales.  Returns ``qkv``.
 
-    Where the call names a row of a cache of 16 bits more than once any of its tokens is kept.  In a cache of 8 bits a block's scale is the smallest power of two under which the largest number written to it fits.  The tokens of a block may
-    stand anywhere in the call; where it names a slot more than once the last is kept.  A block whose first row is written begins anew; in any
-    other the rows that the call does not write keep what they stand for, in codes of the larger scale where it grows.  NaN and infinities become NaN."""
+    In a cache of 16 bits a row that the call names more than once is left with numbers of any of those tokens, of several perhaps: name it once, as with
+    ``kv_append``.  In a cache of 8 bits the last is kept.  There a block's scale is the smallest power of two under which the largest number
+    written to it fits, and the tokens of a block may stand anywhere in the call.  A block whose first row is written begins anew; in any other
+    the rows that the call does not write keep what they stand for, in codes of the larger scale where it grows.  NaN and infinities become NaN."""
     kv_heads = heads if kv_heads is None else kv_heads
     if qkv.is_cuda and native.fast.rope_kv_append(qkv, cos, sin, positions, k_cache, v_cache, slot_mapping, heads, kv_heads, head_dim, k_scale, v_scale) is not None:
         return qkv

@@ -75,7 +75,7 @@ class PluginRegistry:
 
 def _register_builtins(reg: PluginRegistry) -> None:
     from ..ops import functional as ops
-    for name in ("rmsnorm", "layernorm", "rope_packed", "swiglu", "linear", "cross_entropy", "attention", "gemm_raw"):
+    for name in ("rmsnorm", "layernorm", "rope_packed", "swiglu", "linear", "cross_entropy", "token_logprobs", "attention", "gemm_raw"):
         reg.register("kernels", name, getattr(ops, name), overwrite=True)
 
     class NativeScheduler:
