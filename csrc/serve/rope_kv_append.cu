@@ -129,8 +129,8 @@ rope_kv_append_kernel(RopeRows r, uint32_t total, FastDiv per_token, FastDiv per
 // row and head and rotate twice, for want of registers: 8000 tokens, 40 heads of 128 130 us, so 112.)  Blocks of more than twice the rows
 // that 8 warps hold are read twice, by a warp to a head.  The other CTAs rotate q, four units to a thread.
 //
-// Prompts are bound by instructions beside the pass (two rotated rows a lane, maximum, codes; 2 instructions a clock and SM): 8000 tokens, 40 heads of 128 106 us,
-// 4.6 TB/s.  Decoded tokens by the chain slots - block's codes - maximum - codes: one 3.6 us, 64 with 32 heads 6.9.
+// Prompts are bound by instructions beside the pass (two rotated rows a lane, maximum, codes; 2 instructions a clock and SM): 8000 tokens, 40 heads of 128 99 us,
+// 5.0 TB/s, 60000 of 32 heads 560 (5.3).  Decoded tokens by the chain slots - block's codes - maximum - codes: one 3.6 us, 64 with 32 heads 6.9.
 // ---------------------------------------------------------------------------------------------
 namespace append8 {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
@@ -138,8 +138,9 @@ constexpr int kUnits = 4;                    // of q, to a thread
 constexpr int kMaxBlock = 4096;
 constexpr int kStages = 4;                   // heads under way (1: 8000 tokens, 40 heads of 128 142 us)
 constexpr uint32_t kInfinite = 0x7f800000u;
-// CTAs that write blocks: one wave of them, or two to a block.  us by CTAs to a block: 64 decoded tokens, 32 heads of 128 5: 6.6, 8: 8.1; 1000 tokens 5: 14.3, 8:
-// 17.2, 10: 16.3, 16: 18.2; 4000 1: 52.3, 2: 50.7, 3: 49.2; 8000, 40 heads 1: 111, 2: 106.  (Each looks through all slots.)
+// CTAs that write blocks: one wave of them, else two to a block, or one where that is several waves or little work for each.  us by CTAs to a block: 64 decoded
+// tokens, 32 heads of 128 5: 6.6, 8: 8.1; 1000 tokens 6: 13.7, 8: 16.6, 4: 15.5; 4000 1: 49.6, 2: 46.5, 3: 46.6; 60000 1: 561, 2: 592; 12 heads of 64 4000 1:
+// 13.4, 2: 14.8; 8000 1: 22.7, 2: 25.0; 60000 1: 139, 2: 177; 8000, 40 heads 1: 104, 2: 98.7, 3: 104.
 constexpr int resident(int held) { return (held == 2 ? 2 : 3) * kNumSMs; }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -153,6 +154,12 @@ __device__ __forceinline__ float scale_for(uint32_t most) {
   const int e = static_cast<int>(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u ? 1 : 0);
   return __uint_as_float(static_cast<uint32_t>(max(e, 1)) << 23);
 }
+// Of long prompts a kernel before this one marks which blocks each window of kMarked tokens writes to, in a table of 1024 bits by a hash of the
+// block: who looks for a block's tokens then looks through the few windows that have its bit.  (All of the call's slots for each of its blocks
+// are work in the square of its length.)  us without / with marks: 2100 tokens, 32 heads of
+// 128 25.5 / 26.3, 4000 51.5 / 46.6, 8000 89.5 / 82.4, 60000 1350 / 575; 12 heads of 64 8.9 / 9.4, 19.2 / 14.8, 31.9 / 25.2, 624 / 177.
+constexpr int kMarked = 256, kMarkWords = 32, kMarkedFrom = 3000;
+__device__ __forceinline__ uint32_t mark_of(uint32_t block) { return block * 2654435761u >> 22; }
 // 1 / scale, 0 for 0: exact for the powers of two that this file writes
 __device__ __forceinline__ float inverse(float scale) {
   const uint32_t u = __float_as_uint(scale);
@@ -263,10 +270,27 @@ __device__ __forceinline__ void write_alone(const Block& bk, int task) {
 }
 }  // namespace append8
 
+__global__ void __launch_bounds__(append8::kMarked)
+rope_kv_append_marks_kernel(const long long* __restrict__ slots, int tokens, long long rows, int block_size, uint32_t* __restrict__ marks) {
+  using namespace append8;
+  __shared__ uint32_t words[kMarkWords];
+  wait_for_previous(slots, marks);
+  release_dependents();
+  if (threadIdx.x < kMarkWords) words[threadIdx.x] = 0u;
+  __syncthreads();
+  const long long i = static_cast<long long>(blockIdx.x) * kMarked + threadIdx.x, slot = i < tokens ? slots[i] : -1;
+  if (slot >= 0 && slot < rows) {
+    const uint32_t mark = mark_of(static_cast<uint32_t>(slot / block_size));
+    atomicOr(&words[mark >> 5], 1u << (mark & 31u));
+  }
+  __syncthreads();
+  if (threadIdx.x < kMarkWords) marks[static_cast<long long>(blockIdx.x) * kMarkWords + threadIdx.x] = words[threadIdx.x];
+}
+
 // kHeld: rows of a block that a lane has a place in (so many of 8 warps' are a block's at most), or 0: blocks of more.
 template <int kHeld>
 __global__ void __launch_bounds__(append8::kThreads, kHeld == 2 ? 2 : 3)
-rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
+rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, const uint32_t* __restrict__ marks, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
                           float* __restrict__ k_scale, float* __restrict__ v_scale, int blocks, int block_size, int window, int windows, int parts,
                           uint32_t q_units, FastDiv per_token, FastDiv per_head) {
   using namespace append8;
@@ -277,7 +301,7 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
   __nv_bfloat16* qkv = r.qkv;
   const float *cos_t = r.cos_t, *sin_t = r.sin_t;
   const int* positions = r.positions;
-  wait_for_previous(qkv, cos_t, sin_t, positions, slots, k_cache, v_cache, k_scale, v_scale);
+  wait_for_previous(qkv, cos_t, sin_t, positions, slots, marks, k_cache, v_cache, k_scale, v_scale);
   release_dependents();
   const int half = r.head_dim >> 1, per_row = r.head_dim >> 4;      // lanes to a row: eight pairs, or 16 neighbours, each
   const int work = static_cast<int>(blockIdx.x);
@@ -358,25 +382,45 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, uint8
         if (atomicMax(&row_token[s - lo], i) >= 0) twice = 1;
       }
     };
-    const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(slots) >> 3 & 1u);      // a slot before the first 16-byte boundary
-    if (threadIdx.x == 0 && odd != 0) meet(0, slots[0]);
-    const longlong2* two = reinterpret_cast<const longlong2*>(slots + odd);
-    const int pairs = (r.tokens - odd) >> 1;
+    const uint32_t mark = mark_of(static_cast<uint32_t>(block));
+    const int groups_marked = (r.tokens - 1) / kMarked + 1;
+    auto marked = [&](int g) { return (marks[static_cast<long long>(g) * kMarkWords + (mark >> 5)] >> (mark & 31u) & 1u) != 0u; };
+    if (marks != nullptr) {
+      for (int g0 = 0; g0 < groups_marked; g0 += kThreads) {
+        const int g = g0 + lane * kWarps + warp;
+        for (unsigned hit = __ballot_sync(0xffffffffu, g < groups_marked && marked(g)); hit != 0u; hit &= hit - 1u) {
+          const int from = (g0 + (__ffs(hit) - 1) * kWarps + warp) * kMarked + lane;
+          long long s[kMarked / 32];
+#pragma unroll
+          for (int k = 0; k < kMarked / 32; ++k) s[k] = from + k * 32 < r.tokens ? slots[from + k * 32] : -1;
+#pragma unroll
+          for (int k = 0; k < kMarked / 32; ++k) meet(from + k * 32, s[k]);
+        }
+      }
+    } else {
+      const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(slots) >> 3 & 1u);      // a slot before the first 16-byte boundary
+      if (threadIdx.x == 0 && odd != 0) meet(0, slots[0]);
+      const longlong2* two = reinterpret_cast<const longlong2*>(slots + odd);
+      const int pairs = (r.tokens - odd) >> 1;
 #pragma unroll 8
-    for (int i = threadIdx.x; i < pairs; i += kThreads) {
-      const longlong2 s = two[i];
-      meet(odd + 2 * i, s.x);
-      meet(odd + 2 * i + 1, s.y);
+      for (int i = threadIdx.x; i < pairs; i += kThreads) {
+        const longlong2 s = two[i];
+        meet(odd + 2 * i, s.x);
+        meet(odd + 2 * i + 1, s.y);
+      }
+      if (threadIdx.x == 0 && (r.tokens - odd) % 2 != 0) meet(r.tokens - 1, slots[r.tokens - 1]);
     }
-    if (threadIdx.x == 0 && (r.tokens - odd) % 2 != 0) meet(r.tokens - 1, slots[r.tokens - 1]);
     __syncthreads();
     if (first_token != t) continue;
     for (int i = threadIdx.x; i < block_size; i += kThreads)
       if (row_token[i] >= 0) row_list[atomicAdd(&written, 1)] = i;          // in whatever order: rows do not depend on each other
     if (twice)
-      for (int i = 0; i < r.tokens; ++i) {
-        const long long s = slots[i];
-        if (s >= lo && s < hi && row_token[s - lo] != i) rotate_keys(i);
+      for (int g = 0; g < groups_marked; ++g) {
+        if (marks != nullptr && !marked(g)) continue;
+        for (int i = g * kMarked; i < min(r.tokens, (g + 1) * kMarked); ++i) {
+          const long long s = slots[i];
+          if (s >= lo && s < hi && row_token[s - lo] != i) rotate_keys(i);
+        }
       }
     __syncthreads();
     const int n = written, together = warps_together(n, step), groups = kWarps / together, group = warp / together, mine = warp - group * together;
@@ -516,10 +560,17 @@ LLMCTL_API int llmctl_rope_kv_append(void* qkv, long long row_stride, int tokens
   LLMCTL_RETURN_LAST();
 }
 
-// The same into caches [blocks, kv_heads, block_size, head_dim] of e4m3 codes with scales [blocks, kv_heads] (fp32): see the top of this file.
+// Scratch of the call below in 32-bit words; 0: none.
+LLMCTL_API long long llmctl_rope_kv_append_fp8_scratch_elems(int tokens) {
+  using namespace append8;
+  return tokens < kMarkedFrom ? 0 : static_cast<long long>((tokens - 1) / kMarked + 1) * kMarkWords;
+}
+
+// The same into caches [blocks, kv_heads, block_size, head_dim] of e4m3 codes with scales [blocks, kv_heads] (fp32): see the top of this file.  Without
+// scratch (null) it does the same, in the square of the time.
 LLMCTL_API int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int tokens, int heads, int kv_heads, int head_dim, const float* cos_t,
                                          const float* sin_t, int table_rows, const int* positions, const long long* slots, void* k_cache, void* v_cache,
-                                         float* k_scale, float* v_scale, int blocks, int block_size, void* stream) {
+                                         float* k_scale, float* v_scale, int blocks, int block_size, void* scratch, void* stream) {
   LLMCTL_BEGIN();
   using namespace append8;
   const RopeRows r{static_cast<__nv_bfloat16*>(qkv), row_stride, tokens, heads, kv_heads, head_dim, cos_t, sin_t, table_rows, positions};
@@ -530,7 +581,7 @@ LLMCTL_API int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int to
   // A block to each token where they may all be of other sequences, else to each block_size of them.
   const int writers = tokens > 256 ? (tokens + block_size - 1) / block_size : tokens, most = tokens > 256 ? kv_heads : (2 * kv_heads + kWarps - 1) / kWarps;
   const int held = (block_size - 1) / (kWarps * (32 / (head_dim / 16))) + 1;          // rows to a lane
-  int parts = writers <= resident(held) / 2 ? resident(held) / writers : 2;
+  int parts = writers <= resident(held) / 2 ? resident(held) / writers : writers >= 4 * resident(held) || kv_heads <= 2 * kWarps ? 1 : 2;
   if (parts > most) parts = most;
   const long long per_token = static_cast<long long>(heads) * (head_dim / 16), units = per_token * tokens;
   LLMCTL_REQUIRE(units < (1LL << 30));
@@ -539,7 +590,11 @@ LLMCTL_API int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int to
   auto kern = held == 1 ? rope_kv_append_fp8_kernel<1> : held == 2 ? rope_kv_append_fp8_kernel<2> : rope_kv_append_fp8_kernel<0>;
   const cudaError_t e = allow_smem(kern, smem);
   if (e != cudaSuccess) LLMCTL_FAIL(e, "shared memory");
-  LLMCTL_CHECK(launch_dependent(kern, windows * parts + q_ctas, kThreads, smem, (cudaStream_t)stream, r, slots,
+  const uint32_t* marks = tokens < kMarkedFrom ? nullptr : static_cast<const uint32_t*>(scratch);
+  if (marks != nullptr)
+    LLMCTL_CHECK(launch_dependent(rope_kv_append_marks_kernel, (tokens - 1) / kMarked + 1, kMarked, 0, (cudaStream_t)stream, slots, tokens,
+                                  static_cast<long long>(blocks) * block_size, block_size, static_cast<uint32_t*>(scratch)));
+  LLMCTL_CHECK(launch_dependent(kern, windows * parts + q_ctas, kThreads, smem, (cudaStream_t)stream, r, slots, marks,
                                 (uint8_t*)k_cache, (uint8_t*)v_cache, k_scale, v_scale, blocks, block_size, window, windows, parts,
                                 static_cast<uint32_t>(units), FastDiv(static_cast<uint32_t>(per_token)), FastDiv(head_dim / 16)));
   LLMCTL_RETURN_LAST();

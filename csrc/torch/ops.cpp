@@ -46,7 +46,7 @@ using at::Tensor;
   X(llmctl_rmsnorm_fwd) X(llmctl_rmsnorm_bwd_bf16w) X(llmctl_rope_inplace) X(llmctl_gemm_rope_bf16) X(llmctl_gemm_bf16) X(llmctl_gemm_swiglu_bf16)               \
   X(llmctl_gemm_swiglu_bwd_bf16) X(llmctl_swiglu_bwd) X(llmctl_gemm_skinny_bf16) X(llmctl_gemm_skinny_scratch_elems) X(llmctl_flash_attn_fwd) X(llmctl_flash_attn_bwd) X(llmctl_kv_append) \
   X(llmctl_paged_attn_decode) X(llmctl_paged_attn_scratch_elems) X(llmctl_latent_kv_write) X(llmctl_latent_decode) \
-  X(llmctl_rope_kv_append) X(llmctl_rope_kv_append_fp8) X(llmctl_paged_attn_decode_fp8) X(llmctl_paged_attn_fp8_scratch_elems) X(llmctl_token_logprobs) X(llmctl_token_logprobs_bwd)
+  X(llmctl_rope_kv_append) X(llmctl_rope_kv_append_fp8) X(llmctl_rope_kv_append_fp8_scratch_elems) X(llmctl_paged_attn_decode_fp8) X(llmctl_paged_attn_fp8_scratch_elems) X(llmctl_token_logprobs) X(llmctl_token_logprobs_bwd)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
   LLMCTL_ENTRIES(X)
@@ -953,7 +953,7 @@ PyObject* py_rope_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto f32 = [](const Tensor& x) { return static_cast<const float*>(cdata(x)); };
     const bool fp8 = ks.defined() && vs.defined();
     if (fp8) {
-      if (!ready(lib.llmctl_rope_kv_append_fp8) || !here({&ks, &vs}) || !is_fp8_cache(k, ks, D) || !is_fp8_cache(v, vs, D) || k.size(1) != Hk || k.size(2) < 1 || k.size(2) > 4096 || D > 512 ||
+      if (!ready(lib.llmctl_rope_kv_append_fp8) || !lib.llmctl_rope_kv_append_fp8_scratch_elems || !here({&ks, &vs}) || !is_fp8_cache(k, ks, D) || !is_fp8_cache(v, vs, D) || k.size(1) != Hk || k.size(2) < 1 || k.size(2) > 4096 || D > 512 ||
           Hk > 512)
         return none();
     } else if (ks.defined() || vs.defined() || !ready(lib.llmctl_rope_kv_append) || !bf16(k) || !bf16(v) || !k.is_contiguous() || !v.is_contiguous() || !unit16(k) || !unit16(v) ||
@@ -961,12 +961,15 @@ PyObject* py_rope_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return none();
     }
     without_gil([&] {
-      if (fp8)
+      if (fp8) {
+        const long long need = lib.llmctl_rope_kv_append_fp8_scratch_elems(static_cast<int>(T));
+        Tensor scratch = need ? new_f32(qkv, {need}) : Tensor();
         done("llmctl_rope_kv_append_fp8", lib.llmctl_rope_kv_append_fp8(data(qkv), qkv.stride(0), static_cast<int>(T), static_cast<int>(H), static_cast<int>(Hk), static_cast<int>(D), f32(cos),
                                                                         f32(sin), static_cast<int>(cos.size(0)), static_cast<const int*>(cdata(positions)),
                                                                         static_cast<const long long*>(cdata(slots)), data(k), data(v), static_cast<float*>(data(ks)), static_cast<float*>(data(vs)),
-                                                                        static_cast<int>(k.size(0)), static_cast<int>(k.size(2)), stream()));
-      else
+                                                                        static_cast<int>(k.size(0)), static_cast<int>(k.size(2)), need ? data(scratch) : nullptr, stream()),
+             need ? 2 : 1);
+      } else
         done("llmctl_rope_kv_append", lib.llmctl_rope_kv_append(data(qkv), qkv.stride(0), static_cast<int>(T), static_cast<int>(H), static_cast<int>(Hk), static_cast<int>(D), f32(cos), f32(sin),
                                                                 static_cast<int>(cos.size(0)), static_cast<const int*>(cdata(positions)), static_cast<const long long*>(cdata(slots)), data(k),
                                                                 data(v), k.size(0) * k.size(1), stream()));

@@ -21,7 +21,8 @@ native.register_signature("llmctl_paged_attn_decode",
                            c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p])
 native.register_signature("llmctl_paged_attn_scratch_elems", [c_int, c_int, c_int, c_int], restype=c_ll)
 native.register_signature("llmctl_rope_kv_append", [c_void_p, c_ll] + [c_int] * 4 + [c_void_p, c_void_p, c_int] + [c_void_p] * 4 + [c_ll, c_void_p])
-native.register_signature("llmctl_rope_kv_append_fp8", [c_void_p, c_ll] + [c_int] * 4 + [c_void_p, c_void_p, c_int] + [c_void_p] * 6 + [c_int, c_int, c_void_p])
+native.register_signature("llmctl_rope_kv_append_fp8", [c_void_p, c_ll] + [c_int] * 4 + [c_void_p, c_void_p, c_int] + [c_void_p] * 6 + [c_int, c_int, c_void_p, c_void_p])
+native.register_signature("llmctl_rope_kv_append_fp8_scratch_elems", [c_int], restype=c_ll)
 native.register_signature("llmctl_paged_attn_fp8_scratch_elems", [c_int] * 8, restype=c_ll)
 native.register_signature("llmctl_paged_attn_decode_fp8", [c_void_p, c_ll] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 8 + [c_float, c_void_p])
 native.register_signature("llmctl_sample", [c_void_p, c_int, c_ll, c_int, c_int] + [c_void_p] * 6 + [c_void_p])
@@ -228,7 +229,12 @@ def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
                 slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr())
         with _on_device(qkv):
             if fp8:
-                native.call("llmctl_rope_kv_append_fp8", *args, k_scale.data_ptr(), v_scale.data_ptr(), k_cache.shape[0], k_cache.shape[2], native.stream_ptr())
+                need = native.lib().llmctl_rope_kv_append_fp8_scratch_elems(T)
+                scratch = torch.empty(need, dtype=torch.int32, device=qkv.device) if need else None
+                native.call("llmctl_rope_kv_append_fp8", *args, k_scale.data_ptr(), v_scale.data_ptr(), k_cache.shape[0], k_cache.shape[2], native.ptr(scratch),
+                            native.stream_ptr())
+                if need:
+                    native.count_launches(1)        # which windows of tokens write to which blocks
             else:
                 native.call("llmctl_rope_kv_append", *args, k_cache.shape[0] * k_cache.shape[1], native.stream_ptr())
             if rows is not qkv:

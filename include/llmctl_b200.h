@@ -132,7 +132,8 @@ int llmctl_rope_kv_append(void* qkv, long long row_stride, int tokens, int heads
                           void* stream);
 int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int tokens, int heads, int kv_heads, int head_dim, const float* cos_t,
                               const float* sin_t, int table_rows, const int* positions, const long long* slots, void* k_cache, void* v_cache,
-                              float* k_scale, float* v_scale, int blocks, int block_size, void* stream);
+                              float* k_scale, float* v_scale, int blocks, int block_size, void* scratch, void* stream);
+long long llmctl_rope_kv_append_fp8_scratch_elems(int tokens);
 long long llmctl_paged_attn_fp8_scratch_elems(int batch, int heads, int kv_heads, int head_dim, int max_blocks, int block_size, int max_context,
                                               int num_splits);
 int llmctl_paged_attn_decode_fp8(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const float* k_scale,

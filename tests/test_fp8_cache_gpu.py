@@ -63,6 +63,36 @@ def test_append_of_8_bits(sops, size, slots, H, Hk, D):
         assert torch.equal(got[0].cpu().double(), want[0]) and torch.equal(got[1].cpu().double(), want[1])
 
 
+@pytest.mark.parametrize("order", ["prompts", "any"])
+@pytest.mark.parametrize("size", [16, 64, 3])
+@pytest.mark.parametrize("T", [2999, 3000, 5001])
+def test_append_of_long_calls(sops, T, size, order):
+    """Prompts one after the other, and tokens in any order; some without a row, some slots named twice by tokens far from each other."""
+    H, Hk, D = 2, 1, 32
+    blocks = 6000 // size
+    if order == "any":
+        slots = torch.randperm(blocks * size, generator=torch.Generator().manual_seed(T + size))[:T]
+    else:
+        table = torch.randperm(blocks, generator=torch.Generator().manual_seed(T + size))
+        at = torch.cat([torch.arange(7, 7 + T // 3), torch.arange((T // 3 // size + 2) * size, (T // 3 // size + 2) * size + T - T // 3)])
+        slots = table[at // size] * size + at % size
+    slots[T // 5::97] = -1
+    slots[T - 40:] = slots[:40]
+    slots[T // 2] = slots[3]
+    qkv, (cos, sin) = _randn(T, (H + 2 * Hk) * D), _tables(D)
+    qkv *= torch.exp2(torch.randint(-3, 4, (T, 1), device="cuda", generator=_gen(9)).float()).bfloat16()
+    positions = torch.arange(T, dtype=torch.int32, device="cuda") % 4096
+    (k, ks), (v, vs) = _state(blocks, Hk, size, D), _state(blocks, Hk, size, D, seed=2)
+    x = qkv.view(T, H + 2 * Hk, D).clone()
+    rotated = oracle.rotated32(x[:, :H + Hk], cos[positions.long()], sin[positions.long()], fused=True)
+    want_k = oracle.append(rotated[:, H:].cpu(), k.cpu().double(), ks.cpu().double(), slots)
+    want_v = oracle.append(x[:, H + Hk:].float().cpu(), v.cpu().double(), vs.cpu().double(), slots)
+    sops.rope_kv_append(qkv, cos, sin, positions, k, v, slots.cuda(), H, D, kv_heads=Hk, k_scale=ks, v_scale=vs)
+    assert torch.equal(qkv.view(T, -1, D)[:, :H + Hk], rotated.bfloat16()) and torch.equal(qkv.view(T, -1, D)[:, H + Hk:], x[:, H + Hk:])
+    for got, want in (((k, ks), want_k), ((v, vs), want_v)):
+        assert torch.equal(got[0].cpu().double(), want[0]) and torch.equal(got[1].cpu().double(), want[1])
+
+
 def test_numbers_that_are_not_finite(sops):
     H, D = 2, 64
     cos, sin = _tables(D)
