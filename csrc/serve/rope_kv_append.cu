@@ -123,7 +123,8 @@ rope_kv_append_kernel(RopeRows r, uint32_t total, FastDiv per_token, FastDiv per
 // time.
 //
 // CTAs 0 .. windows * parts - 1: of the tokens of a window, one that is the first of the call in its block takes the block.  A scan over the slots tells,
-// which is left out where the token before goes to the same block (in a prompt, 15 of 16).  Then a lane has one place in one row of the block for
+// which is left out where the token before goes to the same block (in a prompt, 15 of 16).  Windows of one token share their blocks' heads instead (a prompt
+// of 200 tokens, 32 heads of 128 6.3 us, 19.2 where the first token's CTAs write alone; over 8 heads in blocks of 64 7.5 / 22.5).  Then a lane has one place in one row of the block for
 // all heads, and keeps its token's angles; as many warps as the block's rows need write a head after the other: the largest rotated number, by
 // all of them, the scale, the codes.  The next head's numbers are asked for beside that.  (A warp to a head's block had to read the angles anew for each
 // row and head and rotate twice, for want of registers: 8000 tokens, 40 heads of 128 130 us, so 112.)  Blocks of more than twice the rows
@@ -135,6 +136,9 @@ rope_kv_append_kernel(RopeRows r, uint32_t total, FastDiv per_token, FastDiv per
 namespace append8 {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kUnits = 4;                    // of q, to a thread
+// Calls of so many tokens may be of as many sequences: CTAs to each token, of which those whose tokens go to one block share its heads.  us with windows of 16
+// tokens / so: 400 decoded tokens, 32 heads of 128 45 / 16, over 8 42 / 8.6; a prompt of 400 8.8 / 11.1, over 8 5.5 / 6.9; 1000 decoded 68 / 36, a prompt 13.8 / 25.4.
+constexpr int kFew = 512;
 constexpr int kMaxBlock = 4096;
 constexpr int kStages = 4;                   // heads under way (1: 8000 tokens, 40 heads of 128 142 us)
 constexpr uint32_t kInfinite = 0x7f800000u;
@@ -295,7 +299,7 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, const
                           uint32_t q_units, FastDiv per_token, FastDiv per_head) {
   using namespace append8;
   extern __shared__ __align__(16) int row_token[];          // [block_size]: the token that a row of the block at hand is written from, or -1; then those rows
-  __shared__ int first_token, twice, written;
+  __shared__ int ahead, others, twice, written;             // tokens of the block: before this one; but this one
   int* const row_list = row_token + (block_size + 3) / 4 * 4;          // (what follows both lies on a 16-byte boundary)
   __shared__ uint32_t warp_most[2][kWarps];
   __nv_bfloat16* qkv = r.qkv;
@@ -338,9 +342,11 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, const
   }
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int part = work / windows, t0 = (work - part * windows) * window, t1 = min(r.tokens, t0 + window);
+  const bool few = window == 1;               // one token, whatever its place in its block
+  const int part0 = work / windows, parts0 = parts, t0 = (work - part0 * windows) * window, t1 = min(r.tokens, t0 + window);
   const long long rows = static_cast<long long>(blocks) * block_size;
   // heads of keys that no block's writer rotates: all of a token's, this part's share
+  int part = part0;
   auto rotate_keys = [&](int tok) {
     for (int i = threadIdx.x; i < r.kv_heads * per_row; i += kThreads)
       if ((i / per_row) % parts == part) {
@@ -366,19 +372,19 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, const
   const bool padded = slot < 0 || slot >= rows, behind = !padded && before >= 0 && before < rows && before / block_size == slot / block_size;
   const unsigned window_mask = t1 - t0 >= 32 ? ~0u : (1u << (t1 - t0)) - 1u;
   for (unsigned left = __ballot_sync(0xffffffffu, padded) & window_mask; left != 0u; left &= left - 1u) rotate_keys(t0 + __ffs(left) - 1);
-  for (unsigned left = __ballot_sync(0xffffffffu, !padded && !behind) & window_mask; left != 0u; left &= left - 1u) {
+  for (unsigned left = __ballot_sync(0xffffffffu, !padded && (few || !behind)) & window_mask; left != 0u; left &= left - 1u) {
     const int t = t0 + __ffs(left) - 1, block = static_cast<int>(__shfl_sync(0xffffffffu, slot, t - t0) / block_size);
     const long long lo = static_cast<long long>(block) * block_size, hi = lo + block_size;
     __syncthreads();                          // the rows of the block before have been read
     for (int i = threadIdx.x; i < block_size; i += kThreads) row_token[i] = -1;
     if (threadIdx.x == 0) {
-      first_token = t;
-      twice = written = 0;
+      ahead = others = twice = written = 0;
     }
     __syncthreads();
     auto meet = [&](int i, long long s) {
       if (s >= lo && s < hi) {
-        if (i < t) atomicMin(&first_token, i);
+        if (few && i != t) atomicAdd(&others, 1);
+        if (i < t) atomicAdd(&ahead, 1);
         if (atomicMax(&row_token[s - lo], i) >= 0) twice = 1;
       }
     };
@@ -411,7 +417,14 @@ rope_kv_append_fp8_kernel(RopeRows r, const long long* __restrict__ slots, const
       if (threadIdx.x == 0 && (r.tokens - odd) % 2 != 0) meet(r.tokens - 1, slots[r.tokens - 1]);
     }
     __syncthreads();
-    if (first_token != t) continue;
+    if (few && others > 0) {                 // as many CTAs for each token: those of a block's tokens share its heads, as far as they go round
+      const int members = others + 1, groups = kWarps / warps_together(members, step), most = min(parts0 * members, max((2 * r.kv_heads + groups - 1) / groups, parts0));
+      part = ahead * parts0 + part0;
+      parts = min(most, r.kv_heads);
+      if (part >= parts) return;
+    } else if (!few && ahead != 0) {
+      continue;
+    }
     for (int i = threadIdx.x; i < block_size; i += kThreads)
       if (row_token[i] >= 0) row_list[atomicAdd(&written, 1)] = i;          // in whatever order: rows do not depend on each other
     if (twice)
@@ -577,9 +590,10 @@ LLMCTL_API int llmctl_rope_kv_append_fp8(void* qkv, long long row_stride, int to
   LLMCTL_REQUIRE(rope_rows_ok(r) && head_dim <= 512 && kv_heads <= 512 && blocks >= 0 && block_size >= 1 && block_size <= kMaxBlock && aligned16(k_cache, v_cache));
   LLMCTL_REQUIRE(static_cast<long long>(blocks) * kv_heads < (1LL << 31) && static_cast<long long>(kv_heads) * block_size * head_dim < (1LL << 31));
   if (tokens == 0) return 0;
-  const int window = tokens > 256 ? 16 : 1, windows = (tokens + window - 1) / window;
+  const bool few = tokens <= kFew;
+  const int window = few ? 1 : 16, windows = (tokens + window - 1) / window;
   // A block to each token where they may all be of other sequences, else to each block_size of them.
-  const int writers = tokens > 256 ? (tokens + block_size - 1) / block_size : tokens, most = tokens > 256 ? kv_heads : (2 * kv_heads + kWarps - 1) / kWarps;
+  const int writers = few ? tokens : (tokens + block_size - 1) / block_size, most = few ? (2 * kv_heads + kWarps - 1) / kWarps : kv_heads;
   const int held = (block_size - 1) / (kWarps * (32 / (head_dim / 16))) + 1;          // rows to a lane
   int parts = writers <= resident(held) / 2 ? resident(held) / writers : writers >= 4 * resident(held) || kv_heads <= 2 * kWarps ? 1 : 2;
   if (parts > most) parts = most;

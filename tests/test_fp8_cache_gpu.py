@@ -65,7 +65,7 @@ def test_append_of_8_bits(sops, size, slots, H, Hk, D):
 
 @pytest.mark.parametrize("order", ["prompts", "any"])
 @pytest.mark.parametrize("size", [16, 64, 3])
-@pytest.mark.parametrize("T", [2999, 3000, 5001])
+@pytest.mark.parametrize("T", [200, 512, 513, 2999, 3000, 5001])
 def test_append_of_long_calls(sops, T, size, order):
     """Prompts one after the other, and tokens in any order; some without a row, some slots named twice by tokens far from each other."""
     H, Hk, D = 2, 1, 32
