@@ -611,6 +611,15 @@ __device__ __forceinline__ void setmaxnreg_dec() {
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
+// The same, and whether any of the threads says so.
+__device__ __forceinline__ bool named_bar_any(uint32_t id, uint32_t nthreads, bool mine) {
+  uint32_t any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(any)
+               : "r"(static_cast<uint32_t>(mine)), "r"(id), "r"(nthreads)
+               : "memory");
+  return any != 0u;
+}
 
 }  // namespace ptx
 }  // namespace llmctl

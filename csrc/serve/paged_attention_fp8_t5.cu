@@ -5,7 +5,7 @@
 //     S^T = K Q^T         128 tokens x N columns, over D                 (A: the key tile as it was loaded, K-major)
 //     O^T = V^T P^T       D dimensions x N columns, over 128 tokens      (A: the value tile as it was loaded, M-major)
 // kind::f8f6f4 wants 8-bit columns too.  A query head, and a row of weights, is therefore FOUR columns: the number rounded to e4m3 (4 significant
-// bits), the rest times 16 rounded, its rest times 16, and so on: 16 bits of what they have, where bf16 has 8, over a range of 2^29.  The products of two
+// bits), the rest times 16 rounded, its rest times 16, and so on: 16 bits of what they have, where bf16 has 8, over a range of 2^28.  The products of two
 // e4m3 numbers are exact and the four columns are added in 32 bits.  N = 16 columns are four heads, 32 eight, 64 sixteen.
 //
 // The scales of keys multiply the scores.  Those of values are added to the exponent of a token's weight, w = 2^(s + log2 sv), which has a running reference of
@@ -43,6 +43,10 @@ constexpr int kThreads = 256;
 constexpr int kPieces = 4, kMaxStages = 8, kMaxBoxes = 16;
 constexpr int kWholeTokens = 768, kLeast = 2;
 constexpr float kStep = 16.f;                // between the columns of a number
+// Eight query heads: the references stay where they are while no score is beyond them by more than kSlack, and no weight by kSlackV (log2; a weight of 1 is then
+// 128, and none above 430), and no maxima are taken.  us, maxima in each tile / so: 70 contexts of up to 31760, 24 heads of 64 over 4 215 / 188, 8 of 8000, 64 heads of 128
+// over 8 31.6 / 31.2; one head 60.9 / 61.2, four 64.5 / 64.6, sixteen 30.9 / 32.9.
+constexpr float kSlack = 32.f, kSlackV = 1.75f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int columns(int GP) { return GP < 4 ? 16 : kPieces * GP; }     // of a product: 16 at least, of which those past 4 GP are nobody's
 constexpr int stage_bytes(int D) { return 2 * kTile * D; }
@@ -205,12 +209,14 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
                                 int stages, float scale_log2, unsigned char* wait_byte) {
   using namespace dec8;
   constexpr int C = kPieces * GP, N = columns(GP), kStage = stage_bytes(D), kHalf = kTile * D;
+  constexpr bool kMayStay = GP == 8;
+  constexpr float kUnit = kMayStay ? 128.f : 256.f;                        // a weight of 1
   constexpr uint32_t kSwizzle = D == 128 ? 2 : 4, kEight = 8 * D;          // layout of the tiles, bytes of eight rows
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bar_q, bar_full[kMaxStages], bar_empty[kMaxStages], bar_s[2], bar_p[2], bar_o[2];
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
-  __shared__ float top[2][4][2 * GP];                                      // per softmax warp: the tile's largest s and s + log2 sv
+  __shared__ __align__(16) float top[2][4][2 * GP];                                      // per softmax warp: the tile's largest s and s + log2 sv
   __shared__ float box_scale[kMaxStages][2][kMaxBoxes];                    // of a stage's boxes: sk, log2 sv
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -450,27 +456,41 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
 #pragma unroll
           for (int g = 0; g < GP; ++g) s[g] = seen ? joined<GP>(c, g) * (sk * factor[g]) : -INFINITY;
         }
+        bool beyond = !kMayStay;
+        if constexpr (kMayStay) {
 #pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          const float a = warp_max_all(s[g]), c = warp_max_all(s[g] + lv);
-          if (lane == 0) {
-            most[w][g] = a;
-            most[w][GP + g] = c;
-          }
+          for (int g = 0; g < GP; ++g) beyond |= !(s[g] - m[g] <= kSlack && s[g] + lv - M[g] <= kSlackV);
         }
-        named_bar_sync(1, 128);
         uint32_t codes[C / 4];                            // this token's row of P: C bytes, piece after piece
         float from[GP];
+        if (!kMayStay || n == first || named_bar_any(1, 128, beyond)) {
 #pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          auto over = [&](int i) { return fmaxf(fmaxf(most[0][i], most[1][i]), fmaxf(most[2][i], most[3][i])); };
-          const float m1 = fmaxf(m[g], over(g)), M1 = fmaxf(M[g], over(GP + g));
-          const float ref = m1 == -INFINITY ? 0.f : m1, Ref = M1 == -INFINITY ? 0.f : M1;
-          l[g] = fmaf(l[g], ex2_approx(m[g] - ref), ex2_approx(s[g] - ref));
-          from[g] = ex2_approx(M[g] - Ref);
-          m[g] = m1;
-          M[g] = M1;
-          s[g] = ex2_approx(s[g] + lv - Ref) * 256.f;
+          for (int g = 0; g < GP; ++g) {
+            const float a = warp_max_all(s[g]), c = warp_max_all(s[g] + lv);
+            if (lane == 0) {
+              most[w][g] = a;
+              most[w][GP + g] = c;
+            }
+          }
+          named_bar_sync(1, 128);
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            auto over = [&](int i) { return fmaxf(fmaxf(most[0][i], most[1][i]), fmaxf(most[2][i], most[3][i])); };
+            const float m1 = fmaxf(m[g], over(g)), M1 = fmaxf(M[g], over(GP + g));
+            const float ref = m1 == -INFINITY ? 0.f : m1, Ref = M1 == -INFINITY ? 0.f : M1;
+            l[g] = fmaf(l[g], ex2_approx(m[g] - ref), ex2_approx(s[g] - ref));
+            from[g] = ex2_approx(M[g] - Ref);
+            m[g] = m1;
+            M[g] = M1;
+            s[g] = ex2_approx(s[g] + lv - Ref) * kUnit;
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            l[g] += ex2_approx(s[g] - m[g]);
+            from[g] = 1.f;
+            s[g] = ex2_approx(s[g] + lv - M[g]) * kUnit;
+          }
         }
 #pragma unroll
         for (int i = 0; i < C / 4; ++i) codes[i] = 0u;
@@ -516,7 +536,7 @@ paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const _
       for (int g = 0; g < GP; ++g) {
         if (g >= group - g0 || !has_dim) continue;
         const float total = (sums[0][g] + sums[1][g]) + (sums[2][g] + sums[3][g]);
-        const float o = acc[g] * (M[g] == -INFINITY ? 1.f / 256.f : exp2f(M[g] - m[g]) * (1.f / 256.f));
+        const float o = acc[g] * (M[g] == -INFINITY ? 1.f / kUnit : exp2f(M[g] - m[g]) * (1.f / kUnit));
         if (whole_item) {
           out[(row0 + g) * D + dim] = __float2bfloat16(o / total);
         } else {

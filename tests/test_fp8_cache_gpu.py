@@ -191,6 +191,26 @@ def test_attention(sops, H, Hk, D, size, lens, splits):
     assert ((got - want).abs() <= oracle.tolerance(want, bound, D)).all()
 
 
+@pytest.mark.parametrize("H,Hk,D", [(8, 1, 128), (6, 1, 64), (32, 4, 64), (2, 2, 64), (16, 1, 128)])
+@pytest.mark.parametrize("key_step,value_step", [(0.01, 0.0), (0.2, 0.0), (0.0, 0.15), (0.05, -0.3), (-0.2, 1.0)])
+@pytest.mark.parametrize("splits", [None, 1])
+def test_attention_of_rising_scores(sops, H, Hk, D, key_step, value_step, splits):
+    """Keys along the query whose scores rise (or fall) from block to block, values whose scales do, by little and by much: as far as any weight's reference is left standing, and beyond."""
+    size, lens = 16, [1900, 131, 700]
+    tables, n, blocks = _batch(lens, size)
+    (k, ks), (v, vs) = _state(blocks, Hk, size, D), _state(blocks, Hk, size, D, seed=2)
+    q = _randn(len(lens), H, D, seed=5, std=0.02) + 0.1
+    for b, c in enumerate(lens):
+        for page in range((c + size - 1) // size):
+            at = int(tables[b, page])
+            k[at] = (k[at].float() * 0.05 + 10 + page * key_step * 10).clamp(-448, 448).to(k.dtype)
+            ks[at] = 2.0 ** -4
+            vs[at] = 2.0 ** round(page * value_step)
+    got = sops.paged_attention_decode_fp8(q, k, v, ks, vs, tables, n, max(lens), num_splits=splits).cpu().double()
+    want, bound = oracle.attend(q.cpu(), k.cpu().float(), ks.cpu(), v.cpu().float(), vs.cpu(), tables.cpu(), n.cpu(), D ** -0.5)
+    assert ((got - want).abs() <= oracle.tolerance(want, bound, D)).all()
+
+
 @pytest.mark.parametrize("size", [16, 5])
 def test_attention_scales(sops, size):
     """Scales of values that differ by 2^60 between pages, a page of zeros, keys that decide alone, and a scale of the softmax."""
