@@ -201,7 +201,7 @@ struct Items {
 // Grid: as many CTAs as there are runs.  GP: query heads of an item.  partial: two rows of items [2 ctas, GP, D + 2] = {sum of w cv at the reference m, m (log2), sum of p}: of the
 // item that the run begins inside of, and of the one that it ends inside of.
 template <int D, int GP>
-__global__ void __launch_bounds__(dec8::kThreads, GP == 16 ? 1 : D == 64 && GP <= 2 ? 3 : 2)
+__global__ void __launch_bounds__(dec8::kThreads, GP == 16 ? 1 : GP == 1 || (D == 64 && GP == 2) ? 3 : 2)
 paged_attn_decode_fp8_t5_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __nv_bfloat16* __restrict__ q,
                                 long long q_stride, const float* __restrict__ k_scale, const float* __restrict__ v_scale,
                                 const int* __restrict__ block_tables, int max_blocks, dec8::Work work, float* __restrict__ partial,
@@ -619,13 +619,16 @@ static Plan plan_of(int batch, int heads, int kv_heads, int head_dim, int limit,
   const int group = heads / kv_heads;
   for (p.GP = 1; p.GP < group && p.GP < 16;) p.GP *= 2;
   p.parts = (group + p.GP - 1) / p.GP;
-  p.per_sm = p.GP == 16 ? 1 : head_dim == 64 && p.GP <= 2 ? 3 : 2;        // registers; stages of 192 KB an SM in all
   p.items = static_cast<long long>(batch) * kv_heads * p.parts;
   const long long tiles = p.items * ((limit + kTile - 1) / kTile);
   // Nothing is split where contexts are short: the second kernel is 2 to 3 us, a tile of a longer chain 0.65.  us, whole / split: 16 contexts of up to 600,
   // 32 heads of 128 15.4 / 18.3, of 1000 21.1 / 21.8, 32 heads over 8 10.5 / 13.7; one of 1000, 32 heads 9.3 / 7.6, 64 of 1000 64.7 / 61.3; 16 of 2000
   // 35.5 / 33.8.
   p.whole = runs == 1 || limit <= kWholeTokens || (limit <= 1024 && p.items >= 128 && p.items <= 1024);
+  // CTAs to an SM: registers; stages of 192 KB an SM in all.  Three for one head of 128, of two stages each, where each has many items or tiles.  us, two / three: 94
+  // contexts of 1, 32 heads 20.9 / 16.2, 64 of 200 23.5 / 20.2, 83 of 425, 40 heads 56.0 / 51.3, 64 of 2000 112 / 109; 16 of 600 15.5 / 17.4, 16 of 4096 61.1 / 61.6.
+  const bool many = p.whole ? p.items >= 2 * 3 * kNumSMs : tiles >= 50 * 3 * kNumSMs;
+  p.per_sm = p.GP == 16 ? 1 : (head_dim == 64 && p.GP <= 2) || (p.GP == 1 && many) ? 3 : 2;
   const long long most = p.whole ? p.items : runs > 1 ? runs : (tiles + kLeast - 1) / kLeast;
   p.ctas = static_cast<int>(most < p.per_sm * kNumSMs ? (most > 1 ? most : 1) : p.per_sm * kNumSMs);
   p.partial = p.whole ? 0 : 2LL * p.ctas * p.GP * (head_dim + 2);
