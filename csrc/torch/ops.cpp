@@ -15,6 +15,7 @@
 #include <ATen/autocast_mode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
@@ -138,6 +139,8 @@ void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 Tensor empty_like_on(const Tensor& t, at::IntArrayRef size, at::ScalarType type) { return at::empty(size, t.options().dtype(type).requires_grad(false)); }
 Tensor new_bf16(const Tensor& t, at::IntArrayRef size) { return empty_like_on(t, size, at::kBFloat16); }
 Tensor new_f32(const Tensor& t, at::IntArrayRef size) { return empty_like_on(t, size, at::kFloat); }
+// The same without the way through the dispatcher (0.5 us each), on the current device: for calls under no mode (quiet()).
+Tensor fresh(at::IntArrayRef size, at::ScalarType type) { return at::detail::empty_cuda(size, type, c10::Device(c10::kCUDA, c10::cuda::current_device()), std::nullopt); }
 void* data(const Tensor& t) { return t.data_ptr(); }
 const void* cdata(const Tensor& t) { return t.const_data_ptr(); }
 
@@ -963,7 +966,7 @@ PyObject* py_rope_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     without_gil([&] {
       if (fp8) {
         const long long need = lib.llmctl_rope_kv_append_fp8_scratch_elems(static_cast<int>(T));
-        Tensor scratch = need ? new_f32(qkv, {need}) : Tensor();
+        Tensor scratch = need ? fresh({need}, at::kFloat) : Tensor();
         done("llmctl_rope_kv_append_fp8", lib.llmctl_rope_kv_append_fp8(data(qkv), qkv.stride(0), static_cast<int>(T), static_cast<int>(H), static_cast<int>(Hk), static_cast<int>(D), f32(cos),
                                                                         f32(sin), static_cast<int>(cos.size(0)), static_cast<const int*>(cdata(positions)),
                                                                         static_cast<const long long*>(cdata(slots)), data(k), data(v), static_cast<float*>(data(ks)), static_cast<float*>(data(vs)),
@@ -998,7 +1001,7 @@ PyObject* py_paged_decode_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Tensor o = without_gil([&] {
       const long long need = lib.llmctl_paged_attn_fp8_scratch_elems(static_cast<int>(B), static_cast<int>(H), static_cast<int>(k.size(1)), static_cast<int>(D), static_cast<int>(tables.size(1)),
                                                                      static_cast<int>(k.size(2)), context, static_cast<int>(splits));
-      Tensor scratch = need ? new_f32(q, {need}) : Tensor(), out = new_bf16(q, q.sizes());
+      Tensor scratch = need ? fresh({need}, at::kFloat) : Tensor(), out = fresh(q.sizes(), at::kBFloat16);
       const auto f32 = [](const Tensor& x) { return static_cast<const float*>(cdata(x)); };
       done("llmctl_paged_attn_decode_fp8",
            lib.llmctl_paged_attn_decode_fp8(cdata(q), q.stride(0), cdata(k), cdata(v), f32(ks), f32(vs), static_cast<const int*>(cdata(tables)), static_cast<int>(tables.size(1)),
@@ -1020,8 +1023,8 @@ struct LogprobsOut {
 };
 LogprobsOut logprobs_fwd(const Tensor& logits, const Tensor& tokens, int64_t top, bool keep) {
   const int64_t rows = logits.size(0), V = logits.size(1);
-  LogprobsOut r{new_f32(logits, {rows}), new_f32(logits, {rows}), top ? empty_like_on(logits, {rows, top}, at::kLong) : Tensor(), top ? new_f32(logits, {rows, top}) : Tensor(),
-                keep ? new_f32(logits, {rows, 2}) : Tensor()};
+  LogprobsOut r{fresh({rows}, at::kFloat), fresh({rows}, at::kFloat), top ? fresh({rows, top}, at::kLong) : Tensor(), top ? fresh({rows, top}, at::kFloat) : Tensor(),
+                keep ? fresh({rows, 2}, at::kFloat) : Tensor()};
   const auto f32 = [](const Tensor& x) { return x.defined() ? static_cast<float*>(data(x)) : nullptr; };
   done("llmctl_token_logprobs",
        lib.llmctl_token_logprobs(cdata(logits), logits.scalar_type() == at::kFloat, logits.stride(0), static_cast<const long long*>(cdata(tokens)), static_cast<int>(rows), static_cast<int>(V),
