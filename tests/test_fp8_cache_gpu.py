@@ -93,6 +93,43 @@ def test_append_of_long_calls(sops, T, size, order):
         assert torch.equal(got[0].cpu().double(), want[0]) and torch.equal(got[1].cpu().double(), want[1])
 
 
+def test_long_calls_captured_and_without_scratch(sops):
+    """A captured long call on other rows and slots, and the C entry without the scratch for its marks: the same bytes as the eager call."""
+    from llmctl_b200.ops import native
+    T, H, D, size, blocks = 4001, 2, 32, 16, 300
+    cos, sin = _tables(D)
+    positions = torch.arange(T, dtype=torch.int32, device="cuda") % 4096
+    rows = [_randn(T, 3 * H * D, seed=s) for s in (1, 2)]
+    slots = [torch.randperm(blocks * size, device="cuda", generator=_gen(s))[:T] for s in (3, 4)]
+    state = [_state(blocks, H, size, D, seed=s) for s in (5, 6)]
+
+    def fresh():
+        return [x.clone() for pair in state for x in pair]
+
+    def run(qkv, at, c):
+        sops.rope_kv_append(qkv, cos, sin, positions, c[0], c[2], at, H, D, k_scale=c[1], v_scale=c[3])
+
+    want = []
+    for i in range(2):
+        qkv, c = rows[i].clone(), fresh()
+        run(qkv, slots[i], c)
+        want.append([qkv, *c])
+    held, at, c = rows[0].clone(), slots[0].clone(), fresh()
+    run(held, at, c)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(held, at, c)
+    for i in (1, 0):
+        for x, y in zip((held, at, *c), (rows[i], slots[i], *fresh())):
+            x.copy_(y)
+        graph.replay()
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip((held, *c), want[i]))
+    qkv, c = rows[0].clone(), fresh()
+    native.call("llmctl_rope_kv_append_fp8", qkv.data_ptr(), qkv.stride(0), T, H, H, D, cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots[0].data_ptr(),
+                c[0].data_ptr(), c[2].data_ptr(), c[1].data_ptr(), c[3].data_ptr(), blocks, size, None, native.stream_ptr())
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip((qkv, *c), want[0]))
+
+
 def test_numbers_that_are_not_finite(sops):
     H, D = 2, 64
     cos, sin = _tables(D)
