@@ -182,7 +182,9 @@ LLMCTL_API int llmctl_paged_attn_decode_fp8(const void* q, long long q_stride, c
     if (rc) LLMCTL_FAIL(rc, "decode over 8 bits");
     LLMCTL_RETURN_LAST();
   }
-  const int splits = decode8_splits(batch, heads, limit, num_splits), per = limit > 0 ? (limit - 1) / splits + 1 : 1;
+  // A cache without blocks, of whatever size they would have, has nothing to split: one part, which needs none of the scratch that the function above answers
+  // for the kernel that this call does not take.
+  const int splits = blocks == 0 ? 1 : decode8_splits(batch, heads, limit, num_splits), per = limit > 0 ? (limit - 1) / splits + 1 : 1;
   LLMCTL_REQUIRE(splits == 1 || scratch != nullptr);
   auto launch = [&](auto kern) {
     return launch_dependent(kern, dim3(heads, splits, batch), 128, 0, s, (const __nv_bfloat16*)q, q_stride, (const uint8_t*)k_cache, (const uint8_t*)v_cache,

@@ -145,6 +145,28 @@ def test_refusals(sops):
             sops.paged_attention_decode_fp8(*fine[:i], bad, *fine[i + 1:])
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="calls the entry point with addresses of nothing: it has to end at the missing device")
+@pytest.mark.parametrize("block_size", [16, 5])
+@pytest.mark.parametrize("batch,heads,kv_heads", [(1, 32, 32), (16, 32, 32), (3, 8, 2)])
+def test_a_cache_without_blocks_needs_no_scratch(sops, block_size, batch, heads, kv_heads):
+    """What a launch writes to scratch has to fit into what is asked for beforehand, which does not know of the cache's blocks: without blocks it writes nothing,
+    so that the entry point takes a null and goes on to the launch (refused arguments are answered with 1)."""
+    from llmctl_b200.ops import native
+    if not native.available():
+        pytest.skip("library not built")
+    for limit in (0, 1, 512, 1000, 4096, 100000):
+        for splits in (0, 1, 3, 256):
+            rc = native.lib().llmctl_paged_attn_decode_fp8(4096, heads * 128, 4096, 4096, 4096, 4096, 4096, limit // block_size + 1, 4096, 4096, None, batch, heads, kv_heads, 128, 0, block_size, limit,
+                                                           splits, 1.0, None)
+            assert rc not in (0, 1)
+
+
+def test_attention_over_a_cache_without_blocks(sops):
+    (k, ks), (v, vs) = (sops.allocate_fp8_cache(0, 16, 2, 64) for _ in range(2))
+    out = sops.paged_attention_decode_fp8(torch.randn(2, 4, 64), k, v, ks, vs, torch.zeros(2, 256, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 4096)
+    assert not out.any()
+
+
 def _engine(**kw):
     from llmctl_b200.comms import mesh
     from llmctl_b200.serve.engine import InferenceEngine

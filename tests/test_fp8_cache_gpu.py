@@ -308,6 +308,20 @@ def test_attention_bad_pages_and_limits(sops):
     assert torch.equal(sops.paged_attention_decode_fp8(q[:1], k, v, ks, vs, tables[:, :2].contiguous(), n2, 10 ** 6), sops.paged_attention_decode_fp8(q[:1], k, v, ks, vs, tables, n2, 32))
 
 
+@pytest.mark.parametrize("size", [16, 5])
+@pytest.mark.parametrize("B,H,Hk,D,limit", [(1, 32, 32, 128, 4096), (16, 32, 32, 128, 4096), (3, 8, 2, 64, 20000), (2, 2, 2, 64, 100)])
+def test_attention_over_a_cache_without_blocks(sops, B, H, Hk, D, limit, size):
+    """Zeros for sequences without tokens, NaN for others (their blocks lie outside of the cache), and what lies behind the results is left."""
+    (k, ks), (v, vs) = (sops.allocate_fp8_cache(0, size, Hk, D, "cuda") for _ in range(2))
+    tables, n = torch.zeros(B, limit // size + 1, device="cuda", dtype=torch.int32), torch.zeros(B, device="cuda", dtype=torch.int32)
+    for splits in (None, 3):
+        assert not sops.paged_attention_decode_fp8(_randn(B, H, D), k, v, ks, vs, tables, n, limit, num_splits=splits).any()
+        n[0] = 70
+        out = sops.paged_attention_decode_fp8(_randn(B, H, D), k, v, ks, vs, tables, n, limit, num_splits=splits)
+        assert out[0].isnan().all() and not out[1:].any()
+        n[0] = 0
+
+
 def test_run_together_in_a_graph_beside_another(sops):
     """Prompt, then decoding steps of append and attention over the same cache: captured twice and replayed side by side on two streams, each against the
     oracle's view of the cache."""
