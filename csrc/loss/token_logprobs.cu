@@ -28,6 +28,7 @@ constexpr int kResident = 4 * kNumSMs;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFloor = -200.f;             // 2^-200 is 0: what lies lower counts as this, so that -inf times its weight is 0 and no NaN
 constexpr float kLow = -1e30f, kUsual = -1e29f;      // beside a maximum above kUsual numbers below kLow weigh nothing, and may be kLow
+constexpr float kMost = 1e30f, kMostGrad = 1e7f;     // up to here differences to a maximum, and their products with the entropy's gradient, are finite with no floor
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -146,7 +147,7 @@ struct Sums {
     s += e;
     t += e * u;
   }
-  // Numbers above kLow beside a maximum above kUsual.
+  // Numbers above kLow beside a maximum between kUsual and kMost.
   template <int U>
   __device__ __forceinline__ void add_usual(const float (&x)[U]) {
     float s2[2] = {0.f, 0.f}, t2[2] = {0.f, 0.f};
@@ -232,7 +233,7 @@ token_logprobs_kernel(const T* __restrict__ logits, long long ld, const long lon
         if (of[e] == most) k = e;
       best_unit = i0 + k * kThreads;
     }
-    const bool usual = a.m > kUsual && a.m < INFINITY;
+    const bool usual = a.m > kUsual && a.m < kMost;
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       float x[U];
@@ -416,7 +417,7 @@ token_logprobs_bwd_kernel(const T* __restrict__ logits, long long ld, const long
   };
   const int parts = gridDim.y, part = blockIdx.y, per = (r.units + parts - 1) / parts, lo = part * per, hi = min(r.units, lo + per);
   const int from = part == 0 ? 0 : r.head + lo * U, to = part == parts - 1 ? V : r.head + hi * U;        // this CTA's numbers
-  const bool usual = m > kUsual;              // (a row with +inf or NaN has a log_s that is no number)
+  const bool usual = m > kUsual && m < kMost && fabsf(gh) < kMostGrad;
   for (int i0 = lo + tid; i0 < hi; i0 += kAhead * kThreads) {
     uint4 raw[kAhead];
 #pragma unroll

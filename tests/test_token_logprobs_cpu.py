@@ -40,6 +40,20 @@ def test_rows_with_masks(ops):
     assert got.top_logprobs[0, 2] == -inf
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_largest_numbers(ops, dtype):
+    """Finite logits up to the type's largest have numbers for all results and gradients."""
+    most, inf = torch.finfo(dtype).max, float("inf")
+    x = torch.tensor([[0.0, most, 1.0, 2.0], [most, 1.0, -most, most], [most] * 4, [1.0, 2.5e38, -inf, 0.0]], dtype=dtype).requires_grad_(True)
+    got = ops.token_logprobs(x, torch.tensor([1, 0, 2, 0]), 2)
+    two, four = torch.log(torch.tensor(2.0)), torch.log(torch.tensor(4.0))
+    assert torch.allclose(got.logprobs[:3], torch.stack([torch.tensor(0.0), -two, -four])) and got.logprobs[3] == 1 - x[3, 1].float()
+    assert torch.allclose(got.entropy, torch.stack([torch.tensor(0.0), two, four, torch.tensor(0.0)])) and got.top_ids.tolist() == [[1, 3], [0, 3], [0, 1], [1, 0]]
+    dx, = torch.autograd.grad(got.logprobs.sum() + 3 * got.entropy.sum(), x)
+    want = torch.tensor([[0.0, 0.0, 0.0, 0.0], [0.5, 0.0, 0.0, -0.5], [-0.25, -0.25, 0.75, -0.25], [1.0, -1.0, 0.0, 0.0]])
+    assert torch.allclose(dx.float(), want, atol=1e-6)
+
+
 def test_tokens_outside_of_the_vocabulary(ops):
     x = _logits(3, 11).requires_grad_(True)
     got = ops.token_logprobs(x, torch.tensor([-100, 4, 11]))

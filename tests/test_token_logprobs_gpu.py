@@ -109,6 +109,54 @@ def test_masks_and_infinities(ops, V, dtype):
     assert got.top_logprobs[0, 1] == -inf
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [9, 5003, 200000])
+def test_the_largest_numbers(ops, V, dtype):
+    """Finite logits up to the type's largest among ordinary ones have numbers for all results and gradients, of the log probability alone and with the
+    entropy's; differences that 32 bits do not hold are -inf."""
+    most = torch.finfo(dtype).max
+    x = _logits(7, V, dtype)
+    x[0, V // 2] = most
+    x[1, 0] = x[1, V - 1] = most
+    x[2] = most
+    x[3, ::2], x[3, 1] = -most, most
+    x[4, 3], x[4, 4:] = 2.4e38, float("-inf")
+    x[5, 2], x[6, 2] = 1e30, 5e29
+    tokens = torch.tensor([V // 2, 1, 0, 0, 3, 2, 0], device="cuda")
+    x.requires_grad_(True)
+    got = ops.token_logprobs(x, tokens, 3)
+    lp, chosen, entropy, order = _want(x, tokens, 3)
+    eps = _slack(lp, V)
+    assert torch.allclose(got.logprobs, chosen.float(), rtol=2.0 ** -22, atol=eps)
+    assert ((got.entropy - entropy).abs() <= eps * (2 + 2 * entropy) + 1e-6).all()
+    assert torch.equal(got.top_ids, order) and torch.allclose(got.top_logprobs, lp.gather(1, order).float(), rtol=2.0 ** -22, atol=eps)
+    g, gh = torch.randn(7, device="cuda"), torch.randn(7, device="cuda")
+    rounding = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    for outs, grads in (((got.logprobs,), (g,)), ((got.logprobs, got.entropy), (g, gh))):
+        dx, = torch.autograd.grad(outs, x, grads, retain_graph=True)
+        want, size = _gradient(x, tokens, 0, None, g, gh if len(grads) == 2 else torch.zeros_like(gh), None)
+        assert ((dx.double() - want).abs() <= rounding * want.abs() + (4 * eps + 2.0 ** -20) * size + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [9, 5003])
+def test_large_gradients_of_the_entropy_beside_masks(ops, V, dtype):
+    """A masked logit has no part in the gradient however large the entropy's is."""
+    x = _logits(4, V, dtype)
+    x[:, ::3], x[1, 1::3] = float("-inf"), torch.finfo(dtype).min
+    x[2, 1] = -1e30
+    tokens = torch.tensor([1, 2, 4, 5], device="cuda")
+    x.requires_grad_(True)
+    got = ops.token_logprobs(x, tokens)
+    for much in (1e7, 1e9, 1e20, 1e35):
+        gh = torch.tensor([much, -much, much, 1.0], device="cuda")
+        dx, = torch.autograd.grad(got.entropy, x, gh, retain_graph=True)
+        want, size = _gradient(x, tokens, 0, None, torch.zeros_like(gh), gh, None)
+        rounding = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+        assert ((dx.double() - want).abs() <= rounding * want.abs() + (4 * _slack(None, V) + 2.0 ** -20) * size + 1e-30).all()
+        assert not dx[:, ::3].any()
+
+
 def _gradient(x, tokens, top, order, g, gh, gt):
     """The formula in 64 bits and the sum of magnitudes of its terms."""
     x = x.detach().double()
