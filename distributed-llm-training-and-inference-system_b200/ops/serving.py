@@ -202,7 +202,8 @@ def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
         return qkv
     fp8 = k_cache.dtype == FP8
     T, width = qkv.shape[0], (heads + 2 * kv_heads) * head_dim
-    _check(heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and head_dim > 0 and head_dim % 16 == 0, "heads: a multiple of kv_heads; head_dim: a multiple of 16")
+    _check(heads > 0 and kv_heads > 0 and heads % kv_heads == 0, "heads: a multiple of kv_heads")
+    _check(head_dim > 0 and head_dim % (16 if qkv.is_cuda or fp8 else 2) == 0, "head_dim: a multiple of 16 on a GPU and in a cache of 8 bits, else even")
     _check(qkv.dim() == 2 and qkv.shape[1] >= width, f"qkv: rows of at least {width} numbers")
     _check(not (torch.is_grad_enabled() and qkv.requires_grad), "rope_kv_append has no backward: call it under no_grad")
     for t in (cos, sin):

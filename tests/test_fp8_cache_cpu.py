@@ -102,6 +102,43 @@ def test_append_of_16_bits_is_rotation_and_append(sops, H, Hk):
         assert not c.any()
 
 
+@pytest.mark.parametrize("D", [2, 8, 24, 40])
+def test_append_of_16_bits_takes_any_even_head(sops, D):
+    """Heads of a multiple of 16 are what kernels and caches of 8 bits need; the plain form of the others' does not."""
+    from llmctl_b200.ops import functional
+    T, H = 5, 3
+    qkv, (cos, sin) = _rows(T, 3 * H, 0, D), _tables(D)
+    positions, slots = torch.tensor([3, 4, 5, 0, 63], dtype=torch.int32), torch.tensor([3, 4, 5, 8, -1])
+    want = functional.rope_packed(qkv.clone(), cos, sin, 2 * H, D, 64, positions)
+    k, v = torch.zeros(4, 4, H, D), torch.zeros(4, 4, H, D)
+    sops.rope_kv_append(qkv, cos, sin, positions, k, v, slots, H, D)
+    assert torch.equal(qkv, want)
+    for c, first in ((k, H), (v, 2 * H)):
+        assert torch.equal(c.view(-1, H, D)[slots[:4]], want.view(T, -1, D)[:4, first:first + H])
+    codes, scales = torch.zeros(1, H, 4, D, dtype=torch.float8_e4m3fn), torch.zeros(1, H)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        sops.rope_kv_append(qkv, cos, sin, positions, codes, codes.clone(), slots, H, D, k_scale=scales, v_scale=scales.clone())
+    with pytest.raises(ValueError, match="even"):
+        sops.rope_kv_append(qkv, cos, sin, positions, k, v, slots, H, D + 1)
+
+
+@pytest.mark.parametrize("head", [8, 24, 40])
+def test_engine_on_the_cpu_serves_any_even_head(head):
+    from llmctl_b200.comms import mesh
+    from llmctl_b200.models.config import ModelConfig
+    from llmctl_b200.serve.engine import InferenceEngine
+    mesh.reset_state()
+    torch.manual_seed(0)
+    cfg = ModelConfig(name="heads-test", layers=2, hidden=4 * head, ffn=64, heads=4, vocab_size=300, max_position_embeddings=64)
+    eng = InferenceEngine(cfg, device="cpu", kv_block_size=4, num_kv_blocks=64, max_batch_size=2, max_batch_tokens=128)
+    prompts = [[5, 6, 7, 8, 9], [11]]
+    for p, o in zip(prompts, eng.generate(prompts, max_tokens=6, temperature=0.0)):
+        assert len(o) == 6
+        for i, t in enumerate(o):
+            logits = eng.model(torch.tensor([p + o[:i]])).float()[-1, :300]
+            assert logits.max() - logits[t] <= 1e-4
+
+
 @pytest.mark.parametrize("H,Hk,size", [(2, 2, 16), (6, 2, 5)])
 def test_attention(sops, H, Hk, size):
     B, D = 4, 64
