@@ -224,9 +224,12 @@ def apply(fn, *args):
         for a in args:
             if isinstance(a, torch.Tensor) and a.requires_grad:
                 return fn.apply(*args)
-    if _forward_ad._current_level >= 0 or _interpreter() is not None or _tracing_state() is not None:
-        return fn.apply(*args)
-    return fn.forward(_NoContext(), *args)
+    return fn.forward(_NoContext(), *args) if unwatched() else fn.apply(*args)
+
+
+def unwatched() -> bool:
+    """No forward-mode AD, functorch transform or tracing is under way."""
+    return not (_forward_ad._current_level >= 0 or _interpreter() is not None or _tracing_state() is not None)
 
 
 def keep(ctx, *tensors) -> None:

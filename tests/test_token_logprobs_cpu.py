@@ -40,6 +40,35 @@ def test_rows_with_masks(ops):
     assert got.top_logprobs[0, 2] == -inf
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("top", [0, 1, 4])
+@pytest.mark.parametrize("numbers", [1, 200, 1 << 21])
+def test_rows_in_portions_and_as_a_whole(ops, monkeypatch, numbers, top, dtype):
+    """With gradients, and under a transform, all rows are computed at once, without some at a time: the same numbers, rows with masks and NaN among them."""
+    monkeypatch.setattr(ops, "_PLAIN_NUMBERS", numbers)
+    x = _logits(2, 4, 60).round().to(dtype)
+    x[0, 0, 1:], x[0, 1], x[0, 2, 7], x[1, 0, ::2], x[1, 1, 5] = float("-inf"), float("-inf"), float("nan"), float("-inf"), float("inf")
+    tokens = torch.randint(-1, 61, (2, 4), generator=torch.Generator().manual_seed(3))
+    got, kept = ops.token_logprobs(x, tokens, top), x.clone()
+    whole = ops.token_logprobs(x.clone().requires_grad_(True), tokens, top)
+    each = torch.vmap(lambda x, t: tuple(v for v in ops.token_logprobs(x, t, top) if v is not None))(x, tokens)
+    # sums of 60 terms in another order: 60 roundings and an exponential's own, relative to sums of at least 1 and weighted logarithms of at most log 60
+    eps = 80 * torch.finfo(torch.float32 if dtype == torch.bfloat16 else dtype).eps / 2 * 5
+    for a, b, c in zip(got, whole, each):
+        assert a.dtype == b.dtype and a.shape == b.shape
+        for other in (b, c):
+            assert torch.equal(a, other) if a.dtype == torch.int64 else torch.allclose(a, other.detach(), rtol=eps, atol=eps, equal_nan=True)
+    assert len([v for v in got if v is not None]) == len(each) == (4 if top else 2) and torch.equal(x.nan_to_num(), kept.nan_to_num())
+
+
+def test_the_best_guess_takes_no_sort(ops):
+    """What evaluation asks for, over a vocabulary of any size, is a pass for the largest number of a row."""
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as p:
+        ops.token_logprobs(_logits(3, 5000), torch.zeros(3, dtype=torch.int64), 1)
+        ops.token_logprobs(_logits(3, 5000).requires_grad_(True), torch.zeros(3, dtype=torch.int64), 1)
+    assert not [e.key for e in p.key_averages() if "sort" in e.key or "topk" in e.key]
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_the_largest_numbers(ops, dtype):
     """Finite logits up to the type's largest have numbers for all results and gradients."""
