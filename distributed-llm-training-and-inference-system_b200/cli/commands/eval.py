@@ -36,7 +36,11 @@ def evaluate_checkpoint(ckpt: Path, tasks, suite=None, batches: int = 8, batch_s
     nll, correct, count, lat = 0.0, 0, 0, []
     with torch.no_grad():
         for b in range(batches):
-            arr = torch.stack([torch.from_numpy(ds[b * batch_size + i]) for i in range(batch_size)]).to(dev)
+            arr = torch.stack([torch.from_numpy(ds[b * batch_size + i]) for i in range(batch_size)])
+            least, most = int(arr[:, 1:].min()), int(arr[:, 1:].max())
+            if least < 0 or most >= mcfg.vocab_size:
+                raise ValueError(f"the data's targets are tokens {least} to {most}, the model's vocabulary is 0 to {mcfg.vocab_size - 1}")
+            arr = arr.to(dev)
             tokens, targets = arr[:, :-1].contiguous(), arr[:, 1:].contiguous()
             t0 = time.perf_counter()
             logits = model(tokens)[:, :mcfg.vocab_size]

@@ -193,3 +193,19 @@ def test_eval_reads_likelihood_and_best_guess_from_one_call(tmp_path):
     task = res["tasks"]["perplexity"]
     assert task["tokens"] == lp.numel() and abs(task["loss"] + float(lp.mean())) < 1e-5 and abs(task["perplexity"] - math.exp(-float(lp.mean()))) < 1e-2
     assert res["tasks"]["accuracy"]["next_token_accuracy"] == float((logits.argmax(-1) == rows[:, 1:].reshape(-1)).double().mean())
+
+
+def test_eval_refuses_tokens_that_the_model_does_not_know(monkeypatch):
+    """A target outside of the vocabulary has no likelihood to be counted."""
+    import numpy as np
+
+    from llmctl_b200.cli.commands.eval import evaluate_checkpoint
+    from llmctl_b200.io import dataset
+    rows = [np.arange(3, 36, dtype=np.int64) for _ in range(4)]
+    monkeypatch.setattr(dataset, "build_dataset", lambda *a, **k: rows)
+    fine = evaluate_checkpoint("gpt-tiny", ["perplexity"], batches=2, batch_size=2, seq_len=32, device="cpu")
+    assert fine["tasks"]["perplexity"]["tokens"] == 4 * 32
+    for bad in (512, -1):
+        rows[3] = np.concatenate([np.arange(3, 35), [bad]])
+        with pytest.raises(ValueError, match="vocabulary"):
+            evaluate_checkpoint("gpt-tiny", ["perplexity"], batches=2, batch_size=2, seq_len=32, device="cpu")
