@@ -308,6 +308,62 @@ def test_attention_bad_pages_and_limits(sops):
     assert torch.equal(sops.paged_attention_decode_fp8(q[:1], k, v, ks, vs, tables[:, :2].contiguous(), n2, 10 ** 6), sops.paged_attention_decode_fp8(q[:1], k, v, ks, vs, tables, n2, 32))
 
 
+def _attend64(q, k, ks, v, vs, tables, lens):
+    """The oracle's formula and bounds, a sequence at a time on the GPU."""
+    B, H, D = q.shape
+    Hk, size = k.shape[1], k.shape[2]
+    out, bound = torch.zeros(B, H, D, device="cuda", dtype=torch.float64), torch.zeros(B, H, 2, device="cuda", dtype=torch.float64)
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        pages = tables[b, :(n + size - 1) // size].long()
+        kk, vv = ((c[pages].double() * s[pages].double()[..., None, None]).transpose(0, 1).reshape(Hk, -1, D)[:, :n] for c, s in ((k, ks), (v, vs)))
+        qq = q[b].double().view(Hk, H // Hk, D)
+        p = torch.softmax(torch.einsum("hgd,hnd->hgn", qq, kk) * D ** -0.5, -1)
+        out[b] = torch.einsum("hgn,hnd->hgd", p, vv).reshape(H, D)
+        bound[b, :, 0] = (torch.einsum("hgd,hnd->hgn", qq.abs(), kk.abs()).amax(-1) * D ** -0.5).reshape(H)
+        bound[b, :, 1] = vv.abs().amax((1, 2)).repeat_interleave(H // Hk)
+    return out, bound
+
+
+def _lens(B, most, every=7):
+    """Contexts of unlike lengths, some sequences without tokens (the first and the last, and runs of them) among them."""
+    return [0 if i % every in (0, 3) or i == B - 1 or 20 <= i < 26 else 1 + (i * 7919 + 13) % most for i in range(B - 1)] + [0]
+
+
+# What a CTA's run is: (sequences, longest context, ...) of whole items, one or two of them and more, two and three CTAs to an SM; of items of four kinds of groups;
+# of tiles that begin and end inside of items, behind the first 32 sequences and the first 64, two and three CTAs to an SM
+MANY = [(70, 200, 16, 16, 128, 16), (70, 200, 8, 8, 128, 16), (150, 300, 24, 4, 64, 16), (300, 140, 16, 1, 64, 8), (200, 260, 8, 4, 64, 32), (300, 150, 4, 4, 64, 16), (40, 1000, 8, 8, 128, 16),
+        (40, 3000, 4, 4, 128, 16), (100, 2000, 4, 2, 64, 16), (70, 2000, 8, 1, 128, 64), (40, 2500, 16, 1, 64, 16), (64, 5200, 16, 16, 128, 64)]
+
+
+@pytest.mark.parametrize("B,most,H,Hk,D,size", MANY)
+@pytest.mark.parametrize("splits", [None, 1, 40])
+def test_attention_of_many_sequences(sops, B, most, H, Hk, D, size, splits):
+    lens = _lens(B, most)
+    tables, n, blocks = _batch(lens, size)
+    (k, ks), (v, vs) = _state(blocks, Hk, size, D), _state(blocks, Hk, size, D, seed=2)
+    q = _randn(B, H, D, seed=5, std=0.1)
+    got = sops.paged_attention_decode_fp8(q, k, v, ks, vs, tables, n, max(lens), num_splits=splits).double()
+    want, bound = _attend64(q, k, ks, v, vs, tables, lens)
+    assert ((got - want).abs() <= oracle.tolerance(want, bound, D)).all()
+
+
+def test_a_wait_that_ran_out_is_raised_by_the_next_call(sops):
+    """The byte that the decode kernel sets when a wait of its runs out, set by a kernel that does nothing else."""
+    from llmctl_b200.ops import native
+    tables, n, blocks = _batch([20], 16)
+    (k, ks), (v, vs) = (sops.allocate_fp8_cache(blocks, 16, 2, 64, "cuda") for _ in range(2))
+    q = _randn(1, 2, 64)
+    native.register_signature("llmctl_wait_status_report", [native.c_int, native.c_void_p])
+    native.call("llmctl_wait_status_report", 4, native.stream_ptr())
+    torch.cuda.synchronize()
+    with pytest.raises(native.NativeError, match=native._OTHER_WAITS[0]):
+        sops.paged_attention_decode_fp8(q, k, v, ks, vs, tables, n, 20)
+    assert sops.paged_attention_decode_fp8(q, k, v, ks, vs, tables, n, 20).isfinite().all()
+    native.check_waits()
+
+
 @pytest.mark.parametrize("size", [16, 5])
 @pytest.mark.parametrize("B,H,Hk,D,limit", [(1, 32, 32, 128, 4096), (16, 32, 32, 128, 4096), (3, 8, 2, 64, 20000), (2, 2, 2, 64, 100)])
 def test_attention_over_a_cache_without_blocks(sops, B, H, Hk, D, limit, size):

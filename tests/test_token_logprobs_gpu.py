@@ -53,6 +53,20 @@ def test_forward(ops, rows, V, top, shift, pad, dtype):
     assert torch.equal(x, kept)
 
 
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 100001), (torch.float32, 50001)])
+@pytest.mark.parametrize("rows,top", [(60, 20), (120, 1), (200, 20), (296, 5), (297, 64)])
+def test_clusters_of_every_size(ops, rows, top, dtype, V):
+    """Rows so long that eight, four, two or one CTA go to each by how many of them there are."""
+    x, tokens = _logits(rows, V, dtype, pad=3), _tokens(rows, V)
+    got = ops.token_logprobs(x, tokens, top)
+    lp, chosen, entropy, order = _want(x, tokens, top)
+    eps = _slack(lp, V)
+    assert ((got.logprobs - chosen).abs() <= eps + 2.0 ** -22 * chosen.abs()).all()
+    assert ((got.entropy - entropy).abs() <= eps * (2 + 2 * entropy) + 1e-6).all()
+    assert torch.equal(got.top_ids, order)
+    assert ((got.top_logprobs - lp.gather(1, order)).abs() <= eps + 2.0 ** -22 * lp.gather(1, order).abs()).all()
+
+
 @pytest.mark.parametrize("V,top", [(4000, 20), (40, 40), (33000, 64)])
 def test_ties_and_order(ops, V, top):
     """Equal logits: the lowest ids; logits that rise or fall along the row, and rows whose largest numbers all stand in one thread's units."""
