@@ -11,7 +11,7 @@
 //
 // 2000 x 50257 in 32 bits 68 us (5.9 TB/s: the pass over the logits bounds it), 4096 x 32000 bf16 48 us (5.4 TB/s; instructions and exponentials are as near: two
 // thirds of either's rate), 64 x 32000 with 5 alternatives 6.3 us, one row with 20 6.9 us (the chain of a cluster's exchanges).
-// Backward: 4096 x 32000 bf16 86 us (6.1 TB/s over logits and their gradient).
+// Backward: 4096 x 32000 bf16 86 us (6.1 TB/s over logits and their gradient), in 32 bits 168 (6.2).
 //
 // Reference: none — the reference offers neither (its server returns text alone, reference llmctl/serve/server.py:57-75).
 #include <type_traits>

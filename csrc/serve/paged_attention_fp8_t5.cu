@@ -45,7 +45,7 @@ constexpr int kWholeTokens = 768, kLeast = 2;
 constexpr float kStep = 16.f;                // between the columns of a number
 // Eight query heads: the references stay where they are while no score is beyond them by more than kSlack, and no weight by kSlackV (log2; a weight of 1 is then
 // 128, and none above 430), and no maxima are taken.  us, maxima in each tile / so: 70 contexts of up to 31760, 24 heads of 64 over 4 215 / 188, 8 of 8000, 64 heads of 128
-// over 8 31.6 / 31.2; one head 60.9 / 61.2, four 64.5 / 64.6, sixteen 30.9 / 32.9.
+// over 8 31.6 / 31.2; one head 60.9 / 61.2, four 64.5 / 64.6, sixteen 30.9 / 32.9 (floors 110, 14; 53, 52, 7).
 constexpr float kSlack = 32.f, kSlackV = 1.75f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int columns(int GP) { return GP < 4 ? 16 : kPieces * GP; }     // of a product: 16 at least, of which those past 4 GP are nobody's

@@ -128,9 +128,10 @@ rope_kv_append_kernel(RopeRows r, uint32_t total, FastDiv per_token, FastDiv per
 // all heads, and keeps its token's angles; as many warps as the block's rows need write a head after the other: the largest rotated number, by
 // all of them, the scale, the codes.  The next head's numbers are asked for beside that.  (A warp to a head's block had to read the angles anew for each
 // row and head and rotate twice, for want of registers: 8000 tokens, 40 heads of 128 130 us, so 112.)  Blocks of more than twice the rows
-// that 8 warps hold are read twice, by a warp to a head.  The other CTAs rotate q, four units to a thread.
+// that 8 warps hold are read twice, by a warp to a head (8000 tokens, 40 heads of 128 in blocks of 64 104 us, of 128 175, of 256 207).  The other CTAs rotate q, four units to a thread.
 //
-// Prompts are bound by reads and writes of memory together: 8000 tokens, 40 heads of 128 99 us, 5.0 TB/s, 60000 of 32 heads 560 (5.3).  A CTA's heads of keys
+// Prompts: 8000 tokens, 40 heads of 128 99 us, 5.0 TB/s (floor 75), 60000 of 32 heads 560 (5.3).  No unit is at its limit (DRAM 54% of its peak, 2.2 instructions a
+// clock and SM, warps 36%).  A CTA's heads of keys
 // take 3.3 thousand clocks each (10 KB read and written), those of values 2.0 (6 KB), and q the rest of the time at the same 18.5 bytes a clock and SM; finding a block's
 // tokens and the first rows take 9 of a CTA's 60 thousand.  Decoded tokens by the chain slots - block's codes - maximum - codes: one 3.6 us, 64 with 32 heads 6.9.
 // ---------------------------------------------------------------------------------------------

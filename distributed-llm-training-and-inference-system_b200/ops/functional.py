@@ -846,7 +846,8 @@ def _token_logprobs_rows(x: torch.Tensor, at: torch.Tensor, top: int):
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
     """Log probabilities of ``tokens`` (int64 [...]; a number that is no token of the vocabulary has 0 and no gradient) under ``logits`` [..., vocabulary], the
     entropy of each row and its ``top`` most probable tokens.  ``logits`` are left as they are; gradients of the log probabilities (``top_logprobs`` among
-    them) and of the entropy flow back to them.  A row that holds a NaN or +inf, or nothing but -inf, has NaN for each."""
+    them) and of the entropy flow back to them, read from the logits once more: ``cross_entropy`` of the same logits, which overwrites them, needs a copy.  A row that
+    holds a NaN or +inf, or nothing but -inf, has NaN for each."""
     if logits.is_cuda and _cfg.elementwise == "native":
         out = native.fast.token_logprobs(logits, tokens, top)
         if out is not None:

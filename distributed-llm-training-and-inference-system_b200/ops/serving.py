@@ -191,7 +191,8 @@ def rope_kv_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posi
                    v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotates q and k of the packed rows ``qkv`` [T, (heads + 2 kv_heads) * head_dim] in place to their ``positions`` (int32 [T], rows of the tables ``cos`` /
     ``sin``, fp32 [positions, head_dim / 2]; one outside of them reads the nearest) and writes k and v to the rows ``slot_mapping`` (int64 [T]; outside of the
-    cache = skip) of the caches: [blocks, block_size, kv_heads, head_dim] of the rows' type, or caches of 8 bits with their scales.  Returns ``qkv``.
+    cache = skip) of the caches: [blocks, block_size, kv_heads, head_dim] of the rows' type, or caches of 8 bits with their scales.  head_dim is a multiple of 16 on a GPU and for
+    caches of 8 bits, else even.  Returns ``qkv``.
 
     In a cache of 16 bits a row that the call names more than once is left with numbers of any of those tokens, of several perhaps: name it once, as with
     ``kv_append``.  In a cache of 8 bits the last is kept.  There a block's scale is the smallest power of two under which the largest number
@@ -270,7 +271,8 @@ def paged_attention_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: 
                                num_splits: Optional[int] = None) -> torch.Tensor:
     """``paged_attention_decode`` over caches of 8 bits: q [B, heads, head_dim], a token per sequence; block_tables: int32 [B, max_blocks]; context_lens: int32
     [B], at most ``max_context`` (tokens beyond it, or beyond the table, are left out) -> [B, heads, head_dim].  heads may be a multiple of the cache's heads:
-    query head h reads head h // (heads / kv_heads).  A sequence without tokens gets zeros.  What the cache holds behind a sequence's last token does not matter."""
+    query head h reads head h // (heads / kv_heads).  A sequence without tokens gets zeros.  What the cache holds behind a sequence's last token does not matter.  On a GPU
+    blocks of a multiple of 8 tokens are read at six times the speed of others."""
     B, H, D = q.shape
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
     if q.is_cuda and num_splits != 0:
