@@ -42,7 +42,7 @@ LLMCTL_API void* llmctl_wait_status_word() { return wait_word(); }
 // Sets a kernel's byte from the device, as its waits do when they run out.
 LLMCTL_API int llmctl_wait_status_report(int which, void* stream) {
   LLMCTL_BEGIN();
-  LLMCTL_REQUIRE(which >= 0 && which < 5);
+  LLMCTL_REQUIRE(which >= 0 && which < 7);
   unsigned char* const byte = wait_report(static_cast<WaitReport>(which));
   LLMCTL_REQUIRE(byte != nullptr);
   wait_report_kernel<<<1, 1, 0, (cudaStream_t)stream>>>(byte);

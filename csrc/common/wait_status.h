@@ -6,7 +6,7 @@
 
 namespace llmctl {
 
-enum WaitReport { kWaitFlashForward = 0, kWaitFlashBackward = 1, kWaitCrossEntropy = 2, kWaitLatentAttention = 3, kWaitPagedFp8 = 4 };
+enum WaitReport { kWaitFlashForward = 0, kWaitFlashBackward = 1, kWaitCrossEntropy = 2, kWaitLatentAttention = 3, kWaitPagedFp8 = 4, kWaitInt4 = 5, kWaitPagedShared = 6 };
 
 // The byte for this kernel, valid on the host and on every device; null if pinned memory cannot be had.
 unsigned char* wait_report(WaitReport which);

@@ -47,7 +47,8 @@ using at::Tensor;
   X(llmctl_rmsnorm_fwd) X(llmctl_rmsnorm_bwd_bf16w) X(llmctl_rope_inplace) X(llmctl_gemm_rope_bf16) X(llmctl_gemm_bf16) X(llmctl_gemm_swiglu_bf16)               \
   X(llmctl_gemm_swiglu_bwd_bf16) X(llmctl_swiglu_bwd) X(llmctl_gemm_skinny_bf16) X(llmctl_gemm_skinny_scratch_elems) X(llmctl_flash_attn_fwd) X(llmctl_flash_attn_bwd) X(llmctl_kv_append) \
   X(llmctl_paged_attn_decode) X(llmctl_paged_attn_scratch_elems) X(llmctl_latent_kv_write) X(llmctl_latent_decode) \
-  X(llmctl_rope_kv_append) X(llmctl_rope_kv_append_fp8) X(llmctl_rope_kv_append_fp8_scratch_elems) X(llmctl_paged_attn_decode_fp8) X(llmctl_paged_attn_fp8_scratch_elems) X(llmctl_token_logprobs) X(llmctl_token_logprobs_bwd)
+  X(llmctl_rope_kv_append) X(llmctl_rope_kv_append_fp8) X(llmctl_rope_kv_append_fp8_scratch_elems) X(llmctl_paged_attn_decode_fp8) X(llmctl_paged_attn_fp8_scratch_elems) X(llmctl_token_logprobs) X(llmctl_token_logprobs_bwd) \
+  X(llmctl_gemm_int4) X(llmctl_gemm_int4_scratch_elems)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
   LLMCTL_ENTRIES(X)
@@ -605,6 +606,43 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                          static_cast<unsigned int*>(data(counters)), static_cast<int>(counters.numel()), 0, stream()));
       else
         gemm(rows, w, out, false, false, false, tile_n, 0);
+      return as_shape_of(out, x);
+    });
+    return THPVariable_Wrap(y);
+  });
+}
+
+// linear_int4(x, w, scale, gated, workspace) -> x @ W.T, or swiglu(x @ W.T), of at most 128 rows with weights of 4 bits
+PyObject* py_linear_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return call(a, n, 5, [&](Args& args) -> PyObject* {
+    const Tensor x = args.tensor(0), w = args.tensor(1), scale = args.tensor(2);
+    const bool gated = args.integer(3);
+    if (!args.ok || !quiet() || !ready(lib.llmctl_gemm_int4) || !lib.llmctl_gemm_int4_scratch_elems || !bf16(x) || x.dim() < 1 || x.numel() == 0 || recorded({&x}) ||
+        x.get_device() != c10::cuda::current_device() || w.get_device() != x.get_device() || scale.get_device() != x.get_device())
+      return none();
+    const int64_t K = x.size(-1), T = x.numel() / K;
+    if (T > 128 || K % 128 || w.scalar_type() != at::kByte || w.dim() != 2 || w.size(1) * 2 != K || w.size(0) == 0 || w.stride(1) != 1 || w.stride(0) % 16 || w.stride(0) < K / 2 || !unit16(w) ||
+        (gated && w.size(0) % 2) || scale.scalar_type() != at::kHalf || scale.dim() != 2 || scale.size(0) != w.size(0) || scale.size(1) != K / 128 || scale.stride(1) != 1 ||
+        scale.stride(0) < scale.size(1) || w.size(0) > (1 << 28) || K > (1 << 28))
+      return none();
+    const Tensor rows = as_rows(x);
+    if (!rows.defined() || rows.stride(0) < K) return none();
+    const int64_t N = w.size(0) / (gated ? 2 : 1);
+    int tickets = 0;
+    const long long elems = lib.llmctl_gemm_int4_scratch_elems(static_cast<int>(T), static_cast<int>(N), static_cast<int>(K), gated, &tickets);
+    Tensor ws, counters;
+    if (elems) {
+      PyObject* pair = PyObject_CallFunction(a[4], "OLi", a[0], elems, tickets);
+      if (pair == nullptr) throw python_error();
+      ws = THPVariable_Unpack(PyTuple_GET_ITEM(pair, 0));
+      counters = THPVariable_Unpack(PyTuple_GET_ITEM(pair, 1));
+      Py_DECREF(pair);
+    }
+    Tensor y = without_gil([&] {
+      Tensor out = fresh({T, N}, at::kBFloat16);
+      done("llmctl_gemm_int4", lib.llmctl_gemm_int4(cdata(rows), rows.stride(0), cdata(w), w.stride(0), cdata(scale), scale.stride(0), data(out), N, static_cast<int>(T), static_cast<int>(N),
+                                                    static_cast<int>(K), gated, elems ? static_cast<float*>(data(ws)) : nullptr, elems ? ws.numel() : 0,
+                                                    elems ? static_cast<unsigned int*>(data(counters)) : nullptr, elems ? static_cast<int>(counters.numel()) : 0, stream()));
       return as_shape_of(out, x);
     });
     return THPVariable_Wrap(y);
@@ -1233,7 +1271,7 @@ PyObject* py_bind(PyObject*, PyObject* args) {
 PyObject* py_launches(PyObject*, PyObject*) { return PyLong_FromLongLong(launches.load(std::memory_order_relaxed)); }
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&py_##name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {{"bind", py_bind, METH_VARARGS, nullptr}, {"launches", py_launches, METH_NOARGS, nullptr}, FAST(rmsnorm), FAST(gemm), FAST(linear), FAST(gemm_swiglu),
+PyMethodDef methods[] = {{"bind", py_bind, METH_VARARGS, nullptr}, {"launches", py_launches, METH_NOARGS, nullptr}, FAST(rmsnorm), FAST(gemm), FAST(linear), FAST(linear_int4), FAST(gemm_swiglu),
                          FAST(mlp), FAST(attention), FAST(rope_attention), FAST(block), FAST(kv_append), FAST(paged_decode), FAST(latent_kv_write), FAST(latent_decode), FAST(rope_kv_append),
                          FAST(paged_decode_fp8), FAST(token_logprobs), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "llmctl_ops", "Host side of the operators (csrc/torch/ops.cpp)", -1, methods};

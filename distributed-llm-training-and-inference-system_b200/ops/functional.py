@@ -15,6 +15,7 @@ can attribute speed-ups.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import threading
 from dataclasses import dataclass
 from typing import NamedTuple, Optional, Tuple
@@ -23,6 +24,8 @@ import torch
 import torch.nn.functional as F
 
 from . import native
+
+c_void_p, c_int, c_ll = native.c_void_p, native.c_int, native.c_ll
 
 # ------------------------------------------------------------------------------------------------
 # backend selection
@@ -626,6 +629,121 @@ def decoder_block(x: torch.Tensor, residual: Optional[torch.Tensor], norm1: torc
         return None
     return native.fast.block(x, residual, norm1, qkv, out, norm2, up, down, cos, sin, None if positions is None else positions.to(torch.int32), batch, seq, heads,
                              head_dim, eps, head_dim ** -0.5, 0, SKINNY_MAX_ROWS)
+
+
+# ------------------------------------------------------------------------------------------------
+# Products with weights of 4 bits  (K0q)
+# ------------------------------------------------------------------------------------------------
+INT4_GROUP = 128                # input channels to a scale
+
+native.register_signature("llmctl_gemm_int4", [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll] + [c_int] * 4 + [c_void_p, c_ll, c_void_p, c_int, c_void_p])
+native.register_signature("llmctl_gemm_int4_scratch_elems", [c_int] * 4 + [c_void_p], restype=c_ll)
+native.register_signature("llmctl_int4_widen", [c_void_p, c_ll, c_void_p, c_ll, c_void_p] + [c_int] * 4 + [c_void_p])
+
+# Tokens up to which the weights are read in 4 bits.  For more of them they are widened to bf16 once, which costs what 60 tokens more would, and the product is
+# the GEMM's (us, in 4 bits / widened: 12288 x 4096 128 tokens 44 / 45, 256 88 / 55).
+_INT4_TOKENS = 128
+
+
+def dequantize_int4(w: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The matrix [N, K] that 4-bit codes ``w`` [N, K / 2] and scales [N, K / 128] stand for (the layout of the ``int4`` quantiser)."""
+    codes = torch.stack([w & 15, w >> 4], dim=2).view(w.shape[0], -1, INT4_GROUP).float() - 8.0
+    return (codes * scale.float().unsqueeze(2)).view(w.shape[0], -1).to(dtype)
+
+
+def _check_int4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, gated: bool) -> None:
+    def need(ok: bool, what: str) -> None:
+        if not ok:
+            raise ValueError(f"weights of 4 bits: {what}")
+    need(x.dim() >= 1 and x.is_floating_point(), "x is a floating tensor [..., K]")
+    K = x.shape[-1]
+    need(K > 0 and K % INT4_GROUP == 0, f"K = {K} is no multiple of {INT4_GROUP}")
+    need(w.dim() == 2 and w.dtype == torch.uint8 and w.shape[1] * 2 == K and w.device == x.device, f"w is uint8 [N, {K // 2}] beside x, two columns to a byte")
+    need(scale.dtype == torch.float16 and scale.shape == (w.shape[0], K // INT4_GROUP) and scale.device == x.device,
+         f"scale is float16 [{w.shape[0]}, {K // INT4_GROUP}] beside x")
+    need(not gated or w.shape[0] % 2 == 0, "gate and up rows are as many")
+    need(not (torch.is_grad_enabled() and x.requires_grad), "the product has no backward: call it under no_grad")
+
+
+def _int4_torch(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, gated: bool) -> torch.Tensor:
+    """In 32 bits with one rounding, whatever the type of x; a block of rows at a time."""
+    x32, step = x.float(), max(1, (1 << 26) // x.shape[-1])
+    parts = [F.linear(x32, dequantize_int4(w[i:i + step], scale[i:i + step], torch.float32)) for i in range(0, w.shape[0], step)]
+    y = torch.cat(parts, -1) if parts else x32.new_zeros(*x.shape[:-1], 0)
+    if gated:
+        gate, up = y.chunk(2, -1)
+        y = F.silu(gate) * up
+    return y.to(x.dtype)
+
+
+def _int4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, gated: bool) -> torch.Tensor:
+    if _cfg.gemm == "native" and x.is_cuda:
+        y = native.fast.linear_int4(x, w, scale, gated, _int4_workspace)
+        if y is not None:
+            return y
+    _check_int4(x, w, scale, gated)
+    if not _use_native(x, "gemm"):
+        return _int4_torch(x, w, scale, gated)
+    K, N = x.shape[-1], w.shape[0] // (2 if gated else 1)
+    out = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    x2, out2 = x.reshape(-1, K), out.view(-1, N)
+    if not _gemm_ok(x2) or x2.stride(0) < K:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    if w.stride(1) != 1 or w.stride(0) % 16 or w.stride(0) < K // 2 or w.data_ptr() % 16:
+        w = w.clone(memory_format=torch.contiguous_format)
+    if scale.stride(1) != 1 or scale.stride(0) < scale.shape[1]:
+        scale = scale.contiguous()
+    with _on_device(x):
+        if x2.shape[0] > _INT4_TOKENS:
+            _int4_prompt(x2, w, scale, gated, out2)
+            return out
+        need, tickets = native.lib().llmctl_gemm_int4_scratch_elems, ctypes.c_int()
+        elems = need(x2.shape[0], N, K, int(gated), ctypes.addressof(tickets))
+        ws = (None, 0, None, 0)
+        if elems:
+            partial, counters = _int4_workspace(x2, elems, tickets.value)
+            ws = (partial.data_ptr(), partial.numel(), counters.data_ptr(), counters.numel())
+        native.call("llmctl_gemm_int4", x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), scale.data_ptr(), scale.stride(0), out2.data_ptr(), N, x2.shape[0], N, K,
+                    int(gated), *ws, native.stream_ptr())
+    return out
+
+
+def _int4_workspace(x: torch.Tensor, elems: int, tickets: int):
+    """Partial sums and counters: the decode GEMM's, or, of matrices too large for them, of this call."""
+    if elems <= _SKINNY_ELEMS and tickets <= _SKINNY_TICKETS:
+        return _skinny_workspace(x, elems)
+    return torch.empty(elems, dtype=torch.float32, device=x.device), torch.zeros(tickets, dtype=torch.int32, device=x.device)
+
+
+def _int4_prompt(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, gated: bool, out: torch.Tensor) -> None:
+    """The product of many tokens: the weights as bf16 rows (in number a multiple of 8, as the GEMM stores them), used once."""
+    K, halves = x.shape[1], 2 if gated else 1
+    N = w.shape[0] // halves
+    padded = -(-N // 8) * 8
+    wide = torch.empty(halves * padded, K, dtype=torch.bfloat16, device=x.device)
+    native.call("llmctl_int4_widen", w.data_ptr(), w.stride(0), scale.data_ptr(), scale.stride(0), wide.data_ptr(), N, padded, halves, K, native.stream_ptr())
+    whole = out if padded == N else torch.empty(x.shape[0], padded, dtype=out.dtype, device=out.device)
+    if gated:
+        native.call("llmctl_gemm_swiglu_bf16", x.data_ptr(), wide.data_ptr(), None, whole.data_ptr(), x.shape[0], padded, K, x.stride(0), K, 2 * padded, padded,
+                    native.stream_ptr())
+    else:
+        gemm_raw(x, wide, out=whole)
+    if whole is not out:
+        out.copy_(whole[:, :N])
+
+
+def linear_int4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """``x @ W.T`` for weights kept in 4 bits, as the ``int4`` quantiser (io/quantize.py) writes them.  x: [..., K]; w: uint8 [N, K / 2], column 2i of a row
+    in the low half of byte i and 2i + 1 in the high one, each the value + 8; scale: fp16 [N, K / 128], one for 128 input channels.  Returns [..., N] of
+    x's type.  No gradients."""
+    return _int4(x, w, scale, False)
+
+
+def linear_swiglu_int4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """``swiglu(x @ W.T)`` for a packed ``W`` [2F, K] (gate rows first) of 4 bits, laid out as ``linear_int4`` takes it: [..., F], rounded once."""
+    return _int4(x, w, scale, True)
 
 
 class _SwiGLULinearFn(torch.autograd.Function):

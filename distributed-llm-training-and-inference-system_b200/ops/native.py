@@ -256,7 +256,7 @@ class NativeError(RuntimeError):
 # the entry points that read and clear their device-side status.
 _WAITS = (("flash attention forward", "llmctl_flash_fwd_status"), ("flash attention backward", "llmctl_flash_bwd_status"),
           ("cross-entropy", "llmctl_cross_entropy_status"), ("latent attention", "llmctl_latent_attention_t5_status"))
-_OTHER_WAITS = ("paged decode attention over 8 bits",)      # behind those: kernels that keep no status on the device
+_OTHER_WAITS = ("paged decode attention over 8 bits", "products with weights of 4 bits", "paged decode attention over shared prefixes")      # behind those: kernels that keep no status on the device
 _wait_word = ctypes.c_uint64(0)         # the library's word once a kernel has been launched
 _wait_bound = False
 

@@ -165,6 +165,17 @@ int llmctl_gemm_skinny_bf16(const void* X, const void* W, void* C, int Mb, int N
 long long llmctl_gemm_skinny_scratch_elems(int Mb, int N, int K, int splits);
 unsigned long long llmctl_stream_capture_id(void* stream);
 
+/* ---- K0q products of up to 512 tokens with weights of 4 bits (csrc/gemm/gemm_int4.cu): out[t, n] = sum_k x[t, k] scale[n, k / 128] (q[n, k] - 8), x bf16
+ * [tokens, K], w uint8 rows of K / 2 bytes (column 2i in the low half of byte i), scale fp16 rows of K / 128, K a multiple of 128.  gated: w has 2 * rows rows,
+ * gate first, and out = silu(gate) * up.  x and w lie on 16-byte boundaries, ldx % 8 == 0, ldw % 16 == 0 (bytes).  partial: fp32 scratch, tickets: zeroed
+ * counters (left zero on return), as many as llmctl_gemm_int4_scratch_elems says (0: not used); one call at a time per pair, as with the skinny GEMM.
+ * llmctl_int4_widen: bf16 [halves * padded, K] of w [halves * rows, K / 2]; rows past a half's last are zeros.
+ * Reference: none (`--quant` is an option of a stub command, llmctl/cli/commands/export.py:17). */
+long long llmctl_gemm_int4_scratch_elems(int tokens, int rows, int K, int gated, int* tickets);
+int llmctl_gemm_int4(const void* x, long long ldx, const void* w, long long ldw, const void* scale, long long lds, void* out, long long ldo, int tokens,
+                     int rows, int K, int gated, float* partial, long long partial_elems, unsigned int* tickets, int n_tickets, void* stream);
+int llmctl_int4_widen(const void* w, long long ldw, const void* scale, long long lds, void* out, int rows, int padded, int halves, int K, void* stream);
+
 /* ---- K6 causal flash attention, head_dim 64 or 128, bf16.  q/k/v/o: [B,S,H,D] views with token strides in
  * elements; lse: fp32 [B,H,S] (natural log).  Any S when causal, else a multiple of 128.  Reference: SDPA/eager inside
  * the HF model (engine.py:284); baseline cuDNN SDPA.
