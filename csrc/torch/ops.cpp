@@ -48,7 +48,7 @@ using at::Tensor;
   X(llmctl_gemm_swiglu_bwd_bf16) X(llmctl_swiglu_bwd) X(llmctl_gemm_skinny_bf16) X(llmctl_gemm_skinny_scratch_elems) X(llmctl_flash_attn_fwd) X(llmctl_flash_attn_bwd) X(llmctl_kv_append) \
   X(llmctl_paged_attn_decode) X(llmctl_paged_attn_scratch_elems) X(llmctl_latent_kv_write) X(llmctl_latent_decode) \
   X(llmctl_rope_kv_append) X(llmctl_rope_kv_append_fp8) X(llmctl_rope_kv_append_fp8_scratch_elems) X(llmctl_paged_attn_decode_fp8) X(llmctl_paged_attn_fp8_scratch_elems) X(llmctl_token_logprobs) X(llmctl_token_logprobs_bwd) \
-  X(llmctl_gemm_int4) X(llmctl_gemm_int4_scratch_elems)
+  X(llmctl_gemm_int4) X(llmctl_gemm_int4_scratch_elems) X(llmctl_paged_attn_decode_shared) X(llmctl_paged_attn_shared_scratch_elems)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
   LLMCTL_ENTRIES(X)
@@ -1053,6 +1053,37 @@ PyObject* py_paged_decode_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// paged_decode_shared(q, k_cache, v_cache, tables, lens, group_starts, shared_lens, scale) -> out
+PyObject* py_paged_decode_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return call(a, n, 8, [&](Args& args) -> PyObject* {
+    const Tensor q = args.tensor(0), k = args.tensor(1), v = args.tensor(2), tables = args.tensor(3), lens = args.tensor(4), starts = args.tensor(5), shared = args.tensor(6);
+    const double scale = args.number(7);
+    if (!args.ok || !quiet() || !ready(lib.llmctl_paged_attn_decode_shared) || !lib.llmctl_paged_attn_shared_scratch_elems ||
+        !here({&q, &k, &v, &tables, &lens, &starts, &shared}) || !bf16(q) || q.dim() != 3 || q.numel() == 0 || q.stride(2) != 1 || q.stride(1) != q.size(2) || q.stride(0) % 8 ||
+        !unit16(q) || recorded({&q}) || !(scale > 0))
+      return none();
+    const int64_t B = q.size(0), H = q.size(1), D = q.size(2), G = shared.numel();
+    if ((D != 64 && D != 128) || B >= 65536 || G > 65536 || !bf16(k) || !bf16(v) || k.dim() != 4 || v.sizes() != k.sizes() || !k.is_contiguous() || !v.is_contiguous() || !unit16(k) ||
+        !unit16(v) || k.size(3) != D || k.numel() == 0 || k.size(0) >= (1LL << 31) || k.size(1) % 8 || k.size(1) >= (1LL << 31) || H % k.size(2))
+      return none();
+    for (const Tensor* t : {&tables, &lens, &starts, &shared})
+      if (t->scalar_type() != at::kInt || !t->is_contiguous() || t->dim() != (t == &tables ? 2 : 1)) return none();
+    if (tables.size(0) < B || tables.size(1) >= (1LL << 31) || lens.size(0) < B || starts.size(0) != G + 1) return none();
+    Tensor o = without_gil([&] {
+      const auto i32 = [](const Tensor& x) { return static_cast<const int*>(cdata(x)); };
+      Tensor scratch = fresh({lib.llmctl_paged_attn_shared_scratch_elems(static_cast<int>(B), static_cast<int>(G), static_cast<int>(H), static_cast<int>(D))}, at::kFloat),
+             out = fresh(q.sizes(), at::kBFloat16);
+      done("llmctl_paged_attn_decode_shared",
+           lib.llmctl_paged_attn_decode_shared(cdata(q), q.stride(0), cdata(k), cdata(v), i32(tables), static_cast<int>(tables.size(1)), i32(lens), i32(starts), i32(shared), data(out),
+                                               static_cast<float*>(data(scratch)), static_cast<int>(B), static_cast<int>(G), static_cast<int>(H), static_cast<int>(k.size(2)),
+                                               static_cast<int>(D), static_cast<int>(k.size(0)), static_cast<int>(k.size(1)), static_cast<float>(scale), stream()),
+           2);
+      return out;
+    });
+    return THPVariable_Wrap(o);
+  });
+}
+
 // ---------------------------------------------------------------------------------------------------------------------------------
 // log probabilities of tokens
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -1273,7 +1304,7 @@ PyObject* py_launches(PyObject*, PyObject*) { return PyLong_FromLongLong(launche
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"bind", py_bind, METH_VARARGS, nullptr}, {"launches", py_launches, METH_NOARGS, nullptr}, FAST(rmsnorm), FAST(gemm), FAST(linear), FAST(linear_int4), FAST(gemm_swiglu),
                          FAST(mlp), FAST(attention), FAST(rope_attention), FAST(block), FAST(kv_append), FAST(paged_decode), FAST(latent_kv_write), FAST(latent_decode), FAST(rope_kv_append),
-                         FAST(paged_decode_fp8), FAST(token_logprobs), {nullptr, nullptr, 0, nullptr}};
+                         FAST(paged_decode_fp8), FAST(token_logprobs), FAST(paged_decode_shared), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "llmctl_ops", "Host side of the operators (csrc/torch/ops.cpp)", -1, methods};
 
 }  // namespace

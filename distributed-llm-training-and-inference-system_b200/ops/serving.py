@@ -27,6 +27,9 @@ native.register_signature("llmctl_paged_attn_fp8_scratch_elems", [c_int] * 8, re
 native.register_signature("llmctl_paged_attn_decode_fp8", [c_void_p, c_ll] + [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 8 + [c_float, c_void_p])
 native.register_signature("llmctl_sample", [c_void_p, c_int, c_ll, c_int, c_int] + [c_void_p] * 6 + [c_void_p])
 
+native.register_signature("llmctl_paged_attn_shared_scratch_elems", [c_int] * 4, restype=c_ll)
+native.register_signature("llmctl_paged_attn_decode_shared", [c_void_p, c_ll, c_void_p, c_void_p, c_void_p, c_int] + [c_void_p] * 5 + [c_int] * 7 + [c_float, c_void_p])
+
 
 def _check(ok: bool, what: str) -> None:
     if not ok:
@@ -312,6 +315,76 @@ def paged_attention_decode_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: 
             continue
         pages = block_tables[b, :(n + block_size - 1) // block_size].long()
         k, v = ((c[pages].float() * s[pages][..., None, None]).transpose(0, 1).reshape(kv_heads, -1, D)[:, :n] for c, s in ((k_cache, k_scale), (v_cache, v_scale)))
+        s = torch.einsum("kgd,knd->kgn", q[b].float().view(kv_heads, H // kv_heads, D), k) * scale
+        out[b] = torch.einsum("kgn,knd->kgd", torch.softmax(s, -1), v).reshape(H, D).to(q.dtype)
+    return out
+
+
+def paged_attention_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+                                  group_starts: torch.Tensor, shared_lens: torch.Tensor, scale: Optional[float] = None) -> torch.Tensor:
+    """``paged_attention_decode`` of groups of sequences whose contexts begin with the same blocks, completions of one prompt for instance, which are read once
+    for a group.  q: [B, heads, head_dim], a token per sequence; caches [blocks, block_size, kv_heads, head_dim] of q's type; block_tables: int32 [B, max_blocks];
+    context_lens: int32 [B] (tokens beyond the table are left out).  group_starts: int32 [G + 1], ascending: the sequences group_starts[g] up to group_starts[g + 1] are
+    one group, whose tables name the same blocks for their first shared_lens[g] (int32 [G]) tokens; a number that is not of whole blocks is taken too.  Sequences in no
+    group, and a group of one, share nothing.  All stand beside q, and what they hold is read when the kernel runs, so that a captured call follows them.
+    -> [B, heads, head_dim].
+
+    heads may be a multiple of the cache's heads: query head h reads head h // (heads / kv_heads).  A sequence without tokens gets zeros, one that is
+    shorter than what its group shares its own tokens of them.  What the cache holds behind a sequence's last token does not matter (but for what its group shares,
+    which has to be numbers).  On a GPU: bfloat16, heads of 64 or 128, blocks of a multiple of 8 tokens."""
+    _check(q.dim() == 3, "q: [sequences, heads, head_dim]")
+    B, H, D = q.shape
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    if q.is_cuda:
+        out = native.fast.paged_decode_shared(q, k_cache, v_cache, block_tables, context_lens, group_starts, shared_lens, scale)
+        if out is not None:
+            return out
+    _check(not (torch.is_grad_enabled() and q.requires_grad), "paged_attention_decode_shared has no backward: call it under no_grad")
+    _check(scale > 0, "scale: positive")
+    for c in (k_cache, v_cache):
+        _check(c.dim() == 4 and c.dtype == q.dtype and c.is_contiguous() and c.device == q.device and c.shape[3] == D and c.data_ptr() % 16 == 0,
+               f"a cache is contiguous [blocks, block_size, kv_heads, {D}] of q's type beside it, from a 16-byte boundary")
+    _check(k_cache.shape == v_cache.shape, "k_cache and v_cache: of one shape")
+    blocks, block_size, kv_heads = k_cache.shape[:3]
+    _check(kv_heads > 0 and H % kv_heads == 0, "heads: a multiple of the cache's")
+    _check(block_tables.dim() == 2 and block_tables.shape[0] >= B and block_tables.dtype == torch.int32 and block_tables.device == q.device, "block_tables: int32 beside the queries, a row per sequence")
+    _check(context_lens.dim() == 1 and context_lens.numel() >= B and context_lens.dtype == torch.int32 and context_lens.device == q.device, "context_lens: int32 beside the queries, one per sequence")
+    G = shared_lens.numel()
+    _check(shared_lens.dim() == 1 and shared_lens.dtype == torch.int32 and shared_lens.device == q.device, "shared_lens: int32 beside the queries, one per group")
+    _check(group_starts.dim() == 1 and group_starts.numel() == G + 1 and group_starts.dtype == torch.int32 and group_starts.device == q.device,
+           "group_starts: int32 beside the queries, one more than groups")
+    if q.is_cuda:
+        _check(q.dtype == torch.bfloat16 and D in (64, 128), "q: bfloat16, heads of 64 or 128")
+        _check(block_size % 8 == 0 and block_size > 0, "blocks of a multiple of 8 tokens")
+        out = torch.empty(B, H, D, dtype=q.dtype, device=q.device)
+        if out.numel() == 0:
+            return out
+        if blocks == 0:
+            return out.zero_()
+        block_tables, context_lens, group_starts, shared_lens = (t.contiguous() for t in (block_tables, context_lens, group_starts, shared_lens))
+        if q.stride(2) != 1 or q.stride(1) != D or q.data_ptr() % 16 or q.stride(0) % 8:
+            q = q.clone(memory_format=torch.contiguous_format)
+        scratch = torch.empty(native.lib().llmctl_paged_attn_shared_scratch_elems(B, G, H, D), dtype=torch.float32, device=q.device)
+        with _on_device(q):
+            native.call("llmctl_paged_attn_decode_shared", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), block_tables.shape[1],
+                        context_lens.data_ptr(), group_starts.data_ptr(), shared_lens.data_ptr(), out.data_ptr(), scratch.data_ptr(), B, G, H, kv_heads, D, blocks, block_size,
+                        float(scale), native.stream_ptr())
+        return out
+    out = torch.zeros(B, H, D, dtype=q.dtype)
+    first, starts = list(range(B)), group_starts.tolist()          # whose table holds a sequence's shared tokens
+    shared = [0] * B
+    limit = block_tables.shape[1] * block_size
+    for g, n in enumerate(shared_lens.tolist()):
+        a, b = (max(0, min(s, B)) for s in starts[g:g + 2])
+        for i in range(a, b):
+            first[i], shared[i] = a, max(0, min(n, int(context_lens[a]), limit)) if b - a > 1 else 0
+    for b in range(B):
+        n = min(int(context_lens[b]), limit)
+        if n <= 0:
+            continue
+        idx = torch.arange(n)
+        table = torch.where(idx < shared[b], block_tables[first[b]][idx // block_size], block_tables[b][idx // block_size]).long()
+        k, v = (c[table, idx % block_size].float().transpose(0, 1) for c in (k_cache, v_cache))
         s = torch.einsum("kgd,knd->kgn", q[b].float().view(kv_heads, H // kv_heads, D), k) * scale
         out[b] = torch.einsum("kgn,knd->kgd", torch.softmax(s, -1), v).reshape(H, D).to(q.dtype)
     return out

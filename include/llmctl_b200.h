@@ -141,6 +141,14 @@ int llmctl_paged_attn_decode_fp8(const void* q, long long q_stride, const void* 
                                  int batch, int heads, int kv_heads, int head_dim, int blocks, int block_size, int max_context, int num_splits,
                                  float scale, void* stream);
 
+/* Decode attention over a paged cache of 16 bits, [blocks, block_size, kv_heads, head_dim], in which the sequences group_starts[g] .. group_starts[g + 1] - 1 have
+ * the same blocks for their first shared_lens[g] tokens, which are read once for the group (csrc/serve/paged_attention_shared.cu).  head_dim 64 or 128, blocks of a
+ * multiple of 8 tokens.  scratch: floats, as many as llmctl_paged_attn_shared_scratch_elems says. */
+long long llmctl_paged_attn_shared_scratch_elems(int batch, int groups, int heads, int head_dim);
+int llmctl_paged_attn_decode_shared(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* block_tables, int max_blocks,
+                                    const int* context_lens, const int* group_starts, const int* shared_lens, void* out, float* scratch, int batch, int groups, int heads,
+                                    int kv_heads, int head_dim, int blocks, int block_size, float scale, void* stream);
+
 /* ---- K14 sampling.  Reference: per-request Python loop with .item() syncs (server.py:209-235). ---- */
 int llmctl_sample(const void* logits, int logits_is_fp32, long long ld, int rows, int V,
                   const float* temperature, const int* top_k, const float* top_p, const float* uniform,
