@@ -4,35 +4,42 @@
 //
 // A group's part of a head of the cache has (sequences x query heads of that head) rows of queries, a sequence's own part its query heads alone: both are items of
 // the same form, 128 rows of queries against a range of tokens, and one kernel walks over all of them:
-//     S = Q K^T       128 rows x 128 tokens, over D         (A: Q, B: the key tile as it was loaded, both K-major)
-//     O += P V        128 rows x D, over 128 tokens         (A: P in tensor memory over S, B: the value tile as it was loaded, N-major)
+//     S = Q K^T       128 rows x 64 tokens, over D          (A: Q, B: the key tile as it was loaded, both K-major)
+//     O += P V        128 rows x D, over 64 tokens          (A: P in tensor memory, B: the value tile as it was loaded, N-major)
 // A row is a thread's: maxima and sums need no exchange.  Weights are rounded to bf16 (2^-9 of each, beside the output's 2^-9) and summed as they were
 // rounded; the reference of a row moves when a score is beyond it by 8 (log2), and O is multiplied then.
 //
-//   warp 0      TMA producer: a box for each cache block and 64 columns, one stage of keys and one of values
-//   warp 1      MMA issuer
+// Items of at most 32 rows (64) stand in the 128 four times (twice), and each of the four softmax warps (pair of them) takes a quarter (half) of a tile's columns, with zeros
+// for weights elsewhere and a reference of its own: a tile's exponentials, 8 clocks for each column of a warp, are shared between the warps.  The copies are
+// parts of their own for the merge.
+//
+//   warp 0      TMA producer: a box for each cache block and 64 columns; keys and values of the tiles in one ring of stages
+//   warp 1      MMA issuer: the next tile's scores while this one's become weights
 //   warps 2-5   queries into shared memory, scores to weights, O to memory
 //
-// Items with few rows leave most of the products' rows to nobody; the tensor cores have room for that: a tile's two products are 1024 clocks, its 64 KB take 2700
-// to come.  Two CTAs to an SM, so that one's tiles are on their way while the other one's are looked at.
+// Bound by the pass over the cache.  The products of rows that nobody has cost nothing that is short: a tile's two are 512 clocks, its 32 KB take 1350 to come.  Two CTAs to an SM,
+// so that one's loads are on their way while the other waits for its item's last ones.
 //
-// The tiles of all items stand in one row, and the CTAs take equal runs of it.  What a CTA finds for an item, O at its reference and the reference and the sum of each row,
-// goes to memory at 128 c + (rows of the items before), c the CTA: a place of its own, since from each part to the next at least one of the two grows by the part's rows.  A
-// second kernel puts the parts together.
+// The tiles of all items stand in one row, a place in front of each item for what it costs beside its tiles, and the CTAs take equal runs of it.  What a CTA finds for an item,
+// O at its reference and the reference and the sum of each row, goes to memory at 128 c + (rows of the items before), c the CTA: a place of its own, since from each part to
+// the next at least one of the two grows by the part's rows.  A second kernel puts the parts together.
 //
 // Every wait is bounded, as in latent_attention_t5.cu.
 // Reference: none.
 #include "../common/dependent.cuh"
+#include "../common/fast_div.h"
 #include "../common/ptx.cuh"
 #include "../common/tma_host.h"
 #include "../common/util.cuh"
 #include "../common/wait_status.h"
 
+#include <type_traits>
+
 namespace llmctl {
 using namespace ptx;
 
 namespace decs {
-constexpr int kTile = 128, kRows = 128, kThreads = 192, kCtas = 2 * kNumSMs;
+constexpr int kTile = 64, kRows = 128, kThreads = 192, kCtas = 2 * kNumSMs;
 constexpr float kLog2e = 1.4426950408889634f, kSlack = 8.f;
 
 struct Work {
@@ -40,14 +47,12 @@ struct Work {
   const int* starts;               // [groups + 1]
   const int* shared;               // [groups]
   int batch, groups, per_head, kv_heads, limit, box;       // query heads of a cache head; tokens that the tables hold; rows of a copy
-  int* before;                     // [groups + batch + 1][2]: tiles and rows of the items before an entry
+  int* found;                      // [groups + batch + 1][8]: of each entry what the merge has to know (Found)
   float* parts;                    // [capacity][D + 4]
   long long capacity;
 
   __device__ __forceinline__ int tokens(int b) const { return max(min(lens[b], limit), 0); }
   __device__ __forceinline__ int start(int g) const { return max(min(starts[g], batch), 0); }
-  // Tokens that a group's sequences share: none of a group of one.
-  __device__ __forceinline__ int shared_of(int g, int first, int end) const { return end - first < 2 ? 0 : max(min(shared[g], tokens(first)), 0); }
   // The group that b belongs to, the last one that does not begin behind it; -1: none.
   __device__ __forceinline__ int group_of(int b) const {
     int lo = 0, hi = groups;       // starts[lo] <= b < starts[hi], as far as they are in order
@@ -60,71 +65,86 @@ struct Work {
     return b < starts[lo + 1] ? lo : -1;
   }
 };
+// How often the rows of an item stand in the 128, and how many rows its parts are.
+__device__ __forceinline__ int copies(int rows) { return rows <= 32 ? 4 : rows <= 64 ? 2 : 1; }
+__device__ __forceinline__ int stored(int rows) { return rows * copies(rows); }
 // The items of one range of tokens: a group's shared ones (e < groups), or those that sequence e - groups has behind them.
 struct Entry {
   int first, count;                // sequences; the first one's table is read
   int t0, t1, from, tiles;         // tokens; the first tile's first
   int rows, row_tiles;             // of queries, for a head of the cache
   __device__ __forceinline__ int items(const Work& w) const { return w.kv_heads * row_tiles; }
+  __device__ __forceinline__ int places() const { return tiles + 1; }                       // of an item
+  __device__ __forceinline__ int rows_of(int row_tile) const { return min(rows - row_tile * kRows, kRows); }
+  __device__ __forceinline__ int stored_rows() const { return (row_tiles - 1) * kRows + stored(rows_of(row_tiles - 1)); }         // for a head of the cache
 };
 __device__ __forceinline__ Entry entry_of(const Work& w, int e) {
   Entry r;
-  if (e < w.groups) {
-    r.first = w.start(e);
-    const int end = w.start(e + 1);
-    r.count = max(end - r.first, 0);
-    r.t0 = 0;
-    r.t1 = r.count > 0 ? w.shared_of(e, r.first, end) : 0;
-  } else {
-    r.first = e - w.groups;
-    r.count = 1;
-    const int g = w.group_of(r.first);
-    r.t0 = 0;
-    if (g >= 0) r.t0 = w.shared_of(g, w.start(g), w.start(g + 1));
-    r.t1 = w.tokens(r.first);
+  const bool own = e >= w.groups;
+  const int mine = own ? w.lens[e - w.groups] : 0, g = own ? w.group_of(e - w.groups) : e;
+  int first = 0, end = 0, shared = 0;
+  if (g >= 0) {
+    shared = w.shared[g];
+    first = w.start(g), end = w.start(g + 1);
+    shared = end - first < 2 ? 0 : max(min(shared, w.tokens(first)), 0);          // a group of one shares nothing
   }
+  r.first = own ? e - w.groups : first;
+  r.count = own ? 1 : max(end - first, 0);
+  r.t0 = own ? shared : 0;
+  r.t1 = own ? max(min(mine, w.limit), 0) : shared;
   r.from = r.t0 - r.t0 % w.box;
   r.tiles = r.t1 > r.t0 ? (r.t1 - r.from + kTile - 1) / kTile : 0;
   r.rows = r.count * w.per_head;
   r.row_tiles = (r.rows + kRows - 1) / kRows;
   return r;
 }
-// Equal runs of `all` tiles.
+struct alignas(16) Found {
+  int places, rows;                // of the items before the entry
+  int tiles, count, first;         // of it; tiles of the last one (behind all entries): nothing, places of all items
+  int group;                       // of a sequence's own: the group that it has shared tokens with, or -1
+  int none[2];
+};
+// Equal runs of `all` places.
 struct Runs {
   int run, longer;
   __device__ __forceinline__ Runs(int all, int ctas) : run(all / ctas), longer(all % ctas) {}
   __device__ __forceinline__ int begin(int c) const { return c * run + min(c, longer); }
-  __device__ __forceinline__ int owner(int tile) const {
+  __device__ __forceinline__ int owner(int place) const {
     const int cut = longer * (run + 1);
-    return tile < cut ? tile / (run + 1) : longer + (tile - cut) / max(run, 1);
+    return place < cut ? place / (run + 1) : longer + (place - cut) / max(run, 1);
   }
 };
-// A CTA's run, part by part: tiles t .. t + n of item x of entry e.
+// A CTA's run, part by part: tiles t .. t + n of item x of entry e, n > 0.
 struct Parts {
   Entry entry;
   int e, x, t, n, left;
   int rows_before;                 // of the items before this one
-  __device__ __forceinline__ Parts(const Work& w, int e_, int tiles_in, int left_, int rows_before_) : e(e_), x(0), t(0), n(0), left(left_), rows_before(rows_before_) {
+  __device__ __forceinline__ Parts(const Work& w, int e_, int in, int left_, int rows_before_) : e(e_), x(0), t(0), n(0), left(left_), rows_before(rows_before_) {
     if (left == 0) return;
     entry = entry_of(w, e);
     if (entry.tiles == 0) {        // (lengths that change meanwhile)
       left = 0;
       return;
     }
-    x = tiles_in / entry.tiles;
-    t = tiles_in - x * entry.tiles;
-    rows_before += x / entry.row_tiles * entry.rows + x % entry.row_tiles * kRows;
-    n = min(entry.tiles - t, left);
+    x = in / entry.places();
+    rows_before += x / entry.row_tiles * entry.stored_rows() + x % entry.row_tiles * kRows;
+    take(in - x * entry.places());     // (n = 0: the run ends with the item's first place)
   }
-  __device__ __forceinline__ bool more() const { return left > 0; }
+  // The places of item x from `from` on.
+  __device__ __forceinline__ void take(int from) {
+    const int places = min(entry.places() - from, left);
+    left -= places;
+    t = max(from - 1, 0);
+    n = places - (from == 0 ? 1 : 0);
+  }
+  __device__ __forceinline__ bool more() const { return n > 0; }
   __device__ __forceinline__ int head() const { return x / entry.row_tiles; }
   __device__ __forceinline__ int row0() const { return x % entry.row_tiles * kRows; }
-  __device__ __forceinline__ int rows() const { return min(entry.rows - row0(), kRows); }
+  __device__ __forceinline__ int rows() const { return entry.rows_of(x % entry.row_tiles); }
   __device__ __forceinline__ void next(const Work& w) {
-    left -= n;
+    n = 0;
     if (left == 0) return;
-    rows_before += rows();
-    t = 0;
+    rows_before += stored(rows());
     if (++x == entry.items(w)) {
       x = 0;
       do {
@@ -135,34 +155,37 @@ struct Parts {
         entry = entry_of(w, e);
       } while (entry.tiles == 0);
     }
-    n = min(entry.tiles, left);
+    const int places = min(entry.places(), left);
+    left -= places;
+    t = 0;
+    n = places - 1;                // 0: the run ends with the item's first place
   }
 };
 constexpr int stage_bytes(int D) { return kTile * D * 2; }
-constexpr int stages(int D) { return D == 64 ? 2 : 1; }
-constexpr int smem_bytes(int D) { return kRows * D * 2 + 2 * stages(D) * stage_bytes(D) + 1024; }
+constexpr int stages(int D) { return D == 64 ? 8 : 4; }        // of keys and values in turn
+constexpr int smem_bytes(int D) { return kRows * D * 2 + stages(D) * stage_bytes(D) + 1024; }
 }  // namespace decs
 
 template <int D>
 __global__ void __launch_bounds__(decs::kThreads, 2)
 paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __nv_bfloat16* q, long long q_stride,
-                         const int* tables, int max_blocks, decs::Work w, int blocks, int block_size, float scale_log2, unsigned char* wait_byte) {
+                         const int* tables, int max_blocks, decs::Work w, int blocks, FastDiv by_block, float scale_log2, unsigned char* wait_byte) {
   using namespace decs;
-  constexpr int kPanels = D / 64, kPanel = kTile * 128, kStage = stage_bytes(D), kStages = stages(D), kQ = kRows * D * 2;
+  constexpr int kPanels = D / 64, kPanel = kTile * 128, kQPanel = kRows * 128, kStage = stage_bytes(D), kStages = stages(D), kQ = kRows * D * 2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], q_full, s_full, p_full, o_full;
+  __shared__ uint64_t full[kStages], empty[kStages], q_full, s_full, s_read, p_full, o_full;
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag, scan[2][kThreads / 32], found[4];
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
-  constexpr int kKAt = kQ, kVAt = kQ + kStages * kStage;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1), mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     mbar_init(&q_full, 4);
     mbar_init(&s_full, 1);
+    mbar_init(&s_read, 4);
     mbar_init(&p_full, 4);
     mbar_init(&o_full, 1);
     abort_flag = 0;
@@ -174,19 +197,18 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tS = tmem_base_smem, tO = tS + kTile;
-  wait_for_previous(q, tables, w.lens, w.starts, w.shared, w.before, w.parts);
+  const uint32_t tS = tmem_base_smem, tP = tS + kTile, tO = tS + 128;
+  wait_for_previous(q, tables, w.lens, w.starts, w.shared, w.found, w.parts);
   release_dependents();
   volatile int* abort = &abort_flag;
 
-  // The run: tiles and rows before each entry, by all threads, an entry each; CTA 0 leaves them for the merge.
+  // The run: places and rows before each entry, by all threads, an entry each; CTA 0 leaves them for the merge.
   const int entries = w.groups + w.batch, ctas = gridDim.x, cta = blockIdx.x;
   auto sums_before = [&](int e0, int& tiles, int& rows) {       // of the entries e0 .. e0 + this thread's, itself left out; returns through the last thread's those of all
     int t = 0, r = 0;
     if (e0 + static_cast<int>(threadIdx.x) < entries) {
       const Entry x = entry_of(w, e0 + threadIdx.x);
-      t = x.items(w) * x.tiles;
-      r = x.tiles > 0 ? w.kv_heads * x.rows : 0;
+      if (x.tiles > 0) t = x.items(w) * x.places(), r = w.kv_heads * x.stored_rows();
     }
     const int own_t = t, own_r = r;
 #pragma unroll
@@ -222,86 +244,121 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     if (e0 + static_cast<int>(threadIdx.x) < entries) {
       if (begin >= at && begin < at + sums.x) found[0] = e0 + threadIdx.x, found[1] = begin - at, found[2] = rows0 + rows;
       if (cta == 0) {
-        w.before[2 * (e0 + threadIdx.x)] = at;
-        w.before[2 * (e0 + threadIdx.x) + 1] = rows0 + rows;
+        const int e = e0 + threadIdx.x;
+        const Entry x = entry_of(w, e);
+        const int g = e < w.groups ? -1 : w.group_of(e - w.groups);
+        reinterpret_cast<Found*>(w.found)[e] = Found{at, rows0 + rows, x.tiles, x.rows, x.first, g, {0, 0}};
       }
     }
     tiles0 += sums.y;
     rows0 += sums.z;
   }
-  if (cta == 0 && threadIdx.x == 0) w.before[2 * entries] = all;
+  if (cta == 0 && threadIdx.x == 0) w.found[8 * entries] = all;
   __syncthreads();
   Parts part(w, found[0], found[1], mine, found[2]);
 
   if (warp == 0) {
     // ------------------------------------ TMA producer: a lane per box ------------------------------------
+    // A part's blocks are asked for 32 at a time, a lane each, one such piece ahead: a table's numbers take as long to come as the tiles that stand before them.
     const int boxes = kTile / w.box, box = lane & 15, panel = lane >> 4;
-    int n = 0;
+    auto divide = [&](int token, uint32_t& row) { return static_cast<int>(by_block.divide(static_cast<uint32_t>(token), row)); };
+    auto first_block = [&](const Parts& p) {
+      uint32_t row;
+      return divide(p.entry.from + p.t * kTile, row);
+    };
+    auto last_block = [&](const Parts& p) {
+      uint32_t row;
+      return divide(min(p.entry.from + (p.t + p.n) * kTile, p.entry.t1) - 1, row);
+    };
+    Parts ahead = part;
+    int piece = 0;                            // of `ahead`
+    auto fetch = [&] {
+      int id = -1;
+      if (!ahead.more()) return id;
+      const int at = first_block(ahead) + piece * 32 + lane, last = last_block(ahead);
+      if (at <= last) id = tables[static_cast<long long>(ahead.entry.first) * max_blocks + at];
+      ++piece;
+      if (at - lane + 32 > last) {
+        ahead.next(w);
+        piece = 0;
+      }
+      return id;
+    };
+    int ids = fetch(), next_ids = fetch(), n = 0;
     for (; part.more(); part.next(w)) {
-      const int head = part.head();
-      const int* table = tables + static_cast<long long>(part.entry.first) * max_blocks;
-      for (int i = 0; i < part.n; ++i, ++n) {
-        const int st = n % kStages, token = part.entry.from + (part.t + i) * kTile + box * w.box;
-        const uint32_t empty = ((n / kStages) & 1u) ^ 1u;
+      const int head = part.head(), b0 = first_block(part);
+      int at = 0;                             // the piece that `ids` is
+      for (int i = 0; i < part.n; ++i) {
+        const int token = part.entry.from + (part.t + i) * kTile + box * w.box;
         const bool has = panel < kPanels && box < boxes && token < part.entry.t1;
-        int block = -1, row = 0;
-        if (has) {
-          block = table[token / block_size];
-          row = token % block_size;
-          if (block < 0 || block >= blocks) block = blocks;     // outside of the cache: zeros
+        uint32_t row = 0;
+        const int index = (has ? divide(token, row) : b0) - b0;
+        if (__shfl_sync(0xffffffffu, index, 0) >= (at + 1) * 32) {
+          ids = next_ids;
+          next_ids = fetch();
+          ++at;
         }
-        const int count = __popc(__ballot_sync(0xffffffffu, has));
+        const int here = __shfl_sync(0xffffffffu, ids, index & 31), there = __shfl_sync(0xffffffffu, next_ids, index & 31);
+        int block = index < (at + 1) * 32 ? here : there;
+        if (block < 0 || block >= blocks) block = blocks;       // outside of the cache: zeros
+        const int bytes = __popc(__ballot_sync(0xffffffffu, has)) * w.box * 128;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          uint64_t* full = kv == 0 ? &k_full[st] : &v_full[st];
-          if (n >= kStages) mbar_wait_or_abort(kv == 0 ? &k_empty[st] : &v_empty[st], empty, abort);
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const int st = n % kStages;
+          if (n >= kStages) mbar_wait_or_abort(&empty[st], ((n / kStages) & 1u) ^ 1u, abort);
           __syncwarp();
-          if (lane == 0) mbar_expect_tx(full, count * w.box * 128);
+          if (lane == 0) mbar_expect_tx(&full[st], bytes);
           __syncwarp();
-          if (has) tma_load_4d(smem + (kv == 0 ? kKAt : kVAt) + st * kStage + panel * kPanel + box * w.box * 128, kv == 0 ? &tmK : &tmV, full, panel * 64, head, row, block);
+          if (has) tma_load_4d(smem + kQ + st * kStage + panel * kPanel + box * w.box * 128, kv == 0 ? &tmK : &tmV, &full[st], panel * 64, head, static_cast<int>(row), block);
         }
+      }
+      for (const int last = (last_block(part) - b0) >> 5; at <= last; ++at) {
+        ids = next_ids;
+        next_ids = fetch();
       }
       if (__any_sync(0xffffffffu, *abort)) break;
     }
     if (__any_sync(0xffffffffu, *abort))      // copies still in flight land before the shared memory is given back
       for (int i = n > kStages ? n - kStages : 0; i < n; ++i) {
         int none = 0;
-        mbar_wait_bounded(&k_full[i % kStages], (i / kStages) & 1u, &none);
-        mbar_wait_bounded(&v_full[i % kStages], (i / kStages) & 1u, &none);
+        mbar_wait_bounded(&full[i % kStages], (i / kStages) & 1u, &none);
       }
   } else if (warp == 1) {
     // ------------------------------------ MMA issuer ------------------------------------
     constexpr uint32_t id_s = make_idesc_bf16(kRows, kTile, 0u, 0u), id_o = make_idesc_bf16(kRows, D, 0u, 1u);
-    const uint64_t q0 = make_smem_desc(smem_base, 16, 1024, 2), k0 = make_smem_desc(smem_base + kKAt, 16, 1024, 2), v0 = make_smem_desc(smem_base + kVAt, kPanel, 1024, 2);
-    int n = 0, item = 0;
+    const uint64_t q0 = make_smem_desc(smem_base, 16, 1024, 2), k0 = make_smem_desc(smem_base + kQ, 16, 1024, 2), v0 = make_smem_desc(smem_base + kQ, kPanel, 1024, 2);
+    int n = 0, item = 0;                      // tiles, items so far
+    auto scores = [&](int tile) {             // tile: of all
+      const int st = 2 * tile % kStages;
+      mbar_wait_or_abort(&full[st], (2 * tile / kStages) & 1u, abort);
+      __syncwarp();
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t k = k0 + (st * kStage >> 4);
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c)
+          umma_ss<1>(tS, q0 + (((c >> 2) * kQPanel + (c & 3) * 32) >> 4), k + (((c >> 2) * kPanel + (c & 3) * 32) >> 4), id_s, c != 0 ? 1u : 0u);
+        umma_commit<1>(&empty[st]);
+        umma_commit<1>(&s_full);
+      }
+    };
     for (; part.more(); part.next(w), ++item) {
       mbar_wait_or_abort(&q_full, item & 1u, abort);
+      scores(n);
       for (int i = 0; i < part.n; ++i, ++n) {
-        const int st = n % kStages;
-        const uint32_t phase = (n / kStages) & 1u;
-        mbar_wait_or_abort(&k_full[st], phase, abort);
-        __syncwarp();
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t k = k0 + (st * kStage >> 4);
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
-            const uint32_t at = ((c >> 2) * kPanel + (c & 3) * 32) >> 4;
-            umma_ss<1>(tS, q0 + at, k + at, id_s, c != 0 ? 1u : 0u);
-          }
-          umma_commit<1>(&k_empty[st]);
-          umma_commit<1>(&s_full);
-        }
-        mbar_wait_or_abort(&v_full[st], phase, abort);
+        mbar_wait_or_abort(&s_read, n & 1u, abort);
+        if (i + 1 < part.n) scores(n + 1);
+        const int st = (2 * n + 1) % kStages;
+        mbar_wait_or_abort(&full[st], ((2 * n + 1) / kStages) & 1u, abort);
         mbar_wait_or_abort(&p_full, n & 1u, abort);
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
           const uint64_t v = v0 + (st * kStage >> 4);
 #pragma unroll
-          for (int c = 0; c < kTile / 16; ++c) umma_ts<1>(tO, tS + c * 8, v + (c * 2048 >> 4), id_o, (i | c) != 0 ? 1u : 0u);
-          umma_commit<1>(&v_empty[st]);
-          if (i + 1 == part.n) umma_commit<1>(&o_full);
+          for (int c = 0; c < kTile / 16; ++c) umma_ts<1>(tO, tP + c * 8, v + (c * 2048 >> 4), id_o, (i | c) != 0 ? 1u : 0u);
+          umma_commit<1>(&empty[st]);
+          umma_commit<1>(&o_full);
         }
       }
       if (__any_sync(0xffffffffu, *abort)) break;
@@ -311,91 +368,166 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     const int quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
     int n = 0, item = 0;
-    for (; part.more(); part.next(w), ++item) {
-      const int rows = part.rows(), r = part.row0() + row, b = part.entry.first + r / w.per_head;
-      const bool mine = row < rows, any = quad * 32 < rows;
-      int limit = part.entry.t1;
-      if (any) {
-        const uint4* src = reinterpret_cast<const uint4*>(q + static_cast<long long>(b) * q_stride + (part.head() * w.per_head + r % w.per_head) * D);
-        uint8_t* dst = smem + row * 128;
-        if (mine) limit = min(w.tokens(b), part.entry.t1);
+    // Where the row stands: copy `copy` of the item's row `in`.
+    struct Row {
+      int copy, in;
+    };
+    auto row_of = [&](int rows) {
+      const int f = copies(rows);
+      return Row{f == 4 ? quad : f == 2 ? quad >> 1 : 0, f == 4 ? lane : f == 2 ? (quad & 1) * 32 + lane : row};
+    };
+    auto query = [&](const Parts& p, int in) {          // of the item's row
+      const int r = p.row0() + in, b = p.entry.first + r / w.per_head;
+      return reinterpret_cast<const uint4*>(q + static_cast<long long>(b) * q_stride + (p.head() * w.per_head + r % w.per_head) * D);
+    };
+    // Items of at most 32 rows: a warp has a quarter of each row's queries and writes it to the four copies.  The next item's are asked for ahead.
+    constexpr int kQuarter = D / 32;          // pieces of 16 bytes
+    uint4 ahead[kQuarter] = {};
+    auto ask = [&](const Parts& p) {
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (mine) x = src[c];
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * kPanel + (((c & 7) ^ (row & 7)) << 4)) = x;
-        }
+      for (int c = 0; c < kQuarter; ++c) ahead[c] = make_uint4(0, 0, 0, 0);
+      if (p.more() && p.rows() <= 32 && lane < p.rows()) {
+        const uint4* src = query(p, lane) + quad * kQuarter;
+#pragma unroll
+        for (int c = 0; c < kQuarter; ++c) ahead[c] = src[c];
+      }
+    };
+    auto put = [&](int to_row, int c, uint4 x) { *reinterpret_cast<uint4*>(smem + to_row * 128 + (c >> 3) * kQPanel + (((c & 7) ^ (to_row & 7)) << 4)) = x; };
+    // Puts an item's queries where the products read them.  The weights' columns that other warps have are zeros, and stay so from item to item of one form.
+    int form = 0;
+    auto begin_item = [&](const Parts& p) {
+      const int rows = p.rows(), f = copies(rows);
+      if (f == 4) {
+#pragma unroll
+        for (int c = 0; c < kQuarter; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) put(k * 32 + lane, quad * kQuarter + c, ahead[c]);
+      } else {
+        const Row me = row_of(rows);
+        const uint4* src = query(p, me.in < rows ? me.in : 0);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) put(row, c, me.in < rows ? src[c] : make_uint4(0, 0, 0, 0));
+      }
+      if (f != form) {
+        const uint32_t zero[8] = {};
+#pragma unroll
+        for (int c = 0; c < kTile / 2; c += 8) tmem_st_x8(tP + lane_off + c, zero);
+        tmem_st_wait();
+        form = f;
       }
       fence_proxy_async_smem();
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
+    };
+    ask(part);
+    if (part.more()) begin_item(part);
+    while (part.more()) {
+      const int rows = part.rows(), t1 = part.entry.t1, t0 = part.entry.t0, tiles = part.n, from0 = part.entry.from + part.t * kTile, f = copies(rows);
+      const Row me = row_of(rows);
+      const bool mine = me.in < rows, any = f == 4 || (f == 2 ? (quad & 1) : quad) * 32 < rows;
+      int limit = t1;                         // of this row's tokens
+      if (mine) limit = min(w.tokens(part.entry.first + (part.row0() + me.in) / w.per_head), t1);
+      const long long at = static_cast<long long>(kRows) * cta + part.rows_before + me.copy * rows + me.in;
+      part.next(w);
       float m = -INFINITY, l = 0.f;
-      for (int i = 0; i < part.n; ++i, ++n) {
-        const int st = n % kStages, from = part.entry.from + (part.t + i) * kTile;
+
+      // The tile before has been multiplied: O may be read and P written.  (All warps wait for each, since a phase more would look like one less.)
+      auto before_done = [&](int i) {
+        if (i != 0) mbar_wait_or_abort(&o_full, (n - 1) & 1u, abort);
+        __syncwarp();
+        tc_fence_after();
+      };
+      auto tile = [&](auto columns, int i, int from) {
+        constexpr int C = decltype(columns)::value, kChunk = C == 16 ? 16 : 32;
+        const uint32_t at_s = tS + lane_off + me.copy * C;
+        const int lo = t0 - from - me.copy * C, hi = limit - from - me.copy * C;         // columns lo .. hi - 1 count
+        const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < C);
+        // 64 columns are read twice, 32 at a time: they and the weights would not fit a thread's registers.
+        uint32_t s[kChunk];
+        auto read = [&](int c0) {
+          if constexpr (C == 16) tmem_ld_x16(at_s, s);
+          else tmem_ld_x32(at_s + c0, s);
+          tmem_ld_wait();
+          if (cut) {
+#pragma unroll
+            for (int c = 0; c < kChunk; ++c)
+              if (c0 + c < lo || c0 + c >= hi) s[c] = 0xff800000u;
+          }
+        };
+        auto have_read = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_read);
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int c0 = 0; c0 < C; c0 += kChunk) {
+          read(c0);
+#pragma unroll
+          for (int c = 0; c < kChunk; c += 2) top = max3(top, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+        }
+        if constexpr (C == kChunk) have_read();
+        top *= scale_log2;
+        const bool moves = top > m + kSlack || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, moves)) {
+          const float to = moves ? top : m, factor = moves ? ex2_approx(m - top) : 1.f;
+          if (i != 0) {
+            before_done(i);
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tmem_ld_x16(tO + lane_off + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+              tmem_st_x16(tO + lane_off + c, o);
+            }
+          }
+          l *= factor;
+          m = to;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float l2 = 0.f;
+        if constexpr (C != kChunk) before_done(i);
+#pragma unroll
+        for (int c0 = 0; c0 < C; c0 += kChunk) {
+          if constexpr (C != kChunk) read(c0);
+          if (C != kChunk && c0 + kChunk == C) have_read();
+          uint32_t p[kChunk / 2];
+#pragma unroll
+          for (int c = 0; c < kChunk / 2; ++c) {
+            const float a = ex2_approx(fmaf(__uint_as_float(s[2 * c]), scale_log2, -ref)), z = ex2_approx(fmaf(__uint_as_float(s[2 * c + 1]), scale_log2, -ref));
+            p[c] = pack_bf16x2(a, z);
+            add2(l, l2, __uint_as_float(p[c] << 16), __uint_as_float(p[c] & 0xffff0000u));
+          }
+          if constexpr (C == kChunk) before_done(i);
+          const uint32_t at_p = tP + lane_off + (me.copy * C + c0) / 2;
+          if constexpr (C == 16) tmem_st_x8(at_p, p);
+          else tmem_st_x16(at_p, p);
+        }
+        l += l2;
+        tmem_st_wait();
+      };
+      for (int i = 0; i < tiles; ++i, ++n) {
+        const int from = from0 + i * kTile;
         mbar_wait_or_abort(&s_full, n & 1u, abort);
         __syncwarp();
         tc_fence_after();
         if (any) {
-          const int lo = part.entry.t0 - from, hi = limit - from;          // columns lo .. hi - 1 count
-          const bool cut = __any_sync(0xffffffffu, lo > 0 || hi < kTile);
-          // Scores are read twice, 64 columns at a time: all 128 and the weights would not fit a thread's registers.
-          auto scores = [&](int at, uint32_t (&s)[64]) {
-            tmem_ld_x32(tS + lane_off + at, s);
-            tmem_ld_x32(tS + lane_off + at + 32, s + 32);
-            tmem_ld_wait();
-            if (cut) {
-#pragma unroll
-              for (int c = 0; c < 64; ++c)
-                if (at + c < lo || at + c >= hi) s[c] = 0xff800000u;
-            }
-          };
-          float top = -INFINITY;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t s[64];
-            scores(h * 64, s);
-#pragma unroll
-            for (int c = 0; c < 64; c += 2) top = max3(top, __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-          }
-          top *= scale_log2;
-          const bool moves = top > m + kSlack || (m == -INFINITY && top > m);
-          if (__any_sync(0xffffffffu, moves)) {
-            const float to = moves ? top : m, factor = moves ? ex2_approx(m - top) : 1.f;
-            if (i != 0) {
-#pragma unroll
-              for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_ld_x32(tO + lane_off + c, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
-                tmem_st_x32(tO + lane_off + c, o);
-              }
-            }
-            l *= factor;
-            m = to;
-          }
-          const float ref = m == -INFINITY ? 0.f : m;
-          float l2 = 0.f;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t s[64], p[32];
-            scores(h * 64, s);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const float a = ex2_approx(fmaf(__uint_as_float(s[2 * c]), scale_log2, -ref)), z = ex2_approx(fmaf(__uint_as_float(s[2 * c + 1]), scale_log2, -ref));
-              p[c] = pack_bf16x2(a, z);
-              add2(l, l2, __uint_as_float(p[c] << 16), __uint_as_float(p[c] & 0xffff0000u));
-            }
-            tmem_st_x32(tS + lane_off + h * 32, p);            // over scores that have been read
-          }
-          l += l2;
-          tmem_st_wait();
+          if (f == 4) tile(std::integral_constant<int, 16>(), i, from);
+          else if (f == 2) tile(std::integral_constant<int, 32>(), i, from);
+          else tile(std::integral_constant<int, 64>(), i, from);
+        } else {
+          if (lane == 0) mbar_arrive(&s_read);
+          before_done(i);
         }
-        if (from + kTile > part.entry.t1) {   // what stands behind the last token may be anything
-          mbar_wait_or_abort(&v_full[st], (n / kStages) & 1u, abort);
-          if (from + row >= part.entry.t1) {
-            uint8_t* dst = smem + kVAt + st * kStage + row * 128;
+        if (i + 1 == tiles) ask(part);
+        if (from + kTile > t1) {              // what stands behind the last token may be anything
+          const int st = (2 * n + 1) % kStages;
+          mbar_wait_or_abort(&full[st], ((2 * n + 1) / kStages) & 1u, abort);
+          if (row < kTile && from + row >= t1) {
+            uint8_t* dst = smem + kQ + st * kStage + row * 128;
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * kPanel + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
           }
@@ -405,11 +537,11 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full);
       }
-      mbar_wait_or_abort(&o_full, item & 1u, abort);
+      mbar_wait_or_abort(&o_full, (n - 1) & 1u, abort);
       __syncwarp();
       tc_fence_after();
+      if (part.more()) begin_item(part);      // the next item's scores come while this one's O is read
       if (any) {
-        const long long at = static_cast<long long>(kRows) * cta + part.rows_before + row;
         float* to = w.parts + at * (D + 4);
         const bool fits = mine && at < w.capacity;
 #pragma unroll
@@ -425,6 +557,7 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         if (fits) st_v4(to + D, make_uint4(__float_as_uint(m), __float_as_uint(l), 0u, 0u));
       }
       tc_fence_before();
+      ++item;
       if (__any_sync(0xffffffffu, *abort)) break;
     }
   }
@@ -436,56 +569,90 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   if (threadIdx.x == 0 && abort_flag) report_wait(wait_byte);
 }
 
-// A warp per sequence and query head: the parts of its group's shared tokens and of its own.
+// A CTA per sequence and query head: the parts of its group's shared tokens and of its own.  Each warp finds the parts' weights for itself, a lane to a part, and adds up
+// every fourth part's row.
 template <int D>
 __global__ void __launch_bounds__(128) paged_attn_shared_merge_kernel(decs::Work w, __nv_bfloat16* out, int ctas) {
   using namespace decs;
   constexpr int kPer = D / 32;
-  wait_for_previous(w.lens, w.starts, w.shared, w.before, w.parts, out);
+  __shared__ float rows_of_warps[4][D];
+  wait_for_previous(w.found, w.parts, out);
   release_dependents();
-  const int lane = threadIdx.x & 31, heads = w.kv_heads * w.per_head, at = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (at >= w.batch * heads) return;
-  const int b = at / heads, h = at - b * heads, head = h / w.per_head;
-  const Runs runs(w.before[2 * (w.groups + w.batch)], ctas);
-  float o[kPer] = {}, m = -INFINITY, l = 0.f;
-  auto add = [&](int e) {
-    const Entry x = entry_of(w, e);
-    if (x.tiles == 0) return;
-    const int r = (b - x.first) * w.per_head + h % w.per_head, row_tile = r / kRows;
-    const int tile0 = w.before[2 * e] + (head * x.row_tiles + row_tile) * x.tiles, c1 = runs.owner(tile0 + x.tiles - 1);
-    const long long rows = static_cast<long long>(w.before[2 * e + 1]) + head * x.rows + r;
-    for (int c = runs.owner(tile0); c <= c1; ++c) {
-      const long long place = static_cast<long long>(kRows) * c + rows;
-      if (place >= w.capacity) return;
-      const float* part = w.parts + place * (D + 4);
-      const float2 ml = *reinterpret_cast<const float2*>(part + D);
-      float v[kPer];
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) v[k] = part[lane * kPer + k];
-      if (ml.y == 0.f) continue;           // no token that counts
-      const float to = fmaxf(m, ml.x), a = m == to ? 1.f : ex2_approx(m - to), z = ml.x == to ? 1.f : ex2_approx(ml.x - to);
-      l = l * a + ml.y * z;
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) o[k] = o[k] * a + v[k] * z;
-      m = to;
-    }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y, h = blockIdx.x, head = h / w.per_head;
+  const Found* found = reinterpret_cast<const Found*>(w.found);
+  const int all = found[w.groups + w.batch].places;
+  const Found own = found[w.groups + b];
+  Found group = own;
+  group.tiles = 0;
+  if (own.group >= 0) group = found[own.group];
+  const Runs runs(all, ctas);
+  // An item's parts: the first one's row, how many CTAs have parts, how many copies of how many rows a part is.
+  struct Item {
+    long long first;
+    int count, f, rows;
   };
-  const int g = w.group_of(b);
-  if (g >= 0) add(g);
-  add(w.groups + b);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16* to = out + static_cast<long long>(at) * D + lane * kPer;
+  auto item = [&](const Found& x) {
+    if (x.tiles == 0) return Item{0, 0, 1, 0};
+    const int r = (b - x.first) * w.per_head + h % w.per_head, row_tile = r / kRows, row_tiles = (x.count + kRows - 1) / kRows, rows = min(x.count - row_tile * kRows, kRows);
+    const int stored_rows = (row_tiles - 1) * kRows + stored(x.count - (row_tiles - 1) * kRows), f = copies(rows);
+    const int place0 = x.places + (head * row_tiles + row_tile) * (x.tiles + 1) + 1, c0 = runs.owner(place0);
+    return Item{static_cast<long long>(kRows) * c0 + x.rows + head * stored_rows + row_tile * kRows + r % kRows, (runs.owner(place0 + x.tiles - 1) - c0 + 1) * f, f, rows};
+  };
+  const Item common = item(group), mine = item(own);
+  const int parts = common.count + mine.count;
+  float o[kPer] = {}, m = -INFINITY, l = 0.f;
+  for (int i0 = 0; i0 < parts; i0 += 32) {
+    const int i = i0 + lane, n = min(parts - i0, 32);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    long long at = 0;
+    if (i < parts) {
+      const bool first = i < common.count;
+      const int j = first ? i : i - common.count, f = first ? common.f : mine.f, c = j / f;
+      at = (first ? common.first : mine.first) + static_cast<long long>(kRows) * c + (j - c * f) * (first ? common.rows : mine.rows);
+      if (at < w.capacity) ml = *reinterpret_cast<const float2*>(w.parts + at * (D + 4) + D);
+      else at = 0;
+    }
+    const bool counts = !(ml.y == 0.f);      // else: no token that counts
+    const float to = fmaxf(m, warp_max(counts ? ml.x : -INFINITY));
+    const float z = !counts ? 0.f : ml.x == to ? 1.f : ex2_approx(ml.x - to), a = m == to ? 1.f : ex2_approx(m - to);
+    l = l * a + warp_sum(counts ? ml.y * z : 0.f);
+    m = to;
+    const unsigned which = __ballot_sync(0xffffffffu, counts);
 #pragma unroll
-  for (int k = 0; k < kPer; k += 2) *reinterpret_cast<__nv_bfloat162*>(to + k) = __floats2bfloat162_rn(o[k] * inv, o[k + 1] * inv);
+    for (int k = 0; k < kPer; ++k) o[k] *= a;
+    // eight rows under way: of parts that do not count some other row is read and not used
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int part = warp + 4 * k, from = min(part, n - 1);
+      const float* row = w.parts + __shfl_sync(0xffffffffu, at, from) * (D + 4) + lane * kPer;
+      const float factor = __shfl_sync(0xffffffffu, z, from);
+      if (4 * k >= n) break;
+      float v[kPer];
+      if constexpr (kPer == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(row);
+      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(row);
+      const bool use = part < n && (which >> part & 1u);
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) o[c] = use ? fmaf(v[c], factor, o[c]) : o[c];
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kPer; ++c) rows_of_warps[warp][lane * kPer + c] = o[c];
+  __syncthreads();
+  if (threadIdx.x < D) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v += rows_of_warps[k][threadIdx.x];
+    out[(static_cast<long long>(b) * gridDim.x + h) * D + threadIdx.x] = __float2bfloat16(l == 0.f ? 0.f : v / l);
+  }
 }
 
 namespace {
 // Floats of scratch: the sums before each entry, then the parts.
-long long parts_at(int batch, int groups) { return (2LL * (groups + batch + 1) + 3) / 4 * 4; }
-long long capacity_of(int batch, int heads) { return static_cast<long long>(decs::kRows) * decs::kCtas + 2LL * batch * heads; }
+long long parts_at(int batch, int groups) { return 8LL * (groups + batch + 1); }
+long long capacity_of(int batch, int heads) { return static_cast<long long>(decs::kRows) * decs::kCtas + 8LL * batch * heads; }
 int box_rows(int block_size) {
   int box = 1;
-  while (box < 128 && block_size % (2 * box) == 0) box *= 2;
+  while (box < decs::kTile && block_size % (2 * box) == 0) box *= 2;
   return box;
 }
 
@@ -495,10 +662,9 @@ cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const __nv_bfloat
   using namespace decs;
   const auto kernel = paged_attn_shared_kernel<D>;
   if (const cudaError_t e = allow_smem(kernel, smem_bytes(D)); e != cudaSuccess) return e;
-  if (const cudaError_t e = launch_dependent(kernel, kCtas, kThreads, smem_bytes(D), s, k, v, q, q_stride, tables, max_blocks, w, blocks, block_size, scale * kLog2e, byte); e != cudaSuccess)
+  if (const cudaError_t e = launch_dependent(kernel, kCtas, kThreads, smem_bytes(D), s, k, v, q, q_stride, tables, max_blocks, w, blocks, FastDiv(block_size), scale * kLog2e, byte); e != cudaSuccess)
     return e;
-  const int all = w.batch * w.kv_heads * w.per_head;
-  return launch_dependent(paged_attn_shared_merge_kernel<D>, (all + 3) / 4, 128, 0, s, w, out, static_cast<int>(kCtas));
+  return launch_dependent(paged_attn_shared_merge_kernel<D>, dim3(w.kv_heads * w.per_head, w.batch), 128, 0, s, w, out, static_cast<int>(kCtas));
 }
 }  // namespace
 }  // namespace llmctl
@@ -520,7 +686,7 @@ LLMCTL_API int llmctl_paged_attn_decode_shared(const void* q, long long q_stride
   const long long limit = static_cast<long long>(max_blocks) * block_size;
   LLMCTL_REQUIRE(limit < (1LL << 31) - 256);
   // tiles of all items, and rows, count in 32 bits
-  LLMCTL_REQUIRE(2LL * batch * heads * ((limit >> 7) + 2) < (1LL << 31) && 2LL * batch * heads < (1LL << 30));
+  LLMCTL_REQUIRE(2LL * batch * heads * ((limit >> 6) + 3) < (1LL << 31) && 8LL * batch * heads < (1LL << 30));
   const int box = box_rows(block_size);
   CUtensorMap k, v;
   const uint64_t D = head_dim, Hk = kv_heads, row = D * Hk;
