@@ -409,6 +409,9 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         for (int c = 0; c < D / 8; ++c) put(row, c, me.in < rows ? src[c] : make_uint4(0, 0, 0, 0));
       }
       if (f != form) {
+        if (n > 0) mbar_wait_or_abort(&o_full, (n - 1) & 1u, abort);
+        __syncwarp();
+        tc_fence_after();
         const uint32_t zero[8] = {};
 #pragma unroll
         for (int c = 0; c < kTile / 2; c += 8) tmem_st_x8(tP + lane_off + c, zero);
@@ -522,7 +525,7 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
           if (lane == 0) mbar_arrive(&s_read);
           before_done(i);
         }
-        if (i + 1 == tiles) ask(part);
+        if (i == 0) ask(part);
         if (from + kTile > t1) {              // what stands behind the last token may be anything
           const int st = (2 * n + 1) % kStages;
           mbar_wait_or_abort(&full[st], ((2 * n + 1) / kStages) & 1u, abort);
@@ -537,10 +540,11 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full);
       }
+      // This item's scores have all been taken, so the next one's queries may stand in the place of its own, and their scores come while O is finished and read.
+      if (part.more()) begin_item(part);
       mbar_wait_or_abort(&o_full, (n - 1) & 1u, abort);
       __syncwarp();
       tc_fence_after();
-      if (part.more()) begin_item(part);      // the next item's scores come while this one's O is read
       if (any) {
         float* to = w.parts + at * (D + 4);
         const bool fits = mine && at < w.capacity;
@@ -569,16 +573,17 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   if (threadIdx.x == 0 && abort_flag) report_wait(wait_byte);
 }
 
-// A CTA per sequence and query head: the parts of its group's shared tokens and of its own.  Each warp finds the parts' weights for itself, a lane to a part, and adds up
-// every fourth part's row.
-template <int D>
-__global__ void __launch_bounds__(128) paged_attn_shared_merge_kernel(decs::Work w, __nv_bfloat16* out, int ctas) {
+// W warps (1 or 4) per sequence and query head: the parts of its group's shared tokens and of its own.  Each warp finds the parts' weights for itself, a lane to a part, and
+// adds up every Wth part's row.  Grid: heads / (4 / W), rounded up, x sequences.
+template <int D, int W>
+__global__ void __launch_bounds__(128, W == 4 ? 8 : 5) paged_attn_shared_merge_kernel(decs::Work w, __nv_bfloat16* out, int ctas) {
   using namespace decs;
-  constexpr int kPer = D / 32;
-  __shared__ float rows_of_warps[4][D];
+  constexpr int kPer = D / 32, kUnderWay = W == 4 ? 4 : 8;
+  __shared__ float rows_of_warps[W][D];
   wait_for_previous(w.found, w.parts, out);
   release_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y, h = blockIdx.x, head = h / w.per_head;
+  const int warp = W == 4 ? threadIdx.x >> 5 : 0, lane = threadIdx.x & 31, b = blockIdx.y, h = W == 4 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5), head = h / w.per_head;
+  if (h >= w.kv_heads * w.per_head) return;
   const Found* found = reinterpret_cast<const Found*>(w.found);
   const int all = found[w.groups + w.batch].places;
   const Found own = found[w.groups + b];
@@ -620,29 +625,41 @@ __global__ void __launch_bounds__(128) paged_attn_shared_merge_kernel(decs::Work
     const unsigned which = __ballot_sync(0xffffffffu, counts);
 #pragma unroll
     for (int k = 0; k < kPer; ++k) o[k] *= a;
-    // eight rows under way: of parts that do not count some other row is read and not used
+    // rows under way at once: of parts that do not count some other row is read and not used
+    for (int k0 = 0; k0 * W < n; k0 += kUnderWay) {
+      float v[kUnderWay][kPer];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int part = warp + 4 * k, from = min(part, n - 1);
-      const float* row = w.parts + __shfl_sync(0xffffffffu, at, from) * (D + 4) + lane * kPer;
-      const float factor = __shfl_sync(0xffffffffu, z, from);
-      if (4 * k >= n) break;
-      float v[kPer];
-      if constexpr (kPer == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(row);
-      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(row);
-      const bool use = part < n && (which >> part & 1u);
+      for (int k = 0; k < kUnderWay; ++k) {
+        const float* row = w.parts + __shfl_sync(0xffffffffu, at, min(warp + W * (k0 + k), n - 1)) * (D + 4) + lane * kPer;
+        if (W * (k0 + k) >= n) continue;
+        if constexpr (kPer == 4) *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(row);
+        else *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(row);
+      }
 #pragma unroll
-      for (int c = 0; c < kPer; ++c) o[c] = use ? fmaf(v[c], factor, o[c]) : o[c];
+      for (int k = 0; k < kUnderWay; ++k) {
+        const int part = warp + W * (k0 + k);
+        const float factor = __shfl_sync(0xffffffffu, z, min(part, n - 1));
+        const bool use = part < n && (which >> (part & 31) & 1u);
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) o[c] = use ? fmaf(v[k][c], factor, o[c]) : o[c];
+      }
     }
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16* to = out + (static_cast<long long>(b) * w.kv_heads * w.per_head + h) * D;
+  if constexpr (W == 1) {
 #pragma unroll
-  for (int c = 0; c < kPer; ++c) rows_of_warps[warp][lane * kPer + c] = o[c];
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float v = 0.f;
+    for (int c = 0; c < kPer; c += 2) *reinterpret_cast<__nv_bfloat162*>(to + lane * kPer + c) = __floats2bfloat162_rn(o[c] * inv, o[c + 1] * inv);
+  } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v += rows_of_warps[k][threadIdx.x];
-    out[(static_cast<long long>(b) * gridDim.x + h) * D + threadIdx.x] = __float2bfloat16(l == 0.f ? 0.f : v / l);
+    for (int c = 0; c < kPer; ++c) rows_of_warps[warp][lane * kPer + c] = o[c];
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float v = 0.f;
+#pragma unroll
+      for (int k = 0; k < W; ++k) v += rows_of_warps[k][threadIdx.x];
+      to[threadIdx.x] = __float2bfloat16(v * inv);
+    }
   }
 }
 
@@ -664,7 +681,10 @@ cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const __nv_bfloat
   if (const cudaError_t e = allow_smem(kernel, smem_bytes(D)); e != cudaSuccess) return e;
   if (const cudaError_t e = launch_dependent(kernel, kCtas, kThreads, smem_bytes(D), s, k, v, q, q_stride, tables, max_blocks, w, blocks, FastDiv(block_size), scale * kLog2e, byte); e != cudaSuccess)
     return e;
-  return launch_dependent(paged_attn_shared_merge_kernel<D>, dim3(w.kv_heads * w.per_head, w.batch), 128, 0, s, w, out, static_cast<int>(kCtas));
+  // Four warps to a sequence and head while all of them are on the chip at once, else one.
+  const int heads = w.kv_heads * w.per_head;
+  if (w.batch * heads <= 8 * kNumSMs) return launch_dependent(paged_attn_shared_merge_kernel<D, 4>, dim3(heads, w.batch), 128, 0, s, w, out, static_cast<int>(kCtas));
+  return launch_dependent(paged_attn_shared_merge_kernel<D, 1>, dim3((heads + 3) / 4, w.batch), 128, 0, s, w, out, static_cast<int>(kCtas));
 }
 }  // namespace
 }  // namespace llmctl
