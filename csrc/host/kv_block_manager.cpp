@@ -147,6 +147,23 @@ API int llmctl_kv_can_allocate(void* h, int num_tokens) {
   return static_cast<int>(kv->free_list.size()) - kv->blocks_for(num_tokens) >= kv->watermark_blocks ? 1 : 0;
 }
 
+API int llmctl_kv_share(void* h, long long from, long long to, int blocks) {
+  KV* kv = static_cast<KV*>(h);
+  std::lock_guard<std::mutex> lk(kv->mu);
+  auto a = kv->seqs.find(from), b = kv->seqs.find(to);
+  if (a == kv->seqs.end() || b == kv->seqs.end() || kv->num_slots > 0 || blocks < 0) return -1;
+  if (blocks > static_cast<int>(a->second.blocks.size()) || blocks > static_cast<int>(b->second.blocks.size())) return -1;
+  for (int i = 0; i < blocks; ++i) {
+    const int shared = a->second.blocks[i];
+    int& own = b->second.blocks[i];
+    if (own == shared) continue;
+    ++kv->refcnt[shared];
+    if (--kv->refcnt[own] == 0) kv->free_list.push_back(own);
+    own = shared;
+  }
+  return 0;
+}
+
 API int llmctl_kv_fork(void* h, long long parent, long long child, int* cow_src, int* cow_dst) {
   KV* kv = static_cast<KV*>(h);
   std::lock_guard<std::mutex> lk(kv->mu);

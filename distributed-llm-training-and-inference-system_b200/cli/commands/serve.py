@@ -26,6 +26,7 @@ def start(
     max_concurrent: int = typer.Option(128, "--max-concurrent"),
     device: str = typer.Option("auto", "--device", help="auto | cuda | cpu"),
     kv_cache_dtype: str = typer.Option("auto", "--kv-cache-dtype", help="auto (the model's type) | fp8 (8 bits, a scale for each block and head)"),
+    weight_dtype: str = typer.Option("auto", "--weight-dtype", help="auto (the model's type) | int4 (projections in 4 bits; one GPU)"),
     tensor_parallel: int = typer.Option(1, "--tensor-parallel", "--tp", help="Shard the model over this many GPUs (one process per GPU, rank 0 serves HTTP)"),
     dry_run: bool = typer.Option(False, "--dry-run", help="Validate and print the configuration, do not serve"),
 ):
@@ -37,12 +38,15 @@ def start(
         fail(f"artifact not found: {artifact}", 2)
     try:
         cfg = ServeConfig(artifact=artifact, host=host, port=port, scheduler=scheduler, max_batch_size=max_batch_size,
-                          max_batch_tokens=max_batch_tokens, max_concurrent=max_concurrent, device=device, kv_cache_dtype=kv_cache_dtype)
+                          max_batch_tokens=max_batch_tokens, max_concurrent=max_concurrent, device=device, kv_cache_dtype=kv_cache_dtype,
+                          weight_dtype=weight_dtype)
     except Exception as e:  # noqa: BLE001 - pydantic validation error
         fail(str(e), 2)
     console.print(f"[bold blue]Starting inference server[/bold blue]  artifact={artifact} {host}:{port} "
                   f"scheduler={scheduler} max_batch_size={max_batch_size} max_batch_tokens={max_batch_tokens} "
                   f"max_concurrent={max_concurrent} device={device}")
+    if tensor_parallel > 1 and weight_dtype != "auto":
+        fail("--weight-dtype int4: one GPU (--tensor-parallel 1)", 2)
     if tensor_parallel > 1:
         # one process per GPU under torchrun: rank 0 runs the HTTP server, the others mirror its engine step by step
         import subprocess
@@ -67,7 +71,7 @@ def start(
     from ...serve.server import create_inference_server
     server = create_inference_server(artifact, host=host, port=port, max_batch_size=max_batch_size,
                                      max_batch_tokens=max_batch_tokens, max_concurrent_requests=max_concurrent,
-                                     scheduler=scheduler, device=None if device == "auto" else device, kv_cache_dtype=kv_cache_dtype)
+                                     scheduler=scheduler, device=None if device == "auto" else device, kv_cache_dtype=kv_cache_dtype, weight_dtype=weight_dtype)
     try:
         asyncio.run(server.start_server())
     except KeyboardInterrupt:

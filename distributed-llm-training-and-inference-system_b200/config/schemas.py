@@ -239,7 +239,15 @@ class ServeConfig(_Base):
     device: str = "auto"
     kv_block_size: int = 16
     kv_cache_dtype: str = "auto"          # auto (the model's type) | fp8 (a scale for each block and head)
+    weight_dtype: str = "auto"            # auto (the model's type) | int4 (projections in 4 bits, a scale for 128 input channels)
     tensor_parallel: int = 1
+
+    @field_validator("weight_dtype")
+    @classmethod
+    def _weights(cls, v):
+        if v not in ("auto", "int4"):
+            raise ValueError("weight_dtype must be auto | int4")
+        return v
 
     @field_validator("kv_cache_dtype")
     @classmethod

@@ -178,10 +178,11 @@ def from_hf_llama(hf: Dict[str, torch.Tensor]) -> Dict[str, torch.Tensor]:
     return out
 
 
-def load_pretrained_state_dict(path: str | Path) -> Dict[str, torch.Tensor]:
+def load_pretrained_state_dict(path: str | Path, dequantise: bool = True) -> Dict[str, torch.Tensor]:
     """Full (unsharded) weights in this framework's names from a directory that holds either one of our checkpoints
     / exports (single file or TP/PP shards + index) or an HF LLaMA checkpoint (``config.json`` + one
-    ``model.safetensors`` or ``model-0000x-of-0000y.safetensors`` shards with a ``weight_map`` index)."""
+    ``model.safetensors`` or ``model-0000x-of-0000y.safetensors`` shards with a ``weight_map`` index).  ``dequantise`` False
+    leaves the tensors of a quantised artifact as they stand in it."""
     from safetensors.torch import load_file
     path = Path(path)
     idx = path / "model.safetensors.index.json"
@@ -196,7 +197,7 @@ def load_pretrained_state_dict(path: str | Path) -> Dict[str, torch.Tensor]:
     if any(k.startswith("model.layers.") or k.startswith("model.embed_tokens") for k in full):
         full = from_hf_llama(full)
     meta = path / "export.json"
-    if meta.exists():
+    if dequantise and meta.exists():
         from .quantize import dequantize_if_needed
         full = dequantize_if_needed(full, json.loads(meta.read_text()).get("quantization"))
     return full

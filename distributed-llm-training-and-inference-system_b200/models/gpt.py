@@ -81,6 +81,8 @@ class MLP(nn.Module):
                                           dtype=dtype, device=device, fused_name="mlp_down")
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.gated and hasattr(self.up, "swiglu"):            # weights held in 4 bits (models/int4.py)
+            return self.down(self.up.swiglu(x))
         if self.gated and not (self.selective_recompute and torch.is_grad_enabled()) and tpl.runs_plain(self.up):
             if tpl.runs_plain(self.down):
                 return ops.swiglu_mlp(x, self.up.weight, self.down.weight)

@@ -11,7 +11,8 @@ prompt, K/V scattered into their cache blocks — kernel K13), all running seque
 together (packed qkv GEMM, rotation to each sequence's own position and append in one kernel, K12 paged attention over the
 block tables, K14 batched sampling) and finished sequences free their blocks.  ``kv_cache_dtype="fp8"`` keeps the cache in 8 bits with a
 scale for each block and head.  Nothing in the step reads
-a value back to the host except the sampled token ids (one small D2H copy per step).
+a value back to the host except the sampled token ids (one small D2H copy per step).  ``weight_dtype="int4"`` keeps the projections in 4 bits.  Completions of one prompt
+(``add_requests``) share its blocks and its prefill, and decode with the prompt's tokens read once for all of them.
 
 Reference: reference llmctl/serve/server.py:127-251 ``InferenceEngine.generate_batch`` right-pads the batch,
 re-runs the HF model over the full sequences (``use_cache`` result discarded), samples from the pad position
@@ -40,11 +41,14 @@ from .ragged import Portion, RaggedBatch
 from .tokenizer import load_tokenizer
 
 
-def load_model_for_inference(artifact, device: Optional[str] = None, dtype: Optional[torch.dtype] = None
+def load_model_for_inference(artifact, device: Optional[str] = None, dtype: Optional[torch.dtype] = None, weight_dtype: str = "auto"
                              ) -> Tuple[GPTModel, ModelConfig, object, torch.device]:
     """Load a checkpoint / exported artifact directory (``model_config.json`` + ``model.safetensors`` or TP/PP
     shards, or the ``config.json`` + ``model.safetensors`` of a registered architecture), or build a random-init model
-    when ``artifact`` names a preset or is a configuration object / dictionary (benchmarks, tests)."""
+    when ``artifact`` names a preset or is a configuration object / dictionary (benchmarks, tests).  ``weight_dtype`` int4 keeps the
+    projections of a GPT model in 4 bits: an ``int4`` artifact's codes as they stand, other weights quantised here."""
+    if weight_dtype not in ("auto", "int4"):
+        raise ValueError(f"weight_dtype {weight_dtype!r}: auto (the model's type) or int4")
     from ..io.export import consolidate_to_state_dict, shard_state_dict_for
     from ..models import registry
     st = get_state()
@@ -71,11 +75,24 @@ def load_model_for_inference(artifact, device: Optional[str] = None, dtype: Opti
     else:
         mcfg = resolve_model(str(artifact) if is_path else artifact)
         model = build_model(mcfg, dtype=dtype, device=dev)
+    if weight_dtype == "int4":
+        if not isinstance(model, GPTModel) or st.tp > 1:
+            raise ValueError("weight_dtype int4: models of the GPT family, without tensor parallelism")
+        from ..io.export import load_pretrained_state_dict
+        from ..models.int4 import hold_in_int4
+        hold_in_int4(model, load_pretrained_state_dict(p, dequantise=False) if p is not None and p.is_dir() else None)
     model.eval()
     for prm in model.parameters():
         prm.requires_grad_(False)
     tok = load_tokenizer(str(artifact) if is_path else None, mcfg.vocab_size)
     return model, mcfg, tok, dev
+
+
+#: Bytes of keys and values of a layer that reading shared prefixes once has to save before a decode step takes the kernel for it (``_in_groups``), which has 8 us more of
+#: start and merge than the one for sequences by themselves, to which a prefix that many read comes from L2.  us, shared / by themselves, 64 tokens behind the prefix: 32 heads
+#: of 128, 8 sequences of 512 tokens (59 MB) 16.6 / 15.1, of 1024 (117) 18.2 / 23.4, 16 of 256 (63) 17.8 / 18.7, 32 of 256 (130) 26.9 / 28.0, of 2048 (1040) 29.8 / 114; 12 heads of
+#: 64, 16 of 1024 (47) 14.2 / 12.2, of 2048 (94) 15.5 / 18.8.
+_SHARED_BYTES = 72 << 20
 
 
 @dataclass
@@ -98,6 +115,9 @@ class Sequence:
     logprobs: Optional[int] = None         # how many alternatives to each token's log probability; None: no log probabilities
     token_logprobs: List[dict] = field(default_factory=list)       # of each generated token: token, logprob, entropy, top [(token, logprob)]
     last_logprob: Optional[dict] = None    # of the token that was sampled last
+    group: Optional[object] = None         # completions of one prompt (``add_requests``): what they have in common
+    prefix: Optional[int] = None           # while the prompt stands in the cache: which copy of it (sequences of one copy share its whole blocks)
+    prompt_logits: Optional[torch.Tensor] = None       # of the prompt's last position, for completions that come after
 
     @property
     def all_ids(self) -> List[int]:
@@ -123,6 +143,8 @@ class _HostViews:
         self.positions = a[4 * B:5 * B]
         self.ctx = a[5 * B:6 * B]
         self.block_tables = a[6 * B:6 * B + B * max_blocks].reshape(B, max_blocks)
+        self.group_starts = a[6 * B + B * max_blocks:7 * B + B * max_blocks + 1]
+        self.shared_lens = a[7 * B + B * max_blocks + 1:]
 
     def fill_pad(self) -> None:
         # padded rows: token 0 at position 0, empty context, no cache slot (K13 skips slot -1)
@@ -131,14 +153,16 @@ class _HostViews:
         self.positions[:] = 0
         self.ctx[:] = 0
         self.block_tables[:] = 0
+        self.group_starts[:] = 0
+        self.shared_lens[:] = 0
 
 
 class _DecodeInputs:
     """Static device inputs of a decode step of (padded) batch ``B`` and ``max_blocks`` table columns, laid out in
-    one int32 buffer: tokens(int64) | slots(int64) | positions | context lengths | block tables."""
+    one int32 buffer: tokens(int64) | slots(int64) | positions | context lengths | block tables | groups that share a prefix (starts, lengths)."""
 
     def __init__(self, B: int, max_blocks: int, device: torch.device):
-        n = 6 * B + B * max_blocks
+        n = 6 * B + B * max_blocks + 2 * B + 1
         pin = device.type == "cuda"
         self._hbuf = torch.zeros(n, dtype=torch.int32, pin_memory=pin)
         self._dbuf = torch.zeros(n, dtype=torch.int32, device=device)
@@ -148,7 +172,9 @@ class _DecodeInputs:
         self.slots = d[2 * B:4 * B].view(torch.int64)
         self.positions = d[4 * B:5 * B]
         self.ctx = d[5 * B:6 * B]
-        self.block_tables = d[6 * B:].view(B, max_blocks)
+        self.block_tables = d[6 * B:6 * B + B * max_blocks].view(B, max_blocks)
+        self.group_starts = d[6 * B + B * max_blocks:7 * B + B * max_blocks + 1]
+        self.shared_lens = d[7 * B + B * max_blocks + 1:]
         self.nbytes = n * 4
 
     def upload(self) -> None:
@@ -159,17 +185,17 @@ class _DecodeGraph:
     """One captured decode step.  Inputs are the static views of ``_DecodeInputs``; the logits land in a static
     output tensor owned by the graph's memory pool."""
 
-    def __init__(self, engine: "InferenceEngine", inp: _DecodeInputs, B: int, max_ctx: int):
+    def __init__(self, engine: "InferenceEngine", inp: _DecodeInputs, B: int, max_ctx: int, shared: bool = False):
         side = torch.cuda.Stream(device=engine.device)
         side.wait_stream(torch.cuda.current_stream(engine.device))
         with torch.cuda.stream(side):
             for _ in range(2):                              # warm-up: tensor-map cache, lazy inits, cuBLAS handles
-                engine._decode_core(inp, B, max_ctx)
+                engine._decode_core(inp, B, max_ctx, shared)
         torch.cuda.current_stream(engine.device).wait_stream(side)
         torch.cuda.synchronize(engine.device)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph, capture_error_mode="thread_local"):
-            self.logits = engine._decode_core(inp, B, max_ctx)
+            self.logits = engine._decode_core(inp, B, max_ctx, shared)
 
     def replay(self) -> torch.Tensor:
         self.graph.replay()
@@ -226,8 +252,9 @@ class InferenceEngine:
                  scheduler: str = "dynamic", device: Optional[str] = None, kv_block_size: int = 16,
                  kv_memory_fraction: float = 0.5, num_kv_blocks: Optional[int] = None, seed: int = 0,
                  cuda_graphs: Optional[bool] = None, fused_tp_decode: Optional[bool] = None,
-                 dtype: Optional[torch.dtype] = None, kv_watermark: float = 0.01, kv_cache_dtype: str = "auto"):
-        self.model, self.cfg, self.tokenizer, self.device = load_model_for_inference(artifact, device, dtype)
+                 dtype: Optional[torch.dtype] = None, kv_watermark: float = 0.01, kv_cache_dtype: str = "auto",
+                 weight_dtype: str = "auto"):
+        self.model, self.cfg, self.tokenizer, self.device = load_model_for_inference(artifact, device, dtype, weight_dtype)
         self.st = get_state()
         self.lockstep = False       # True under serve/lockstep.py: cancellations take effect on all TP ranks at once
         m = self.model
@@ -317,7 +344,8 @@ class InferenceEngine:
             if symm.available() and native.has_symbol("llmctl_ar_residual_rmsnorm") and ops.kernel_config().gemm == "native":
                 self._ar = _DecodeAllReduce(self.st, max(max_batch_size, 8), self.cfg.hidden, self.device)
                 self._ar.calls_per_step = 2 * len(self.model.blocks)
-        self._graphs: Dict[Tuple[int, int], "_DecodeGraph"] = {}
+        self._graphs: Dict[Tuple[int, int, bool], "_DecodeGraph"] = {}
+        self._next_prefix = 1
         self._staging: Dict[Tuple[int, int], "_DecodeInputs"] = {}
 
     def check_logprobs(self, logprobs: Optional[int]) -> None:
@@ -327,7 +355,7 @@ class InferenceEngine:
 
     # ---- request API ---------------------------------------------------------------------------------
     def add_request(self, prompt_ids: List[int], max_tokens: int = 100, temperature: float = 1.0, top_p: float = 1.0,
-                    top_k: int = -1, on_token=None, logprobs: Optional[int] = None) -> Sequence:
+                    top_k: int = -1, on_token=None, logprobs: Optional[int] = None, group: Optional[object] = None) -> Sequence:
         """``logprobs``: the sequence's ``token_logprobs`` get each generated token's log probability under the model (before temperature, top_k and top_p), the
         entropy and that many of the most probable tokens."""
         self.check_logprobs(logprobs)
@@ -339,7 +367,7 @@ class InferenceEngine:
         with self._lock:
             rid = self._next_id
             self._next_id += 1
-            seq = Sequence(rid, list(prompt_ids), max_tokens, temperature, top_p, top_k, on_token=on_token, logprobs=logprobs)
+            seq = Sequence(rid, list(prompt_ids), max_tokens, temperature, top_p, top_k, on_token=on_token, logprobs=logprobs, group=group)
             if self._plugin_sched is not None and max_tokens > 0:
                 self._staged.append(_StagedRequest(rid, len(prompt_ids), max_tokens, time.time()))
                 self.seqs[rid] = seq
@@ -350,6 +378,15 @@ class InferenceEngine:
                 return seq
             self.seqs[rid] = seq
         return seq
+
+    def add_requests(self, prompt_ids: List[int], n: int, max_tokens: int = 100, temperature: float = 1.0, top_p: float = 1.0, top_k: int = -1, on_token=None,
+                     logprobs: Optional[int] = None) -> List[Sequence]:
+        """``n`` completions of one prompt.  They are sequences of their own, but the prompt is run once for those that are admitted while another one of them runs, and
+        its whole blocks are kept once for them."""
+        if n < 1:
+            raise ValueError(f"n: at least one completion, not {n}")
+        group = object() if n > 1 and not self.ragged and self.st.tp == 1 else None
+        return [self.add_request(prompt_ids, max_tokens, temperature, top_p, top_k, on_token, logprobs, group) for _ in range(n)]
 
     def has_work(self) -> bool:
         return self.sched.num_waiting + self.sched.num_running + len(self._staged) > 0
@@ -474,7 +511,10 @@ class InferenceEngine:
     @torch.no_grad()
     def _prefill(self, seq: Sequence) -> torch.Tensor:
         """Dense causal attention over prompt (+ already generated tokens after a preemption); returns the
-        last position's logits [V]."""
+        last position's logits [V].  A completion of a prompt that stands in the cache already takes its blocks and its logits."""
+        logits = self._prefill_shared(seq)
+        if logits is not None:
+            return logits
         ids = seq.all_ids
         n = len(ids)
         H, D = self.heads_local, self.head_dim
@@ -494,9 +534,55 @@ class InferenceEngine:
         y, _ = m.final_norm(x[-1:], residual[-1:] if residual is not None else None)
         logits = m.lm_head(y) if m.lm_head is not None else ops.linear(y, m.embed.weight)
         self.stats["prefill_tokens"] += n
+        if seq.group is not None:
+            seq.prefix, self._next_prefix = self._next_prefix, self._next_prefix + 1
+            if not seq.generated:
+                seq.prompt_logits = logits[0].clone()
         return logits[0]
 
-    def _decode_core(self, inp: "_DecodeInputs", B: int, max_ctx: int) -> torch.Tensor:
+    def _prefill_shared(self, seq: Sequence) -> Optional[torch.Tensor]:
+        """Puts the prompt of ``seq`` into the cache from another completion of it that is there: whole blocks are shared, a last one that is not full is copied."""
+        if seq.group is None or seq.generated:
+            return None
+        other = next((s for s in self.seqs.values() if s is not seq and s.group is seq.group and s.prefix is not None and s.prompt_logits is not None), None)
+        if other is None:
+            return None
+        n, bs = len(seq.prompt_ids), self.block_size
+        whole = n // bs
+        self.kv.share(other.req_id, seq.req_id, whole)
+        if n % bs:
+            a, b = self.kv.block_table(other.req_id)[whole], self.kv.block_table(seq.req_id)[whole]
+            for caches in (self.k_caches, self.v_caches, *((self.k_scales, self.v_scales) if self.fp8_cache else ())):
+                for c in caches:
+                    c[b].copy_(c[a])            # (what stands behind the prompt is the other one's, and will be written over)
+        seq.prefix, seq.prompt_logits = other.prefix, other.prompt_logits
+        return seq.prompt_logits
+
+    def _forget(self, ids) -> None:
+        """Sequences whose blocks have been given back."""
+        for rid in ids:
+            s = self.seqs.get(rid)
+            if s is not None:
+                s.prefix = s.prompt_logits = None
+
+    def _in_groups(self, seqs: List[Sequence]) -> Tuple[List[Sequence], List[Tuple[int, int]]]:
+        """Sequences that share a prefix beside one another, in front; and of each such group how many they are and how many tokens they share, if reading those once
+        is worth a kernel of its own."""
+        if self.fp8_cache or self.device.type == "cuda" and (self.dtype != torch.bfloat16 or self.head_dim not in (64, 128) or self.block_size % 8):
+            return seqs, []
+        by: Dict[int, List[Sequence]] = {}
+        for s in seqs:
+            if s.prefix is not None and len(s.prompt_ids) >= self.block_size:
+                by.setdefault(s.prefix, []).append(s)
+        groups = [g for g in by.values() if len(g) > 1]
+        shared = [len(g[0].prompt_ids) // self.block_size * self.block_size for g in groups]
+        if not groups or sum((len(g) - 1) * n for g, n in zip(groups, shared)) * 2 * self.heads_local * self.head_dim * self.dtype.itemsize < _SHARED_BYTES:
+            return seqs, []
+        front = [s for g in groups for s in g]
+        ids = {s.req_id for s in front}
+        return front + [s for s in seqs if s.req_id not in ids], [(len(g), n) for g, n in zip(groups, shared)]
+
+    def _decode_core(self, inp: "_DecodeInputs", B: int, max_ctx: int, shared: bool = False) -> torch.Tensor:
         """Device-only part of a decode step over the static input views (capturable in a CUDA graph)."""
         H, D = self.heads_local, self.head_dim
         m = self.model
@@ -505,6 +591,8 @@ class InferenceEngine:
             q = self._append(i, qkv, positions, inp.slots)[:, :H * D].reshape(B, H, D)
             if self.fp8_cache:
                 o = sops.paged_attention_decode_fp8(q, self.k_caches[i], self.v_caches[i], self.k_scales[i], self.v_scales[i], inp.block_tables, inp.ctx, max_ctx)
+            elif shared:
+                o = sops.paged_attention_decode_shared(q, self.k_caches[i], self.v_caches[i], inp.block_tables, inp.ctx, inp.group_starts, inp.shared_lens)
             else:
                 o = sops.paged_attention_decode(q, self.k_caches[i], self.v_caches[i], inp.block_tables, inp.ctx, max_ctx)
             return o.reshape(B, H * D)
@@ -549,8 +637,8 @@ class InferenceEngine:
         return min(b, max(hi, n))
 
     @torch.no_grad()
-    def _decode(self, seqs: List[Sequence]) -> torch.Tensor:
-        """One token for every sequence in ``seqs``; returns logits [B, V].  The step's inputs (last tokens,
+    def _decode(self, seqs: List[Sequence], groups: Optional[List[Tuple[int, int]]] = None) -> torch.Tensor:
+        """One token for every sequence in ``seqs`` (``groups``: see ``_in_groups``); returns logits [B, V].  The step's inputs (last tokens,
         positions, context lengths, cache slots, block tables) are packed into one pinned host buffer and reach
         the device in a single copy."""
         B = len(seqs)
@@ -572,6 +660,10 @@ class InferenceEngine:
             inp = self._staging[key] = _DecodeInputs(Bb, max_blocks, self.device)
         h = inp.host
         h.fill_pad()
+        at = 0
+        for g, (count, n) in enumerate(groups or []):
+            at += count
+            h.group_starts[g + 1:], h.shared_lens[g] = at, n
         bs = self.block_size
         for r, (s, c) in enumerate(zip(seqs, ctx)):
             table = self.kv.block_table(s.req_id)
@@ -583,10 +675,10 @@ class InferenceEngine:
         inp.upload()
         self.stats["decode_tokens"] += B
         if not use_graph:
-            return self._decode_core(inp, Bb, cb)[:B]
-        g = self._graphs.get(key)
+            return self._decode_core(inp, Bb, cb, bool(groups))[:B]
+        g = self._graphs.get((*key, bool(groups)))
         if g is None:
-            g = self._graphs[key] = _DecodeGraph(self, inp, Bb, cb)
+            g = self._graphs[(*key, bool(groups))] = _DecodeGraph(self, inp, Bb, cb, bool(groups))
         return g.replay()[:B]
 
     def _gather_vocab(self, logits: torch.Tensor) -> torch.Tensor:
@@ -651,19 +743,25 @@ class InferenceEngine:
                 s = self.seqs[r]
                 tok = self._sample(self._prefill(s), [s])[0]
                 self._emit(s, tok, finished)
-                evicted.update(self.sched.pop_preempted())
+                evicted.update(self._preempted())
         t1 = time.perf_counter()
         self.stats["prefill_time_s"] += t1 - t0
         decode = [s for s in decode if s.req_id not in evicted and not s.finished]
         if decode:
-            toks = self._sample(self._decode(decode), decode)
+            decode, groups = self._in_groups(decode)
+            toks = self._sample(self._decode(decode, groups), decode)
             for s, tok in zip(decode, toks):
                 self._emit(s, tok, finished)
             self.stats["decode_time_s"] += time.perf_counter() - t1
             self.stats["decode_steps"] += 1
-        evicted.update(self.sched.pop_preempted())
+        evicted.update(self._preempted())
         self.stats["preemptions"] += len(evicted)
         return finished
+
+    def _preempted(self) -> List[int]:
+        ids = self.sched.pop_preempted()
+        self._forget(ids)
+        return ids
 
     def _emit(self, s: Sequence, tok: int, finished: List[Sequence]) -> None:
         if s.finished:
@@ -687,6 +785,7 @@ class InferenceEngine:
             s.finish_reason = "length"
         if s.finish_reason:
             s.finished = True
+            s.prefix = s.prompt_logits = None
             self.sched.finish(s.req_id)
             self.seqs.pop(s.req_id, None)
             s.done_event.set()
@@ -697,14 +796,16 @@ class InferenceEngine:
     def abort(self, seq: Sequence, reason: str = "error") -> None:
         if not seq.finished:
             seq.finished, seq.finish_reason = True, reason
+            seq.prefix = seq.prompt_logits = None
             self.sched.finish(seq.req_id)
             self.seqs.pop(seq.req_id, None)
             seq.done_event.set()
 
     # ---- convenience: synchronous generation -------------------------------------------------------------
     def generate(self, prompts: List[List[int]], max_tokens: int = 16, temperature: float = 0.0, top_p: float = 1.0,
-                 top_k: int = -1) -> List[List[int]]:
-        seqs = [self.add_request(p, max_tokens, temperature, top_p, top_k) for p in prompts]
+                 top_k: int = -1, n: int = 1) -> List[List[int]]:
+        """``n`` completions of each prompt, one behind the other."""
+        seqs = [s for p in prompts for s in self.add_requests(p, n, max_tokens, temperature, top_p, top_k)]
         idle = 0
         while any(not s.finished for s in seqs):
             if not self.has_work():

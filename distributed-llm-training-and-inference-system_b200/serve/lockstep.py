@@ -67,6 +67,10 @@ class LockstepEngine:
         holder["event"].wait()
         return holder["seq"]
 
+    def add_requests(self, prompt_ids: List[int], n: int, *args, **kwargs) -> List[Sequence]:
+        """``n`` completions of one prompt, each by itself: prefixes are shared on one GPU only."""
+        return [self.add_request(prompt_ids, *args, **kwargs) for _ in range(n)]
+
     def has_work(self) -> bool:
         with self._lock:
             pending = bool(self._pending)

@@ -29,7 +29,7 @@ def lib() -> ctypes.CDLL:
             "llmctl_kv_block_table": (c_int, [c_void_p, c_ll, PI, c_int]),
             "llmctl_kv_free_blocks": (c_int, [c_void_p]), "llmctl_kv_total_blocks": (c_int, [c_void_p]),
             "llmctl_kv_block_size": (c_int, [c_void_p]), "llmctl_kv_can_allocate": (c_int, [c_void_p, c_int]),
-            "llmctl_kv_fork": (c_int, [c_void_p, c_ll, c_ll, PI, PI]),
+            "llmctl_kv_fork": (c_int, [c_void_p, c_ll, c_ll, PI, PI]), "llmctl_kv_share": (c_int, [c_void_p, c_ll, c_ll, c_int]),
             "llmctl_kv_set_state_slots": (c_int, [c_void_p, c_int]), "llmctl_kv_state_slot": (c_int, [c_void_p, c_ll]),
             "llmctl_kv_free_state_slots": (c_int, [c_void_p]),
             "llmctl_sched_create": (c_void_p, [c_int, c_int, c_int, c_void_p]),
@@ -99,6 +99,11 @@ class KVBlockManager:
         if r < 0:
             raise RuntimeError("fork failed (unknown parent, existing child, or no free block)")
         return (s.value, d.value) if r == 1 else None
+
+    def share(self, source: int, target: int, blocks: int) -> None:
+        """``target`` reads the first ``blocks`` blocks of ``source`` in place of its own, which are given back."""
+        if lib().llmctl_kv_share(self._h, source, target, blocks) != 0:
+            raise RuntimeError("share failed (unknown sequence, or fewer blocks)")
 
     def clear_cache(self, request_id) -> None:   # name kept from the reference's KVCacheManager
         self.free(int(request_id))

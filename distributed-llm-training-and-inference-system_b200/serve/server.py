@@ -27,6 +27,7 @@ class GenerationRequest(BaseModel):
     top_p: float = Field(1.0, gt=0.0, le=1.0)
     top_k: int = -1
     stream: bool = False
+    n: int = Field(1, ge=1, le=128)                         # completions of the prompt (not of a stream)
     logprobs: Optional[int] = Field(None, ge=0, le=20)      # log probabilities of the generated tokens, with so many alternatives to each
 
 
@@ -41,6 +42,13 @@ class GenerationLogprobsResponse(GenerationResponse):
     """The response to a request with ``logprobs``: of each token its text, its id, its log probability, the entropy of the distribution it was drawn
     from and the most probable tokens; null where a number is not finite."""
     logprobs: Dict[str, list]
+
+
+class GenerationChoicesResponse(BaseModel):
+    """The response to a request with ``n`` above 1: each completion as a response of its own."""
+    id: str
+    choices: List[Dict]
+    usage: Dict[str, int]
 
 
 def _finite(x: float) -> Optional[float]:
@@ -98,7 +106,7 @@ class EngineLoop(threading.Thread):
 class InferenceServer:
     def __init__(self, model_path: str, host: str = "0.0.0.0", port: int = 8080, max_batch_size: int = 8,
                  max_batch_tokens: int = 8192, max_concurrent_requests: int = 128, scheduler: str = "dynamic",
-                 device: Optional[str] = None, engine: Optional[InferenceEngine] = None, kv_cache_dtype: str = "auto"):
+                 device: Optional[str] = None, engine: Optional[InferenceEngine] = None, kv_cache_dtype: str = "auto", weight_dtype: str = "auto"):
         from fastapi import FastAPI, HTTPException
         from fastapi.middleware.cors import CORSMiddleware
         from fastapi.responses import PlainTextResponse, StreamingResponse
@@ -107,7 +115,7 @@ class InferenceServer:
         self.max_concurrent_requests = max_concurrent_requests
         self.engine = engine or InferenceEngine(model_path, max_batch_size=max_batch_size,
                                                 max_batch_tokens=max_batch_tokens, scheduler=scheduler, device=device,
-                                                kv_cache_dtype=kv_cache_dtype)
+                                                kv_cache_dtype=kv_cache_dtype, weight_dtype=weight_dtype)
         self.scheduler = self.engine.sched
         self.active_requests: Dict[str, RequestState] = {}
         self.completed = 0
@@ -133,6 +141,10 @@ class InferenceServer:
         async def create_completion(req: GenerationRequest):
             if len(self.active_requests) >= self.max_concurrent_requests:
                 raise HTTPException(status_code=503, detail="Server at capacity")
+            if req.stream and req.n > 1:
+                raise HTTPException(status_code=422, detail="n: one completion of a stream")
+            if req.n > 1:
+                return await self.handle_choices_request(req)
             if req.stream:
                 return StreamingResponse(self._stream(req), media_type="text/event-stream")
             return await self.handle_generation_request(req)
@@ -210,6 +222,30 @@ class InferenceServer:
             if not seq.finished:
                 seq.cancel_requested = True
             self.active_requests.pop(rid, None)
+
+    async def handle_choices_request(self, req: GenerationRequest) -> GenerationChoicesResponse:
+        loop = asyncio.get_running_loop()
+        ids = self.engine.tokenizer.encode(req.prompt)
+        more = {} if req.logprobs is None else {"logprobs": min(req.logprobs, self.engine.cfg.vocab_size)}
+        seqs = await loop.run_in_executor(None, lambda: self.engine.add_requests(ids, req.n, req.max_tokens, req.temperature, req.top_p, req.top_k, **more))
+        rids = [str(uuid.uuid4()) for _ in seqs]
+        for rid, seq in zip(rids, seqs):
+            self.active_requests[rid] = RequestState(rid, seq)
+        self.loop_thread.wake.set()
+        try:
+            for seq in seqs:
+                await loop.run_in_executor(None, seq.done_event.wait)
+            self.completed += len(seqs)
+            self.errors += sum(seq.finish_reason == "error" for seq in seqs)
+            of = [self._response(rid, seq, len(ids)).model_dump() for rid, seq in zip(rids, seqs)]
+            completion = sum(len(seq.generated) for seq in seqs)
+            return GenerationChoicesResponse(id=rids[0], choices=[{"index": i, **r} for i, r in enumerate(of)],
+                                             usage={"prompt_tokens": len(ids), "completion_tokens": completion, "total_tokens": len(ids) + completion})
+        finally:
+            for rid, seq in zip(rids, seqs):
+                if not seq.finished:
+                    seq.cancel_requested = True
+                self.active_requests.pop(rid, None)
 
     async def _stream(self, req: GenerationRequest):
         loop = asyncio.get_running_loop()

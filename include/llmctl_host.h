@@ -32,6 +32,9 @@ int llmctl_kv_can_allocate(void* kv, int num_tokens);
 /* Share parent's blocks with child (prefix sharing).  If the last block is partially filled it must be
  * copied before the child appends: returns 1 and sets *cow_src / *cow_dst, else 0; -1 on error. */
 int llmctl_kv_fork(void* kv, long long parent, long long child, int* cow_src, int* cow_dst);
+/* Puts the first `blocks` blocks of `from` in the place of those of `to`, which are given back: both then read the same tokens there.  Neither may write to
+ * them.  0 = ok, -1: unknown sequence, fewer blocks than that, or state slots in use (nothing is changed). */
+int llmctl_kv_share(void* kv, long long from, long long to, int blocks);
 /* State slots for models with recurrent layers: `num_slots` fixed-size per-sequence states beside the pages (call
  * before any sequence exists; 0 = none).  A sequence takes a slot at its first allocation, which fails (-1) when no
  * slot is free, and returns it in llmctl_kv_free.  Fork is refused while slots are in use. */
