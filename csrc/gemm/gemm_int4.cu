@@ -1,6 +1,7 @@
 // Entry points of the products with weights of 4 bits; which kernel a call takes; weights widened to bf16 for prompts.
 // Reference: none (quantisation is an option of a stub command, llmctl/cli/commands/export.py:17).
 #include "../common/dependent.cuh"
+#include "../common/fast_div.h"
 #include "../common/util.cuh"
 #include "gemm_int4.h"
 
@@ -8,37 +9,56 @@
 
 namespace llmctl {
 
-// bf16 [halves * padded, K] of W [halves * rows, K / 2]: each number (q - 8) s rounded once, rows past the last of a half zeros.  A thread has 32 columns: 16 bytes in,
-// 64 out.  Bound by what it writes: 22016 x 4096 38 us (5.9 TB/s).
-__global__ void __launch_bounds__(256) int4_widen_kernel(const uint8_t* __restrict__ w, long long ldw, const __half* __restrict__ scale, long long lds, __nv_bfloat16* __restrict__ out,
-                                                         int rows, int padded, int pieces, long long all) {
+// bf16 [halves * padded, K] of W [halves * rows, K / 2]: each number (q - 8) s rounded once, rows past the last of a half zeros.  A thread has 8 columns of a row at a time, 4
+// bytes in and 16 out.  The whole number n = q - 8 is exact in bf16 (128 + q less 136), and s = s1 + s0 with 8 and at most 3 significant bits, so that n s0 is exact and
+// fma(n, s1, n s0) the product rounded once.  Bound by what it writes.
+__global__ void __launch_bounds__(256) int4_widen_kernel(const uint8_t* w, long long ldw, const __half* scale, long long lds, __nv_bfloat16* out, int rows, int padded, FastDiv by_words,
+                                                         int all) {
   wait_for_previous(w, scale, out);
   release_dependents();
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
-    const int row = static_cast<int>(i / pieces), piece = static_cast<int>(i - static_cast<long long>(row) * pieces), half = row / padded, in = row - half * padded;
-    uint4 words = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-    float s = 0.f;
-    if (in < rows) {
+  const int stride = gridDim.x * 256;
+  for (long long i0 = blockIdx.x * 256 + threadIdx.x; i0 < all; i0 += 4LL * stride) {
+    uint32_t words[4];
+    float s[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const long long i = i0 + static_cast<long long>(k) * stride;
+      words[k] = 0x88888888u;
+      s[k] = 0.f;
+      if (i >= all) continue;
+      uint32_t word;
+      const int row = static_cast<int>(by_words.divide(static_cast<uint32_t>(i), word)), half = row >= padded ? 1 : 0, in = row - half * padded;
+      if (in >= rows) continue;
       const long long from = static_cast<long long>(half) * rows + in;
-      words = *reinterpret_cast<const uint4*>(w + from * ldw + piece * 16);
-      s = __half2float(scale[from * lds + (piece >> 2)]);
+      words[k] = *reinterpret_cast<const uint32_t*>(w + from * ldw + word * 4);
+      s[k] = __half2float(scale[from * lds + (word >> 4)]);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t v = reinterpret_cast<const uint32_t*>(&words)[j];
-      float f[8];
+    for (int k = 0; k < 4; ++k) {
+      const long long i = i0 + static_cast<long long>(k) * stride;
+      if (i >= all) continue;
+      const __nv_bfloat16 high = __float2bfloat16(s[k]);
+      const float rest = s[k] - __bfloat162float(high);
+      const __nv_bfloat162 s1 = __bfloat162bfloat162(high), s0 = __bfloat162bfloat162(__float2bfloat16(fabsf(s[k]) < INFINITY ? rest : 0.f));
+      const uint32_t even = words[k] & 0x0f0f0f0fu, odd = (words[k] >> 4) & 0x0f0f0f0fu;
+      const uint32_t lo = __byte_perm(even, odd, 0x5140), hi = __byte_perm(even, odd, 0x7362);             // columns 0 .. 3, 4 .. 7
+      const uint32_t pair[4] = {__byte_perm(lo, 0x43434343u, 0x4140), __byte_perm(lo, 0x43434343u, 0x4342), __byte_perm(hi, 0x43434343u, 0x4140), __byte_perm(hi, 0x43434343u, 0x4342)};
+      bf16x8 r;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) f[c] = static_cast<float>(static_cast<int>((v >> 4 * c) & 15u) - 8) * s;
-      store8(out + i * 32 + j * 8, pack8(f));
+      for (int c = 0; c < 4; ++c) {
+        const __nv_bfloat162 n = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair[c]), __floats2bfloat162_rn(136.f, 136.f));
+        r.v[c] = __hfma2(n, s1, __hmul2(n, s0));
+      }
+      store8(out + i * 8, r);
     }
   }
 }
 
 namespace {
-// Chunks of 8 tokens read the weights again, from L2; the tensor cores' kernel reads them once but has 6 us of start and merge.  us, chunks / tensor cores: 4096 x 4096 (8.4 MB)
-// 16 tokens 8.0 / 9.4, 24 11.8 / 12.5, 32 14.1 / 12.8; gated 2048 -> 5632 (11.5 MB) 16 tokens 11.5 / 12.0, 24 16.8 / 15.0; 6144 rows of 2048 (6.3 MB) 24 tokens 9.3 / 11.4, 32
-// 12.6 / 11.8; 2048 x 2048 64 tokens 8.9 / 16.0; 12288 x 4096 (25 MB) 9 tokens 18 / 15.6.
-bool in_chunks(int tokens, long long matrix_rows, int K) { return tokens <= 8 || (tokens + 7) / 8 * (matrix_rows * (K / 2)) <= (24LL << 20); }
+// Chunks of 8 tokens read the weights again, from L2; the tensor cores' kernel reads them once for 64 tokens but has some 5 us of start and merge.  us, chunks / tensor cores:
+// 4096 x 4096 (8.4 MB) 16 tokens 8.0 / 8.0, 24 11.8 / 9.8; gated 2048 -> 5632 (11.5 MB) 12 tokens 11.2 / 10.9; 6144 rows of 2048 (6.3 MB) 24 tokens 9.3 / 11.0, 32 12.6 /
+// 11.0; 2048 rows of 5632 (5.8 MB) 32 tokens 9.9 / 12.3, 48 14.5 / 14.7; 2048 x 2048 64 tokens 8.9 / 10.8; 12288 x 4096 (25 MB) 9 tokens 18 / 14.0.
+bool in_chunks(int tokens, long long matrix_rows, int K) { return tokens <= 8 || (tokens + 7) / 8 * (matrix_rows * (K / 2)) <= (23LL << 20); }
 }  // namespace
 }  // namespace llmctl
 
@@ -72,9 +92,10 @@ LLMCTL_API int llmctl_int4_widen(const void* w, long long ldw, const void* scale
   LLMCTL_BEGIN();
   LLMCTL_REQUIRE(rows > 0 && padded >= rows && (halves == 1 || halves == 2) && K > 0 && K % 128 == 0 && static_cast<long long>(padded) * halves < (1LL << 31));
   LLMCTL_REQUIRE(aligned16(w, out) && ldw >= K / 2 && ldw % 16 == 0 && lds >= K / 128);
-  const long long all = static_cast<long long>(padded) * halves * (K / 32);
-  const int grid = static_cast<int>(min((all + 255) / 256, 8LL * kNumSMs));
+  const long long all = static_cast<long long>(padded) * halves * (K / 8);
+  LLMCTL_REQUIRE(all < (1LL << 31));
+  const int grid = static_cast<int>(min((all + 1023) / 1024, 8LL * kNumSMs));
   LLMCTL_CHECK(launch_dependent(int4_widen_kernel, grid, 256, 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(w), ldw, static_cast<const __half*>(scale), lds,
-                                static_cast<__nv_bfloat16*>(out), rows, padded, K / 32, all));
+                                static_cast<__nv_bfloat16*>(out), rows, padded, FastDiv(K / 8), static_cast<int>(all)));
   return 0;
 }

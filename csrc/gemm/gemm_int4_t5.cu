@@ -9,10 +9,11 @@
 // D_g leaves tensor memory after each group, and its rows are multiplied by their scales and added up in 32 bits, so that nothing is rounded before the
 // output.  For that the whole numbers need no scale of their own: 0x4300 | q is 128 + q in bf16, less 136: 13 instructions for 8 columns.
 //
-//   warp 0      TMA producer of weights and of tokens, a ring of stages each
-//   warp 1      MMA issuer: 8 products to a group
-//   4 or 8      a row and up to 32 tokens per thread: D_g times its scale into the row's sums; outputs
-//   16          a row and a group per thread: from shared memory, widened, to tensor memory; four warps to every fourth group
+//   1 warp      TMA producer of weights and of tokens, a ring of stages each
+//   2 warps     MMA issuers, of a unit's first and of its second group: 8 products each (one warp's issuing took 400 clocks for a group)
+//   8           a row and up to 32 tokens per thread: D_g times its scale into the row's sums; outputs.  Up to 32 tokens the first four look at a unit's first group and the
+//               others at its second, above that each at half of the tokens
+//   12          a row and a group per thread: from shared memory, widened, to tensor memory; four warps to every third group
 //
 // The work is one row of units, tile after tile, and the CTAs take equal runs of it, whatever the sizes (4096 rows are 32 tiles, for 148 SMs).  A tile that
 // more than one CTA has a part of is put together by the last of them to come, which finds the others' sums in memory and adds all up in the order of the
@@ -32,10 +33,16 @@ using namespace ptx;
 
 namespace int4t5 {
 constexpr int kRows = 128, kUnitBytes = kRows * 128;
-constexpr int kRingW = 6, kRingA = 4, kRingD = 4;
+// A barrier's phases are told by their parity, so that whoever waits at a stage has to wait for each of its phases: a stage of A belongs to one set of widening warps
+// and to one issuer, one of D to one issuer, one of W to the same sets each time around.  The rings are multiples of those.
+constexpr int kRingW = 6, kRingA = 6;
+constexpr int ring_d(int P) { return P <= 32 ? 4 : 2; }
 constexpr int ring_x(int P) { return P <= 32 ? 6 : 3; }
-constexpr int sum_warps(int P) { return P > 32 ? 8 : 4; }
-constexpr int threads(int P) { return 32 * (2 + sum_warps(P) + 16); }
+constexpr int kSumAt = 3, kSumWarps = 8, kWidenAt = kSumAt + kSumWarps, kSets = 3, kThreads = 32 * (kWidenAt + 4 * kSets);
+constexpr bool by_group(int P) { return P <= 32; }              // the sums' warps share a unit's groups, not the tokens
+// Shared memory behind the rings: the second group's sums, and the up rows'.
+constexpr int sums_bytes(int P) { return by_group(P) ? P * kRows * 4 : 0; }
+constexpr int up_bytes(int P, bool gated) { return gated ? P * (kRows / 2) * 4 : 0; }
 
 struct Args {
   const __half* scale;
@@ -45,33 +52,35 @@ struct Args {
   unsigned char* wait_byte;
   long long lds, ldo;
   int tokens, rows, groups, tiles; // rows: of the output (F where gated)
-  int run, longer;                 // units of a CTA; the first `longer` have one more
+  int run;                         // units of a CTA (of the last one fewer)
 };
 }  // namespace int4t5
 
 template <int P, bool GATED>
-__global__ void __launch_bounds__(int4t5::threads(P), 1)
+__global__ void __launch_bounds__(int4t5::kThreads, 1)
 gemm_int4_t5_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, int4t5::Args a) {
   using namespace int4t5;
-  constexpr int kOutRows = GATED ? kRows / 2 : kRows, kPanel = P * 128, kStageX = 4 * kPanel, kRingX = ring_x(P);
+  constexpr int kOutRows = GATED ? kRows / 2 : kRows, kPanel = P * 128, kStageX = 4 * kPanel, kRingX = ring_x(P), kRingD = ring_d(P);
   constexpr int kA = kRingD * P;              // of tensor memory: the ring of D, then that of A
-  constexpr int kColumns = 512, kSumWarps = sum_warps(P), kSumThreads = 32 * kSumWarps, kMine = P * 4 / kSumWarps;        // tokens of a thread
+  constexpr bool kByGroup = by_group(P);
+  static_assert(kRingD * P + kRingA * 64 <= 512 && kRingA % kSets == 0 && kRingA % 2 == 0 && kRingW % kSets == 0 && kRingD % 2 == 0);
+  constexpr int kColumns = 512, kOutThreads = kByGroup ? 128 : 256, kMine = kByGroup ? P : P / 2;           // tokens of a thread
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t w_full[kRingW], w_empty[kRingW], x_full[kRingX], x_empty[kRingX], a_full[kRingA], a_empty[kRingA], d_full[kRingD], d_empty[kRingD];
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag, last_one;
-  __shared__ uint4 kept_scales[32 * sum_warps(P)];
+  __shared__ uint4 kept_scales[32 * kSumWarps];
 
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
-  constexpr int kXAt = kRingW * kUnitBytes, kUpAt = kXAt + kRingX * kStageX;
+  constexpr int kXAt = kRingW * kUnitBytes, kSumsAt = kXAt + kRingX * kStageX, kUpAt = kSumsAt + sums_bytes(P);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRingW; ++i) mbar_init(&w_full[i], 1), mbar_init(&w_empty[i], 8);
-    for (int i = 0; i < kRingX; ++i) mbar_init(&x_full[i], 1), mbar_init(&x_empty[i], 1);
+    for (int i = 0; i < kRingX; ++i) mbar_init(&x_full[i], 1), mbar_init(&x_empty[i], 2);
     for (int i = 0; i < kRingA; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
-    for (int i = 0; i < kRingD; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], kSumWarps);
+    for (int i = 0; i < kRingD; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], kByGroup ? 4 : 8);
     abort_flag = 0;
     fence_mbar_init();
     prefetch_tmap(&tmW);
@@ -86,7 +95,7 @@ gemm_int4_t5_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
 
   // This CTA's run of units.
   const int ctas = gridDim.x, cta = blockIdx.x, G = (a.groups + 1) / 2;       // pairs of groups; of an odd number the last one's second is zeros
-  const int u0 = cta * a.run + min(cta, a.longer), units = a.run + (cta < a.longer ? 1 : 0), tile0 = u0 / G, g0 = u0 - tile0 * G;
+  const int u0 = cta * a.run, units = min(a.run, a.tiles * G - u0), tile0 = u0 / G, g0 = u0 - tile0 * G;
   const int token0 = blockIdx.y * P;
 
   auto load_w = [&](int tile, int g, auto&& load) {
@@ -139,38 +148,39 @@ gemm_int4_t5_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
         for (int i = units > kRingX ? units - kRingX : 0; i < units; ++i) mbar_wait_bounded(&x_full[i % kRingX], (i / kRingX) & 1u, &none);
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------ MMA issuer ------------------------------------
+  } else if (warp < kSumAt) {
+    // ------------------------------------ MMA issuers: the units' first groups, their second ones ------------------------------------
     constexpr uint32_t id = make_idesc_bf16(kRows, P, 0u, 0u);
-    const uint64_t b0 = make_smem_desc(smem_base + kXAt, 16, 1024, 2);
+    const int second = warp - 1;
+    const uint64_t b0 = make_smem_desc(smem_base + kXAt + second * 2 * kPanel, 16, 1024, 2);
     int xs = 0;
     uint32_t xp = 0;
-    for (int i = 0; i < 2 * units; ++i) {      // groups
-      const int as = i % kRingA;
-      if (i >= kRingD) mbar_wait_or_abort(&d_empty[i % kRingD], ((i / kRingD) & 1u) ^ 1u, abort);
-      if ((i & 1) == 0) mbar_wait_or_abort(&x_full[xs], xp, abort);
+    for (int i = second; i < 2 * units; i += 2) {
+      const int as = i % kRingA, ds = i % kRingD;
+      if (i >= kRingD) mbar_wait_or_abort(&d_empty[ds], ((i / kRingD) & 1u) ^ 1u, abort);
+      mbar_wait_or_abort(&x_full[xs], xp, abort);
       mbar_wait_or_abort(&a_full[as], (i / kRingA) & 1u, abort);
       __syncwarp();
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t b = b0 + ((xs * kStageX + (i & 1) * 2 * kPanel) >> 4);
+        const uint64_t b = b0 + (xs * kStageX >> 4);
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          umma_ts<1>(tmem_base + i % kRingD * P, tmem_base + kA + as * 64 + k * 8, b + (((k >> 2) * kPanel + (k & 3) * 32) >> 4), id, k != 0 ? 1u : 0u);
+          umma_ts<1>(tmem_base + ds * P, tmem_base + kA + as * 64 + k * 8, b + (((k >> 2) * kPanel + (k & 3) * 32) >> 4), id, k != 0 ? 1u : 0u);
+        umma_commit<1>(&d_full[ds]);
         umma_commit<1>(&a_empty[as]);
-        if (i & 1) umma_commit<1>(&x_empty[xs]);
-        umma_commit<1>(&d_full[i % kRingD]);
+        umma_commit<1>(&x_empty[xs]);
       }
-      if ((i & 1) && ++xs == kRingX) xs = 0, xp ^= 1u;
+      if (++xs == kRingX) xs = 0, xp ^= 1u;
     }
-  } else if (warp >= 2 + kSumWarps) {
-    // ------------------------------------ widening: a row of every fourth group per thread ------------------------------------
-    const int first = (warp - 2 - kSumWarps) >> 2, quad = warp & 3, row = quad * 32 + lane;
-    const uint32_t to = tmem_base + kA + first * 64 + (static_cast<uint32_t>(quad * 32) << 16);
+  } else if (warp >= kWidenAt) {
+    // ------------------------------------ widening: a row of every third group per thread ------------------------------------
+    const int first = (warp - kWidenAt) >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t to = tmem_base + kA + (static_cast<uint32_t>(quad * 32) << 16);
     const uint8_t* from = smem + row * 128;
     const int swz = row & 7;                  // of the 16-byte pieces of a row, as TMA lays them
-    for (int i = first; i < 2 * units; i += kRingA) {
-      const int u = i >> 1, ws = u % kRingW;
+    for (int i = first; i < 2 * units; i += kSets) {
+      const int u = i >> 1, ws = u % kRingW, as = i % kRingA;
       mbar_wait_or_abort(&w_full[ws], (u / kRingW) & 1u, abort);
       uint4 words[4];
 #pragma unroll
@@ -192,26 +202,28 @@ gemm_int4_t5_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
           }
         }
         if (half == 0) {
-          if (i >= kRingA) mbar_wait_or_abort(&a_empty[first], ((i / kRingA) & 1u) ^ 1u, abort);
+          if (i >= kRingA) mbar_wait_or_abort(&a_empty[as], ((i / kRingA) & 1u) ^ 1u, abort);
           __syncwarp();
           tc_fence_after();
         }
-        tmem_st_x32(to + half * 32, r);
+        tmem_st_x32(to + as * 64 + half * 32, r);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&a_full[first]);
+        mbar_arrive(&a_full[as]);
         mbar_arrive(&w_empty[ws]);
       }
     }
   } else {
     // ------------------------------------ sums: a row per thread ------------------------------------
-    const int quad = warp & 3, row = quad * 32 + lane, n0 = (warp - 2) / 4 * kMine;
+    const int quad = warp & 3, row = quad * 32 + lane, part = (warp - kSumAt) >> 2, n0 = kByGroup ? 0 : part * kMine;
     const uint32_t from = tmem_base + n0 + (static_cast<uint32_t>(quad * 32) << 16);
     const int tokens = min(a.tokens - token0 - n0, kMine);
+    float* second_sums = reinterpret_cast<float*>(smem + kSumsAt);        // [token][row]
     float* up_sums = reinterpret_cast<float*>(smem + kUpAt);              // gated: [token][up row]
+    constexpr int kGroups = kByGroup ? 1 : 2;                             // of a unit, that a thread looks at
     int tile = tile0, g = g0;
     auto scale_at = [&](int tile, int group) {
       if (group >= a.groups) return __half();
@@ -219,14 +231,14 @@ gemm_int4_t5_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
       return a.scale[static_cast<long long>(min(out, a.rows - 1) + (GATED && row >= 64 ? a.rows : 0)) * a.lds + group];
     };
     // Scales are asked for four units at a time, and four ahead: a row's come from memory, a microsecond away.  They are kept where only their thread looks.
-    __half* kept = reinterpret_cast<__half*>(&kept_scales[threadIdx.x - 64]);
-    __half next[8];
+    __half* kept = reinterpret_cast<__half*>(&kept_scales[threadIdx.x - 32 * kSumAt]);
+    __half next[4 * kGroups];
     int next_tile = tile, next_g = g, next_u = 0;
     auto fetch_scales = [&] {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        next[2 * j] = next_u < units ? scale_at(next_tile, 2 * next_g) : __half();
-        next[2 * j + 1] = next_u < units ? scale_at(next_tile, 2 * next_g + 1) : __half();
+#pragma unroll
+        for (int h = 0; h < kGroups; ++h) next[kGroups * j + h] = next_u < units ? scale_at(next_tile, 2 * next_g + (kByGroup ? part : h)) : __half();
         ++next_u;
         if (++next_g == G) next_g = 0, ++next_tile;
       }
@@ -239,14 +251,14 @@ gemm_int4_t5_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     for (int u = 0; u < units; ++u) {
       if ((u & 3) == 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) kept[j] = next[j];
+        for (int j = 0; j < 4 * kGroups; ++j) kept[j] = next[j];
         fetch_scales();
       }
-      const float2 s = __half22float2(reinterpret_cast<const __half2*>(kept)[u & 3]);
       const bool ends = g + 1 == G;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int i = 2 * u + h;
+      for (int h = 0; h < kGroups; ++h) {
+        const int i = 2 * u + (kByGroup ? part : h);
+        const float s = __half2float(kept[kGroups * (u & 3) + h]);
         mbar_wait_or_abort(&d_full[i % kRingD], (i / kRingD) & 1u, abort);
         __syncwarp();
         tc_fence_after();
@@ -256,7 +268,7 @@ gemm_int4_t5_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
           tmem_ld_x16(from + i % kRingD * P + n, d);
           tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 16; ++c) total[n + c] = fmaf(h ? s.y : s.x, __uint_as_float(d[c]), total[n + c]);
+          for (int c = 0; c < 16; ++c) total[n + c] = fmaf(s, __uint_as_float(d[c]), total[n + c]);
         }
         tc_fence_before();
         __syncwarp();
@@ -267,57 +279,81 @@ gemm_int4_t5_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
         continue;
       }
       // The tile, or this CTA's part of it, is done.
-      bool write = true;
-      if (!whole || !ends) {
-        const int t0 = tile * G, cut = a.longer * (a.run + 1);
-        auto owner = [&](int unit) { return unit < cut ? unit / (a.run + 1) : a.longer + (unit - cut) / a.run; };
-        const int c0 = owner(t0), c1 = owner(t0 + G - 1);       // the first and the last CTA with a part
-        float* slots = a.partial + static_cast<long long>(blockIdx.y) * 2 * ctas * P * kRows + n0 * kRows + row;
-        const long long pitch = P * kRows;
-        float* mine = slots + (2 * cta + (cta == c0 ? 1 : 0)) * pitch;
+      if constexpr (kByGroup) {
+        if (part == 1) {
 #pragma unroll
-        for (int n = 0; n < kMine; ++n) __stcg(mine + n * kRows, total[n]);
-        __threadfence();
-        named_bar_sync(1, kSumThreads);
-        if (threadIdx.x == 64) {
-          unsigned int* ticket = a.tickets + static_cast<long long>(blockIdx.y) * a.tiles + tile;
-          last_one = atomicAdd(ticket, 1u) == static_cast<unsigned int>(c1 - c0);
-          if (last_one) *ticket = 0;
-          __threadfence();
+          for (int n = 0; n < kMine; ++n) second_sums[n * kRows + row] = total[n];
         }
-        named_bar_sync(1, kSumThreads);
-        write = last_one;
-        if (write) {
+        named_bar_sync(2, 256);
+        if (part == 0) {
 #pragma unroll
-          for (int n = 0; n < kMine; ++n) total[n] = 0.f;
-          for (int c = c0; c <= c1; ++c) {
-            const float* part = slots + (2 * c + (c == c0 ? 1 : 0)) * pitch;
-#pragma unroll
-            for (int n = 0; n < kMine; ++n) total[n] += __ldcg(part + n * kRows);
-          }
+          for (int n = 0; n < kMine; ++n) total[n] += second_sums[n * kRows + row];
         }
+        named_bar_sync(3, 256);
       }
-      if (write) {
-        const int out = tile * kOutRows + (GATED ? row & 63 : row);
-        __nv_bfloat16* to = a.out + static_cast<long long>(token0 + n0) * a.ldo + out;
-        if constexpr (GATED) {
-          if (row >= 64) {
+      if (!kByGroup || part == 0) {
+        bool write = true;
+        if (!whole || !ends) {
+          const int t0 = tile * G, c0 = t0 / a.run, c1 = (t0 + G - 1) / a.run;      // the first and the last CTA with a part
+          float* slots = a.partial + static_cast<long long>(blockIdx.y) * 2 * ctas * P * kRows + n0 * kRows + row;
+          const long long pitch = P * kRows;
+          float* mine = slots + (2 * cta + (cta == c0 ? 1 : 0)) * pitch;
 #pragma unroll
-            for (int n = 0; n < kMine; ++n) up_sums[(n0 + n) * 64 + row - 64] = total[n];
+          for (int n = 0; n < kMine; ++n) __stcg(mine + n * kRows, total[n]);
+          __threadfence();
+          named_bar_sync(1, kOutThreads);
+          if (threadIdx.x == 32 * kSumAt) {
+            unsigned int* ticket = a.tickets + static_cast<long long>(blockIdx.y) * a.tiles + tile;
+            last_one = atomicAdd(ticket, 1u) == static_cast<unsigned int>(c1 - c0);
+            if (last_one) *ticket = 0;
+            __threadfence();
           }
-          named_bar_sync(1, kSumThreads);
-          if (row < 64 && out < a.rows) {
+          named_bar_sync(1, kOutThreads);
+          write = last_one;
+          if (write) {
+#pragma unroll
+            for (int n = 0; n < kMine; ++n) total[n] = 0.f;
+            // (two parts under way at once; behind the last one its neighbour is read again and not used)
+            for (int c = c0; c <= c1; c += 2) {
+              const float* one = slots + (2 * c + (c == c0 ? 1 : 0)) * pitch;
+              const float* other = slots + 2 * min(c + 1, c1) * pitch;
+              const float use = c + 1 <= c1 ? 1.f : 0.f;
+#pragma unroll
+              for (int n = 0; n < kMine; n += 16) {
+                float v[16], z[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = __ldcg(one + (n + k) * kRows), z[k] = __ldcg(other + (n + k) * kRows);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  total[n + k] += v[k];
+                  if (use != 0.f) total[n + k] += z[k];
+                }
+              }
+            }
+          }
+        }
+        if (write) {
+          const int out = tile * kOutRows + (GATED ? row & 63 : row);
+          __nv_bfloat16* to = a.out + static_cast<long long>(token0 + n0) * a.ldo + out;
+          if constexpr (GATED) {
+            if (row >= 64) {
+#pragma unroll
+              for (int n = 0; n < kMine; ++n) up_sums[(n0 + n) * 64 + row - 64] = total[n];
+            }
+            named_bar_sync(1, kOutThreads);
+            if (row < 64 && out < a.rows) {
+#pragma unroll
+              for (int n = 0; n < kMine; ++n)
+                if (n < tokens) to[n * a.ldo] = __float2bfloat16(total[n] / (1.f + __expf(-total[n])) * up_sums[(n0 + n) * 64 + row]);
+            }
+          } else if (out < a.rows) {
 #pragma unroll
             for (int n = 0; n < kMine; ++n)
-              if (n < tokens) to[n * a.ldo] = __float2bfloat16(total[n] / (1.f + __expf(-total[n])) * up_sums[(n0 + n) * 64 + row]);
+              if (n < tokens) to[n * a.ldo] = __float2bfloat16(total[n]);
           }
-        } else if (out < a.rows) {
-#pragma unroll
-          for (int n = 0; n < kMine; ++n)
-            if (n < tokens) to[n * a.ldo] = __float2bfloat16(total[n]);
         }
+        if (GATED || !whole || !ends) named_bar_sync(1, kOutThreads);           // the flag and the up rows have been read
       }
-      named_bar_sync(1, kSumThreads);                 // the flag and the up rows have been read
 #pragma unroll
       for (int n = 0; n < kMine; ++n) total[n] = 0.f;
       ++tile;
@@ -334,16 +370,21 @@ gemm_int4_t5_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
 }
 
 namespace {
-int ctas_of(int tiles, int groups) { return static_cast<int>(min(static_cast<long long>(kNumSMs), static_cast<long long>(tiles) * ((groups + 1) / 2))); }
+// Runs of one length, as short as one CTA to an SM allows.
+int run_of(long long units) { return static_cast<int>((units + kNumSMs - 1) / kNumSMs); }
+int ctas_of(int tiles, int groups) {
+  const long long units = static_cast<long long>(tiles) * ((groups + 1) / 2);
+  return static_cast<int>((units + run_of(units) - 1) / run_of(units));
+}
 int padded(int tokens) { return tokens <= 16 ? 16 : tokens <= 32 ? 32 : 64; }
 
 template <int P, bool GATED>
 cudaError_t launch(const CUtensorMap& w, const CUtensorMap& x, const int4t5::Args& a, int chunks, cudaStream_t s) {
   using namespace int4t5;
-  constexpr int smem = kRingW * kUnitBytes + ring_x(P) * 4 * P * 128 + (GATED ? P * 64 * 4 : 0) + 1024;
+  constexpr int smem = kRingW * kUnitBytes + ring_x(P) * 4 * P * 128 + sums_bytes(P) + up_bytes(P, GATED) + 1024;
   const auto kernel = gemm_int4_t5_kernel<P, GATED>;
   if (const cudaError_t e = allow_smem(kernel, smem); e != cudaSuccess) return e;
-  return launch_dependent(kernel, dim3(ctas_of(a.tiles, a.groups), chunks), threads(P), smem, s, w, x, a);
+  return launch_dependent(kernel, dim3(ctas_of(a.tiles, a.groups), chunks), kThreads, smem, s, w, x, a);
 }
 template <bool GATED>
 cudaError_t dispatch(const CUtensorMap& w, const CUtensorMap& x, const int4t5::Args& a, int p, int chunks, cudaStream_t s) {
@@ -367,8 +408,8 @@ cudaError_t gemm_int4_t5(const void* x, long long ldx, const void* w, long long 
   if (const int e = get_tmap_2d_bf16(&tx, x, tokens, groups * 128LL, ldx, p, 64, 1); e != 0) return static_cast<cudaError_t>(e);
   unsigned char* const byte = wait_report(kWaitInt4);
   if (byte == nullptr) return cudaErrorMemoryAllocation;
-  const int tiles = (rows + tile_rows - 1) / tile_rows, units = tiles * ((groups + 1) / 2), ctas = ctas_of(tiles, groups);
-  const int4t5::Args a = {static_cast<const __half*>(scale), static_cast<__nv_bfloat16*>(out), partial, tickets, byte, lds, ldo, tokens, rows, groups, tiles, units / ctas, units % ctas};
+  const int tiles = (rows + tile_rows - 1) / tile_rows;
+  const int4t5::Args a = {static_cast<const __half*>(scale), static_cast<__nv_bfloat16*>(out), partial, tickets, byte, lds, ldo, tokens, rows, groups, tiles, run_of(static_cast<long long>(tiles) * ((groups + 1) / 2))};
   return gated ? dispatch<true>(tw, tx, a, p, chunks, s) : dispatch<false>(tw, tx, a, p, chunks, s);
 }
 

@@ -612,7 +612,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// linear_int4(x, w, scale, gated, workspace) -> x @ W.T, or swiglu(x @ W.T), of at most 128 rows with weights of 4 bits
+// linear_int4(x, w, scale, gated, workspace) -> x @ W.T, or swiglu(x @ W.T), of at most 192 rows with weights of 4 bits
 PyObject* py_linear_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return call(a, n, 5, [&](Args& args) -> PyObject* {
     const Tensor x = args.tensor(0), w = args.tensor(1), scale = args.tensor(2);
@@ -621,7 +621,7 @@ PyObject* py_linear_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         x.get_device() != c10::cuda::current_device() || w.get_device() != x.get_device() || scale.get_device() != x.get_device())
       return none();
     const int64_t K = x.size(-1), T = x.numel() / K;
-    if (T > 128 || K % 128 || w.scalar_type() != at::kByte || w.dim() != 2 || w.size(1) * 2 != K || w.size(0) == 0 || w.stride(1) != 1 || w.stride(0) % 16 || w.stride(0) < K / 2 || !unit16(w) ||
+    if (T > (w.dim() == 2 && w.size(0) * w.size(1) >= 16 << 20 ? 192 : 128) || K % 128 || w.scalar_type() != at::kByte || w.dim() != 2 || w.size(1) * 2 != K || w.size(0) == 0 || w.stride(1) != 1 || w.stride(0) % 16 || w.stride(0) < K / 2 || !unit16(w) ||
         (gated && w.size(0) % 2) || scale.scalar_type() != at::kHalf || scale.dim() != 2 || scale.size(0) != w.size(0) || scale.size(1) != K / 128 || scale.stride(1) != 1 ||
         scale.stride(0) < scale.size(1) || w.size(0) > (1 << 28) || K > (1 << 28))
       return none();

@@ -640,9 +640,11 @@ native.register_signature("llmctl_gemm_int4", [c_void_p, c_ll, c_void_p, c_ll, c
 native.register_signature("llmctl_gemm_int4_scratch_elems", [c_int] * 4 + [c_void_p], restype=c_ll)
 native.register_signature("llmctl_int4_widen", [c_void_p, c_ll, c_void_p, c_ll, c_void_p] + [c_int] * 4 + [c_void_p])
 
-# Tokens up to which the weights are read in 4 bits.  For more of them they are widened to bf16 once, which costs what 60 tokens more would, and the product is
-# the GEMM's (us, in 4 bits / widened: 12288 x 4096 128 tokens 44 / 45, 256 88 / 55).
-_INT4_TOKENS = 128
+def _int4_tokens(w: torch.Tensor) -> int:
+    """Tokens up to which the weights are read in 4 bits, once for 64 of them.  For more they are widened to bf16 and the product is the GEMM's, whose time hardly depends
+    on the number of tokens up to 256 (us, in 4 bits / widened: 4096 rows of 11008 190 tokens 48 / 58, 256 63 / 58; 32000 x 4096 190 95 / 123; 12288 x 4096 129 53 / 52; smaller ones,
+    4096 x 4096 100 19 / 25, 129 27 / 25, gated 2048 -> 5632 100 31 / 27, 129 42 / 27)."""
+    return 192 if w.shape[0] * w.shape[1] >= 16 << 20 else 128
 
 
 def dequantize_int4(w: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -696,7 +698,7 @@ def _int4(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, gated: bool) ->
     if scale.stride(1) != 1 or scale.stride(0) < scale.shape[1]:
         scale = scale.contiguous()
     with _on_device(x):
-        if x2.shape[0] > _INT4_TOKENS:
+        if x2.shape[0] > _int4_tokens(w):
             _int4_prompt(x2, w, scale, gated, out2)
             return out
         need, tickets = native.lib().llmctl_gemm_int4_scratch_elems, ctypes.c_int()

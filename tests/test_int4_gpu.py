@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from llmctl_b200.ops import functional as ops
+from llmctl_b200.ops import functional as ops, native
 
 from int4_oracle import check, matrix, product
 
@@ -11,7 +11,9 @@ pytestmark = pytest.mark.gpu
 
 @pytest.fixture(autouse=True)
 def _gpu(cuda_device):
-    return cuda_device
+    yield
+    torch.cuda.synchronize()
+    native.check_waits("test")
 
 
 def tokens(n, width, seed=1):
@@ -26,15 +28,15 @@ def run(x, w, scale, gated):
 
 # chunks of 8 tokens with one and two tiles of rows, the tensor cores' kernel with 16, 32 and 64 tokens and several chunks of them, widened weights
 @pytest.mark.parametrize("n,width,rows", [(1, 128, 1), (1, 4096, 4096), (2, 256, 33), (7, 1280, 9500), (8, 11008, 130), (9, 128, 16), (16, 4096, 12289), (31, 384, 200), (33, 5120, 9000),
-                                          (64, 11008, 4096), (65, 4096, 13001), (128, 4224, 12800), (129, 256, 24), (200, 4096, 1001)])
+                                          (64, 11008, 4096), (65, 4096, 13001), (128, 4224, 12800), (129, 256, 24), (190, 5120, 9000), (193, 5120, 9000), (200, 4096, 1001)])
 @pytest.mark.parametrize("gated", [False, True])
 def test_against_64_bits(n, width, rows, gated):
     x = tokens(n, width)
     w, scale = matrix(rows * (2 if gated else 1), width, 2, "cuda")
-    check(run(x, w, scale, gated), product(x, w, scale, gated, widened=n > 128))
+    check(run(x, w, scale, gated), product(x, w, scale, gated, widened=n > ops._int4_tokens(w)))
 
 
-@pytest.mark.parametrize("n", [3, 40, 150])
+@pytest.mark.parametrize("n", [3, 40, 250])
 @pytest.mark.parametrize("gated", [False, True])
 def test_layouts(n, gated):
     x, (w, scale) = tokens(n, 5120), matrix(9216, 5120, 3, "cuda")
@@ -61,7 +63,7 @@ def test_nothing_to_do():
     assert ops.linear_int4(torch.empty(3, 256, device="cuda", dtype=torch.bfloat16), w[:0], scale[:0]).shape == (3, 0)
 
 
-@pytest.mark.parametrize("n", [2, 20, 140])
+@pytest.mark.parametrize("n", [2, 20, 240])
 def test_numbers_that_are_not_finite_stay_with_their_token(n):
     x, (w, scale) = tokens(n, 4096), matrix(13000, 4096, 5, "cuda")
     clean = ops.linear_int4(x, w, scale)
@@ -114,3 +116,14 @@ def test_streams_and_graphs(n):
         torch.cuda.synchronize()
         for i in range(2):
             assert all(torch.equal(o, want[i]) for o in outs[i]) and all(torch.equal(o, want[2 + i]) for o in eager[i])
+
+
+def test_long_runs_of_many_tokens():
+    """Many units to a CTA, several chunks: stages of every ring are handed on many times."""
+    w, scale = matrix(40000, 4096, 9, "cuda")
+    for n in (16, 32, 64, 130):
+        x = tokens(n, 4096)
+        want, first = product(x, w, scale), ops.linear_int4(x, w, scale)
+        check(first, want)
+        for _ in range(30):
+            assert torch.equal(ops.linear_int4(x, w, scale), first)
