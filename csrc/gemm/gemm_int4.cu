@@ -9,47 +9,70 @@
 
 namespace llmctl {
 
-// bf16 [halves * padded, K] of W [halves * rows, K / 2]: each number (q - 8) s rounded once, rows past the last of a half zeros.  A thread has 8 columns of a row at a time, 4
-// bytes in and 16 out.  The whole number n = q - 8 is exact in bf16 (128 + q less 136), and s = s1 + s0 with 8 and at most 3 significant bits, so that n s0 is exact and
-// fma(n, s1, n s0) the product rounded once.  Bound by what it writes.
-__global__ void __launch_bounds__(256) int4_widen_kernel(const uint8_t* w, long long ldw, const __half* scale, long long lds, __nv_bfloat16* out, int rows, int padded, FastDiv by_words,
-                                                         int all) {
-  wait_for_previous(w, scale, out);
+// Operands of a prompt's product: x and the numbers (q - 8) s in fp16, each row brought to one range by a power of two, which the product's epilogue takes back.  bf16 would round
+// (q - 8) s to 8 bits, as far off as the output's own rounding (1.4 times the error, 1.7 gated); in fp16 it is off by 2^-12 and x, of 8 bits, is exact, both down to 2^-25 of what
+// the row's largest is brought to, 2^14: 2^-39 of it, below the products' fp32.  Infinities and NaN stay what they are and have no part in the range.  A warp has a row; 8 columns of
+// it in a lane at a time, which a warp stores as 512 whole bytes.  Bound by what it writes.
+__global__ void __launch_bounds__(256) int4_prepare_kernel(const __nv_bfloat16* x, long long ldx, int tokens, const uint8_t* w, long long ldw, const __half* scale, long long lds, int rows,
+                                                           int padded, int K, int all, __half* x_out, float* x_by, __half* w_out, float* w_by, long long w_by_half) {
+  wait_for_previous(x_out, x_by, w_out, w_by);
   release_dependents();
-  const int stride = gridDim.x * 256;
-  for (long long i0 = blockIdx.x * 256 + threadIdx.x; i0 < all; i0 += 4LL * stride) {
-    uint32_t words[4];
-    float s[4];
+  const int lane = threadIdx.x & 31, words = K / 8;
+  auto largest = [](uint32_t bits, uint32_t none, uint32_t most) { return bits < none ? max(bits, most) : most; };
+  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < all; i += gridDim.x * 8) {
+    if (i < tokens) {
+      const uint4* from = reinterpret_cast<const uint4*>(x + i * ldx);
+      uint32_t most = 0;
+#pragma unroll 4
+      for (int c = lane; c < words; c += 32) {
+        const uint4 v = from[c];
+        const uint32_t two[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const long long i = i0 + static_cast<long long>(k) * stride;
-      words[k] = 0x88888888u;
-      s[k] = 0.f;
-      if (i >= all) continue;
-      uint32_t word;
-      const int row = static_cast<int>(by_words.divide(static_cast<uint32_t>(i), word)), half = row >= padded ? 1 : 0, in = row - half * padded;
-      if (in >= rows) continue;
-      const long long from = static_cast<long long>(half) * rows + in;
-      words[k] = *reinterpret_cast<const uint32_t*>(w + from * ldw + word * 4);
-      s[k] = __half2float(scale[from * lds + (word >> 4)]);
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const long long i = i0 + static_cast<long long>(k) * stride;
-      if (i >= all) continue;
-      const __nv_bfloat16 high = __float2bfloat16(s[k]);
-      const float rest = s[k] - __bfloat162float(high);
-      const __nv_bfloat162 s1 = __bfloat162bfloat162(high), s0 = __bfloat162bfloat162(__float2bfloat16(fabsf(s[k]) < INFINITY ? rest : 0.f));
-      const uint32_t even = words[k] & 0x0f0f0f0fu, odd = (words[k] >> 4) & 0x0f0f0f0fu;
-      const uint32_t lo = __byte_perm(even, odd, 0x5140), hi = __byte_perm(even, odd, 0x7362);             // columns 0 .. 3, 4 .. 7
-      const uint32_t pair[4] = {__byte_perm(lo, 0x43434343u, 0x4140), __byte_perm(lo, 0x43434343u, 0x4342), __byte_perm(hi, 0x43434343u, 0x4140), __byte_perm(hi, 0x43434343u, 0x4342)};
-      bf16x8 r;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const __nv_bfloat162 n = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair[c]), __floats2bfloat162_rn(136.f, 136.f));
-        r.v[c] = __hfma2(n, s1, __hmul2(n, s0));
+        for (int k = 0; k < 4; ++k) most = largest(two[k] & 0x7fffu, 0x7f80u, largest((two[k] >> 16) & 0x7fffu, 0x7f80u, most));
       }
-      store8(out + i * 8, r);
+      const int e = max(static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 7), 15);          // exponents of both factors stay within fp32's
+      const float up = __uint_as_float(static_cast<uint32_t>(268 - e) << 23);
+      if (lane == 0) x_by[i] = __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
+      uint4* to = reinterpret_cast<uint4*>(x_out + static_cast<long long>(i) * K);
+#pragma unroll 4
+      for (int c = lane; c < words; c += 32) {
+        const uint4 v = from[c];
+        const uint32_t two[4] = {v.x, v.y, v.z, v.w};
+        __half2 h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = __floats2half2_rn(__uint_as_float(two[k] << 16) * up, __uint_as_float(two[k] & 0xffff0000u) * up);
+        to[c] = *reinterpret_cast<const uint4*>(h);
+      }
+      continue;
+    }
+    const int row = i - tokens, half = row >= padded ? 1 : 0, in = row - half * padded;
+    uint4* to = reinterpret_cast<uint4*>(w_out + static_cast<long long>(row) * K);
+    float* by = w_by + half * w_by_half + in;
+    if (in >= rows) {
+      for (int c = lane; c < words; c += 32) to[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (lane == 0) *by = 1.f;
+      continue;
+    }
+    const long long at = static_cast<long long>(half) * rows + in;
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(w + at * ldw);
+    const __half* s = scale + at * lds;
+    uint32_t most = 0;
+    for (int g = lane; g < words / 16; g += 32) most = largest(__half_as_ushort(s[g]) & 0x7fffu, 0x7c00u, most);
+    const int e = max(static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10), 1);
+    const float up = __uint_as_float(static_cast<uint32_t>(153 - e) << 23);                         // the largest scale to 2^11, times 8
+    if (lane == 0) *by = __uint_as_float(static_cast<uint32_t>(e + 101) << 23);
+#pragma unroll 4
+    for (int c = lane; c < words; c += 32) {
+      const uint32_t word = from[c];
+      const __half2 one = __float2half2_rn(__half2float(s[c >> 4]) * up);
+      const uint32_t even = word & 0x0f0f0f0fu, odd = (word >> 4) & 0x0f0f0f0fu;
+      const uint32_t lo = __byte_perm(even, odd, 0x5140), hi = __byte_perm(even, odd, 0x7362);       // columns 0 .. 3, 4 .. 7
+      const uint32_t pair[4] = {__byte_perm(lo, 0x64646464u, 0x4140), __byte_perm(lo, 0x64646464u, 0x4342), __byte_perm(hi, 0x64646464u, 0x4140), __byte_perm(hi, 0x64646464u, 0x4342)};
+      __half2 h[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)                                                                     // 1024 + q less 1032, exact; one rounding
+        h[k] = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&pair[k]), __floats2half2_rn(1032.f, 1032.f)), one);
+      to[c] = *reinterpret_cast<const uint4*>(h);
     }
   }
 }
@@ -88,14 +111,14 @@ LLMCTL_API int llmctl_gemm_int4(const void* x, long long ldx, const void* w, lon
   return 0;
 }
 
-LLMCTL_API int llmctl_int4_widen(const void* w, long long ldw, const void* scale, long long lds, void* out, int rows, int padded, int halves, int K, void* stream) {
+LLMCTL_API int llmctl_int4_prepare(const void* x, long long ldx, int tokens, const void* w, long long ldw, const void* scale, long long lds, int rows, int padded, int halves, int K,
+                                   void* x_out, float* x_by, void* w_out, float* w_by, void* stream) {
   LLMCTL_BEGIN();
-  LLMCTL_REQUIRE(rows > 0 && padded >= rows && (halves == 1 || halves == 2) && K > 0 && K % 128 == 0 && static_cast<long long>(padded) * halves < (1LL << 31));
-  LLMCTL_REQUIRE(aligned16(w, out) && ldw >= K / 2 && ldw % 16 == 0 && lds >= K / 128);
-  const long long all = static_cast<long long>(padded) * halves * (K / 8);
-  LLMCTL_REQUIRE(all < (1LL << 31));
-  const int grid = static_cast<int>(min((all + 1023) / 1024, 8LL * kNumSMs));
-  LLMCTL_CHECK(launch_dependent(int4_widen_kernel, grid, 256, 0, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(w), ldw, static_cast<const __half*>(scale), lds,
-                                static_cast<__nv_bfloat16*>(out), rows, padded, FastDiv(K / 8), static_cast<int>(all)));
+  LLMCTL_REQUIRE(tokens > 0 && rows > 0 && padded >= rows && (halves == 1 || halves == 2) && K > 0 && K % 128 == 0 && static_cast<long long>(padded) * halves + tokens < (1LL << 30));
+  LLMCTL_REQUIRE(aligned16(x, w, x_out, w_out) && ldx >= K && ldx % 8 == 0 && ldw >= K / 2 && ldw % 16 == 0 && lds >= K / 128);
+  const int all = padded * halves + tokens;
+  LLMCTL_CHECK(launch_dependent(int4_prepare_kernel, min((all + 7) / 8, 8 * kNumSMs), 256, 0, static_cast<cudaStream_t>(stream), static_cast<const __nv_bfloat16*>(x), ldx, tokens,
+                                static_cast<const uint8_t*>(w), ldw, static_cast<const __half*>(scale), lds, rows, padded, K, all, static_cast<__half*>(x_out), x_by,
+                                static_cast<__half*>(w_out), w_by, (padded + 63LL) / 64 * 64));
   return 0;
 }

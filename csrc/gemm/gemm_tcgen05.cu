@@ -101,8 +101,10 @@ constexpr int kGemmThreads = 192;
 // CTAs fitted, where their registers allow two; beside a gated activation's 196-209 registers they allow one.
 constexpr int kOutBox = 32 * 128;
 constexpr int kSmShared = 228 * 1024, kNeighbourShared = 1280;      // of an SM; of such a CTA (static, the reserved KB, rounded up)
-enum class Gated { kNone, kForward, kBackward, kRotate };       // what the epilogue does besides storing
-constexpr bool plain_output(Gated g) { return g == Gated::kNone || g == Gated::kRotate; }
+enum class Gated { kNone, kForward, kBackward, kRotate, kScale, kForwardScale };       // what the epilogue does besides storing
+constexpr bool plain_output(Gated g) { return g == Gated::kNone || g == Gated::kRotate || g == Gated::kScale; }
+constexpr bool gated_forward(Gated g) { return g == Gated::kForward || g == Gated::kForwardScale; }
+constexpr bool scaled(Gated g) { return g == Gated::kScale || g == Gated::kForwardScale; }      // fp16 operands, rows and columns times powers of two
 constexpr int out_bufs(Gated g) { return plain_output(g) ? 1 : 2; }
 
 template <int BN, Gated kGated = Gated::kNone>
@@ -242,6 +244,9 @@ struct SwigluMaps {
   const float *cos, *sin;
   const int* positions;
   int seq, rotated;
+  // scales (kScale, kForwardScale): a factor for each row of the product and for each of its columns (the up columns' follow columns_to further on)
+  const float *rows_by, *columns_by;
+  long long columns_to;
 };
 
 // Rotation of heads of 64 on their way out (llmctl_gemm_rope_bf16): a chunk of 64 columns is a head, and a lane holds its row of it, halves and all.
@@ -281,8 +286,35 @@ __device__ __forceinline__ void rotate_epilogue(uint32_t t_row, OutStage<1>& out
     stage_box(out, tmC, col, row0, lane, [&](int e) { return pack_bf16x2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])); });
   }
 }
+// Products of fp16 operands whose rows were brought to one range by powers of two (llmctl_gemm_f16_scaled): they are taken back here, the columns' first,
+// which are those of weights and small (the product of the two may pass fp32's range where the result does not).  `by` has whole chunks of 64.
+__device__ __forceinline__ void scale_columns(uint32_t (&r)[64], const float* by, float row_by) {
+#pragma unroll
+  for (int i = 0; i < 64; i += 4) {
+    const float4 c = *reinterpret_cast<const float4*>(by + i);
+    r[i] = __float_as_uint(__uint_as_float(r[i]) * c.x * row_by);
+    r[i + 1] = __float_as_uint(__uint_as_float(r[i + 1]) * c.y * row_by);
+    r[i + 2] = __float_as_uint(__uint_as_float(r[i + 2]) * c.z * row_by);
+    r[i + 3] = __float_as_uint(__uint_as_float(r[i + 3]) * c.w * row_by);
+  }
+}
 template <int BN>
-__device__ __forceinline__ void swiglu_epilogue(uint32_t t_row, OutStage<2>& out, const SwigluMaps& maps, int row0, int f0,
+__device__ __forceinline__ void scale_epilogue(uint32_t t_row, OutStage<1>& out, const CUtensorMap* tmC, const SwigluMaps& sw, float row_by, int row0, int n0, int M,
+                                               int N, int lane) {
+#pragma unroll 1
+  for (int c = 0; c < BN / 64; ++c) {
+    uint32_t r[64];
+    tmem_ld_x32(t_row + c * 64, r);
+    tmem_ld_x32(t_row + c * 64 + 32, r + 32);
+    tmem_ld_wait();
+    const int col = n0 + c * 64;
+    if (row0 >= M || col >= N) continue;               // uniform over the warp
+    scale_columns(r, sw.columns_by + col, row_by);
+    stage_box(out, tmC, col, row0, lane, [&](int e) { return pack_bf16x2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])); });
+  }
+}
+template <int BN, bool kScaled>
+__device__ __forceinline__ void swiglu_epilogue(uint32_t t_row, OutStage<2>& out, const SwigluMaps& maps, [[maybe_unused]] float row_by, int row0, int f0,
                                                 int M, int F, int lane) {
 #pragma unroll 1
   for (int c = 0; c < BN / 128; ++c) {
@@ -294,6 +326,10 @@ __device__ __forceinline__ void swiglu_epilogue(uint32_t t_row, OutStage<2>& out
     tmem_ld_wait();
     const int col = f0 + c * 64;
     if (row0 >= M || col >= F) continue;               // uniform over the warp
+    if constexpr (kScaled) {
+      scale_columns(g, maps.columns_by + col, row_by);
+      scale_columns(u, maps.columns_by + maps.columns_to + col, row_by);
+    }
     auto packed = [](const uint32_t* r, int e) { return pack_bf16x2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])); };
     if (maps.keep) {
       stage_box(out, &maps.gate, col, row0, lane, [&](int e) { return packed(g, e); });
@@ -395,7 +431,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int lane = threadIdx.x & 31;
 
   const int num_m = (M + kBM - 1) / kBM;
-  constexpr bool kSwiglu = kGated == Gated::kForward;
+  constexpr bool kSwiglu = gated_forward(kGated);
   constexpr int kCols = kSwiglu ? BN / 2 : BN;         // output columns per tile; with the gate N counts those of one half
   const int num_n = (N + kCols - 1) / kCols;
   const int num_tiles = num_m * num_n;
@@ -473,7 +509,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     // ------------------------------ MMA issuer ------------------------------
     // The whole warp walks the loop, one elected lane issues: stage addresses and descriptors stay in uniform registers, which
     // the instruction reads.  From a single lane's branch a product took 85-107 clocks to issue, more than a 128-wide tile's 64.
-    constexpr uint32_t idesc = make_idesc_bf16(kBM, BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u);
+    constexpr uint32_t idesc = (scaled(kGated) ? make_idesc_f16 : make_idesc_bf16)(kBM, BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u);
     int stage = 0;
     uint32_t phase = 0;
     int acc = 0;
@@ -525,16 +561,20 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       if (grouped_b_row(gate, mb_, n0, N) < 0) continue;
       [[maybe_unused]] Angles angles;
       if constexpr (kGated == Gated::kRotate) angles.load(sw, m0 + q * 32 + lane, M);
+      float row_by = 1.f;
+      if constexpr (scaled(kGated)) row_by = m0 + q * 32 + lane < M ? sw.rows_by[m0 + q * 32 + lane] : 0.f;
       mbar_wait(&bar_tfull[acc], aphase);
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
       out.begin(smem + Cfg::kOutAt, smem, q, BN / 64, plain_output(kGated) && tile + static_cast<int>(gridDim.x) >= num_tiles);
       if constexpr (kSwiglu)
-        swiglu_epilogue<BN>(t_row, out, sw, m0 + q * 32, n0, M, N, lane);
+        swiglu_epilogue<BN, scaled(kGated)>(t_row, out, sw, row_by, m0 + q * 32, n0, M, N, lane);
       else if constexpr (kGated == Gated::kBackward)
         swiglu_bwd_epilogue<BN>(t_row, out.at, sw, m0 + q * 32, n0, M, N, lane);
       else if constexpr (kGated == Gated::kRotate)
         rotate_epilogue<BN>(t_row, out, &tmC, angles, sw.rotated, m0 + q * 32, n0, M, N, lane);
+      else if constexpr (kGated == Gated::kScale)
+        scale_epilogue<BN>(t_row, out, &tmC, sw, row_by, m0 + q * 32, n0, M, N, lane);
       else
         gemm_epilogue<BN, OutT>(t_row, out, &tmC, C, ldc, m0 + q * 32, n0, M, N, beta, lane);
       tc_fence_before();
@@ -604,7 +644,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   const int num_pairs = gridDim.x >> 1;
 
   const int num_m = (M + 2 * kBM - 1) / (2 * kBM);
-  constexpr bool kSwiglu = kGated == Gated::kForward;
+  constexpr bool kSwiglu = gated_forward(kGated);
   constexpr int kCols = kSwiglu ? BN / 2 : BN;         // output columns per tile; with the gate N counts those of one half
   const int num_n = (N + kCols - 1) / kCols;
   const int num_tiles = num_m * num_n;
@@ -679,7 +719,7 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   } else if (warp == 1) {
     // ------------------------------ MMA issuer (leader CTA only) ------------------------------
     if (cta_rank == 0) {
-      constexpr uint32_t idesc = make_idesc_bf16(2 * kBM, BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u);
+      constexpr uint32_t idesc = (scaled(kGated) ? make_idesc_f16 : make_idesc_bf16)(2 * kBM, BN, A_MN ? 1u : 0u, B_MN ? 1u : 0u);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -726,16 +766,20 @@ gemm2_tcgen05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const int n0 = nb_ * kCols;
       [[maybe_unused]] Angles angles;
       if constexpr (kGated == Gated::kRotate) angles.load(sw, m0 + q * 32 + lane, M);
+      float row_by = 1.f;
+      if constexpr (scaled(kGated)) row_by = m0 + q * 32 + lane < M ? sw.rows_by[m0 + q * 32 + lane] : 0.f;
       mbar_wait(&bar_tfull[acc], aphase);
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(acc * BN);
       out.begin(smem + Cfg::kOutAt, smem, q, BN / 64, plain_output(kGated) && tile + num_pairs >= num_tiles);
       if constexpr (kSwiglu)
-        swiglu_epilogue<BN>(t_row, out, sw, m0 + q * 32, n0, M, N, lane);
+        swiglu_epilogue<BN, scaled(kGated)>(t_row, out, sw, row_by, m0 + q * 32, n0, M, N, lane);
       else if constexpr (kGated == Gated::kBackward)
         swiglu_bwd_epilogue<BN>(t_row, out.at, sw, m0 + q * 32, n0, M, N, lane);
       else if constexpr (kGated == Gated::kRotate)
         rotate_epilogue<BN>(t_row, out, &tmC, angles, sw.rotated, m0 + q * 32, n0, M, N, lane);
+      else if constexpr (kGated == Gated::kScale)
+        scale_epilogue<BN>(t_row, out, &tmC, sw, row_by, m0 + q * 32, n0, M, N, lane);
       else
         gemm_epilogue<BN, OutT>(t_row, out, &tmC, C, ldc, m0 + q * 32, n0, M, N, beta, lane);
       tc_fence_before();
@@ -1063,13 +1107,12 @@ static int dispatch_layout2(int a_mn, int b_mn, const void* A, const void* B, vo
   return launch_gemm2<PBN, true, true, OutT>(A, B, C, M, N, K, lda, ldb, ldc, beta, max_ctas, s, g);
 }
 
-template <bool kPair>
+template <bool kPair, Gated kGated = Gated::kForward>
 static int launch_swiglu(const void* X, const void* W, void* GU, void* ACT, int M, int F, int K, long long ldx, long long ldw, long long ldgu,
-                         long long ldact, cudaStream_t s) {
+                         long long ldact, cudaStream_t s, SwigluMaps sw = SwigluMaps{}) {
   constexpr int kCols = kPair ? 128 : 64;            // gate rows (and up rows) per tile
   const __nv_bfloat16 *w = (const __nv_bfloat16*)W, *gu = (const __nv_bfloat16*)GU;
   CUtensorMap tmA, tmW;
-  SwigluMaps sw;
   int rc = get_tmap_2d_bf16(&tmA, X, M, K, ldx, kBM, kBK, 1);
   if (!rc) rc = get_tmap_2d_bf16(&tmW, w, F, K, ldw, kCols, kBK, 1);
   if (!rc) rc = get_tmap_2d_bf16(&sw.w_up, w + static_cast<long long>(F) * ldw, F, K, ldw, kCols, kBK, 1);
@@ -1081,22 +1124,22 @@ static int launch_swiglu(const void* X, const void* W, void* GU, void* ACT, int 
   if (rc) LLMCTL_FAIL(rc, "tensor maps");
   const int tiles = ((M + (kPair ? 2 : 1) * kBM - 1) / ((kPair ? 2 : 1) * kBM)) * ((F + kCols - 1) / kCols);
   if constexpr (kPair) {
-    auto kern = gemm2_tcgen05_kernel<256, false, false, __nv_bfloat16, Gated::kForward>;
-    LLMCTL_CHECK(allow_smem(kern, Gemm2Cfg<256, Gated::kForward>::kSmemBytes));
+    auto kern = gemm2_tcgen05_kernel<256, false, false, __nv_bfloat16, kGated>;
+    LLMCTL_CHECK(allow_smem(kern, Gemm2Cfg<256, kGated>::kSmemBytes));
     const int pairs = tiles < num_sms() / 2 ? tiles : num_sms() / 2;
-    LLMCTL_CHECK(launch_gemm_kernel(kern, 2 * pairs, Gemm2Cfg<256, Gated::kForward>::kSmemBytes, s, tmA, tmW, tmA, (__nv_bfloat16*)ACT, ldact, M, F, K, 0, GemmGate{}, sw));
+    LLMCTL_CHECK(launch_gemm_kernel(kern, 2 * pairs, Gemm2Cfg<256, kGated>::kSmemBytes, s, tmA, tmW, tmA, (__nv_bfloat16*)ACT, ldact, M, F, K, 0, GemmGate{}, sw));
   } else {
-    auto kern = gemm_tcgen05_kernel<128, false, false, __nv_bfloat16, Gated::kForward>;
-    LLMCTL_CHECK(allow_smem(kern, GemmCfg<128, Gated::kForward>::kSmemBytes));
-    LLMCTL_CHECK(launch_gemm_kernel(kern, tiles < num_sms() ? tiles : num_sms(), GemmCfg<128, Gated::kForward>::kSmemBytes, s, tmA, tmW, tmA, (__nv_bfloat16*)ACT, ldact,
+    auto kern = gemm_tcgen05_kernel<128, false, false, __nv_bfloat16, kGated>;
+    LLMCTL_CHECK(allow_smem(kern, GemmCfg<128, kGated>::kSmemBytes));
+    LLMCTL_CHECK(launch_gemm_kernel(kern, tiles < num_sms() ? tiles : num_sms(), GemmCfg<128, kGated>::kSmemBytes, s, tmA, tmW, tmA, (__nv_bfloat16*)ACT, ldact,
                                     M, F, K, 0, GemmGate{}, sw));
   }
   LLMCTL_RETURN_LAST();
 }
 
 // kBN: 64 or 128 (one CTA), 256 (CTA pair).
-template <int kBN>
-static int launch_rotate(const void* X, const void* W, void* C, int M, int N, int K, long long ldx, long long ldw, long long ldc, const SwigluMaps& sw, cudaStream_t s) {
+template <int kBN, Gated kGated>
+static int launch_plain(const void* X, const void* W, void* C, int M, int N, int K, long long ldx, long long ldw, long long ldc, const SwigluMaps& sw, cudaStream_t s) {
   constexpr bool kPair = kBN == 256;
   constexpr int kRows = (kPair ? 2 : 1) * kBM;
   CUtensorMap tmA, tmW, tmC;
@@ -1107,13 +1150,13 @@ static int launch_rotate(const void* X, const void* W, void* C, int M, int N, in
   const int tiles = ((M + kRows - 1) / kRows) * ((N + kBN - 1) / kBN), most = kPair ? num_sms() / 2 : num_sms();
   const int grid = tiles < most ? tiles : most;
   if constexpr (kPair) {
-    auto kern = gemm2_tcgen05_kernel<256, false, false, __nv_bfloat16, Gated::kRotate>;
-    LLMCTL_CHECK(allow_smem(kern, Gemm2Cfg<256, Gated::kRotate>::kSmemBytes));
-    LLMCTL_CHECK(launch_gemm_kernel(kern, 2 * grid, Gemm2Cfg<256, Gated::kRotate>::kSmemBytes, s, tmA, tmW, tmC, (__nv_bfloat16*)C, ldc, M, N, K, 0, GemmGate{}, sw));
+    auto kern = gemm2_tcgen05_kernel<256, false, false, __nv_bfloat16, kGated>;
+    LLMCTL_CHECK(allow_smem(kern, Gemm2Cfg<256, kGated>::kSmemBytes));
+    LLMCTL_CHECK(launch_gemm_kernel(kern, 2 * grid, Gemm2Cfg<256, kGated>::kSmemBytes, s, tmA, tmW, tmC, (__nv_bfloat16*)C, ldc, M, N, K, 0, GemmGate{}, sw));
   } else {
-    auto kern = gemm_tcgen05_kernel<kBN, false, false, __nv_bfloat16, Gated::kRotate>;
-    LLMCTL_CHECK(allow_smem(kern, GemmCfg<kBN, Gated::kRotate>::kSmemBytes));
-    LLMCTL_CHECK(launch_gemm_kernel(kern, grid, GemmCfg<kBN, Gated::kRotate>::kSmemBytes, s, tmA, tmW, tmC, (__nv_bfloat16*)C, ldc, M, N, K, 0, GemmGate{}, sw));
+    auto kern = gemm_tcgen05_kernel<kBN, false, false, __nv_bfloat16, kGated>;
+    LLMCTL_CHECK(allow_smem(kern, GemmCfg<kBN, kGated>::kSmemBytes));
+    LLMCTL_CHECK(launch_gemm_kernel(kern, grid, GemmCfg<kBN, kGated>::kSmemBytes, s, tmA, tmW, tmC, (__nv_bfloat16*)C, ldc, M, N, K, 0, GemmGate{}, sw));
   }
   LLMCTL_RETURN_LAST();
 }
@@ -1266,7 +1309,28 @@ LLMCTL_API int llmctl_gemm_swiglu_bf16(const void* X, const void* W, void* GU, v
   LLMCTL_REQUIRE(((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(GU) |
                    reinterpret_cast<uintptr_t>(ACT)) & 15) == 0 && static_cast<long long>(ldact) >= F);
   const bool one_wave = static_cast<long long>((M + kBM - 1) / kBM) * ((F + 63) / 64) <= num_sms();
-  return (one_wave || M <= 128 ? launch_swiglu<false> : launch_swiglu<true>)(X, W, GU, ACT, M, F, K, ldx, ldw, ldgu, ldact, (cudaStream_t)stream);
+  return (one_wave || M <= 128 ? launch_swiglu<false> : launch_swiglu<true>)(X, W, GU, ACT, M, F, K, ldx, ldw, ldgu, ldact, (cudaStream_t)stream, SwigluMaps{});
+}
+
+// C[M, N] = rows_by[m] columns_by[n] sum_k X[m, k] W[n, k], X and W fp16, C bf16; gated: W has 2 N rows, gate first, columns_by of the up rows starts at the next
+// multiple of 64, and C = silu(gate) * up.  The products of prompts with weights of 4 bits, whose eight bits of sum and scale bf16 would round once more.
+LLMCTL_API int llmctl_gemm_f16_scaled(const void* X, const void* W, const float* rows_by, const float* columns_by, void* C, int M, int N, int K, long long ldx,
+                                      long long ldw, long long ldc, int gated, void* stream) {
+  LLMCTL_BEGIN();
+  LLMCTL_REQUIRE(M > 0 && N > 0 && K > 0 && N % 8 == 0 && ldx % 8 == 0 && ldw % 8 == 0 && ldc % 8 == 0 && ldx >= K && ldw >= K && ldc >= N);
+  LLMCTL_REQUIRE(rows_by != nullptr && aligned16(X, W, C, columns_by));
+  SwigluMaps sw{};
+  sw.rows_by = rows_by;
+  sw.columns_by = columns_by;
+  sw.columns_to = (N + 63LL) / 64 * 64;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (gated) {
+    const bool one_wave = static_cast<long long>((M + kBM - 1) / kBM) * ((N + 63) / 64) <= num_sms();
+    return (one_wave || M <= 128 ? launch_swiglu<false, Gated::kForwardScale> : launch_swiglu<true, Gated::kForwardScale>)(X, W, nullptr, C, M, N, K, ldx, ldw, 0, ldc, s, sw);
+  }
+  const int bn = one_wave_tile(M, N);
+  const auto launch = bn == 64 ? launch_plain<64, Gated::kScale> : bn == 128 || M <= 128 || N <= 128 ? launch_plain<128, Gated::kScale> : launch_plain<256, Gated::kScale>;
+  return launch(X, W, C, M, N, K, ldx, ldw, ldc, sw, s);
 }
 
 // DGU[M, 2F] = (d gate | d up) of a gated MLP from dy [M, K], the down-projection W [K, F] and the forward's GU [M, 2F] (row stride ldgu for
@@ -1301,7 +1365,7 @@ LLMCTL_API int llmctl_gemm_rope_bf16(const void* X, const void* W, void* C, int 
   sw.seq = seq_len;
   sw.rotated = rotated;
   const int bn = one_wave_tile(M, N);
-  const auto launch = bn == 64 ? launch_rotate<64> : bn == 128 || M <= 128 ? launch_rotate<128> : launch_rotate<256>;
+  const auto launch = bn == 64 ? launch_plain<64, Gated::kRotate> : bn == 128 || M <= 128 ? launch_plain<128, Gated::kRotate> : launch_plain<256, Gated::kRotate>;
   return launch(X, W, C, M, N, K, ldx, ldw, ldc, sw, (cudaStream_t)stream);
 }
 

@@ -638,10 +638,11 @@ INT4_GROUP = 128                # input channels to a scale
 
 native.register_signature("llmctl_gemm_int4", [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll] + [c_int] * 4 + [c_void_p, c_ll, c_void_p, c_int, c_void_p])
 native.register_signature("llmctl_gemm_int4_scratch_elems", [c_int] * 4 + [c_void_p], restype=c_ll)
-native.register_signature("llmctl_int4_widen", [c_void_p, c_ll, c_void_p, c_ll, c_void_p] + [c_int] * 4 + [c_void_p])
+native.register_signature("llmctl_int4_prepare", [c_void_p, c_ll, c_int, c_void_p, c_ll, c_void_p, c_ll] + [c_int] * 4 + [c_void_p] * 5)
+native.register_signature("llmctl_gemm_f16_scaled", [c_void_p] * 5 + [c_int] * 3 + [c_ll] * 3 + [c_int, c_void_p])
 
 def _int4_tokens(w: torch.Tensor) -> int:
-    """Tokens up to which the weights are read in 4 bits, once for 64 of them.  For more they are widened to bf16 and the product is the GEMM's, whose time hardly depends
+    """Tokens up to which the weights are read in 4 bits, once for 64 of them.  For more they are widened to fp16 and the product is the GEMM's, whose time hardly depends
     on the number of tokens up to 256 (us, in 4 bits / widened: 4096 rows of 11008 190 tokens 48 / 58, 256 63 / 58; 32000 x 4096 190 95 / 123; 12288 x 4096 129 53 / 52; smaller ones,
     4096 x 4096 100 19 / 25, 129 27 / 25, gated 2048 -> 5632 100 31 / 27, 129 42 / 27)."""
     return 192 if w.shape[0] * w.shape[1] >= 16 << 20 else 128
@@ -720,18 +721,18 @@ def _int4_workspace(x: torch.Tensor, elems: int, tickets: int):
 
 
 def _int4_prompt(x: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, gated: bool, out: torch.Tensor) -> None:
-    """The product of many tokens: the weights as bf16 rows (in number a multiple of 8, as the GEMM stores them), used once."""
-    K, halves = x.shape[1], 2 if gated else 1
+    """The product of many tokens: x and the weights in fp16 (rows of weights in number a multiple of 8, as the GEMM stores them), used once; each row is brought to
+    one range by a power of two, which the product takes back."""
+    (M, K), halves = x.shape, 2 if gated else 1
     N = w.shape[0] // halves
     padded = -(-N // 8) * 8
-    wide = torch.empty(halves * padded, K, dtype=torch.bfloat16, device=x.device)
-    native.call("llmctl_int4_widen", w.data_ptr(), w.stride(0), scale.data_ptr(), scale.stride(0), wide.data_ptr(), N, padded, halves, K, native.stream_ptr())
-    whole = out if padded == N else torch.empty(x.shape[0], padded, dtype=out.dtype, device=out.device)
-    if gated:
-        native.call("llmctl_gemm_swiglu_bf16", x.data_ptr(), wide.data_ptr(), None, whole.data_ptr(), x.shape[0], padded, K, x.stride(0), K, 2 * padded, padded,
-                    native.stream_ptr())
-    else:
-        gemm_raw(x, wide, out=whole)
+    x16, w16 = (torch.empty(n, K, dtype=torch.float16, device=x.device) for n in (M, halves * padded))
+    w_by, x_by = torch.empty(-(-padded // 64) * 64 * halves + M, dtype=torch.float32, device=x.device).tensor_split([-(-padded // 64) * 64 * halves])
+    stream = native.stream_ptr()
+    native.call("llmctl_int4_prepare", x.data_ptr(), x.stride(0), M, w.data_ptr(), w.stride(0), scale.data_ptr(), scale.stride(0), N, padded, halves, K,
+                x16.data_ptr(), x_by.data_ptr(), w16.data_ptr(), w_by.data_ptr(), stream)
+    whole = out if padded == N else torch.empty(M, padded, dtype=out.dtype, device=out.device)
+    native.call("llmctl_gemm_f16_scaled", x16.data_ptr(), w16.data_ptr(), x_by.data_ptr(), w_by.data_ptr(), whole.data_ptr(), M, padded, K, K, K, padded, int(gated), stream)
     if whole is not out:
         out.copy_(whole[:, :N])
 

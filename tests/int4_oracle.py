@@ -21,10 +21,10 @@ def wide(w, scale):
 
 def product(x, w, scale, gated=False, widened=False):
     """(value, bound on the error of a bf16 result).  A sum of n numbers in 32 bits is off by at most n 2^-23 of the sum of their sizes, a group's 128 and those
-    between the groups; weights rounded to bf16 (``widened``) add 2^-8 of it, the result's own rounding 2^-8 of the value (half a step: eps / 2)."""
+    between the groups; weights rounded to fp16 (``widened``) add 2^-12 of it, the result's own rounding 2^-8 of the value (half a step: eps / 2)."""
     full, x = wide(w, scale), x.double()
     y, size = x @ full.t(), x.abs() @ full.abs().t()
-    off = size * ((GROUP + x.shape[-1] // GROUP) * 2.0 ** -23 + (2.0 ** -8 if widened else 0.0))
+    off = size * ((GROUP + x.shape[-1] // GROUP) * 2.0 ** -23 + (2.0 ** -12 if widened else 0.0))
     if gated:
         (g, u), (eg, eu) = y.chunk(2, -1), off.chunk(2, -1)
         act = torch.nn.functional.silu(g)

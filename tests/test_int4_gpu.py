@@ -127,3 +127,30 @@ def test_long_runs_of_many_tokens():
         check(first, want)
         for _ in range(30):
             assert torch.equal(ops.linear_int4(x, w, scale), first)
+
+
+@pytest.mark.parametrize("n", [3, 40, 250, 700])
+@pytest.mark.parametrize("gated", [False, True])
+def test_rows_of_any_size(n, gated):
+    """Tokens and rows of weights whose sizes lie far apart, scales from fp16's least to its largest, rows of zeros."""
+    g = torch.Generator().manual_seed(11)
+    x = (tokens(n, 1024).float() * torch.exp2(torch.randint(-40, 20, (n, 1), generator=g).float()).cuda()).bfloat16()
+    x[n // 2] = 0
+    w, scale = matrix(4000, 1024, 12, "cuda")
+    scale *= torch.exp2(torch.randint(-14, 14, (4000, 1), generator=g).float()).cuda().half()
+    scale[7], scale[8, 0], scale[9, 1], scale[10, 2] = 0, 65504.0, 2.0 ** -24, 2.0 ** -15
+    check(run(x, w, scale, gated), product(x, w, scale, gated, widened=n > ops._int4_tokens(w)))
+
+
+def test_the_largest_numbers_of_a_prompt():
+    """Products that pass fp16's range, and fp32's where only a factor does."""
+    w, scale = matrix(512, 256, 13, "cuda")
+    for size in (2.0 ** 110, 2.0 ** -120):
+        x = (tokens(300, 256).float().clamp(-4, 4) * size).bfloat16()
+        y, _ = product(x, w, scale, widened=True)
+        got = ops.linear_int4(x, w, scale).double()
+        assert torch.isfinite(got).all() and ((got - y).norm() / y.norm()).item() < 2.0 ** -8
+    scale[3, 1] = float("inf")
+    scale[4, 0] = float("nan")
+    got = ops.linear_int4(tokens(300, 256), w, scale)
+    assert not got[:, 3:5].isfinite().any() and got[:, :3].isfinite().all() and got[:, 5:].isfinite().all()
