@@ -82,10 +82,21 @@ namespace {
 // 4096 x 4096 (8.4 MB) 16 tokens 8.0 / 8.0, 24 11.8 / 9.8; gated 2048 -> 5632 (11.5 MB) 12 tokens 11.2 / 10.9; 6144 rows of 2048 (6.3 MB) 24 tokens 9.3 / 11.0, 32 12.6 /
 // 11.0; 2048 rows of 5632 (5.8 MB) 32 tokens 9.9 / 12.3, 48 14.5 / 14.7; 2048 x 2048 64 tokens 8.9 / 10.8; 12288 x 4096 (25 MB) 9 tokens 18 / 14.0.
 bool in_chunks(int tokens, long long matrix_rows, int K) { return tokens <= 8 || (tokens + 7) / 8 * (matrix_rows * (K / 2)) <= (23LL << 20); }
+
+// Tokens up to which the weights are read in 4 bits, once for 64 of them.  For more they are widened to fp16, and the time of the GEMM that follows hardly depends on the number
+// of tokens up to 256.  us, in 4 bits / widened: many bytes or a long K, 32000 x 4096 190 tokens 95 / 144, 256 128 / 146; 12288 x 4096 190 53 / 60, 256 71 / 61; 4096 x 4096 190
+// 27 / 30, 256 35 / 31; 2048 x 5632 190 27 / 36; 5120 x 5120 190 36 / 38.  Neither, 6144 x 2048 60 13 / 17, 65 22 / 17; gated 2048 -> 5632 65 29 / 25, 1024 -> 4096 65 19 / 16.
+// So few bytes that up to 11 chunks read them, 2048 x 2048 65 9 / 16, 96 16 / 16; gated 768 -> 2048 65 10 / 11, 96 13 / 11; 2304 x 768 65 6.4 / 8.2, 100 8.5 / 8.4.
+int most_tokens(long long matrix_rows, int K) {
+  const long long bytes = matrix_rows * (K / 2);
+  return bytes >= (16LL << 20) || K >= 4096 ? 192 : bytes <= (2LL << 20) ? 88 : 64;
+}
 }  // namespace
 }  // namespace llmctl
 
 using namespace llmctl;
+
+LLMCTL_API int llmctl_gemm_int4_tokens(long long matrix_rows, int K) { return most_tokens(matrix_rows, K); }
 
 LLMCTL_API long long llmctl_gemm_int4_scratch_elems(int tokens, int rows, int K, int gated, int* tickets) {
   *tickets = 0;

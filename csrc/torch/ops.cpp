@@ -48,7 +48,7 @@ using at::Tensor;
   X(llmctl_gemm_swiglu_bwd_bf16) X(llmctl_swiglu_bwd) X(llmctl_gemm_skinny_bf16) X(llmctl_gemm_skinny_scratch_elems) X(llmctl_flash_attn_fwd) X(llmctl_flash_attn_bwd) X(llmctl_kv_append) \
   X(llmctl_paged_attn_decode) X(llmctl_paged_attn_scratch_elems) X(llmctl_latent_kv_write) X(llmctl_latent_decode) \
   X(llmctl_rope_kv_append) X(llmctl_rope_kv_append_fp8) X(llmctl_rope_kv_append_fp8_scratch_elems) X(llmctl_paged_attn_decode_fp8) X(llmctl_paged_attn_fp8_scratch_elems) X(llmctl_token_logprobs) X(llmctl_token_logprobs_bwd) \
-  X(llmctl_gemm_int4) X(llmctl_gemm_int4_scratch_elems) X(llmctl_paged_attn_decode_shared) X(llmctl_paged_attn_shared_scratch_elems)
+  X(llmctl_gemm_int4) X(llmctl_gemm_int4_scratch_elems) X(llmctl_gemm_int4_tokens) X(llmctl_paged_attn_decode_shared) X(llmctl_paged_attn_shared_scratch_elems)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
   LLMCTL_ENTRIES(X)
@@ -617,13 +617,13 @@ PyObject* py_linear_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return call(a, n, 5, [&](Args& args) -> PyObject* {
     const Tensor x = args.tensor(0), w = args.tensor(1), scale = args.tensor(2);
     const bool gated = args.integer(3);
-    if (!args.ok || !quiet() || !ready(lib.llmctl_gemm_int4) || !lib.llmctl_gemm_int4_scratch_elems || !bf16(x) || x.dim() < 1 || x.numel() == 0 || recorded({&x}) ||
+    if (!args.ok || !quiet() || !ready(lib.llmctl_gemm_int4) || !lib.llmctl_gemm_int4_scratch_elems || !lib.llmctl_gemm_int4_tokens || !bf16(x) || x.dim() < 1 || x.numel() == 0 || recorded({&x}) ||
         x.get_device() != c10::cuda::current_device() || w.get_device() != x.get_device() || scale.get_device() != x.get_device())
       return none();
     const int64_t K = x.size(-1), T = x.numel() / K;
-    if (T > (w.dim() == 2 && w.size(0) * w.size(1) >= 16 << 20 ? 192 : 128) || K % 128 || w.scalar_type() != at::kByte || w.dim() != 2 || w.size(1) * 2 != K || w.size(0) == 0 || w.stride(1) != 1 || w.stride(0) % 16 || w.stride(0) < K / 2 || !unit16(w) ||
+    if (K % 128 || w.scalar_type() != at::kByte || w.dim() != 2 || w.size(1) * 2 != K || w.size(0) == 0 || w.stride(1) != 1 || w.stride(0) % 16 || w.stride(0) < K / 2 || !unit16(w) ||
         (gated && w.size(0) % 2) || scale.scalar_type() != at::kHalf || scale.dim() != 2 || scale.size(0) != w.size(0) || scale.size(1) != K / 128 || scale.stride(1) != 1 ||
-        scale.stride(0) < scale.size(1) || w.size(0) > (1 << 28) || K > (1 << 28))
+        scale.stride(0) < scale.size(1) || w.size(0) > (1 << 28) || K > (1 << 28) || T > lib.llmctl_gemm_int4_tokens(w.size(0), static_cast<int>(K)))
       return none();
     const Tensor rows = as_rows(x);
     if (!rows.defined() || rows.stride(0) < K) return none();

@@ -638,14 +638,13 @@ INT4_GROUP = 128                # input channels to a scale
 
 native.register_signature("llmctl_gemm_int4", [c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll] + [c_int] * 4 + [c_void_p, c_ll, c_void_p, c_int, c_void_p])
 native.register_signature("llmctl_gemm_int4_scratch_elems", [c_int] * 4 + [c_void_p], restype=c_ll)
+native.register_signature("llmctl_gemm_int4_tokens", [c_ll, c_int])
 native.register_signature("llmctl_int4_prepare", [c_void_p, c_ll, c_int, c_void_p, c_ll, c_void_p, c_ll] + [c_int] * 4 + [c_void_p] * 5)
 native.register_signature("llmctl_gemm_f16_scaled", [c_void_p] * 5 + [c_int] * 3 + [c_ll] * 3 + [c_int, c_void_p])
 
 def _int4_tokens(w: torch.Tensor) -> int:
-    """Tokens up to which the weights are read in 4 bits, once for 64 of them.  For more they are widened to fp16 and the product is the GEMM's, whose time hardly depends
-    on the number of tokens up to 256 (us, in 4 bits / widened: 4096 rows of 11008 190 tokens 48 / 58, 256 63 / 58; 32000 x 4096 190 95 / 123; 12288 x 4096 129 53 / 52; smaller ones,
-    4096 x 4096 100 19 / 25, 129 27 / 25, gated 2048 -> 5632 100 31 / 27, 129 42 / 27)."""
-    return 192 if w.shape[0] * w.shape[1] >= 16 << 20 else 128
+    """Tokens up to which the weights are read in 4 bits; for more they are widened."""
+    return native.lib().llmctl_gemm_int4_tokens(w.shape[0], 2 * w.shape[1])
 
 
 def dequantize_int4(w: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:

@@ -177,10 +177,11 @@ unsigned long long llmctl_stream_capture_id(void* stream);
  * [tokens, K], w uint8 rows of K / 2 bytes (column 2i in the low half of byte i), scale fp16 rows of K / 128, K a multiple of 128.  gated: w has 2 * rows rows,
  * gate first, and out = silu(gate) * up.  x and w lie on 16-byte boundaries, ldx % 8 == 0, ldw % 16 == 0 (bytes).  partial: fp32 scratch, tickets: zeroed
  * counters (left zero on return), as many as llmctl_gemm_int4_scratch_elems says (0: not used); one call at a time per pair, as with the skinny GEMM.
- * More tokens: llmctl_int4_prepare writes x_out fp16 [tokens, K] and w_out fp16 [halves * padded, K] (rows past a half's last are zeros), rows in one range, and the powers
+ * More tokens than llmctl_gemm_int4_tokens: llmctl_int4_prepare writes x_out fp16 [tokens, K] and w_out fp16 [halves * padded, K] (rows past a half's last are zeros), rows in one range, and the powers
  * of two that they are to be multiplied by: x_by [tokens], w_by [halves][padded up to a multiple of 64].  llmctl_gemm_f16_scaled (csrc/gemm/gemm_tcgen05.cu): bf16
  * C[m, n] = rows_by[m] columns_by[n] sum_k X[m, k] W[n, k], N a multiple of 8; gated: W [2 N, K], columns_by as w_by is laid out, C = silu(gate) * up.
  * Reference: none (`--quant` is an option of a stub command, llmctl/cli/commands/export.py:17). */
+int llmctl_gemm_int4_tokens(long long matrix_rows, int K);
 long long llmctl_gemm_int4_scratch_elems(int tokens, int rows, int K, int gated, int* tickets);
 int llmctl_gemm_int4(const void* x, long long ldx, const void* w, long long ldw, const void* scale, long long lds, void* out, long long ldo, int tokens,
                      int rows, int K, int gated, float* partial, long long partial_elems, unsigned int* tickets, int n_tickets, void* stream);
