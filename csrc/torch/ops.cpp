@@ -48,7 +48,7 @@ using at::Tensor;
   X(llmctl_gemm_swiglu_bwd_bf16) X(llmctl_swiglu_bwd) X(llmctl_gemm_skinny_bf16) X(llmctl_gemm_skinny_scratch_elems) X(llmctl_flash_attn_fwd) X(llmctl_flash_attn_bwd) X(llmctl_kv_append) \
   X(llmctl_paged_attn_decode) X(llmctl_paged_attn_scratch_elems) X(llmctl_latent_kv_write) X(llmctl_latent_decode) \
   X(llmctl_rope_kv_append) X(llmctl_rope_kv_append_fp8) X(llmctl_rope_kv_append_fp8_scratch_elems) X(llmctl_paged_attn_decode_fp8) X(llmctl_paged_attn_fp8_scratch_elems) X(llmctl_token_logprobs) X(llmctl_token_logprobs_bwd) \
-  X(llmctl_gemm_int4) X(llmctl_gemm_int4_scratch_elems) X(llmctl_gemm_int4_tokens) X(llmctl_paged_attn_decode_shared) X(llmctl_paged_attn_shared_scratch_elems)
+  X(llmctl_gemm_int4) X(llmctl_gemm_int4_scratch_elems) X(llmctl_gemm_int4_tokens) X(llmctl_int4_prepare) X(llmctl_gemm_f16_scaled) X(llmctl_paged_attn_decode_shared) X(llmctl_paged_attn_shared_scratch_elems)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
   LLMCTL_ENTRIES(X)
@@ -612,7 +612,7 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// linear_int4(x, w, scale, gated, workspace) -> x @ W.T, or swiglu(x @ W.T), of at most 192 rows with weights of 4 bits
+// linear_int4(x, w, scale, gated, workspace) -> x @ W.T, or swiglu(x @ W.T), with weights of 4 bits
 PyObject* py_linear_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return call(a, n, 5, [&](Args& args) -> PyObject* {
     const Tensor x = args.tensor(0), w = args.tensor(1), scale = args.tensor(2);
@@ -623,11 +623,24 @@ PyObject* py_linear_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t K = x.size(-1), T = x.numel() / K;
     if (K % 128 || w.scalar_type() != at::kByte || w.dim() != 2 || w.size(1) * 2 != K || w.size(0) == 0 || w.stride(1) != 1 || w.stride(0) % 16 || w.stride(0) < K / 2 || !unit16(w) ||
         (gated && w.size(0) % 2) || scale.scalar_type() != at::kHalf || scale.dim() != 2 || scale.size(0) != w.size(0) || scale.size(1) != K / 128 || scale.stride(1) != 1 ||
-        scale.stride(0) < scale.size(1) || w.size(0) > (1 << 28) || K > (1 << 28) || T > lib.llmctl_gemm_int4_tokens(w.size(0), static_cast<int>(K)))
+        scale.stride(0) < scale.size(1) || w.size(0) > (1 << 28) || K > (1 << 28))
       return none();
     const Tensor rows = as_rows(x);
     if (!rows.defined() || rows.stride(0) < K) return none();
     const int64_t N = w.size(0) / (gated ? 2 : 1);
+    if (T > lib.llmctl_gemm_int4_tokens(w.size(0), static_cast<int>(K))) {             // a prompt: operands in fp16
+      if (!ready(lib.llmctl_gemm_f16_scaled) || !lib.llmctl_int4_prepare || T + w.size(0) >= (1 << 30)) return none();
+      return THPVariable_Wrap(without_gil([&] {
+        const int halves = gated ? 2 : 1, t = static_cast<int>(T), k = static_cast<int>(K);
+        const int64_t padded = (N + 7) / 8 * 8, columns = (N + 63) / 64 * 64 * halves;         // rows stored by TMA begin at multiples of 16 bytes
+        Tensor x16 = fresh({T, K}, at::kHalf), w16 = fresh({halves * padded, K}, at::kHalf), by = fresh({columns + T}, at::kFloat), out = fresh({T, padded}, at::kBFloat16);
+        float* by_at = static_cast<float*>(data(by));
+        done("llmctl_int4_prepare", lib.llmctl_int4_prepare(cdata(rows), rows.stride(0), t, cdata(w), w.stride(0), cdata(scale), scale.stride(0), static_cast<int>(N), static_cast<int>(padded), halves, k, data(x16),
+                                                            by_at + columns, data(w16), by_at, stream()));
+        done("llmctl_gemm_f16_scaled", lib.llmctl_gemm_f16_scaled(cdata(x16), cdata(w16), by_at + columns, by_at, data(out), t, static_cast<int>(padded), k, K, K, padded, gated, stream()));
+        return as_shape_of(padded == N ? out : out.narrow(1, 0, N).contiguous(), x);
+      }));
+    }
     int tickets = 0;
     const long long elems = lib.llmctl_gemm_int4_scratch_elems(static_cast<int>(T), static_cast<int>(N), static_cast<int>(K), gated, &tickets);
     Tensor ws, counters;
