@@ -56,23 +56,37 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(const __nv_bfloat16* 
     const long long at = static_cast<long long>(half) * rows + in;
     const uint32_t* from = reinterpret_cast<const uint32_t*>(w + at * ldw);
     const __half* s = scale + at * lds;
-    uint32_t most = 0;
+    uint32_t next[4], most = 0;                                                                     // under way while the row's range is found, and while the words before are widened
+#pragma unroll
+    for (int k = 0; k < 4; ++k) next[k] = lane + 32 * k < words ? from[lane + 32 * k] : 0u;
     for (int g = lane; g < words / 16; g += 32) most = largest(__half_as_ushort(s[g]) & 0x7fffu, 0x7c00u, most);
     const int e = max(static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10), 1);
     const float up = __uint_as_float(static_cast<uint32_t>(153 - e) << 23);                         // the largest scale to 2^11, times 8
     if (lane == 0) *by = __uint_as_float(static_cast<uint32_t>(e + 101) << 23);
-#pragma unroll 4
-    for (int c = lane; c < words; c += 32) {
-      const uint32_t word = from[c];
-      const __half2 one = __float2half2_rn(__half2float(s[c >> 4]) * up);
-      const uint32_t even = word & 0x0f0f0f0fu, odd = (word >> 4) & 0x0f0f0f0fu;
-      const uint32_t lo = __byte_perm(even, odd, 0x5140), hi = __byte_perm(even, odd, 0x7362);       // columns 0 .. 3, 4 .. 7
-      const uint32_t pair[4] = {__byte_perm(lo, 0x64646464u, 0x4140), __byte_perm(lo, 0x64646464u, 0x4342), __byte_perm(hi, 0x64646464u, 0x4140), __byte_perm(hi, 0x64646464u, 0x4342)};
-      __half2 h[4];
+    for (int c0 = lane; c0 < words; c0 += 128) {
+      uint32_t now[4];
+      __half sc[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)                                                                     // 1024 + q less 1032, exact; one rounding
-        h[k] = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&pair[k]), __floats2half2_rn(1032.f, 1032.f)), one);
-      to[c] = *reinterpret_cast<const uint4*>(h);
+      for (int k = 0; k < 4; ++k) {
+        const int c = c0 + 32 * k;
+        now[k] = next[k];
+        if (c < words) sc[k] = s[c >> 4];
+        if (c + 128 < words) next[k] = from[c + 128];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = c0 + 32 * k;
+        if (c >= words) break;
+        const __half2 one = __float2half2_rn(__half2float(sc[k]) * up);
+        const uint32_t even = now[k] & 0x0f0f0f0fu, odd = (now[k] >> 4) & 0x0f0f0f0fu;
+        const uint32_t lo = __byte_perm(even, odd, 0x5140), hi = __byte_perm(even, odd, 0x7362);     // columns 0 .. 3, 4 .. 7
+        const uint32_t pair[4] = {__byte_perm(lo, 0x64646464u, 0x4140), __byte_perm(lo, 0x64646464u, 0x4342), __byte_perm(hi, 0x64646464u, 0x4140), __byte_perm(hi, 0x64646464u, 0x4342)};
+        __half2 h[4];
+#pragma unroll
+        for (int i2 = 0; i2 < 4; ++i2)                                                              // 1024 + q less 1032, exact; one rounding
+          h[i2] = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&pair[i2]), __floats2half2_rn(1032.f, 1032.f)), one);
+        to[c] = *reinterpret_cast<const uint4*>(h);
+      }
     }
   }
 }
