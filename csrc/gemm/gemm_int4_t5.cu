@@ -18,6 +18,10 @@
 // The work is one row of units, tile after tile, and the CTAs take equal runs of it, whatever the sizes (4096 rows are 32 tiles, for 148 SMs).  A tile that
 // more than one CTA has a part of is put together by the last of them to come, which finds the others' sums in memory and adds all up in the order of the
 // CTAs: the result does not depend on which that is, and nobody waits.
+//
+// us, weights not in L2 (a kernel that only reads them / this one): 4096 rows of 11008, 16 tokens 5.4 / 13.5, 32 16.5; 12288 x 4096, 16 tokens 5.7 / 14.0; 15360 x 5120, 61 tokens
+// 7.6 / 23.3; 32000 x 4096, 16 tokens 11.3 / 24.8; gated 2048 -> 5632, 32 tokens 3.4 / 14.6.  Bound by what a unit passes through between the barriers (bytes, whole numbers,
+// products, scaled sums, 1 us each way in) and by its ends: 3 us until the first products, 2 to 3 for the tiles in parts.  The tensor cores have 6% (16 tokens) to 21% (64) to do.
 // Reference: none.
 #include "../common/dependent.cuh"
 #include "../common/ptx.cuh"

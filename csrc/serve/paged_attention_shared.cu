@@ -17,8 +17,11 @@
 //   warp 1      MMA issuer: the next tile's scores while this one's become weights
 //   warps 2-5   queries into shared memory, scores to weights, O to memory
 //
-// Bound by the pass over the cache.  The products of rows that nobody has cost nothing that is short: a tile's two are 512 clocks, its 32 KB take 1350 to come.  Two CTAs to an SM,
-// so that one's loads are on their way while the other waits for its item's last ones.
+// Bound by the pass over the cache: us with the merge, sequences x (shared + own tokens), 32 heads of 128: 16 x (50000 + 2000) 210 - 226 (its bytes at the copy rate 179; 174 - 184
+// in this kernel), 32 x (4096 + 256) 48.5 (24; 2.5 of start, 1.5 between the kernels, 7 of merge), 67 in 8 groups x (8000 + 1001), 8 heads of the cache 87 (54); 40 heads, 48 in 3
+// groups x (400 + 777) 122 (78: the ends of items, one after the other in each CTA); 12 heads of 64, 4 x (288 + 20) 12.6: launches and the chain of one item.  The products of rows that
+// nobody has cost nothing that is short: a tile's two are 512 clocks, its 32 KB take 1350 to come.  Two CTAs to an SM, so that one's loads are on their way while the other waits
+// for its item's last ones.
 //
 // The tiles of all items stand in one row, a place in front of each item for what it costs beside its tiles, and the CTAs take equal runs of it.  What a CTA finds for an item,
 // O at its reference and the reference and the sum of each row, goes to memory at 128 c + (rows of the items before), c the CTA: a place of its own, since from each part to
