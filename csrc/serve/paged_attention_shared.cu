@@ -550,7 +550,7 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       tc_fence_after();
       if (any) {
         float* to = w.parts + at * (D + 4);
-        const bool fits = mine && at < w.capacity;
+        const bool fits = mine && at >= 0 && at < w.capacity;          // (groups that overlap may count past 32 bits)
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
@@ -617,7 +617,7 @@ __global__ void __launch_bounds__(128, W == 4 ? 8 : 5) paged_attn_shared_merge_k
       const bool first = i < common.count;
       const int j = first ? i : i - common.count, f = first ? common.f : mine.f, c = j / f;
       at = (first ? common.first : mine.first) + static_cast<long long>(kRows) * c + (j - c * f) * (first ? common.rows : mine.rows);
-      if (at < w.capacity) ml = *reinterpret_cast<const float2*>(w.parts + at * (D + 4) + D);
+      if (at >= 0 && at < w.capacity) ml = *reinterpret_cast<const float2*>(w.parts + at * (D + 4) + D);
       else at = 0;
     }
     const bool counts = !(ml.y == 0.f);      // else: no token that counts

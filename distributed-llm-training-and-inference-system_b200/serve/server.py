@@ -139,7 +139,7 @@ class InferenceServer:
 
         @app.post("/v1/completions")
         async def create_completion(req: GenerationRequest):
-            if len(self.active_requests) >= self.max_concurrent_requests:
+            if len(self.active_requests) + req.n > self.max_concurrent_requests:
                 raise HTTPException(status_code=503, detail="Server at capacity")
             if req.stream and req.n > 1:
                 raise HTTPException(status_code=422, detail="n: one completion of a stream")

@@ -116,6 +116,19 @@ def test_server_gives_choices():
         server.shutdown()
 
 
+def test_a_server_takes_no_more_completions_than_requests():
+    from fastapi.testclient import TestClient
+    from llmctl_b200.serve.server import InferenceServer
+    server = InferenceServer("gpt-tiny", engine=_engine(), max_concurrent_requests=3)
+    server.start_background()
+    try:
+        with TestClient(server.app) as client:
+            ask = lambda n: client.post("/v1/completions", json={"prompt": "a", "max_tokens": 2, "n": n}).status_code  # noqa: E731
+            assert [ask(n) for n in (4, 3, 1)] == [503, 200, 200] and not server.active_requests
+    finally:
+        server.shutdown()
+
+
 def test_weights_in_4_bits(tmp_path):
     """An int4 artifact's codes are served as they stand; other weights are quantised."""
     from safetensors.torch import save_file

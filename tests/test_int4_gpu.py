@@ -154,3 +154,29 @@ def test_the_largest_numbers_of_a_prompt():
     scale[4, 0] = float("nan")
     got = ops.linear_int4(tokens(300, 256), w, scale)
     assert not got[:, 3:5].isfinite().any() and got[:, :3].isfinite().all() and got[:, 5:].isfinite().all()
+
+
+@pytest.mark.parametrize("n", [2, 12, 300])
+def test_offsets_past_32_bits(n):
+    """The last rows of a matrix of more than 2^31 bytes are what they are by themselves."""
+    rows, width = 1_100_008, 4096
+    w = torch.empty(rows, width // 2, dtype=torch.uint8, device="cuda").random_(0, 256)
+    scale = torch.empty(rows, width // 128, dtype=torch.half, device="cuda").normal_(0, 0.01)
+    x = tokens(n, width)
+    got = ops.linear_int4(x, w, scale)
+    for part in (slice(0, 8), slice(rows - 72, rows)):
+        check(got[:, part], product(x, w[part], scale[part], widened=n > 192))
+
+
+@pytest.mark.parametrize("n", [1, 20, 300])
+@pytest.mark.parametrize("gated", [False, True])
+def test_ways_to_call(n, gated):
+    x, (w, scale) = tokens(n, 512), matrix(264, 512, 14, "cuda")
+    want = run(x, w, scale, gated)
+    with torch.inference_mode():
+        assert torch.equal(run(x, w, scale, gated), want)
+    with torch.no_grad():
+        assert torch.equal(run(x.clone().requires_grad_(True), w, scale, gated), want)
+    assert torch.equal(run(x.view(n, 1, 1, 512), w, scale, gated), want.view(n, 1, 1, -1))
+    assert torch.equal(run(x[0], w, scale, gated), run(x[:1], w, scale, gated)[0])
+    assert run(x.expand(2, n, 512), w, scale, gated).shape == (2, n, 132 if gated else 264)
