@@ -23,7 +23,7 @@
 // nobody has cost nothing that is short: a tile's two are 512 clocks, its 32 KB take 1350 to come.  Two CTAs to an SM, so that one's loads are on their way while the other waits
 // for its item's last ones.
 //
-// The tiles of all items stand in one row, a place in front of each item for what it costs beside its tiles, and the CTAs take equal runs of it.  What a CTA finds for an item,
+// The tiles of all items stand in one row, places in front of each item for what it costs beside its tiles, and the CTAs take equal runs of it.  What a CTA finds for an item,
 // O at its reference and the reference and the sum of each row, goes to memory at 128 c + (rows of the items before), c the CTA: a place of its own, since from each part to
 // the next at least one of the two grows by the part's rows.  A second kernel puts the parts together.
 //
@@ -71,13 +71,17 @@ struct Work {
 // How often the rows of an item stand in the 128, and how many rows its parts are.
 __device__ __forceinline__ int copies(int rows) { return rows <= 32 ? 4 : rows <= 64 ? 2 : 1; }
 __device__ __forceinline__ int stored(int rows) { return rows * copies(rows); }
+// Places in front of an item of an entry of so many rows: what it costs beside its tiles.  O of many rows takes 3400 clocks to leave, of one row 1000 (48 sequences of 3 groups, 400 tokens
+// shared and 777 of their own, 40 heads: the CTAs with the groups' items ended 15 us after the others, at 105; us with 1 place for all 122, 2 for those 117, 3 115).  Stored
+// side by side, [D / 4][rows], it leaves faster and is gathered slower (119; 32 sequences of 4096 + 256 tokens 47.5 -> 52).
+__device__ __forceinline__ int front(int rows) { return rows >= 8 ? 3 : 1; }
 // The items of one range of tokens: a group's shared ones (e < groups), or those that sequence e - groups has behind them.
 struct Entry {
   int first, count;                // sequences; the first one's table is read
   int t0, t1, from, tiles;         // tokens; the first tile's first
   int rows, row_tiles;             // of queries, for a head of the cache
   __device__ __forceinline__ int items(const Work& w) const { return w.kv_heads * row_tiles; }
-  __device__ __forceinline__ int places() const { return tiles + 1; }                       // of an item
+  __device__ __forceinline__ int places() const { return tiles + front(rows); }                       // of an item
   __device__ __forceinline__ int rows_of(int row_tile) const { return min(rows - row_tile * kRows, kRows); }
   __device__ __forceinline__ int stored_rows() const { return (row_tiles - 1) * kRows + stored(rows_of(row_tiles - 1)); }         // for a head of the cache
 };
@@ -131,14 +135,15 @@ struct Parts {
     }
     x = in / entry.places();
     rows_before += x / entry.row_tiles * entry.stored_rows() + x % entry.row_tiles * kRows;
-    take(in - x * entry.places());     // (n = 0: the run ends with the item's first place)
+    take(in - x * entry.places());     // (n = 0: the run ends in front of the item)
   }
   // The places of item x from `from` on.
   __device__ __forceinline__ void take(int from) {
     const int places = min(entry.places() - from, left);
     left -= places;
-    t = max(from - 1, 0);
-    n = places - (from == 0 ? 1 : 0);
+    const int before = front(entry.rows);
+    t = max(from - before, 0);
+    n = max(places - max(before - from, 0), 0);
   }
   __device__ __forceinline__ bool more() const { return n > 0; }
   __device__ __forceinline__ int head() const { return x / entry.row_tiles; }
@@ -161,7 +166,7 @@ struct Parts {
     const int places = min(entry.places(), left);
     left -= places;
     t = 0;
-    n = places - 1;                // 0: the run ends with the item's first place
+    n = max(places - front(entry.rows), 0);            // 0: the run ends in front of the item
   }
 };
 constexpr int stage_bytes(int D) { return kTile * D * 2; }
@@ -603,7 +608,7 @@ __global__ void __launch_bounds__(128, W == 4 ? 8 : 5) paged_attn_shared_merge_k
     if (x.tiles == 0) return Item{0, 0, 1, 0};
     const int r = (b - x.first) * w.per_head + h % w.per_head, row_tile = r / kRows, row_tiles = (x.count + kRows - 1) / kRows, rows = min(x.count - row_tile * kRows, kRows);
     const int stored_rows = (row_tiles - 1) * kRows + stored(x.count - (row_tiles - 1) * kRows), f = copies(rows);
-    const int place0 = x.places + (head * row_tiles + row_tile) * (x.tiles + 1) + 1, c0 = runs.owner(place0);
+    const int place0 = x.places + (head * row_tiles + row_tile) * (x.tiles + front(x.count)) + front(x.count), c0 = runs.owner(place0);
     return Item{static_cast<long long>(kRows) * c0 + x.rows + head * stored_rows + row_tile * kRows + r % kRows, (runs.owner(place0 + x.tiles - 1) - c0 + 1) * f, f, rows};
   };
   const Item common = item(group), mine = item(own);
@@ -620,6 +625,18 @@ __global__ void __launch_bounds__(128, W == 4 ? 8 : 5) paged_attn_shared_merge_k
       if (at >= 0 && at < w.capacity) ml = *reinterpret_cast<const float2*>(w.parts + at * (D + 4) + D);
       else at = 0;
     }
+    // Rows under way at once, the first ones beside their weights: of parts that do not count some other row is read and not used.
+    float v[kUnderWay][kPer];
+    auto fetch = [&](int k0) {
+#pragma unroll
+      for (int k = 0; k < kUnderWay; ++k) {
+        const float* row = w.parts + __shfl_sync(0xffffffffu, at, min(warp + W * (k0 + k), n - 1)) * (D + 4) + lane * kPer;
+        if (W * (k0 + k) >= n) continue;
+        if constexpr (kPer == 4) *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(row);
+        else *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(row);
+      }
+    };
+    fetch(0);
     const bool counts = !(ml.y == 0.f);      // else: no token that counts
     const float to = fmaxf(m, warp_max(counts ? ml.x : -INFINITY));
     const float z = !counts ? 0.f : ml.x == to ? 1.f : ex2_approx(ml.x - to), a = m == to ? 1.f : ex2_approx(m - to);
@@ -628,16 +645,8 @@ __global__ void __launch_bounds__(128, W == 4 ? 8 : 5) paged_attn_shared_merge_k
     const unsigned which = __ballot_sync(0xffffffffu, counts);
 #pragma unroll
     for (int k = 0; k < kPer; ++k) o[k] *= a;
-    // rows under way at once: of parts that do not count some other row is read and not used
     for (int k0 = 0; k0 * W < n; k0 += kUnderWay) {
-      float v[kUnderWay][kPer];
-#pragma unroll
-      for (int k = 0; k < kUnderWay; ++k) {
-        const float* row = w.parts + __shfl_sync(0xffffffffu, at, min(warp + W * (k0 + k), n - 1)) * (D + 4) + lane * kPer;
-        if (W * (k0 + k) >= n) continue;
-        if constexpr (kPer == 4) *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(row);
-        else *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(row);
-      }
+      if (k0 > 0) fetch(k0);
 #pragma unroll
       for (int k = 0; k < kUnderWay; ++k) {
         const int part = warp + W * (k0 + k);
@@ -709,7 +718,7 @@ LLMCTL_API int llmctl_paged_attn_decode_shared(const void* q, long long q_stride
   const long long limit = static_cast<long long>(max_blocks) * block_size;
   LLMCTL_REQUIRE(limit < (1LL << 31) - 256);
   // tiles of all items, and rows, count in 32 bits
-  LLMCTL_REQUIRE(2LL * batch * heads * ((limit >> 6) + 3) < (1LL << 31) && 8LL * batch * heads < (1LL << 30));
+  LLMCTL_REQUIRE(2LL * batch * heads * ((limit >> 6) + 5) < (1LL << 31) && 8LL * batch * heads < (1LL << 30));
   const int box = box_rows(block_size);
   CUtensorMap k, v;
   const uint64_t D = head_dim, Hk = kv_heads, row = D * Hk;
