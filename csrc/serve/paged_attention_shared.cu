@@ -53,6 +53,7 @@ struct Work {
   int* found;                      // [groups + batch + 1][8]: of each entry what the merge has to know (Found)
   float* parts;                    // [capacity][D + 4]
   long long capacity;
+  FastDiv by_head;                 // by per_head
 
   __device__ __forceinline__ int tokens(int b) const { return max(min(lens[b], limit), 0); }
   __device__ __forceinline__ int start(int g) const { return max(min(starts[g], batch), 0); }
@@ -99,7 +100,7 @@ __device__ __forceinline__ Entry entry_of(const Work& w, int e) {
   r.count = own ? 1 : max(end - first, 0);
   r.t0 = own ? shared : 0;
   r.t1 = own ? max(min(mine, w.limit), 0) : shared;
-  r.from = r.t0 - r.t0 % w.box;
+  r.from = r.t0 & ~(w.box - 1);             // (a power of two)
   r.tiles = r.t1 > r.t0 ? (r.t1 - r.from + kTile - 1) / kTile : 0;
   r.rows = r.count * w.per_head;
   r.row_tiles = (r.rows + kRows - 1) / kRows;
@@ -111,33 +112,40 @@ struct alignas(16) Found {
   int group;                       // of a sequence's own: the group that it has shared tokens with, or -1
   int none[2];
 };
-// Equal runs of `all` places.
+// Equal runs of `all` places.  (A quotient of at most some hundred: an approximate one is off by one at most.)
+__device__ __forceinline__ int quotient(int n, int d) {
+  const unsigned q = __float2uint_rz(__fdividef(static_cast<float>(n), static_cast<float>(d))), all = n, of = d;
+  return static_cast<int>(q * of > all ? q - 1 : (q + 1) * of <= all ? q + 1 : q);
+}
 struct Runs {
   int run, longer;
-  __device__ __forceinline__ Runs(int all, int ctas) : run(all / ctas), longer(all % ctas) {}
+  __device__ __forceinline__ explicit Runs(int all) : run(all / kCtas), longer(all % kCtas) {}
   __device__ __forceinline__ int begin(int c) const { return c * run + min(c, longer); }
   __device__ __forceinline__ int owner(int place) const {
     const int cut = longer * (run + 1);
-    return place < cut ? place / (run + 1) : longer + (place - cut) / max(run, 1);
+    return place < cut ? quotient(place, run + 1) : longer + quotient(place - cut, max(run, 1));
   }
 };
-// A CTA's run, part by part: tiles t .. t + n of item x of entry e, n > 0.
+// A CTA's run, part by part: tiles t .. t + n of an item of entry e, n > 0.
 struct Parts {
   Entry entry;
-  int e, x, t, n, left;
+  int e, t, n, left;
+  int head, row_tile;              // the item of the entry
   int rows_before;                 // of the items before this one
-  __device__ __forceinline__ Parts(const Work& w, int e_, int in, int left_, int rows_before_) : e(e_), x(0), t(0), n(0), left(left_), rows_before(rows_before_) {
+  __device__ __forceinline__ Parts(const Work& w, int e_, int in, int left_, int rows_before_) : e(e_), t(0), n(0), left(left_), head(0), row_tile(0), rows_before(rows_before_) {
     if (left == 0) return;
     entry = entry_of(w, e);
     if (entry.tiles == 0) {        // (lengths that change meanwhile)
       left = 0;
       return;
     }
-    x = in / entry.places();
-    rows_before += x / entry.row_tiles * entry.stored_rows() + x % entry.row_tiles * kRows;
+    const int x = in / entry.places();
+    head = x / entry.row_tiles;
+    row_tile = x - head * entry.row_tiles;
+    rows_before += head * entry.stored_rows() + row_tile * kRows;
     take(in - x * entry.places());     // (n = 0: the run ends in front of the item)
   }
-  // The places of item x from `from` on.
+  // The item's places from `from` on.
   __device__ __forceinline__ void take(int from) {
     const int places = min(entry.places() - from, left);
     left -= places;
@@ -146,15 +154,15 @@ struct Parts {
     n = max(places - max(before - from, 0), 0);
   }
   __device__ __forceinline__ bool more() const { return n > 0; }
-  __device__ __forceinline__ int head() const { return x / entry.row_tiles; }
-  __device__ __forceinline__ int row0() const { return x % entry.row_tiles * kRows; }
-  __device__ __forceinline__ int rows() const { return entry.rows_of(x % entry.row_tiles); }
+  __device__ __forceinline__ int row0() const { return row_tile * kRows; }
+  __device__ __forceinline__ int rows() const { return entry.rows_of(row_tile); }
   __device__ __forceinline__ void next(const Work& w) {
     n = 0;
     if (left == 0) return;
     rows_before += stored(rows());
-    if (++x == entry.items(w)) {
-      x = 0;
+    if (++row_tile == entry.row_tiles) row_tile = 0, ++head;
+    if (head == w.kv_heads) {
+      head = 0;
       do {
         if (++e >= w.groups + w.batch) {
           left = 0;
@@ -211,7 +219,7 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   volatile int* abort = &abort_flag;
 
   // The run: places and rows before each entry, by all threads, an entry each; CTA 0 leaves them for the merge.
-  const int entries = w.groups + w.batch, ctas = gridDim.x, cta = blockIdx.x;
+  const int entries = w.groups + w.batch, cta = blockIdx.x;
   auto sums_before = [&](int e0, int& tiles, int& rows) {       // of the entries e0 .. e0 + this thread's, itself left out; returns through the last thread's those of all
     int t = 0, r = 0;
     if (e0 + static_cast<int>(threadIdx.x) < entries) {
@@ -241,7 +249,7 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     sums = sums_before(e0, tiles, rows);
     all += sums.y;
   }
-  const Runs runs(all, ctas);
+  const Runs runs(all);
   const int begin = runs.begin(cta), mine = runs.begin(cta + 1) - begin;
   if (threadIdx.x == 0) found[0] = 0, found[1] = 0, found[2] = 0;
   __syncthreads();
@@ -294,7 +302,7 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     };
     int ids = fetch(), next_ids = fetch(), n = 0;
     for (; part.more(); part.next(w)) {
-      const int head = part.head(), b0 = first_block(part);
+      const int head = part.head, b0 = first_block(part);
       int at = 0;                             // the piece that `ids` is
       for (int i = 0; i < part.n; ++i) {
         const int token = part.entry.from + (part.t + i) * kTile + box * w.box;
@@ -385,8 +393,9 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       return Row{f == 4 ? quad : f == 2 ? quad >> 1 : 0, f == 4 ? lane : f == 2 ? (quad & 1) * 32 + lane : row};
     };
     auto query = [&](const Parts& p, int in) {          // of the item's row
-      const int r = p.row0() + in, b = p.entry.first + r / w.per_head;
-      return reinterpret_cast<const uint4*>(q + static_cast<long long>(b) * q_stride + (p.head() * w.per_head + r % w.per_head) * D);
+      uint32_t of_head;
+      const int b = p.entry.first + static_cast<int>(w.by_head.divide(p.row0() + in, of_head));
+      return reinterpret_cast<const uint4*>(q + static_cast<long long>(b) * q_stride + (p.head * w.per_head + of_head) * D);
     };
     // Items of at most 32 rows: a warp has a quarter of each row's queries and writes it to the four copies.  The next item's are asked for ahead.
     constexpr int kQuarter = D / 32;          // pieces of 16 bytes
@@ -438,7 +447,8 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
       const Row me = row_of(rows);
       const bool mine = me.in < rows, any = f == 4 || (f == 2 ? (quad & 1) : quad) * 32 < rows;
       int limit = t1;                         // of this row's tokens
-      if (mine) limit = min(w.tokens(part.entry.first + (part.row0() + me.in) / w.per_head), t1);
+      uint32_t of_head;
+      if (mine) limit = min(w.tokens(part.entry.first + static_cast<int>(w.by_head.divide(part.row0() + me.in, of_head))), t1);
       const long long at = static_cast<long long>(kRows) * cta + part.rows_before + me.copy * rows + me.in;
       part.next(w);
       float m = -INFINITY, l = 0.f;
@@ -584,13 +594,15 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
 // W warps (1 or 4) per sequence and query head: the parts of its group's shared tokens and of its own.  Each warp finds the parts' weights for itself, a lane to a part, and
 // adds up every Wth part's row.  Grid: heads / (4 / W), rounded up, x sequences.
 template <int D, int W>
-__global__ void __launch_bounds__(128, W == 4 ? 8 : 5) paged_attn_shared_merge_kernel(decs::Work w, __nv_bfloat16* out, int ctas) {
+__global__ void __launch_bounds__(128, W == 4 ? 8 : 5) paged_attn_shared_merge_kernel(decs::Work w, __nv_bfloat16* out) {
   using namespace decs;
   constexpr int kPer = D / 32, kUnderWay = W == 4 ? 4 : 8;
   __shared__ float rows_of_warps[W][D];
   wait_for_previous(w.found, w.parts, out);
   release_dependents();
-  const int warp = W == 4 ? threadIdx.x >> 5 : 0, lane = threadIdx.x & 31, b = blockIdx.y, h = W == 4 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5), head = h / w.per_head;
+  const int warp = W == 4 ? threadIdx.x >> 5 : 0, lane = threadIdx.x & 31, b = blockIdx.y, h = W == 4 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5);
+  uint32_t of_head;
+  const int head = static_cast<int>(w.by_head.divide(h, of_head));
   if (h >= w.kv_heads * w.per_head) return;
   const Found* found = reinterpret_cast<const Found*>(w.found);
   const int all = found[w.groups + w.batch].places;
@@ -598,7 +610,7 @@ __global__ void __launch_bounds__(128, W == 4 ? 8 : 5) paged_attn_shared_merge_k
   Found group = own;
   group.tiles = 0;
   if (own.group >= 0) group = found[own.group];
-  const Runs runs(all, ctas);
+  const Runs runs(all);
   // An item's parts: the first one's row, how many CTAs have parts, how many copies of how many rows a part is.
   struct Item {
     long long first;
@@ -606,7 +618,7 @@ __global__ void __launch_bounds__(128, W == 4 ? 8 : 5) paged_attn_shared_merge_k
   };
   auto item = [&](const Found& x) {
     if (x.tiles == 0) return Item{0, 0, 1, 0};
-    const int r = (b - x.first) * w.per_head + h % w.per_head, row_tile = r / kRows, row_tiles = (x.count + kRows - 1) / kRows, rows = min(x.count - row_tile * kRows, kRows);
+    const int r = (b - x.first) * w.per_head + static_cast<int>(of_head), row_tile = r / kRows, row_tiles = (x.count + kRows - 1) / kRows, rows = min(x.count - row_tile * kRows, kRows);
     const int stored_rows = (row_tiles - 1) * kRows + stored(x.count - (row_tiles - 1) * kRows), f = copies(rows);
     const int place0 = x.places + (head * row_tiles + row_tile) * (x.tiles + front(x.count)) + front(x.count), c0 = runs.owner(place0);
     return Item{static_cast<long long>(kRows) * c0 + x.rows + head * stored_rows + row_tile * kRows + r % kRows, (runs.owner(place0 + x.tiles - 1) - c0 + 1) * f, f, rows};
@@ -695,8 +707,8 @@ cudaError_t launch(const CUtensorMap& k, const CUtensorMap& v, const __nv_bfloat
     return e;
   // Four warps to a sequence and head while all of them are on the chip at once, else one.
   const int heads = w.kv_heads * w.per_head;
-  if (w.batch * heads <= 8 * kNumSMs) return launch_dependent(paged_attn_shared_merge_kernel<D, 4>, dim3(heads, w.batch), 128, 0, s, w, out, static_cast<int>(kCtas));
-  return launch_dependent(paged_attn_shared_merge_kernel<D, 1>, dim3((heads + 3) / 4, w.batch), 128, 0, s, w, out, static_cast<int>(kCtas));
+  if (w.batch * heads <= 8 * kNumSMs) return launch_dependent(paged_attn_shared_merge_kernel<D, 4>, dim3(heads, w.batch), 128, 0, s, w, out);
+  return launch_dependent(paged_attn_shared_merge_kernel<D, 1>, dim3((heads + 3) / 4, w.batch), 128, 0, s, w, out);
 }
 }  // namespace
 }  // namespace llmctl
@@ -727,7 +739,7 @@ LLMCTL_API int llmctl_paged_attn_decode_shared(const void* q, long long q_stride
   unsigned char* const byte = wait_report(kWaitPagedShared);
   LLMCTL_REQUIRE(byte != nullptr);
   decs::Work w = {context_lens, group_starts, shared_lens, batch, groups, heads / kv_heads, kv_heads, static_cast<int>(limit), box, reinterpret_cast<int*>(scratch),
-                  scratch + parts_at(batch, groups), capacity_of(batch, heads)};
+                  scratch + parts_at(batch, groups), capacity_of(batch, heads), FastDiv(heads / kv_heads)};
   const auto* qs = static_cast<const __nv_bfloat16*>(q);
   auto* o = static_cast<__nv_bfloat16*>(out);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
