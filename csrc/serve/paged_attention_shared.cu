@@ -75,7 +75,7 @@ __device__ __forceinline__ int stored(int rows) { return rows * copies(rows); }
 // Places in front of an item of an entry of so many rows: what it costs beside its tiles.  O of many rows takes 3400 clocks to leave, of one row 1000 (48 sequences of 3 groups, 400 tokens
 // shared and 777 of their own, 40 heads: the CTAs with the groups' items ended 15 us after the others, at 105; us with 1 place for all 122, 2 for those 117, 3 115).  Stored
 // side by side, [D / 4][rows], it leaves faster and is gathered slower (119; 32 sequences of 4096 + 256 tokens 47.5 -> 52).
-__device__ __forceinline__ int front(int rows) { return rows >= 8 ? 3 : 1; }
+__device__ __forceinline__ int front(int rows) { return rows >= 8 ? 2 : 1; }
 // The items of one range of tokens: a group's shared ones (e < groups), or those that sequence e - groups has behind them.
 struct Entry {
   int first, count;                // sequences; the first one's table is read
@@ -547,11 +547,10 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         if (from + kTile > t1) {              // what stands behind the last token may be anything
           const int st = (2 * n + 1) % kStages;
           mbar_wait_or_abort(&full[st], ((2 * n + 1) / kStages) & 1u, abort);
-          if (row < kTile && from + row >= t1) {
-            uint8_t* dst = smem + kQ + st * kStage + row * 128;
+          uint8_t* dst = smem + kQ + st * kStage + (t1 - from) * 128;
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * kPanel + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-          }
+          for (int c = 0; c < kPanels; ++c)
+            for (int i = row; i < (from + kTile - t1) * 8; i += kRows) *reinterpret_cast<uint4*>(dst + c * kPanel + i * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async_smem();
         }
         tc_fence_before();
