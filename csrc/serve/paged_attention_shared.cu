@@ -18,9 +18,9 @@
 //   warps 2-5   queries into shared memory, scores to weights, O to memory
 //
 // Bound by the pass over the cache: us with the merge, sequences x (shared + own tokens), 32 heads of 128: 16 x (50000 + 2000) 210 - 226 (its bytes at the copy rate 179; 174 - 184
-// in this kernel), 32 x (4096 + 256) 48.5 (24; 2.5 of start, 1.5 between the kernels, 7 of merge), 67 in 8 groups x (8000 + 1001), 8 heads of the cache 87 (54); 40 heads, 48 in 3
-// groups x (400 + 777) 122 (78: the ends of items, one after the other in each CTA); 12 heads of 64, 4 x (288 + 20) 12.6: launches and the chain of one item.  The products of rows that
-// nobody has cost nothing that is short: a tile's two are 512 clocks, its 32 KB take 1350 to come.  Two CTAs to an SM, so that one's loads are on their way while the other waits
+// in this kernel), 32 x (4096 + 256) 47.5 (24; 2.5 of start, 1.5 between the kernels, 6.5 of merge), 67 in 8 groups x (8000 + 1001), 8 heads of the cache 86 (54); 40 heads, 48 in 3
+// groups x (400 + 777) 114 (78: the ends of items, one after the other in each CTA), 128 in 4 groups x (512 + 10) 85 (8: 17 items to a CTA, 5300 clocks each); 12 heads of 64, 4 x
+// (288 + 20) 11.4: launches and the chain of one item.  The products of rows that nobody has cost nothing that is short: a tile's two are 512 clocks, its 32 KB take 1350 to come.  Two CTAs to an SM, so that one's loads are on their way while the other waits
 // for its item's last ones.
 //
 // The tiles of all items stand in one row, places in front of each item for what it costs beside its tiles, and the CTAs take equal runs of it.  What a CTA finds for an item,
@@ -73,7 +73,8 @@ struct Work {
 __device__ __forceinline__ int copies(int rows) { return rows <= 32 ? 4 : rows <= 64 ? 2 : 1; }
 __device__ __forceinline__ int stored(int rows) { return rows * copies(rows); }
 // Places in front of an item of an entry of so many rows: what it costs beside its tiles.  O of many rows takes 3400 clocks to leave, of one row 1000 (48 sequences of 3 groups, 400 tokens
-// shared and 777 of their own, 40 heads: the CTAs with the groups' items ended 15 us after the others, at 105; us with 1 place for all 122, 2 for those 117, 3 115).  Stored
+// shared and 777 of their own, 40 heads: the CTAs with the groups' items ended 15 us after the others, at 105, and end with them now; us with 1 place for all 122, with 2 for
+// those 117).  Stored
 // side by side, [D / 4][rows], it leaves faster and is gathered slower (119; 32 sequences of 4096 + 256 tokens 47.5 -> 52).
 __device__ __forceinline__ int front(int rows) { return rows >= 8 ? 2 : 1; }
 // The items of one range of tokens: a group's shared ones (e < groups), or those that sequence e - groups has behind them.
