@@ -11,11 +11,12 @@ namespace llmctl {
 
 // Operands of a prompt's product: x and the numbers (q - 8) s in fp16, each row brought to one range by a power of two, which the product's epilogue takes back.  bf16 would round
 // (q - 8) s to 8 bits, as far off as the output's own rounding (1.4 times the error, 1.7 gated); in fp16 it is off by 2^-12 and x, of 8 bits, is exact, both down to 2^-25 of what
-// the row's largest is brought to, 2^14: 2^-39 of it, below the products' fp32.  Infinities and NaN stay what they are and have no part in the range.  A warp has a row; 8 columns of
-// it in a lane at a time, which a warp stores as 512 whole bytes.  Bound by what it writes: 12288 x 4096 and 1777 tokens 32 us (its 155 MB at the copy rate: 24), 22528 x 4096 and
+// the row's largest is brought to, 2^14: 2^-39 of it, below the products' fp32.  Infinities and NaN stay what they are and have no part in the range.  A warp has a row of x, or up to
+// 2048 columns of a row of weights (whose range it finds for itself, in the scales); 8 columns in a lane at a time, which a warp stores as 512 whole bytes.  Bound by what it writes: 12288 x 4096 and 1777 tokens 32 us (its 155 MB at the copy rate: 24), 22528 x 4096 and
 // 4096 tokens 56 (45).  With the product behind it 151 and 523 (124 and 487 alone); as bf16, without x, 146 and 544 - and where the power limit holds the clocks down 6% less.
+constexpr int kPiece = 256;          // words of 8 columns
 __global__ void __launch_bounds__(256) int4_prepare_kernel(const __nv_bfloat16* x, long long ldx, int tokens, const uint8_t* w, long long ldw, const __half* scale, long long lds, int rows,
-                                                           int padded, int K, int all, __half* x_out, float* x_by, __half* w_out, float* w_by, long long w_by_half) {
+                                                           int padded, int K, FastDiv by_pieces, int all, __half* x_out, float* x_by, __half* w_out, float* w_by, long long w_by_half) {
   wait_for_previous(x_out, x_by, w_out, w_by);
   release_dependents();
   const int lane = threadIdx.x & 31, words = K / 8;
@@ -24,7 +25,7 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(const __nv_bfloat16* 
     if (i < tokens) {
       const uint4* from = reinterpret_cast<const uint4*>(x + i * ldx);
       uint32_t most = 0;
-#pragma unroll 4
+#pragma unroll 8
       for (int c = lane; c < words; c += 32) {
         const uint4 v = from[c];
         const uint32_t two[4] = {v.x, v.y, v.z, v.w};
@@ -35,7 +36,7 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(const __nv_bfloat16* 
       const float up = __uint_as_float(static_cast<uint32_t>(268 - e) << 23);
       if (lane == 0) x_by[i] = __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
       uint4* to = reinterpret_cast<uint4*>(x_out + static_cast<long long>(i) * K);
-#pragma unroll 4
+#pragma unroll 8
       for (int c = lane; c < words; c += 32) {
         const uint4 v = from[c];
         const uint32_t two[4] = {v.x, v.y, v.z, v.w};
@@ -46,48 +47,43 @@ __global__ void __launch_bounds__(256) int4_prepare_kernel(const __nv_bfloat16* 
       }
       continue;
     }
-    const int row = i - tokens, half = row >= padded ? 1 : 0, in = row - half * padded;
+    uint32_t piece;
+    const int row = static_cast<int>(by_pieces.divide(i - tokens, piece)), half = row >= padded ? 1 : 0, in = row - half * padded, c0 = static_cast<int>(piece) * kPiece + lane, end = min(words, c0 - lane + kPiece);
     uint4* to = reinterpret_cast<uint4*>(w_out + static_cast<long long>(row) * K);
     float* by = w_by + half * w_by_half + in;
     if (in >= rows) {
-      for (int c = lane; c < words; c += 32) to[c] = make_uint4(0u, 0u, 0u, 0u);
-      if (lane == 0) *by = 1.f;
+      for (int c = c0; c < end; c += 32) to[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (c0 == 0) *by = 1.f;
       continue;
     }
     const long long at = static_cast<long long>(half) * rows + in;
     const uint32_t* from = reinterpret_cast<const uint32_t*>(w + at * ldw);
     const __half* s = scale + at * lds;
-    uint32_t next[4], most = 0;                                                                     // under way while the row's range is found, and while the words before are widened
+    uint32_t now[kPiece / 32], most = 0;
+    __half sc[kPiece / 32];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) next[k] = lane + 32 * k < words ? from[lane + 32 * k] : 0u;
+    for (int k = 0; k < kPiece / 32; ++k) {
+      const int c = c0 + 32 * k;
+      now[k] = c < end ? from[c] : 0u;
+      sc[k] = c < end ? s[c >> 4] : __ushort_as_half(0);
+    }
     for (int g = lane; g < words / 16; g += 32) most = largest(__half_as_ushort(s[g]) & 0x7fffu, 0x7c00u, most);
     const int e = max(static_cast<int>(__reduce_max_sync(0xffffffffu, most) >> 10), 1);
     const float up = __uint_as_float(static_cast<uint32_t>(153 - e) << 23);                         // the largest scale to 2^11, times 8
-    if (lane == 0) *by = __uint_as_float(static_cast<uint32_t>(e + 101) << 23);
-    for (int c0 = lane; c0 < words; c0 += 128) {
-      uint32_t now[4];
-      __half sc[4];
+    if (c0 == 0) *by = __uint_as_float(static_cast<uint32_t>(e + 101) << 23);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int c = c0 + 32 * k;
-        now[k] = next[k];
-        if (c < words) sc[k] = s[c >> 4];
-        if (c + 128 < words) next[k] = from[c + 128];
-      }
+    for (int k = 0; k < kPiece / 32; ++k) {
+      const int c = c0 + 32 * k;
+      if (c >= end) break;
+      const __half2 one = __float2half2_rn(__half2float(sc[k]) * up);
+      const uint32_t even = now[k] & 0x0f0f0f0fu, odd = (now[k] >> 4) & 0x0f0f0f0fu;
+      const uint32_t lo = __byte_perm(even, odd, 0x5140), hi = __byte_perm(even, odd, 0x7362);       // columns 0 .. 3, 4 .. 7
+      const uint32_t pair[4] = {__byte_perm(lo, 0x64646464u, 0x4140), __byte_perm(lo, 0x64646464u, 0x4342), __byte_perm(hi, 0x64646464u, 0x4140), __byte_perm(hi, 0x64646464u, 0x4342)};
+      __half2 h[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int c = c0 + 32 * k;
-        if (c >= words) break;
-        const __half2 one = __float2half2_rn(__half2float(sc[k]) * up);
-        const uint32_t even = now[k] & 0x0f0f0f0fu, odd = (now[k] >> 4) & 0x0f0f0f0fu;
-        const uint32_t lo = __byte_perm(even, odd, 0x5140), hi = __byte_perm(even, odd, 0x7362);     // columns 0 .. 3, 4 .. 7
-        const uint32_t pair[4] = {__byte_perm(lo, 0x64646464u, 0x4140), __byte_perm(lo, 0x64646464u, 0x4342), __byte_perm(hi, 0x64646464u, 0x4140), __byte_perm(hi, 0x64646464u, 0x4342)};
-        __half2 h[4];
-#pragma unroll
-        for (int i2 = 0; i2 < 4; ++i2)                                                              // 1024 + q less 1032, exact; one rounding
-          h[i2] = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&pair[i2]), __floats2half2_rn(1032.f, 1032.f)), one);
-        to[c] = *reinterpret_cast<const uint4*>(h);
-      }
+      for (int j = 0; j < 4; ++j)                                                                   // 1024 + q less 1032, exact; one rounding
+        h[j] = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&pair[j]), __floats2half2_rn(1032.f, 1032.f)), one);
+      to[c] = *reinterpret_cast<const uint4*>(h);
     }
   }
 }
@@ -140,11 +136,11 @@ LLMCTL_API int llmctl_gemm_int4(const void* x, long long ldx, const void* w, lon
 LLMCTL_API int llmctl_int4_prepare(const void* x, long long ldx, int tokens, const void* w, long long ldw, const void* scale, long long lds, int rows, int padded, int halves, int K,
                                    void* x_out, float* x_by, void* w_out, float* w_by, void* stream) {
   LLMCTL_BEGIN();
-  LLMCTL_REQUIRE(tokens > 0 && rows > 0 && padded >= rows && (halves == 1 || halves == 2) && K > 0 && K % 128 == 0 && static_cast<long long>(padded) * halves + tokens < (1LL << 30));
+  LLMCTL_REQUIRE(tokens > 0 && rows > 0 && padded >= rows && (halves == 1 || halves == 2) && K > 0 && K % 128 == 0 && static_cast<long long>(padded) * halves * ((K / 8 + kPiece - 1) / kPiece) + tokens < (1LL << 30));
   LLMCTL_REQUIRE(aligned16(x, w, x_out, w_out) && ldx >= K && ldx % 8 == 0 && ldw >= K / 2 && ldw % 16 == 0 && lds >= K / 128);
-  const int all = padded * halves + tokens;
+  const int pieces = (K / 8 + kPiece - 1) / kPiece, all = padded * halves * pieces + tokens;
   LLMCTL_CHECK(launch_dependent(int4_prepare_kernel, min((all + 7) / 8, 8 * kNumSMs), 256, 0, static_cast<cudaStream_t>(stream), static_cast<const __nv_bfloat16*>(x), ldx, tokens,
-                                static_cast<const uint8_t*>(w), ldw, static_cast<const __half*>(scale), lds, rows, padded, K, all, static_cast<__half*>(x_out), x_by,
+                                static_cast<const uint8_t*>(w), ldw, static_cast<const __half*>(scale), lds, rows, padded, K, FastDiv(pieces), all, static_cast<__half*>(x_out), x_by,
                                 static_cast<__half*>(w_out), w_by, (padded + 63LL) / 64 * 64));
   return 0;
 }

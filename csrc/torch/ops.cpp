@@ -629,7 +629,7 @@ PyObject* py_linear_int4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!rows.defined() || rows.stride(0) < K) return none();
     const int64_t N = w.size(0) / (gated ? 2 : 1);
     if (T > lib.llmctl_gemm_int4_tokens(w.size(0), static_cast<int>(K))) {             // a prompt: operands in fp16
-      if (!ready(lib.llmctl_gemm_f16_scaled) || !lib.llmctl_int4_prepare || T + w.size(0) >= (1 << 30)) return none();
+      if (!ready(lib.llmctl_gemm_f16_scaled) || !lib.llmctl_int4_prepare || T + w.size(0) * ((K + 2047) / 2048) >= (1 << 30)) return none();
       return THPVariable_Wrap(without_gil([&] {
         const int halves = gated ? 2 : 1, t = static_cast<int>(T), k = static_cast<int>(K);
         const int64_t padded = (N + 7) / 8 * 8, columns = (N + 63) / 64 * 64 * halves;         // rows stored by TMA begin at multiples of 16 bytes
