@@ -159,10 +159,11 @@ class _HostViews:
 
 class _DecodeInputs:
     """Static device inputs of a decode step of (padded) batch ``B`` and ``max_blocks`` table columns, laid out in
-    one int32 buffer: tokens(int64) | slots(int64) | positions | context lengths | block tables | groups that share a prefix (starts, lengths)."""
+    one int32 buffer: tokens(int64) | slots(int64) | positions | context lengths | block tables, and, of a step
+    with ``groups`` that share a prefix, their starts | lengths."""
 
-    def __init__(self, B: int, max_blocks: int, device: torch.device):
-        n = 6 * B + B * max_blocks + 2 * B + 1
+    def __init__(self, B: int, max_blocks: int, device: torch.device, groups: bool = False):
+        n = 6 * B + B * max_blocks + (2 * B + 1 if groups else 0)
         pin = device.type == "cuda"
         self._hbuf = torch.zeros(n, dtype=torch.int32, pin_memory=pin)
         self._dbuf = torch.zeros(n, dtype=torch.int32, device=device)
@@ -346,7 +347,7 @@ class InferenceEngine:
                 self._ar.calls_per_step = 2 * len(self.model.blocks)
         self._graphs: Dict[Tuple[int, int, bool], "_DecodeGraph"] = {}
         self._next_prefix = 1
-        self._staging: Dict[Tuple[int, int], "_DecodeInputs"] = {}
+        self._staging: Dict[Tuple[int, int, bool], "_DecodeInputs"] = {}
 
     def check_logprobs(self, logprobs: Optional[int]) -> None:
         most = min(ops.MAX_TOP_LOGPROBS, self.cfg.vocab_size)
@@ -651,13 +652,13 @@ class InferenceEngine:
         else:
             Bb, cb = B, max_ctx
         max_blocks = (cb + self.block_size - 1) // self.block_size
-        key = (Bb, max_blocks)
+        key = (Bb, max_blocks, bool(groups))
         inp = self._staging.get(key)
         if inp is None:
             if len(self._staging) > 64:
                 self._staging.clear()
                 self._graphs.clear()
-            inp = self._staging[key] = _DecodeInputs(Bb, max_blocks, self.device)
+            inp = self._staging[key] = _DecodeInputs(Bb, max_blocks, self.device, bool(groups))
         h = inp.host
         h.fill_pad()
         at = 0
@@ -676,9 +677,9 @@ class InferenceEngine:
         self.stats["decode_tokens"] += B
         if not use_graph:
             return self._decode_core(inp, Bb, cb, bool(groups))[:B]
-        g = self._graphs.get((*key, bool(groups)))
+        g = self._graphs.get(key)
         if g is None:
-            g = self._graphs[(*key, bool(groups))] = _DecodeGraph(self, inp, Bb, cb, bool(groups))
+            g = self._graphs[key] = _DecodeGraph(self, inp, Bb, cb, bool(groups))
         return g.replay()[:B]
 
     def _gather_vocab(self, logits: torch.Tensor) -> torch.Tensor:
