@@ -12,8 +12,8 @@ namespace llmctl {
 // Operands of a prompt's product: x and the numbers (q - 8) s in fp16, each row brought to one range by a power of two, which the product's epilogue takes back.  bf16 would round
 // (q - 8) s to 8 bits, as far off as the output's own rounding (1.4 times the error, 1.7 gated); in fp16 it is off by 2^-12 and x, of 8 bits, is exact, both down to 2^-25 of what
 // the row's largest is brought to, 2^14: 2^-39 of it, below the products' fp32.  Infinities and NaN stay what they are and have no part in the range.  A warp has a row of x, or up to
-// 2048 columns of a row of weights (whose range it finds for itself, in the scales); 8 columns in a lane at a time, which a warp stores as 512 whole bytes.  Bound by what it writes: 12288 x 4096 and 1777 tokens 32 us (its 155 MB at the copy rate: 24), 22528 x 4096 and
-// 4096 tokens 56 (45).  With the product behind it 151 and 523 (124 and 487 alone); as bf16, without x, 146 and 544 - and where the power limit holds the clocks down 6% less.
+// 2048 columns of a row of weights (whose range it finds for itself, in the scales); 8 columns in a lane at a time, which a warp stores as 512 whole bytes.  Bound by what it writes: 12288 x 4096 and 1777 tokens 30.5 us (its 155 MB at the copy rate: 24), 22528 x 4096 and
+// 4096 tokens 52 (45).  With the product behind it 146 and 518 (122 and 474 alone); as bf16, without x, 146 and 544 - and where the power limit holds the clocks down 6% less.
 constexpr int kPiece = 256;          // words of 8 columns
 __global__ void __launch_bounds__(256) int4_prepare_kernel(const __nv_bfloat16* x, long long ldx, int tokens, const uint8_t* w, long long ldw, const __half* scale, long long lds, int rows,
                                                            int padded, int K, FastDiv by_pieces, int all, __half* x_out, float* x_by, __half* w_out, float* w_by, long long w_by_half) {
@@ -95,12 +95,13 @@ namespace {
 bool in_chunks(int tokens, long long matrix_rows, int K) { return tokens <= 8 || (tokens + 7) / 8 * (matrix_rows * (K / 2)) <= (23LL << 20); }
 
 // Tokens up to which the weights are read in 4 bits, once for 64 of them.  For more they are widened to fp16, and the time of the GEMM that follows hardly depends on the number
-// of tokens up to 256.  us, in 4 bits / widened: many bytes or a long K, 32000 x 4096 190 tokens 95 / 144, 256 128 / 146; 12288 x 4096 190 53 / 60, 256 71 / 61; 4096 x 4096 190
-// 27 / 30, 256 35 / 31; 2048 x 5632 190 27 / 36; 5120 x 5120 190 36 / 38.  Neither, 6144 x 2048 60 13 / 17, 65 22 / 17; gated 2048 -> 5632 65 29 / 25, 1024 -> 4096 65 19 / 16.
-// So few bytes that up to 11 chunks read them, 2048 x 2048 65 9 / 16, 96 16 / 16; gated 768 -> 2048 65 10 / 11, 96 13 / 11; 2304 x 768 65 6.4 / 8.2, 100 8.5 / 8.4.
+// of tokens up to 256.  us, in 4 bits / widened: many bytes or a long K, 32000 x 4096 190 tokens 95 / 116, 256 128 / 117; 2048 x 5632 190 26 / 30, 256 35 / 31; fewer, 12288 x 4096
+// 100 36 / 45, 190 53 / 50; 4096 x 4096 100 19 / 23, 190 27 / 25; 5120 x 5120 100 27 / 31, 190 37 / 36; neither, 6144 x 2048 60 13 / 16, 65 22 / 16; gated 2048 -> 5632 65
+// 29 / 21, 1024 -> 4096 65 19 / 14.  So few bytes that chunks of 8 tokens read them, 2048 x 2048 65 9 / 13, 96 16 / 13; gated 768 -> 2048 65 10.1 / 10.3, 96 13 / 10; 2304 x 768 65
+// 6.5 / 7.8, 100 8.6 / 8.0.
 int most_tokens(long long matrix_rows, int K) {
   const long long bytes = matrix_rows * (K / 2);
-  return bytes >= (16LL << 20) || K >= 4096 ? 192 : bytes <= (2LL << 20) ? 88 : 64;
+  return bytes >= (32LL << 20) || K > 5120 ? 192 : bytes >= (16LL << 20) || K >= 4096 ? 128 : bytes <= (2LL << 20) ? 72 : 64;
 }
 }  // namespace
 }  // namespace llmctl

@@ -69,6 +69,8 @@ class LockstepEngine:
 
     def add_requests(self, prompt_ids: List[int], n: int, *args, **kwargs) -> List[Sequence]:
         """``n`` completions of one prompt, each by itself: prefixes are shared on one GPU only."""
+        if n < 1:
+            raise ValueError(f"n: at least one completion, not {n}")
         return [self.add_request(prompt_ids, *args, **kwargs) for _ in range(n)]
 
     def has_work(self) -> bool:

@@ -91,7 +91,7 @@ def test_refusals_on_the_gpu():
         ops.linear_swiglu_int4(x.requires_grad_(True), w, scale)
 
 
-@pytest.mark.parametrize("n", [1, 50])
+@pytest.mark.parametrize("n", [1, 50, 300])
 def test_streams_and_graphs(n):
     """Calls on two streams and two replayed graphs at once, each with partial sums of its own."""
     w, scale = matrix(12800, 4096, 8, "cuda")
