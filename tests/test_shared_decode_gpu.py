@@ -96,6 +96,17 @@ def test_strides_and_no_sequences():
     assert run({**s, "q": s["q"][:0]}).shape == (0, 4, 64)
 
 
+def test_caches_past_32_bits():
+    """Blocks at the end of a cache of more than 2^31 numbers."""
+    s = oracle.batch([(5, 320)], [50, 9], 16, 32, 32, 128, device="cuda")
+    want, blocks, need = run(s), 40_000, s["k_cache"].shape[0]
+    far = {**s, "block_tables": s["block_tables"] + (blocks - need)}
+    for name in ("k_cache", "v_cache"):
+        far[name] = torch.empty(blocks, 16, 32, 128, dtype=torch.bfloat16, device="cuda")
+        far[name][-need:] = s[name]
+    assert far["k_cache"].numel() > 2 ** 31 and torch.equal(run(far), want)
+
+
 def test_refusals_on_the_gpu():
     s = oracle.batch([(2, 16)], [3], 8, 4, 2, 64, device="cuda")
     for change in [dict(q=s["q"].cpu()), dict(q=s["q"].float(), k_cache=s["k_cache"].float(), v_cache=s["v_cache"].float()), dict(context_lens=s["context_lens"].cpu()),
