@@ -608,8 +608,18 @@ __global__ void __launch_bounds__(128, W == 4 ? 8 : 5) paged_attn_shared_merge_k
   const int all = found[w.groups + w.batch].places;
   const Found own = found[w.groups + b];
   Found group = own;
-  group.tiles = 0;
-  if (own.group >= 0) group = found[own.group];
+  if (w.groups <= 32) {                      // a lane to each, beside the sequence's: one after the other they come 0.7 us later
+    const Found x = found[min(lane, max(w.groups - 1, 0))];
+    const int from = max(own.group, 0);
+    group.places = __shfl_sync(0xffffffffu, x.places, from);
+    group.rows = __shfl_sync(0xffffffffu, x.rows, from);
+    group.tiles = __shfl_sync(0xffffffffu, x.tiles, from);
+    group.count = __shfl_sync(0xffffffffu, x.count, from);
+    group.first = __shfl_sync(0xffffffffu, x.first, from);
+  } else if (own.group >= 0) {
+    group = found[own.group];
+  }
+  if (own.group < 0) group.tiles = 0;
   const Runs runs(all);
   // An item's parts: the first one's row, how many CTAs have parts, how many copies of how many rows a part is.
   struct Item {
