@@ -496,7 +496,7 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
           const float to = moves ? top : m, factor = moves ? ex2_approx(m - top) : 1.f;
           if (i != 0) {
             before_done(i);
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D; c += 16) {
               uint32_t o[16];
               tmem_ld_x16(tO + lane_off + c, o);
@@ -549,7 +549,7 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
           const int st = (2 * n + 1) % kStages;
           mbar_wait_or_abort(&full[st], ((2 * n + 1) / kStages) & 1u, abort);
           uint8_t* dst = smem + kQ + st * kStage + (t1 - from) * 128;
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < kPanels; ++c)
             for (int i = row; i < (from + kTile - t1) * 8; i += kRows) *reinterpret_cast<uint4*>(dst + c * kPanel + i * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async_smem();
