@@ -18,9 +18,9 @@
 //   warps 2-5   queries into shared memory, scores to weights, O to memory
 //
 // Bound by the pass over the cache: us with the merge, sequences x (shared + own tokens), 32 heads of 128: 16 x (50000 + 2000) 210 - 226 (its bytes at the copy rate 179; 174 - 184
-// in this kernel), 32 x (4096 + 256) 47.5 (24; 2.5 of start, 1.5 between the kernels, 6.5 of merge), 67 in 8 groups x (8000 + 1001), 8 heads of the cache 86 (54); 40 heads, 48 in 3
-// groups x (400 + 777) 114 (78: the ends of items, one after the other in each CTA), 128 in 4 groups x (512 + 10) 85 (8: 17 items to a CTA, 5300 clocks each); 12 heads of 64, 4 x
-// (288 + 20) 11.4: launches and the chain of one item.  The products of rows that nobody has cost nothing that is short: a tile's two are 512 clocks, its 32 KB take 1350 to come.  Two CTAs to an SM, so that one's loads are on their way while the other waits
+// in this kernel), 32 x (4096 + 256) 46.7 (24; 2.5 of start, 1.5 between the kernels, 6.5 of merge), 67 in 8 groups x (8000 + 1001), 8 heads of the cache 85 (54); 40 heads, 48 in 3
+// groups x (400 + 777) 112 (78: the ends of items, one after the other in each CTA), 128 in 4 groups x (512 + 10) 83 (8: 17 items to a CTA, 5300 clocks each); 12 heads of 64, 4 x
+// (288 + 20) 9.6: launches and the chain of one item.  The products of rows that nobody has cost nothing that is short: a tile's two are 512 clocks, its 32 KB take 1350 to come.  Two CTAs to an SM, so that one's loads are on their way while the other waits
 // for its item's last ones.
 //
 // The tiles of all items stand in one row, places in front of each item for what it costs beside its tiles, and the CTAs take equal runs of it.  What a CTA finds for an item,
@@ -221,54 +221,52 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
 
   // The run: places and rows before each entry, by all threads, an entry each; CTA 0 leaves them for the merge.
   const int entries = w.groups + w.batch, cta = blockIdx.x;
-  auto sums_before = [&](int e0, int& tiles, int& rows) {       // of the entries e0 .. e0 + this thread's, itself left out; returns through the last thread's those of all
-    int t = 0, r = 0;
-    if (e0 + static_cast<int>(threadIdx.x) < entries) {
-      const Entry x = entry_of(w, e0 + threadIdx.x);
-      if (x.tiles > 0) t = x.items(w) * x.places(), r = w.kv_heads * x.stored_rows();
-    }
-    const int own_t = t, own_r = r;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int a = __shfl_up_sync(0xffffffffu, t, o), b = __shfl_up_sync(0xffffffffu, r, o);
-      if (lane >= o) t += a, r += b;
-    }
-    if (lane == 31) scan[0][warp] = t, scan[1][warp] = r;
-    __syncthreads();
-    int all_t = 0, all_r = 0;
-    for (int i = 0; i < kThreads / 32; ++i) {
-      if (i == warp) tiles = all_t + t - own_t, rows = all_r + r - own_r;
-      all_t += scan[0][i], all_r += scan[1][i];
-    }
-    __syncthreads();
-    return make_int3(own_t, all_t, all_r);
-  };
-  int all = 0;
-  int3 sums;
-  int tiles, rows;
-  for (int e0 = 0; e0 < entries; e0 += kThreads) {
-    sums = sums_before(e0, tiles, rows);
-    all += sums.y;
-  }
-  const Runs runs(all);
-  const int begin = runs.begin(cta), mine = runs.begin(cta + 1) - begin;
   if (threadIdx.x == 0) found[0] = 0, found[1] = 0, found[2] = 0;
-  __syncthreads();
-  int tiles0 = 0, rows0 = 0;
-  for (int e0 = 0; e0 < entries; e0 += kThreads) {
-    if (entries > kThreads) sums = sums_before(e0, tiles, rows);           // (else they are at hand)
-    const int at = tiles0 + tiles;
-    if (e0 + static_cast<int>(threadIdx.x) < entries) {
-      if (begin >= at && begin < at + sums.x) found[0] = e0 + threadIdx.x, found[1] = begin - at, found[2] = rows0 + rows;
-      if (cta == 0) {
-        const int e = e0 + threadIdx.x;
-        const Entry x = entry_of(w, e);
-        const int g = e < w.groups ? -1 : w.group_of(e - w.groups);
-        reinterpret_cast<Found*>(w.found)[e] = Found{at, rows0 + rows, x.tiles, x.rows, x.first, g, {0, 0}};
+  int all = 0, begin = 0, mine = 0;
+  Entry x{};
+  int own_t = 0, before_t = 0, before_r = 0, all_t = 0, all_r = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {     // sums of all, then where the run begins
+    int tiles0 = 0, rows0 = 0;
+#pragma unroll 1
+    for (int e0 = 0; e0 < entries; e0 += kThreads) {
+      const int e = e0 + threadIdx.x;
+      if (pass == 0 || entries > kThreads) {           // (else they are at hand)
+        int t = 0, r = 0;
+        if (e < entries) {
+          x = entry_of(w, e);
+          if (x.tiles > 0) t = x.items(w) * x.places(), r = w.kv_heads * x.stored_rows();
+        }
+        own_t = t;
+        const int own_r = r;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int a = __shfl_up_sync(0xffffffffu, t, o), b = __shfl_up_sync(0xffffffffu, r, o);
+          if (lane >= o) t += a, r += b;
+        }
+        if (lane == 31) scan[0][warp] = t, scan[1][warp] = r;
+        __syncthreads();
+        all_t = all_r = 0;
+        for (int i = 0; i < kThreads / 32; ++i) {
+          if (i == warp) before_t = all_t + t - own_t, before_r = all_r + r - own_r;
+          all_t += scan[0][i], all_r += scan[1][i];
+        }
+        __syncthreads();
       }
+      if (pass == 1 && e < entries) {
+        const int at = tiles0 + before_t;
+        if (begin >= at && begin < at + own_t) found[0] = e, found[1] = begin - at, found[2] = rows0 + before_r;
+        if (cta == 0) reinterpret_cast<Found*>(w.found)[e] = Found{at, rows0 + before_r, x.tiles, x.rows, x.first, e < w.groups ? -1 : w.group_of(e - w.groups), {0, 0}};
+      }
+      tiles0 += all_t;
+      rows0 += all_r;
     }
-    tiles0 += sums.y;
-    rows0 += sums.z;
+    if (pass == 0) {
+      all = tiles0;
+      const Runs runs(all);
+      begin = runs.begin(cta);
+      mine = runs.begin(cta + 1) - begin;
+    }
   }
   if (cta == 0 && threadIdx.x == 0) w.found[8 * entries] = all;
   __syncthreads();
