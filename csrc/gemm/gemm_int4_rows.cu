@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) gemm_int4_rows_kernel(Int4Args
     const int token = i / kOutRows, row = i % kOutRows, at_sum = token * kPitch + (GATED ? (row >> 3) * 16 + (row & 7) : row);
     if (row0 + row >= a.rows) continue;
     float v = joined(at_sum);
-    if constexpr (GATED) v = v / (1.f + __expf(-v)) * joined(at_sum + 8);
+    if constexpr (GATED) v = v * __fdividef(1.f, 1.f + __expf(-v)) * joined(at_sum + 8);
     a.out[(token0 + token) * a.ldo + row0 + row] = __float2bfloat16(v);
   }
 }

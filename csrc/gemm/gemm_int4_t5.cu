@@ -20,8 +20,9 @@
 // CTAs: the result does not depend on which that is, and nobody waits.
 //
 // us, weights not in L2 (a kernel that only reads them / this one): 4096 rows of 11008, 16 tokens 5.4 / 13.5, 32 16.5; 12288 x 4096, 16 tokens 5.7 / 14.0; 15360 x 5120, 61 tokens
-// 7.6 / 23.3; 32000 x 4096, 16 tokens 11.3 / 24.8; gated 2048 -> 5632, 32 tokens 3.4 / 14.6.  Bound by what a unit passes through between the barriers (bytes, whole numbers,
-// products, scaled sums, 1 us each way in) and by its ends: 3 us until the first products, 2 to 3 for the tiles in parts.  The tensor cores have 6% (16 tokens) to 21% (64) to do.
+// 7.6 / 23.3; 32000 x 4096, 16 tokens 11.3 / 24.8; gated 2048 -> 5632, 32 tokens 3.4 / 13.3 (14.8 with
+// IEEE quotients, whose code, run once by each warp, comes from memory).  Bound by what a unit passes through between the barriers (bytes, whole numbers, products, scaled sums, 1 us
+// each way in) and by its ends: 3 us until the first products, 2 to 3 for the tiles in parts.  The tensor cores have 6% (16 tokens) to 21% (64) to do.
 // Reference: none.
 #include "../common/dependent.cuh"
 #include "../common/ptx.cuh"
@@ -348,7 +349,7 @@ gemm_int4_t5_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             if (row < 64 && out < a.rows) {
 #pragma unroll
               for (int n = 0; n < kMine; ++n)
-                if (n < tokens) to[n * a.ldo] = __float2bfloat16(total[n] / (1.f + __expf(-total[n])) * up_sums[(n0 + n) * 64 + row]);
+                if (n < tokens) to[n * a.ldo] = __float2bfloat16(total[n] * __fdividef(1.f, 1.f + __expf(-total[n])) * up_sums[(n0 + n) * 64 + row]);
             }
           } else if (out < a.rows) {
 #pragma unroll
