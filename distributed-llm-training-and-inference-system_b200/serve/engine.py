@@ -95,6 +95,13 @@ def load_model_for_inference(artifact, device: Optional[str] = None, dtype: Opti
 _SHARED_BYTES = 72 << 20
 
 
+class _Prompt:
+    """What completions of one prompt have in common.  Only the thread that steps the engine looks into it."""
+
+    def __init__(self):
+        self.held: List["Sequence"] = []       # those whose prompt stands in the cache, with its logits
+
+
 @dataclass
 class Sequence:
     req_id: int
@@ -115,7 +122,7 @@ class Sequence:
     logprobs: Optional[int] = None         # how many alternatives to each token's log probability; None: no log probabilities
     token_logprobs: List[dict] = field(default_factory=list)       # of each generated token: token, logprob, entropy, top [(token, logprob)]
     last_logprob: Optional[dict] = None    # of the token that was sampled last
-    group: Optional[object] = None         # completions of one prompt (``add_requests``): what they have in common
+    group: Optional["_Prompt"] = None      # completions of one prompt (``add_requests``): what they have in common
     prefix: Optional[int] = None           # while the prompt stands in the cache: which copy of it (sequences of one copy share its whole blocks)
     prompt_logits: Optional[torch.Tensor] = None       # of the prompt's last position, for completions that come after
 
@@ -356,7 +363,7 @@ class InferenceEngine:
 
     # ---- request API ---------------------------------------------------------------------------------
     def add_request(self, prompt_ids: List[int], max_tokens: int = 100, temperature: float = 1.0, top_p: float = 1.0,
-                    top_k: int = -1, on_token=None, logprobs: Optional[int] = None, group: Optional[object] = None) -> Sequence:
+                    top_k: int = -1, on_token=None, logprobs: Optional[int] = None, group: Optional[_Prompt] = None) -> Sequence:
         """``logprobs``: the sequence's ``token_logprobs`` get each generated token's log probability under the model (before temperature, top_k and top_p), the
         entropy and that many of the most probable tokens."""
         self.check_logprobs(logprobs)
@@ -386,7 +393,7 @@ class InferenceEngine:
         its whole blocks are kept once for them."""
         if n < 1:
             raise ValueError(f"n: at least one completion, not {n}")
-        group = object() if n > 1 and not self.ragged and self.st.tp == 1 else None
+        group = _Prompt() if n > 1 and not self.ragged and self.st.tp == 1 else None
         return [self.add_request(prompt_ids, max_tokens, temperature, top_p, top_k, on_token, logprobs, group) for _ in range(n)]
 
     def has_work(self) -> bool:
@@ -539,16 +546,14 @@ class InferenceEngine:
             seq.prefix, self._next_prefix = self._next_prefix, self._next_prefix + 1
             if not seq.generated:
                 seq.prompt_logits = logits[0].clone()
+                seq.group.held.append(seq)
         return logits[0]
 
     def _prefill_shared(self, seq: Sequence) -> Optional[torch.Tensor]:
         """Puts the prompt of ``seq`` into the cache from another completion of it that is there: whole blocks are shared, a last one that is not full is copied."""
-        if seq.group is None or seq.generated:
+        if seq.group is None or seq.generated or not seq.group.held:
             return None
-        other = next((s for s in self.seqs.values() if s is not seq and s.group is seq.group and s.prefix is not None and s.prompt_logits is not None), None)
-        if other is None:
-            return None
-        n, bs = len(seq.prompt_ids), self.block_size
+        other, n, bs = seq.group.held[0], len(seq.prompt_ids), self.block_size
         whole = n // bs
         self.kv.share(other.req_id, seq.req_id, whole)
         if n % bs:
@@ -557,14 +562,15 @@ class InferenceEngine:
                 for c in caches:
                     c[b].copy_(c[a])            # (what stands behind the prompt is the other one's, and will be written over)
         seq.prefix, seq.prompt_logits = other.prefix, other.prompt_logits
+        seq.group.held.append(seq)
         return seq.prompt_logits
 
-    def _forget(self, ids) -> None:
-        """Sequences whose blocks have been given back."""
-        for rid in ids:
-            s = self.seqs.get(rid)
-            if s is not None:
-                s.prefix = s.prompt_logits = None
+    @staticmethod
+    def _forget(seq: Sequence) -> None:
+        """The sequence's blocks are given back."""
+        if seq.group is not None:
+            seq.group.held = [s for s in seq.group.held if s is not seq]
+        seq.prefix = seq.prompt_logits = None
 
     def _in_groups(self, seqs: List[Sequence]) -> Tuple[List[Sequence], List[Tuple[int, int]]]:
         """Sequences that share a prefix beside one another, in front; and of each such group how many they are and how many tokens they share, if reading those once
@@ -761,7 +767,8 @@ class InferenceEngine:
 
     def _preempted(self) -> List[int]:
         ids = self.sched.pop_preempted()
-        self._forget(ids)
+        for s in filter(None, map(self.seqs.get, ids)):
+            self._forget(s)
         return ids
 
     def _emit(self, s: Sequence, tok: int, finished: List[Sequence]) -> None:
@@ -786,7 +793,7 @@ class InferenceEngine:
             s.finish_reason = "length"
         if s.finish_reason:
             s.finished = True
-            s.prefix = s.prompt_logits = None
+            self._forget(s)
             self.sched.finish(s.req_id)
             self.seqs.pop(s.req_id, None)
             s.done_event.set()
@@ -797,7 +804,7 @@ class InferenceEngine:
     def abort(self, seq: Sequence, reason: str = "error") -> None:
         if not seq.finished:
             seq.finished, seq.finish_reason = True, reason
-            seq.prefix = seq.prompt_logits = None
+            self._forget(seq)
             self.sched.finish(seq.req_id)
             self.seqs.pop(seq.req_id, None)
             seq.done_event.set()
