@@ -376,15 +376,15 @@ class InferenceEngine:
             rid = self._next_id
             self._next_id += 1
             seq = Sequence(rid, list(prompt_ids), max_tokens, temperature, top_p, top_k, on_token=on_token, logprobs=logprobs, group=group)
+            if max_tokens > 0:
+                self.seqs[rid] = seq               # before the scheduler has it: a step of another thread may plan it at once
             if self._plugin_sched is not None and max_tokens > 0:
                 self._staged.append(_StagedRequest(rid, len(prompt_ids), max_tokens, time.time()))
-                self.seqs[rid] = seq
                 return seq
             if max_tokens <= 0 or not self.sched.add_request(rid, len(prompt_ids), max_tokens):
+                self.seqs.pop(rid, None)
                 seq.finished, seq.finish_reason = True, "error"
                 seq.done_event.set()
-                return seq
-            self.seqs[rid] = seq
         return seq
 
     def add_requests(self, prompt_ids: List[int], n: int, max_tokens: int = 100, temperature: float = 1.0, top_p: float = 1.0, top_k: int = -1, on_token=None,

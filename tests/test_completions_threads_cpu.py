@@ -64,3 +64,43 @@ def test_a_completion_finds_its_prompt_whatever_stands_before_it():
     assert len({tuple(s.generated) for s in seqs}) == 1 and all(len(s.generated) == 4 for s in seqs)
     assert eng.kv.free_blocks == 64 and all(s.prompt_logits is None and s.prefix is None for s in seqs)
     assert sum(spent) <= 3 * 9                 # two at a time: once for each pair
+
+
+def test_a_server_that_many_ask_at_once(_threads_take_turns_often):
+    """Nobody's request ends in an error because others hand in theirs."""
+    from llmctl_b200.serve.server import EngineLoop
+    eng = _engine()
+    loop, seqs = EngineLoop(eng), [[] for _ in range(3)]
+
+    def ask(i):
+        for k in range(40):
+            seqs[i] += eng.add_requests([4 + i, 5, 6, 7, 8, 9], 3, 3, 0.0) if i else [eng.add_request([9, 8, 7 + k % 3], 3, 0.0)]
+            loop.wake.set()
+
+    loop.start()
+    threads = [threading.Thread(target=ask, args=(i,)) for i in range(3)]
+    try:
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        for s in sum(seqs, []):
+            assert s.done_event.wait(60)
+    finally:
+        loop.stop()
+    assert loop.error is None and all(s.finish_reason in ("length", "stop") for s in sum(seqs, []))
+    assert eng.kv.free_blocks == 64
+
+
+def test_a_request_may_be_planned_as_soon_as_it_is_handed_in():
+    """The engine's thread steps between the scheduler's taking a request and the return of the call that brings it."""
+    eng = _engine()
+    take = eng.sched.add_request
+    eng.sched.add_request = lambda *a: (take(*a), eng.step())[0]
+    seq = eng.add_request([9, 8, 7], 3, 0.0)
+    assert len(seq.generated) == 1
+    while eng.has_work():
+        eng.step()
+    assert len(seq.generated) == 3 and not eng.seqs
+    refused = eng.add_request([1] * 400, 200, 0.0)          # more than the engine's tokens
+    assert refused.finish_reason == "error" and not eng.seqs
