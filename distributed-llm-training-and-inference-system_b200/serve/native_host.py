@@ -156,9 +156,10 @@ class BatchScheduler:
         return lib().llmctl_sched_num_running(self._h)
 
     def pop_preempted(self) -> List[int]:
-        buf = (c_ll * 64)()
-        n = lib().llmctl_sched_pop_preempted(self._h, buf, 64)
-        return list(buf[:n])
+        buf, ids = (c_ll * 64)(), []
+        while n := lib().llmctl_sched_pop_preempted(self._h, buf, 64):
+            ids += buf[:n]
+        return ids
 
     def __del__(self):
         try:

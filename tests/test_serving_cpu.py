@@ -319,3 +319,21 @@ def test_bench_e2e_tensor_parallel_cli_on_gloo():
     out = r.stdout
     res = json.loads(out[out.index("{"):out.rindex("}") + 1])
     assert res["tensor_parallel"] == 2 and res["steps"] == 4 and res["decode_tokens_per_s"] > 0
+
+
+def test_preempted_sequences_are_all_told_at_once():
+    """However many lose their blocks in a step, none is left for a later step, when it may run again."""
+    from llmctl_b200.serve.native_host import BatchScheduler, KVBlockManager
+    kv = KVBlockManager(151, 1, 0.0)
+    sched = BatchScheduler(160, 100000, "vllm-like", kv)
+    assert sched.add_request(1, 1, 149)
+    for i in range(150):
+        assert sched.add_request(2 + i, 1, 4)
+    sched.step()
+    assert sched.num_running > 140
+    for _ in range(140):
+        assert sched.on_token(1)
+    running = sched.num_running
+    gone = sched.pop_preempted()
+    assert len(gone) == len(set(gone)) == sched.num_waiting > 64 and running + len(gone) == 151
+    assert sched.pop_preempted() == []
