@@ -100,6 +100,9 @@ class _Prompt:
 
     def __init__(self):
         self.held: List["Sequence"] = []       # those whose prompt stands in the cache, with its logits
+        # The block that the prompt does not fill, of each cache, as the prompt left it (8 bits: what a completion writes behind the prompt may change the
+        # block's scale, and the codes of the prompt's rows with it).
+        self.tail: Optional[List[torch.Tensor]] = None
 
 
 @dataclass
@@ -547,6 +550,9 @@ class InferenceEngine:
             if not seq.generated:
                 seq.prompt_logits = logits[0].clone()
                 seq.group.held.append(seq)
+                if self.fp8_cache and n % self.block_size:
+                    b = self.kv.block_table(seq.req_id)[n // self.block_size]
+                    seq.group.tail = [c[b].clone() for c in self._cache_tensors()]
         return logits[0]
 
     def _prefill_shared(self, seq: Sequence) -> Optional[torch.Tensor]:
@@ -558,18 +564,22 @@ class InferenceEngine:
         self.kv.share(other.req_id, seq.req_id, whole)
         if n % bs:
             a, b = self.kv.block_table(other.req_id)[whole], self.kv.block_table(seq.req_id)[whole]
-            for caches in (self.k_caches, self.v_caches, *((self.k_scales, self.v_scales) if self.fp8_cache else ())):
-                for c in caches:
-                    c[b].copy_(c[a])            # (what stands behind the prompt is the other one's, and will be written over)
+            for i, c in enumerate(self._cache_tensors()):          # (what stands behind the prompt is the other one's, and will be written over)
+                c[b].copy_(c[a] if seq.group.tail is None else seq.group.tail[i])
         seq.prefix, seq.prompt_logits = other.prefix, other.prompt_logits
         seq.group.held.append(seq)
         return seq.prompt_logits
+
+    def _cache_tensors(self) -> List[torch.Tensor]:
+        return [*self.k_caches, *self.v_caches, *((*self.k_scales, *self.v_scales) if self.fp8_cache else ())]
 
     @staticmethod
     def _forget(seq: Sequence) -> None:
         """The sequence's blocks are given back."""
         if seq.group is not None:
             seq.group.held = [s for s in seq.group.held if s is not seq]
+            if not seq.group.held:
+                seq.group.tail = None
         seq.prefix = seq.prompt_logits = None
 
     def _in_groups(self, seqs: List[Sequence]) -> Tuple[List[Sequence], List[Tuple[int, int]]]:
