@@ -196,11 +196,16 @@ def load_pretrained_state_dict(path: str | Path, dequantise: bool = True) -> Dic
         raise FileNotFoundError(f"no model.safetensors (or index) under {path}")
     if any(k.startswith("model.layers.") or k.startswith("model.embed_tokens") for k in full):
         full = from_hf_llama(full)
-    meta = path / "export.json"
-    if dequantise and meta.exists():
+    if dequantise:
         from .quantize import dequantize_if_needed
-        full = dequantize_if_needed(full, json.loads(meta.read_text()).get("quantization"))
+        full = dequantize_if_needed(full, quantisation_of(path))
     return full
+
+
+def quantisation_of(path: str | Path) -> Optional[str]:
+    """The scheme in which an artifact's matrices are quantised, as its ``export.json`` says."""
+    meta = Path(path) / "export.json"
+    return json.loads(meta.read_text()).get("quantization") if meta.exists() else None
 
 
 def has_weights(path: str | Path) -> bool:

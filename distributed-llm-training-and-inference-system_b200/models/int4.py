@@ -10,7 +10,7 @@ from typing import Dict, Optional
 import torch
 import torch.nn as nn
 
-from ..io.quantize import SCALE_SUFFIX, Int4GroupQuantizer
+from ..io.quantize import INT4_GROUP, SCALE_SUFFIX, Int4GroupQuantizer
 from ..ops import functional as ops
 from ..parallel import tp as tpl
 
@@ -31,16 +31,21 @@ class Int4Linear(nn.Module):
         return ops.linear_swiglu_int4(x, self.weight, self.scale)
 
 
+def _fit(codes: torch.Tensor, scale: torch.Tensor, rows: int, width: int) -> bool:
+    return (codes.dtype == torch.uint8 and codes.shape == (rows, width // 2) and scale.dtype == torch.float16 and width % INT4_GROUP == 0
+            and scale.shape == (rows, width // INT4_GROUP))
+
+
 def hold_in_int4(model: nn.Module, codes: Optional[Dict[str, torch.Tensor]] = None) -> int:
-    """Puts an ``Int4Linear`` in the place of every projection of ``model`` that the quantiser takes; returns how many.  ``codes``: tensors of an ``int4`` artifact
-    by name, used as they are; a projection that is not among them is quantised from its weights."""
+    """Puts an ``Int4Linear`` in the place of every projection of ``model`` that the quantiser takes (a head of its own among them); returns how many.  ``codes``:
+    tensors of an ``int4`` artifact by name, used as they are; a projection that is not among them, or not as its codes and scales would be, is quantised from its weights."""
     codes, quantiser, done = codes or {}, Int4GroupQuantizer(), 0
     for path, module in list(model.named_modules()):
         if not isinstance(module, (tpl.ColumnParallelLinear, tpl.RowParallelLinear)):
             continue
         name, device = path + ".weight", module.weight.device
         got = {k: codes[k] for k in (name, name + SCALE_SUFFIX) if k in codes}
-        if len(got) != 2 or got[name].dtype != torch.uint8:
+        if len(got) != 2 or not _fit(*got.values(), *module.weight.shape):
             got = quantiser.quantize({name: module.weight.detach()})
         if name + SCALE_SUFFIX not in got:
             continue

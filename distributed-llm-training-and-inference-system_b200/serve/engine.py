@@ -57,17 +57,22 @@ def load_model_for_inference(artifact, device: Optional[str] = None, dtype: Opti
     else:
         dev = torch.device(device)
     dtype = dtype or (torch.bfloat16 if dev.type == "cuda" else torch.float32)
+    codes: Dict[str, torch.Tensor] = {}                          # of an int4 artifact, if they are to be kept
     is_path = isinstance(artifact, (str, Path))
     p = Path(str(artifact)) if is_path else None
     if p is not None and p.is_dir():
-        from ..io.export import load_pretrained_state_dict
+        from ..io.export import load_pretrained_state_dict, quantisation_of
+        from ..io.quantize import Int4GroupQuantizer, dequantize_if_needed, get_quantizer
         mcfg = resolve_model(p)                                  # model_config.json, an HF config.json, or a registered design
         model = build_model(mcfg, dtype=dtype, device=dev)
         arch = registry.architecture_of(mcfg)
         if arch is not None and arch.load_weights is not None:
             arch.load_weights(model, p)
         else:
-            full = load_pretrained_state_dict(p)                 # our names or HF LlamaForCausalLM names
+            stored, scheme = load_pretrained_state_dict(p, dequantise=False), quantisation_of(p)       # our names or HF LlamaForCausalLM names
+            full = dequantize_if_needed(stored, scheme)
+            if weight_dtype == "int4" and scheme == "int4" and type(get_quantizer(scheme)) is Int4GroupQuantizer:
+                codes = stored
             local = shard_state_dict_for(full, model)
             with torch.no_grad():
                 for k, prm in model.named_parameters():
@@ -78,9 +83,8 @@ def load_model_for_inference(artifact, device: Optional[str] = None, dtype: Opti
     if weight_dtype == "int4":
         if not isinstance(model, GPTModel) or st.tp > 1:
             raise ValueError("weight_dtype int4: models of the GPT family, without tensor parallelism")
-        from ..io.export import load_pretrained_state_dict
         from ..models.int4 import hold_in_int4
-        hold_in_int4(model, load_pretrained_state_dict(p, dequantise=False) if p is not None and p.is_dir() else None)
+        hold_in_int4(model, codes)
     model.eval()
     for prm in model.parameters():
         prm.requires_grad_(False)
