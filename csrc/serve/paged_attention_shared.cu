@@ -6,8 +6,10 @@
 // the same form, 128 rows of queries against a range of tokens, and one kernel walks over all of them:
 //     S = Q K^T       128 rows x 64 tokens, over D          (A: Q, B: the key tile as it was loaded, both K-major)
 //     O += P V        128 rows x D, over 64 tokens          (A: P in tensor memory, B: the value tile as it was loaded, N-major)
-// A row is a thread's: maxima and sums need no exchange.  Weights are rounded to bf16 (2^-9 of each, beside the output's 2^-9) and summed as they were
-// rounded; the reference of a row moves when a score is beyond it by 8 (log2), and O is multiplied then.
+// A row is a thread's: maxima and sums need no exchange.  A weight is two numbers of bf16, itself and what that leaves of it (2^-16 of it is lost at most), each multiplied
+// with the values; as one, off by up to 2^-8, they make 1.1 to 1.4 times the error of the output's own rounding and cost less: us, one / two, the cases below, 46.7 / 50.5, 85 / 91.5,
+// 112 / 123, 223 / 248, 9.6 / 9.7.  That is what the sequences read by themselves get, and how many completions a prompt has should not show in their numbers.  The reference of a row
+// moves when a score is beyond it by 8 (log2), and O is multiplied then.
 //
 // Items of at most 32 rows (64) stand in the 128 four times (twice), and each of the four softmax warps (pair of them) takes a quarter (half) of a tile's columns, with zeros
 // for weights elsewhere and a reference of its own: a tile's exponentials, 8 clocks for each column of a warp, are shared between the warps.  The copies are
@@ -215,6 +217,7 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tS = tmem_base_smem, tP = tS + kTile, tO = tS + 128;
+  static_assert(2 * kTile <= 128 && 128 + D <= 256);
   wait_for_previous(q, tables, w.lens, w.starts, w.shared, w.found, w.parts);
   release_dependents();
   volatile int* abort = &abort_flag;
@@ -371,7 +374,8 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         if (elect_one()) {
           const uint64_t v = v0 + (st * kStage >> 4);
 #pragma unroll
-          for (int c = 0; c < kTile / 16; ++c) umma_ts<1>(tO, tP + c * 8, v + (c * 2048 >> 4), id_o, (i | c) != 0 ? 1u : 0u);
+          for (int c = 0; c < kTile / 8; ++c)               // 16 tokens' weights, and their rests
+            umma_ts<1>(tO, tP + c * 8, v + ((c >> 1) * 2048 >> 4), id_o, (i | c) != 0 ? 1u : 0u);
           umma_commit<1>(&empty[st]);
           umma_commit<1>(&o_full);
         }
@@ -430,7 +434,7 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         tc_fence_after();
         const uint32_t zero[8] = {};
 #pragma unroll
-        for (int c = 0; c < kTile / 2; c += 8) tmem_st_x8(tP + lane_off + c, zero);
+        for (int c = 0; c < kTile; c += 8) tmem_st_x8(tP + lane_off + c, zero);
         tmem_st_wait();
         form = f;
       }
@@ -510,21 +514,23 @@ paged_attn_shared_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         const float ref = m == -INFINITY ? 0.f : m;
         float l2 = 0.f;
         if constexpr (C != kChunk) before_done(i);
-#pragma unroll
+#pragma unroll 1
         for (int c0 = 0; c0 < C; c0 += kChunk) {
           if constexpr (C != kChunk) read(c0);
           if (C != kChunk && c0 + kChunk == C) have_read();
-          uint32_t p[kChunk / 2];
 #pragma unroll
-          for (int c = 0; c < kChunk / 2; ++c) {
-            const float a = ex2_approx(fmaf(__uint_as_float(s[2 * c]), scale_log2, -ref)), z = ex2_approx(fmaf(__uint_as_float(s[2 * c + 1]), scale_log2, -ref));
-            p[c] = pack_bf16x2(a, z);
-            add2(l, l2, __uint_as_float(p[c] << 16), __uint_as_float(p[c] & 0xffff0000u));
+          for (int c1 = 0; c1 < kChunk; c1 += 16) {
+            uint32_t p[16];                    // of 16 tokens eight columns of what bf16 holds, and eight of the rest
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const float a = ex2_approx(fmaf(__uint_as_float(s[c1 + 2 * c]), scale_log2, -ref)), z = ex2_approx(fmaf(__uint_as_float(s[c1 + 2 * c + 1]), scale_log2, -ref));
+              p[c] = pack_bf16x2(a, z);
+              p[8 + c] = pack_bf16x2(a - __uint_as_float(p[c] << 16), z - __uint_as_float(p[c] & 0xffff0000u));
+              add2(l, l2, a, z);
+            }
+            if (C == kChunk && c1 == 0) before_done(i);
+            tmem_st_x16(tP + lane_off + me.copy * C + c0 + c1, p);
           }
-          if constexpr (C == kChunk) before_done(i);
-          const uint32_t at_p = tP + lane_off + (me.copy * C + c0) / 2;
-          if constexpr (C == 16) tmem_st_x8(at_p, p);
-          else tmem_st_x16(at_p, p);
         }
         l += l2;
         tmem_st_wait();
