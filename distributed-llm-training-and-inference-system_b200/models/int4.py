@@ -40,9 +40,8 @@ def hold_in_int4(model: nn.Module, codes: Optional[Dict[str, torch.Tensor]] = No
     """Puts an ``Int4Linear`` in the place of every projection of ``model`` that the quantiser takes (a head of its own among them); returns how many.  ``codes``:
     tensors of an ``int4`` artifact by name, used as they are; a projection that is not among them, or not as its codes and scales would be, is quantised from its weights."""
     codes, quantiser, done = codes or {}, Int4GroupQuantizer(), 0
-    for path, module in list(model.named_modules()):
-        if not isinstance(module, (tpl.ColumnParallelLinear, tpl.RowParallelLinear)):
-            continue
+    for path in [p for p, m in model.named_modules() if isinstance(m, (tpl.ColumnParallelLinear, tpl.RowParallelLinear))]:
+        module = model.get_submodule(path)          # (one at a time: what is replaced gives its weights back)
         name, device = path + ".weight", module.weight.device
         got = {k: codes[k] for k in (name, name + SCALE_SUFFIX) if k in codes}
         if len(got) != 2 or not _fit(*got.values(), *module.weight.shape):

@@ -76,3 +76,20 @@ def test_an_artifact_is_read_once(tmp_path, monkeypatch, quantised):
     held = _engine(str(tmp_path), weight_dtype="int4")
     assert len(reads) == 1
     assert held.generate([[5, 6, 7]], max_tokens=4, temperature=0.0) == _engine("gpt-tiny", weight_dtype="int4").generate([[5, 6, 7]], max_tokens=4, temperature=0.0)
+
+
+def test_a_projection_gives_its_weights_back_as_it_is_replaced(monkeypatch):
+    """While a model is rounded, never more than one of its wide matrices stands beside those that are still to come."""
+    import weakref
+    from llmctl_b200.models import int4
+    model, seen, alive = _engine("gpt-tiny").model, [], []
+    quantise = int4.Int4GroupQuantizer.quantize
+
+    def watched(self, sd):
+        alive.append(sum(r() is not None for r in seen))
+        seen.extend(weakref.ref(model.get_submodule(k.removesuffix(".weight"))) for k in sd)
+        return quantise(self, sd)
+
+    monkeypatch.setattr(int4.Int4GroupQuantizer, "quantize", watched)
+    replaced = int4.hold_in_int4(model)
+    assert len(seen) == replaced > 4 and max(alive) <= 1
