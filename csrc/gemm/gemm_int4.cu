@@ -10,10 +10,11 @@
 namespace llmctl {
 
 // Operands of a prompt's product: x and the numbers (q - 8) s in fp16, each row brought to one range by a power of two, which the product's epilogue takes back.  bf16 would round
-// (q - 8) s to 8 bits, as far off as the output's own rounding (1.4 times the error, 1.7 gated); in fp16 it is off by 2^-12 and x, of 8 bits, is exact, both down to 2^-25 of what
+// (q - 8) s to 8 bits, as far off as the output's own rounding (1.4 times the error, 1.7 gated); in fp16 it is off by 2^-11 of itself at most and x, of 8 bits, is exact, both down to 2^-25 of what
 // the row's largest is brought to, 2^14: 2^-39 of it, below the products' fp32.  Infinities and NaN stay what they are and have no part in the range.  A warp has a row of x, or up to
 // 2048 columns of a row of weights (whose range it finds for itself, in the scales); 8 columns in a lane at a time, which a warp stores as 512 whole bytes.  Bound by what it writes: 12288 x 4096 and 1777 tokens 30.5 us (its 155 MB at the copy rate: 24), 22528 x 4096 and
-// 4096 tokens 52 (45).  With the product behind it 146 and 518 (122 and 474 alone); as bf16, without x, 146 and 544 - and where the power limit holds the clocks down 6% less.
+// 4096 tokens 52 (45).  With the product behind it 146 and 518 (122 and 474 alone) with the chip's full clocks, 172 and 610 with what the power limit leaves to passes back to back; as bf16, without x, 146 and 544, under
+// the power limit 6% less.
 constexpr int kPiece = 256;          // words of 8 columns
 __global__ void __launch_bounds__(256) int4_prepare_kernel(const __nv_bfloat16* x, long long ldx, int tokens, const uint8_t* w, long long ldw, const __half* scale, long long lds, int rows,
                                                            int padded, int K, FastDiv by_pieces, int all, __half* x_out, float* x_by, __half* w_out, float* w_by, long long w_by_half) {

@@ -7,8 +7,8 @@
 //     S = Q K^T       128 rows x 64 tokens, over D          (A: Q, B: the key tile as it was loaded, both K-major)
 //     O += P V        128 rows x D, over 64 tokens          (A: P in tensor memory, B: the value tile as it was loaded, N-major)
 // A row is a thread's: maxima and sums need no exchange.  A weight is two numbers of bf16, itself and what that leaves of it (2^-16 of it is lost at most), each multiplied
-// with the values; as one, off by up to 2^-8, they make 1.1 to 1.4 times the error of the output's own rounding and cost less: us, one / two, the cases below, 46.7 / 50.5, 85 / 91.5,
-// 112 / 123, 223 / 248, 9.6 / 9.7.  That is what the sequences read by themselves get, and how many completions a prompt has should not show in their numbers.  The reference of a row
+// with the values; as one, off by up to 2^-8, they make 1.1 to 1.4 times the error of the output's own rounding and cost less: us, one / two, cases below, 46.7 / 50.5, 85 / 91.5,
+// 112 / 123, 223 / 248, 9.6 / 9.7 (the second product alone: its numbers computed and not multiplied take nothing).  That is what the sequences read by themselves get, and how many completions a prompt has should not show in their numbers.  The reference of a row
 // moves when a score is beyond it by 8 (log2), and O is multiplied then.
 //
 // Items of at most 32 rows (64) stand in the 128 four times (twice), and each of the four softmax warps (pair of them) takes a quarter (half) of a tile's columns, with zeros
@@ -19,10 +19,10 @@
 //   warp 1      MMA issuer: the next tile's scores while this one's become weights
 //   warps 2-5   queries into shared memory, scores to weights, O to memory
 //
-// Bound by the pass over the cache: us with the merge, sequences x (shared + own tokens), 32 heads of 128: 16 x (50000 + 2000) 210 - 226 (its bytes at the copy rate 179; 174 - 184
-// in this kernel), 32 x (4096 + 256) 46.7 (24; 2.5 of start, 1.5 between the kernels, 6.5 of merge), 67 in 8 groups x (8000 + 1001), 8 heads of the cache 85 (54); 40 heads, 48 in 3
-// groups x (400 + 777) 112 (78: the ends of items, one after the other in each CTA), 128 in 4 groups x (512 + 10) 83 (8: 17 items to a CTA, 5300 clocks each); 12 heads of 64, 4 x
-// (288 + 20) 9.6: launches and the chain of one item.  The products of rows that nobody has cost nothing that is short: a tile's two are 512 clocks, its 32 KB take 1350 to come.  Two CTAs to an SM, so that one's loads are on their way while the other waits
+// Bound by the pass over the cache: us with the merge, sequences x (shared + own tokens), 32 heads of 128: 16 x (50000 + 2000) 235 - 248 (its bytes at the copy rate 179; 203
+// in this kernel by itself, the power limit holds the clocks of passes back to back), 32 x (4096 + 256) 50 (24; 2.5 of start, 1.5 between the kernels, 6.5 of merge), 67 in 8 groups x (8000 + 1001), 8 heads of the cache 88 - 92 (54); 40 heads, 48 in 3
+// groups x (400 + 777) 118 - 123 (78: the ends of items, one after the other in each CTA), 128 in 4 groups x (512 + 10) 84 (8: 17 items to a CTA, 5300 clocks each); 12 heads of 64, 4 x
+// (288 + 20) 9.7: launches and the chain of one item.  The products of rows that nobody has cost little: a tile's three are 768 clocks, its 32 KB take 1350 to come.  Two CTAs to an SM, so that one's loads are on their way while the other waits
 // for its item's last ones.
 //
 // The tiles of all items stand in one row, places in front of each item for what it costs beside its tiles, and the CTAs take equal runs of it.  What a CTA finds for an item,

@@ -94,8 +94,8 @@ def load_model_for_inference(artifact, device: Optional[str] = None, dtype: Opti
 
 #: Bytes of keys and values of a layer that reading shared prefixes once has to save before a decode step takes the kernel for it (``_in_groups``), which has 8 us more of
 #: start and merge than the one for sequences by themselves, to which a prefix that many read comes from L2.  us, shared / by themselves, 64 tokens behind the prefix: 32 heads
-#: of 128, 8 sequences of 512 tokens (59 MB) 16.6 / 15.1, of 1024 (117) 18.2 / 23.4, 16 of 256 (63) 17.8 / 18.7, 32 of 256 (130) 26.9 / 28.0, of 2048 (1040) 29.8 / 114; 12 heads of
-#: 64, 16 of 1024 (47) 14.2 / 12.2, of 2048 (94) 15.5 / 18.8.
+#: of 128, 8 sequences of 512 tokens (59 MB) 15.5 / 15.1, of 1024 (117) 16.3 / 23.4, 16 of 256 (63) 16.6 / 19.0, 32 of 256 (130) 26.1 / 28.1, of 2048 (1040) 30.2 / 113; 12 heads of
+#: 64, 16 of 1024 (47) 14.4 / 12.2, of 2048 (94) 15.5 / 18.8.
 _SHARED_BYTES = 72 << 20
 
 
